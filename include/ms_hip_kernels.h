@@ -419,6 +419,95 @@ int ms_hip_gqa(const ms_hip_gqa_desc* desc, const float* dQ, const float* dK, co
                float* dPresentK, float* dPresentV, void* dWorkspace, int64_t workspace_bytes,
                void* stream);
 
+/* ---- a serving step over many requests ----------------------------------------
+ * The attention block of a step that answers many requests at once, next to the
+ * projections (MatMulNBits) above: norms and rotation of the new queries and keys with their
+ * append to a paged cache, attention over the pages, low-rank adapters beside a
+ * projection. On device pointers and a stream, nothing allocated, only kernel launches (so
+ * every call can be captured). The calling thread's current device must be the buffers'. No
+ * counterpart in the reference, whose GroupQueryAttention holds one contiguous cache.
+ *
+ * The cache: K and V [num_pages, page_size, kv_num_heads, head_dim], fp32 or fp16
+ * (cache_type MS_HIP_DTYPE_F32 or _F16), 16-byte aligned. A step: `requests` requests, the new
+ * tokens of request r in rows [cu[r], cu[r+1]) of the step's tensors (dCu int32
+ * [requests + 1], not decreasing, cu[requests] <= tokens), after past[r] cached ones (dPast
+ * int32 [requests]); its position p lies in page table[r][p / page_size] (dTable int32
+ * [requests, max_pages]). A request may have no new token. Rows behind the last request's are
+ * left as they were, in every output. A table entry outside [0, num_pages), or a position past
+ * the table, is a page that is not there: its keys are masked, appends to it dropped. The lengths
+ * and the table are read on the device, so a captured step is replayed with new ones.
+ *   max_new, max_total   bounds of any request's new tokens and of past + new tokens (0: not
+ *                        known). They choose the launch; results do not depend on them.
+ *   q_stride, ...        floats from one token's row to the next (0: rows lie back to back);
+ *                        packed QKV rows are three pointers with one stride.
+ *   rotary               as ms_hip_gqa's: cos/sin [cos_rows, cos_cols], positions past the
+ *                        last row take it, 2 * cos_cols channels turn (at most head_dim).
+ *   eps                  of the norms. scale 0 means 1/sqrt(head_dim); local_window_size < 0:
+ *                        no window, else the key range of ms_hip_gqa. */
+typedef struct ms_hip_paged_desc {
+    int tokens, requests, max_new, max_total;
+    int num_heads, kv_num_heads, head_dim;
+    int page_size, num_pages, max_pages;
+    int cache_type;
+    int q_stride, k_stride, v_stride;
+    int do_rotary, rotary_interleaved, cos_rows, cos_cols;
+    int local_window_size;
+    float scale;
+    float eps;
+} ms_hip_paged_desc;
+int ms_hip_paged_check(const ms_hip_paged_desc* desc);
+/* Norms, rotation and append: queries and keys are normed per head, x * inv * gamma with inv =
+ * 1 / sqrt(mean(x^2) + eps) (dQGamma / dKGamma [head_dim], null: that one is not normed),
+ * rotated by their positions (do_rotary), the queries written to dQOut [tokens,
+ * num_heads * head_dim] and the keys and the values to the cache. head_dim up to 1024. dQOut
+ * may be dQ where its rows lie back to back; no other output may overlap an input
+ * (MS_HIP_ERR_INVALID). Two requests must not share a page that either appends to. */
+int ms_hip_paged_append(const ms_hip_paged_desc* desc, const float* dQ, const float* dK, const float* dV,
+                        const float* dQGamma, const float* dKGamma, const int32_t* dCu, const int32_t* dPast,
+                        const int32_t* dTable, const float* dCos, const float* dSin, float* dQOut,
+                        void* dKCache, void* dVCache, void* stream);
+/* Attention of the new tokens (their keys and values appended) over each request's positions
+ * [max(0, pos - window + 1), pos]: dOut [tokens, num_heads * head_dim]. head_dim a multiple
+ * of 8 up to 256 (else MS_HIP_ERR_UNSUPPORTED). A row that sees no key is zero. fp32 accuracy
+ * for both cache types; what a query does not see does not reach it, infinities and NaN
+ * included. The workspace is optional (a smaller, misaligned or NULL one: the keys of a tile of
+ * queries are not shared out); calls that may overlap need one each. */
+int64_t ms_hip_paged_attention_workspace_size(const ms_hip_paged_desc* desc);
+int ms_hip_paged_attention(const ms_hip_paged_desc* desc, const float* dQ, const int32_t* dCu,
+                           const int32_t* dPast, const int32_t* dTable, const void* dKCache,
+                           const void* dVCache, float* dOut, void* dWorkspace, int64_t workspace_bytes,
+                           void* stream);
+/* The norms and the rotation alone, for GroupQueryAttention with do_rotary = 0: dQ [tokens,
+ * num_heads * head_dim] and dK [tokens, kv_num_heads * head_dim] to dQOut and dKOut of the
+ * same shape (each may be its input where rows lie back to back), at dPositions int32 [tokens]
+ * (below zero: zero; needed with do_rotary). */
+typedef struct ms_hip_qk_norm_desc {
+    int tokens, num_heads, kv_num_heads, head_dim;
+    int q_stride, k_stride;
+    int do_rotary, rotary_interleaved, cos_rows, cos_cols;
+    float eps;
+} ms_hip_qk_norm_desc;
+int ms_hip_qk_norm_check(const ms_hip_qk_norm_desc* desc);
+int ms_hip_qk_norm_rotary(const ms_hip_qk_norm_desc* desc, const float* dQ, const float* dK,
+                          const float* dQGamma, const float* dKGamma, const int32_t* dPositions,
+                          const float* dCos, const float* dSin, float* dQOut, float* dKOut, void* stream);
+/* Low-rank adapters of many requests beside a shared projection:
+ * y[t] = base[t] + scale[a] * B_a (A_a x[t]) with a = adapter[t] (dAdapters int32 [tokens]; outside
+ * [0, adapters): no adapter, y[t] = base[t]). dX [tokens, K], dBase and dY [tokens, N] fp32 (dY
+ * may be dBase; dBase null: zero); dA [adapters, max_rank, K], dB [adapters, N, max_rank],
+ * fp32 or fp16 (weight_type); dRanks int32 [adapters] (null: max_rank; rows of A and columns of
+ * B from an adapter's rank on are not used), dScales fp32 [adapters] (null: 1). max_rank up to
+ * 1024. fp32 accuracy, no atomics. The workspace is needed, 16-byte aligned (a smaller or
+ * misaligned one: MS_HIP_ERR_INVALID); calls that may overlap need one each. */
+typedef struct ms_hip_lora_desc {
+    int tokens, K, N, adapters, max_rank, weight_type;
+} ms_hip_lora_desc;
+int ms_hip_lora_check(const ms_hip_lora_desc* desc);
+int64_t ms_hip_lora_workspace_size(const ms_hip_lora_desc* desc);
+int ms_hip_lora(const ms_hip_lora_desc* desc, const float* dX, const void* dA, const void* dB,
+                const int32_t* dRanks, const float* dScales, const int32_t* dAdapters,
+                const float* dBase, float* dY, void* dWorkspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -54,6 +54,7 @@
 #include "mfma_w4.h"
 #include "mfma_w4_pipe.h"
 #include "mfma_w4_rb.h"
+#include "serving.h"
 #include "skinny_w4.h"
 
 using namespace msnb;
@@ -3173,6 +3174,330 @@ int ms_hip_gqa(const ms_hip_gqa_desc* d, const float* dQ, const float* dK, const
             MS_HIP_CHECK(hipGetLastError());
         }
     }
+    return MS_HIP_OK;
+}
+
+}  // extern "C"
+
+// =========================================================================================
+// A serving step over many requests (kernels in ms_hip_serving.hip).
+namespace {
+
+// Whether [a, a + na) and [b, b + nb) share a byte.
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+int check_heads(const char* op, int tokens, int heads, int kv_heads, int head_dim)
+{
+    if (heads <= 0 || kv_heads <= 0 || heads > 65535)
+        return fail(MS_HIP_ERR_INVALID, "%s requires positive 'num_heads' (up to 65535) and 'kv_num_heads'.", op);
+    if (heads % kv_heads != 0)
+        return fail(MS_HIP_ERR_INVALID, "%s num_heads=%d must be a multiple of kv_num_heads=%d.", op, heads, kv_heads);
+    if (head_dim <= 0 || head_dim > kAppendMaxDim)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: head_dim=%d is not in [1, %d]", op, head_dim, kAppendMaxDim);
+    if (tokens < 0 || tokens > (1 << 29) || (int64_t)tokens * heads > INT_MAX)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: %d tokens of %d heads are out of range", op, tokens, heads);
+    return MS_HIP_OK;
+}
+
+int check_rotary(const char* op, int do_rotary, int rows, int cols)
+{
+    if (do_rotary && (rows <= 0 || cols <= 0))
+        return fail(MS_HIP_ERR_INVALID, "%s do_rotary=1 requires cos_cache and sin_cache.", op);
+    return MS_HIP_OK;
+}
+
+// Floats from the first of `rows` rows to the end of the last.
+int64_t span(int64_t rows, int64_t stride, int64_t width) { return rows > 0 ? (rows - 1) * stride + width : 0; }
+
+int64_t cache_bytes(const ms_hip_paged_desc& d)
+{
+    return (int64_t)d.num_pages * d.page_size * d.kv_num_heads * d.head_dim * (d.cache_type == MS_HIP_DTYPE_F16 ? 2 : 4);
+}
+
+PagedBatch paged_batch(const ms_hip_paged_desc& d, const int32_t* cu, const int32_t* past, const int32_t* table)
+{
+    PagedBatch b;
+    b.cu = cu;
+    b.past = past;
+    b.table = table;
+    b.tokens = d.tokens;
+    b.requests = d.requests;
+    b.num_pages = d.num_pages;
+    b.max_pages = d.max_pages;
+    b.page = FastDiv(d.page_size);
+    return b;
+}
+
+PagedAttnPlan paged_plan(const ms_hip_paged_desc& d, int64_t ws_avail)
+{
+    const int64_t reach = std::min<int64_t>((int64_t)d.max_pages * d.page_size, INT_MAX);
+    return paged_attention_plan(d.tokens, d.requests, d.max_new > 0 ? std::min(d.max_new, d.tokens) : d.tokens,
+                                d.max_total > 0 ? std::min<int64_t>(d.max_total, reach) : reach, d.num_heads,
+                                d.kv_num_heads, d.head_dim, d.cache_type == MS_HIP_DTYPE_F16, ws_avail, device_cus());
+}
+
+// What append and qk_norm_rotary share; the strides are in place.
+void append_rotary(AppendArgs& p, int do_rotary, int interleaved, int cos_rows, int cos_cols, const float* cos,
+                   const float* sin)
+{
+    p.cos = cos;
+    p.sin = sin;
+    p.cos_rows = cos_rows;
+    p.half = cos_cols;
+    p.rot_half = do_rotary ? std::min(2 * cos_cols, p.D) / 2 : 0;
+    p.interleaved = interleaved ? 1 : 0;
+    p.vec = (p.q_stride & 3) == 0 && (p.k_stride & 3) == 0 && (p.v_stride & 3) == 0 && (!do_rotary || (cos_cols & 3) == 0);
+    for (const void* x : {(const void*)p.q, (const void*)p.k, (const void*)p.v, (const void*)p.gq, (const void*)p.gk,
+                          (const void*)p.cos, (const void*)p.sin, (const void*)p.q_out, (const void*)p.k_out,
+                          (const void*)p.v_out})
+        if (misaligned16(x)) p.vec = 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ms_hip_paged_check(const ms_hip_paged_desc* d)
+{
+    if (!d) return fail(MS_HIP_ERR_INVALID, "[ms_hip] null PagedAttention descriptor");
+    if (int st = check_heads("PagedAttention", d->tokens, d->num_heads, d->kv_num_heads, d->head_dim)) return st;
+    if (int st = check_rotary("PagedAttention", d->do_rotary, d->cos_rows, d->cos_cols)) return st;
+    if (d->requests < 0 || d->max_new < 0 || d->max_total < 0 || d->max_pages < 0)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] PagedAttention: negative sizes");
+    if (d->page_size <= 0 || d->num_pages <= 0)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] PagedAttention: page_size and num_pages must be positive");
+    if ((int64_t)d->num_pages * d->page_size > INT_MAX)
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] PagedAttention: the cache has more than 2^31-1 rows");
+    if (d->cache_type != MS_HIP_DTYPE_F32 && d->cache_type != MS_HIP_DTYPE_F16)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] PagedAttention: cache_type must be fp32 or fp16");
+    const int qw = d->num_heads * d->head_dim, kw = d->kv_num_heads * d->head_dim;
+    if ((d->q_stride && d->q_stride < qw) || (d->k_stride && d->k_stride < kw) || (d->v_stride && d->v_stride < kw))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] PagedAttention: a row stride is below the row's width");
+    return MS_HIP_OK;
+}
+
+int ms_hip_paged_append(const ms_hip_paged_desc* d, const float* dQ, const float* dK, const float* dV,
+                        const float* dQGamma, const float* dKGamma, const int32_t* dCu, const int32_t* dPast,
+                        const int32_t* dTable, const float* dCos, const float* dSin, float* dQOut, void* dKCache,
+                        void* dVCache, void* stream)
+{
+    if (int st = gate()) return st;
+    if (int st = ms_hip_paged_check(d)) return st;
+    if (d->tokens == 0 || d->requests == 0) return MS_HIP_OK;
+    if (!dQ || !dK || !dV || !dCu || !dPast || (!dTable && d->max_pages > 0) || !dQOut || !dKCache || !dVCache)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_append: null query, key, value, lengths, table, output or cache");
+    if (d->do_rotary && (!dCos || !dSin))
+        return fail(MS_HIP_ERR_INVALID, "PagedAttention do_rotary=1 requires cos_cache and sin_cache.");
+    for (const void* x : {(const void*)dQ, (const void*)dK, (const void*)dV, (const void*)dQGamma, (const void*)dKGamma,
+                          (const void*)dCu, (const void*)dPast, (const void*)dTable, (const void*)dCos, (const void*)dSin,
+                          (const void*)dQOut})
+        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_append: buffers must be 4-byte aligned");
+    if (misaligned16(dKCache) || misaligned16(dVCache))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_append: the cache must be 16-byte aligned");
+    AppendArgs p{};
+    p.b = paged_batch(*d, dCu, dPast, dTable);
+    p.q = dQ;
+    p.k = dK;
+    p.v = dV;
+    p.gq = dQGamma;
+    p.gk = dKGamma;
+    p.q_out = dQOut;
+    p.k_out = dKCache;
+    p.v_out = dVCache;
+    p.H = d->num_heads;
+    p.kvH = d->kv_num_heads;
+    p.D = d->head_dim;
+    const int64_t qw = (int64_t)p.H * p.D, kw = (int64_t)p.kvH * p.D, T = d->tokens, f = sizeof(float);
+    p.q_stride = d->q_stride ? d->q_stride : qw;
+    p.k_stride = d->k_stride ? d->k_stride : kw;
+    p.v_stride = d->v_stride ? d->v_stride : kw;
+    p.eps = d->eps;
+    p.f16 = d->cache_type == MS_HIP_DTYPE_F16;
+    append_rotary(p, d->do_rotary, d->rotary_interleaved, d->cos_rows, d->cos_cols, dCos, dSin);
+    const int64_t qs = span(T, p.q_stride, qw) * f, ks = span(T, p.k_stride, kw) * f, vs = span(T, p.v_stride, kw) * f;
+    const int64_t cb = cache_bytes(*d), ob = T * qw * f;
+    bool clash = overlap(dQOut, ob, dQ, qs) && !(dQOut == dQ && p.q_stride == qw);
+    clash |= overlap(dQOut, ob, dK, ks) || overlap(dQOut, ob, dV, vs) || overlap(dQOut, ob, dKCache, cb) ||
+             overlap(dQOut, ob, dVCache, cb) || overlap(dKCache, cb, dVCache, cb);
+    for (const void* c : {(const void*)dKCache, (const void*)dVCache})
+        clash |= overlap(c, cb, dQ, qs) || overlap(c, cb, dK, ks) || overlap(c, cb, dV, vs);
+    if (clash) return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_append: an output overlaps an input or another output");
+    MS_HIP_CHECK(launch_append(p, static_cast<hipStream_t>(stream)));
+    return MS_HIP_OK;
+}
+
+int ms_hip_qk_norm_check(const ms_hip_qk_norm_desc* d)
+{
+    if (!d) return fail(MS_HIP_ERR_INVALID, "[ms_hip] null QkNormRotary descriptor");
+    if (int st = check_heads("QkNormRotary", d->tokens, d->num_heads, d->kv_num_heads, d->head_dim)) return st;
+    if (int st = check_rotary("QkNormRotary", d->do_rotary, d->cos_rows, d->cos_cols)) return st;
+    if ((d->q_stride && d->q_stride < d->num_heads * d->head_dim) ||
+        (d->k_stride && d->k_stride < d->kv_num_heads * d->head_dim))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] QkNormRotary: a row stride is below the row's width");
+    return MS_HIP_OK;
+}
+
+int ms_hip_qk_norm_rotary(const ms_hip_qk_norm_desc* d, const float* dQ, const float* dK, const float* dQGamma,
+                          const float* dKGamma, const int32_t* dPositions, const float* dCos, const float* dSin,
+                          float* dQOut, float* dKOut, void* stream)
+{
+    if (int st = gate()) return st;
+    if (int st = ms_hip_qk_norm_check(d)) return st;
+    if (d->tokens == 0) return MS_HIP_OK;
+    if (!dQ || !dK || !dQOut || !dKOut) return fail(MS_HIP_ERR_INVALID, "[ms_hip] qk_norm_rotary: null query, key or output");
+    if (d->do_rotary && (!dCos || !dSin || !dPositions))
+        return fail(MS_HIP_ERR_INVALID, "QkNormRotary do_rotary=1 requires positions, cos_cache and sin_cache.");
+    for (const void* x : {(const void*)dQ, (const void*)dK, (const void*)dQGamma, (const void*)dKGamma,
+                          (const void*)dPositions, (const void*)dCos, (const void*)dSin, (const void*)dQOut,
+                          (const void*)dKOut})
+        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] qk_norm_rotary: buffers must be 4-byte aligned");
+    AppendArgs p{};
+    p.b.tokens = d->tokens;
+    p.positions = d->do_rotary ? dPositions : nullptr;
+    p.q = dQ;
+    p.k = dK;
+    p.gq = dQGamma;
+    p.gk = dKGamma;
+    p.q_out = dQOut;
+    p.k_out = dKOut;
+    p.H = d->num_heads;
+    p.kvH = d->kv_num_heads;
+    p.D = d->head_dim;
+    const int64_t qw = (int64_t)p.H * p.D, kw = (int64_t)p.kvH * p.D, T = d->tokens, f = sizeof(float);
+    p.q_stride = d->q_stride ? d->q_stride : qw;
+    p.k_stride = d->k_stride ? d->k_stride : kw;
+    p.eps = d->eps;
+    append_rotary(p, d->do_rotary, d->rotary_interleaved, d->cos_rows, d->cos_cols, dCos, dSin);
+    const int64_t qs = span(T, p.q_stride, qw) * f, ks = span(T, p.k_stride, kw) * f, qb = T * qw * f, kb = T * kw * f;
+    if ((overlap(dQOut, qb, dQ, qs) && !(dQOut == dQ && p.q_stride == qw)) ||
+        (overlap(dKOut, kb, dK, ks) && !(dKOut == dK && p.k_stride == kw)) || overlap(dQOut, qb, dK, ks) ||
+        overlap(dKOut, kb, dQ, qs) || overlap(dQOut, qb, dKOut, kb))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] qk_norm_rotary: an output overlaps an input or another output");
+    MS_HIP_CHECK(launch_append(p, static_cast<hipStream_t>(stream)));
+    return MS_HIP_OK;
+}
+
+int64_t ms_hip_paged_attention_workspace_size(const ms_hip_paged_desc* d)
+{
+    return d && ms_hip_paged_check(d) == MS_HIP_OK ? paged_plan(*d, -1).ws_bytes : 0;
+}
+
+int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const int32_t* dCu, const int32_t* dPast,
+                           const int32_t* dTable, const void* dKCache, const void* dVCache, float* dOut,
+                           void* dWorkspace, int64_t workspace_bytes, void* stream)
+{
+    if (int st = gate()) return st;
+    if (int st = ms_hip_paged_check(d)) return st;
+    if (d->head_dim % 8 != 0 || d->head_dim > 256)
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_attention: head_dim=%d is not a multiple of 8 up to 256",
+                    d->head_dim);
+    if (d->tokens == 0 || d->requests == 0) return MS_HIP_OK;
+    if (!dQ || !dCu || !dPast || (!dTable && d->max_pages > 0) || !dKCache || !dVCache || !dOut)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: null query, lengths, table, cache or output");
+    for (const void* x : {(const void*)dQ, (const void*)dCu, (const void*)dPast, (const void*)dTable, (const void*)dOut})
+        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: buffers must be 4-byte aligned");
+    if (misaligned16(dKCache) || misaligned16(dVCache))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the cache must be 16-byte aligned");
+    const PagedAttnPlan plan = paged_plan(*d, dWorkspace && !misaligned16(dWorkspace) ? workspace_bytes : 0);
+    PagedAttnArgs p{};
+    p.b = paged_batch(*d, dCu, dPast, dTable);
+    p.q = dQ;
+    p.kc = dKCache;
+    p.vc = dVCache;
+    p.out = dOut;
+    p.part = static_cast<float*>(dWorkspace);
+    p.H = d->num_heads;
+    p.kvH = d->kv_num_heads;
+    p.D = d->head_dim;
+    p.window = d->local_window_size;
+    p.f16 = d->cache_type == MS_HIP_DTYPE_F16;
+    p.splits = plan.splits;
+    const int64_t qw = (int64_t)p.H * p.D, T = d->tokens, f = sizeof(float);
+    p.q_stride = d->q_stride ? d->q_stride : qw;
+    p.grp = FastDiv(p.H / p.kvH);
+    p.scale2 = (d->scale != 0.0f ? d->scale : 1.0f / std::sqrt((float)p.D)) * 1.44269504088896341f;
+    const int64_t ob = T * qw * f, cb = cache_bytes(*d);
+    if (overlap(dOut, ob, dQ, span(T, p.q_stride, qw) * f) || overlap(dOut, ob, dKCache, cb) || overlap(dOut, ob, dVCache, cb) ||
+        overlap(dOut, ob, dWorkspace, plan.ws_bytes))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the output overlaps an input or the workspace");
+    MS_HIP_CHECK(launch_paged_attention(p, plan, static_cast<hipStream_t>(stream)));
+    return MS_HIP_OK;
+}
+
+int ms_hip_lora_check(const ms_hip_lora_desc* d)
+{
+    if (!d) return fail(MS_HIP_ERR_INVALID, "[ms_hip] null LoRA descriptor");
+    if (d->tokens < 0 || d->K <= 0 || d->N <= 0 || d->adapters <= 0 || d->max_rank <= 0)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: tokens must be at least 0, K, N, adapters and max_rank at least 1");
+    if (d->max_rank > 1024) return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] lora: max_rank %d is above 1024", d->max_rank);
+    if (d->weight_type != MS_HIP_DTYPE_F32 && d->weight_type != MS_HIP_DTYPE_F16)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: weight_type must be fp32 or fp16");
+    if (d->tokens > (1 << 24) || d->K > (1 << 26) || d->N > (1 << 26) ||
+        ((int64_t)d->tokens / 16 + 1) * (d->N / 64 + 1) * 16 > INT_MAX)
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] lora: %d tokens of K=%d, N=%d are out of range", d->tokens, d->K, d->N);
+    return MS_HIP_OK;
+}
+
+int64_t ms_hip_lora_workspace_size(const ms_hip_lora_desc* d)
+{
+    if (!d || ms_hip_lora_check(d) != MS_HIP_OK || d->tokens == 0) return 0;
+    return lora_plan(d->tokens, d->K, d->N, d->adapters, d->max_rank, device_cus()).ws_bytes;
+}
+
+int ms_hip_lora(const ms_hip_lora_desc* d, const float* dX, const void* dA, const void* dB, const int32_t* dRanks,
+                const float* dScales, const int32_t* dAdapters, const float* dBase, float* dY, void* dWorkspace,
+                int64_t workspace_bytes, void* stream)
+{
+    if (int st = gate()) return st;
+    if (int st = ms_hip_lora_check(d)) return st;
+    if (d->tokens == 0) return MS_HIP_OK;
+    if (!dX || !dA || !dB || !dAdapters || !dY)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: null input, weights, adapter list or output");
+    for (const void* x : {(const void*)dX, (const void*)dRanks, (const void*)dScales, (const void*)dAdapters,
+                          (const void*)dBase, (const void*)dY})
+        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: buffers must be 4-byte aligned");
+    const bool f16 = d->weight_type == MS_HIP_DTYPE_F16;
+    for (const void* x : {dA, dB})
+        if (reinterpret_cast<uintptr_t>(x) & (f16 ? 1 : 3))
+            return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: weights must be aligned to their type");
+    const LoraPlan plan = lora_plan(d->tokens, d->K, d->N, d->adapters, d->max_rank, device_cus());
+    if (!dWorkspace || misaligned16(dWorkspace) || workspace_bytes < plan.ws_bytes)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora needs a 16-byte aligned workspace of %lld bytes (got %lld)",
+                    (long long)plan.ws_bytes, (long long)(dWorkspace ? workspace_bytes : 0));
+    LoraArgs p{};
+    p.x = dX;
+    p.a = dA;
+    p.b = dB;
+    p.ranks = dRanks;
+    p.scales = dScales;
+    p.which = dAdapters;
+    p.base = dBase;
+    p.y = dY;
+    p.h = static_cast<float*>(dWorkspace);
+    p.T = d->tokens;
+    p.K = d->K;
+    p.N = d->N;
+    p.adapters = d->adapters;
+    p.rank = d->max_rank;
+    p.rank16 = (d->max_rank + 15) / 16 * 16;
+    p.f16 = f16;
+    p.splits = plan.splits;
+    p.vec = (p.K & 7) == 0 && (p.N & 3) == 0 && (p.rank & 3) == 0;
+    for (const void* x : {(const void*)dX, dA, dB, (const void*)dBase, (const void*)dY})
+        if (misaligned16(x)) p.vec = 0;
+    const int64_t f = sizeof(float), yb = (int64_t)p.T * p.N * f, xb = (int64_t)p.T * p.K * f, e = f16 ? 2 : 4;
+    const int64_t ab = (int64_t)p.adapters * p.rank * p.K * e, bb = (int64_t)p.adapters * p.rank * p.N * e;
+    if (overlap(dY, yb, dX, xb) || overlap(dY, yb, dA, ab) || overlap(dY, yb, dB, bb) ||
+        (dBase != dY && overlap(dY, yb, dBase, yb)))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: the output overlaps an input");
+    for (const void* x : {(const void*)dX, (const void*)dBase, (const void*)dY})
+        if (overlap(dWorkspace, plan.ws_bytes, x, x == dX ? xb : yb))
+            return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: the workspace overlaps a buffer of the call");
+    MS_HIP_CHECK(launch_lora(p, plan, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;
 }
 

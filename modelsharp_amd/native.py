@@ -74,6 +74,15 @@ _PROTOTYPES = {
     "ms_hip_gqa_check": (_c_int, [_vp]),
     "ms_hip_gqa": (_c_int, [_vp] * 13 + [_c_i64, _vp]),
     "ms_hip_gqa_workspace_size": (_c_i64, [_vp]),
+    "ms_hip_paged_check": (_c_int, [_vp]),
+    "ms_hip_paged_append": (_c_int, [_vp] * 15),
+    "ms_hip_paged_attention_workspace_size": (_c_i64, [_vp]),
+    "ms_hip_paged_attention": (_c_int, [_vp] * 9 + [_c_i64, _vp]),
+    "ms_hip_qk_norm_check": (_c_int, [_vp]),
+    "ms_hip_qk_norm_rotary": (_c_int, [_vp] * 11),
+    "ms_hip_lora_check": (_c_int, [_vp]),
+    "ms_hip_lora_workspace_size": (_c_i64, [_vp]),
+    "ms_hip_lora": (_c_int, [_vp] * 10 + [_c_i64, _vp]),
     "ms_hip_nbits_weights_create_from_files": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int,
                                                         ctypes.POINTER(_vp)]),
     "ms_hip_debug_force_failure": (_c_int, [_c_int]),
@@ -469,3 +478,58 @@ def gqa(desc: GqaDesc, dQ, dK, dV, dPastK, dPastV, dSeqlens, dCos, dSin, dOut, d
     check(load().ms_hip_gqa(ctypes.byref(desc), _d(dQ), _d(dK), _d(dV), _d(dPastK), _d(dPastV), _d(dSeqlens),
                             _d(dCos), _d(dSin), _d(dOut), _d(dPresentK), _d(dPresentV), _d(dWorkspace),
                             int(workspace_bytes), _d(stream)))
+
+
+# ---- a serving step over many requests (device pointers; 0 / None for an absent optional buffer) ----
+class PagedDesc(ctypes.Structure):
+    """ms_hip_paged_desc."""
+    _fields_ = [(n, ctypes.c_int) for n in (
+        "tokens", "requests", "max_new", "max_total", "num_heads", "kv_num_heads", "head_dim", "page_size", "num_pages",
+        "max_pages", "cache_type", "q_stride", "k_stride", "v_stride", "do_rotary", "rotary_interleaved", "cos_rows",
+        "cos_cols", "local_window_size")] + [("scale", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+class QkNormDesc(ctypes.Structure):
+    """ms_hip_qk_norm_desc."""
+    _fields_ = [(n, ctypes.c_int) for n in (
+        "tokens", "num_heads", "kv_num_heads", "head_dim", "q_stride", "k_stride", "do_rotary", "rotary_interleaved",
+        "cos_rows", "cos_cols")] + [("eps", ctypes.c_float)]
+
+
+class LoraDesc(ctypes.Structure):
+    """ms_hip_lora_desc."""
+    _fields_ = [(n, ctypes.c_int) for n in ("tokens", "K", "N", "adapters", "max_rank", "weight_type")]
+
+
+def paged_append(desc: PagedDesc, dQ, dK, dV, dQGamma, dKGamma, dCu, dPast, dTable, dCos, dSin, dQOut, dKCache,
+                 dVCache, stream=None):
+    """Norms per head, rotation, and append of the new keys and values to their pages."""
+    check(load().ms_hip_paged_append(ctypes.byref(desc), dQ, dK, dV, dQGamma, dKGamma, dCu, dPast, dTable, dCos, dSin,
+                                     dQOut, dKCache, dVCache, stream))
+
+
+def paged_attention_workspace_size(desc: PagedDesc) -> int:
+    return int(load().ms_hip_paged_attention_workspace_size(ctypes.byref(desc)))
+
+
+def paged_attention(desc: PagedDesc, dQ, dCu, dPast, dTable, dKCache, dVCache, dOut, dWorkspace=None,
+                    workspace_bytes=0, stream=None):
+    """Attention of each request's new tokens over its pages."""
+    check(load().ms_hip_paged_attention(ctypes.byref(desc), dQ, dCu, dPast, dTable, dKCache, dVCache, dOut, dWorkspace,
+                                        workspace_bytes, stream))
+
+
+def qk_norm_rotary(desc: QkNormDesc, dQ, dK, dQGamma, dKGamma, dPositions, dCos, dSin, dQOut, dKOut, stream=None):
+    """Norms per head and rotation onto contiguous rows."""
+    check(load().ms_hip_qk_norm_rotary(ctypes.byref(desc), dQ, dK, dQGamma, dKGamma, dPositions, dCos, dSin, dQOut, dKOut,
+                                       stream))
+
+
+def lora_workspace_size(desc: LoraDesc) -> int:
+    return int(load().ms_hip_lora_workspace_size(ctypes.byref(desc)))
+
+
+def lora(desc: LoraDesc, dX, dA, dB, dRanks, dScales, dAdapters, dBase, dY, dWorkspace, workspace_bytes, stream=None):
+    """y[t] = base[t] + scale[a] B_a (A_a x[t]) with a = adapters[t]."""
+    check(load().ms_hip_lora(ctypes.byref(desc), dX, dA, dB, dRanks, dScales, dAdapters, dBase, dY, dWorkspace,
+                             workspace_bytes, stream))

@@ -10,6 +10,7 @@ from .decoder_kernels import (HipGateUpSiluMulKernel, HipSkipNormGateUpSiluMulKe
                               fuse_gate_up_silu, fuse_silu_mul, fuse_skipnorm, register_decoder_kernels)
 from .graph import Engine, KernelRegistry, ModelGraph
 from .hip_kernel import HipMatMulNBitsKernel, register_kernels
+from .serving_kernels import HipLoraMatMulNBitsKernel, register_serving_kernels
 
 
 def build(graph: ModelGraph, registry: KernelRegistry | None = None) -> Engine:
@@ -17,10 +18,12 @@ def build(graph: ModelGraph, registry: KernelRegistry | None = None) -> Engine:
     replace the managed ones) and uploads every MatMulNBits weight triple."""
     registry = registry if registry is not None else KernelRegistry()
     register_decoder_kernels(registry)
+    register_serving_kernels(registry)
     register_kernels(registry)
     for op, cls in (("MatMulNBits", HipMatMulNBitsKernel), ("GateUpSiluMul", HipGateUpSiluMulKernel),
                     ("SkipNormMatMulNBits", HipSkipNormMatMulNBitsKernel),
-                    ("SkipNormGateUpSiluMul", HipSkipNormGateUpSiluMulKernel)):
+                    ("SkipNormGateUpSiluMul", HipSkipNormGateUpSiluMulKernel),
+                    ("LoraMatMulNBits", HipLoraMatMulNBitsKernel)):
         ok, k = registry.try_get(op)
         if ok and isinstance(k, cls):
             k.preload(graph)
