@@ -30,26 +30,40 @@ hipError_t launch_append(const AppendArgs& p, hipStream_t s)
 }
 
 // ---- attention over pages ----------------------------------------------------------------------
+namespace {
+// Requests of up to this many rows go to paged_rows_kernel (16 rows a tile).
+constexpr int kFewRows = 32;
+// Which cases paged_blocks_kernel takes.
+bool blocks_fit(int D, int f16) { return f16 && D > 0; }
+}  // namespace
+
 PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new, int64_t max_total, int H, int kvH,
                                    int D, int f16, int64_t ws_avail, int cus)
 {
     PagedAttnPlan pl;
-    const int grp = H / kvH;
-    const int64_t tiles = tokens * grp / 16 + requests;
-    const int64_t likely = std::max<int64_t>(1, std::min(tiles, (max_new * grp + 15) / 16 * (int64_t)requests)) * kvH;
-    int64_t splits = std::max<int64_t>(1, 4 * (int64_t)cus / likely);
-    splits = std::min<int64_t>({splits, std::max<int64_t>(1, max_total / 128), 64});
+    const int64_t grp = H / kvH;
+    const bool few = max_new * grp <= kFewRows || !blocks_fit(D, f16);   // as far as is known
+    const bool one = requests == 1 && !few;
+    // tiles at the most, and as many as the bounds make likely
+    const int64_t blocks = few ? 0 : tokens * grp / 128 + std::min<int64_t>(requests, tokens * grp / (kFewRows + 1) + 1);
+    const int64_t rows = one   ? 0
+                         : few ? tokens * grp / 16 + requests
+                               : (int64_t)std::min<int64_t>(requests, tokens) * ((kFewRows + 15) / 16);
+    const int64_t likely = few ? std::max<int64_t>(1, std::min(rows, (max_new * grp + 15) / 16 * requests)) : blocks;
+    int64_t splits = std::max<int64_t>(1, (few ? 4 : 2) * (int64_t)cus / (likely * kvH));
+    splits = std::min<int64_t>({splits, std::max<int64_t>(1, max_total / (few ? 128 : 256)), 64});
     const int64_t ws = splits > 1 ? splits * tokens * H * (D + 2) * (int64_t)sizeof(float) : 0;
     if (ws_avail >= 0 && ws > ws_avail) splits = 1;
     pl.splits = (int)splits;
     pl.ws_bytes = splits > 1 ? ws : 0;
-    pl.grid = (int)std::min<int64_t>(tiles * splits * kvH, INT32_MAX);
+    pl.rows_grid = rows * splits * kvH;
+    pl.blocks_grid = blocks * splits * kvH;
     return pl;
 }
 
 namespace {
 template <typename T>
-void launch_rows(const PagedAttnArgs& p, int grid, hipStream_t s)
+void launch_rows(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
 {
     if (p.D <= 64)
         hipLaunchKernelGGL((paged_rows_kernel<T, 64, 2>), dim3(grid), dim3(256), 0, s, p);
@@ -58,15 +72,39 @@ void launch_rows(const PagedAttnArgs& p, int grid, hipStream_t s)
     else
         hipLaunchKernelGGL((paged_rows_kernel<T, 256, 1>), dim3(grid), dim3(256), 0, s, p);
 }
+
+template <typename T>
+void launch_blocks(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
+{
+    if (p.D <= 64)
+        hipLaunchKernelGGL((paged_blocks_kernel<T, 64>), dim3(grid), dim3(256), 0, s, p);
+    else if (p.D <= 96)
+        hipLaunchKernelGGL((paged_blocks_kernel<T, 96>), dim3(grid), dim3(256), 0, s, p);
+    else if (p.D <= 128)
+        hipLaunchKernelGGL((paged_blocks_kernel<T, 128>), dim3(grid), dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((paged_blocks_kernel<T, 256>), dim3(grid), dim3(256), 0, s, p);
+}
 }  // namespace
 
-hipError_t launch_paged_attention(const PagedAttnArgs& p, const PagedAttnPlan& plan, hipStream_t s)
+hipError_t launch_paged_attention(const PagedAttnArgs& args, const PagedAttnPlan& plan, hipStream_t s)
 {
-    if (p.f16)
-        launch_rows<_Float16>(p, plan.grid, s);
-    else
-        launch_rows<float>(p, plan.grid, s);
-    if (hipError_t e = hipGetLastError()) return e;
+    PagedAttnArgs p = args;
+    if (plan.blocks_grid) {
+        p.rows_min = plan.rows_grid ? kFewRows + 1 : 0;
+        p.rows_max = INT32_MAX;
+        launch_blocks<_Float16>(p, (unsigned)plan.blocks_grid, s);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    if (plan.rows_grid) {
+        p.rows_min = 0;
+        p.rows_max = plan.blocks_grid ? kFewRows : INT32_MAX;
+        if (p.f16)
+            launch_rows<_Float16>(p, (unsigned)plan.rows_grid, s);
+        else
+            launch_rows<float>(p, (unsigned)plan.rows_grid, s);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
     if (p.splits > 1) {
         const int64_t rows = (int64_t)p.b.tokens * p.H;
         hipLaunchKernelGGL(paged_merge_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);

@@ -34,8 +34,9 @@ __device__ __forceinline__ int wave_scan(int x)
     return x;
 }
 
-// Tile `idx` of the batch, the requests in order and each one's tiles from its last (the longest
-// range of keys) to its first; false past the end. Every wave by itself, with a uniform idx.
+// Tile `idx` of the launch's requests (those of rows_min to rows_max rows) in order, each one's tiles
+// from its last (the longest range of keys) to its first; false past the end. Every wave by
+// itself, with a uniform idx.
 template <int BM>
 __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, PagedTile& t)
 {
@@ -45,7 +46,8 @@ __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, Page
         const int i = min(base + lane, b.requests - 1);
         const int c0 = max(b.cu[i], 0), c1 = min(b.cu[i + 1], b.tokens);
         const int n = base + lane < b.requests ? max(c1 - c0, 0) : 0;
-        const int tiles = (n * p.grp.div + BM - 1) / BM;
+        const int nr = n * p.grp.div;
+        const int tiles = nr >= p.rows_min && nr <= p.rows_max ? (nr + BM - 1) / BM : 0;
         const int sum = wave_scan(tiles);
         const uint64_t past_idx = __ballot(sum > idx);
         if (past_idx) {
@@ -415,6 +417,270 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs p)
     __syncthreads();
     if (flag)
         for (int lr = wave; lr < t.rows; lr += 4) paged_exact_row<T>(p, t, lr, sp, kr);
+}
+
+// ---- chunks: tiles of 128 rows -----------------------------------------------------------------
+typedef float floatx16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef short short8_t __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+
+constexpr float kGrow = 4.0f;     // the running maximum moves in steps above 2^4
+constexpr int kWeightExp = 11;    // weights times 2^11: at most 2^15 in fp16
+
+// How an operand's fp32 values are held for the 16-bit matrix cores.
+//   fp16 cache: K and V are fp16 already; queries and weights are two fp16 halves (22 bits), two
+//   products an operand pair.
+template <typename T> struct PagedSplit;
+template <> struct PagedSplit<_Float16> {
+    static constexpr int kPlanes = 1, kParts = 2;   // of the cache, of queries and weights
+    static constexpr int kProducts = 2;
+    static constexpr int pair[kProducts][2] = {{0, 0}, {0, 1}};   // (plane, part)
+    __device__ static __forceinline__ void part(const float (&x)[8], short8_t (&out)[2])
+    {
+        half8_t h, l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l[i] = (_Float16)__builtin_fmaf((float)h[i], -1.0f, x[i]);
+        out[0] = __builtin_bit_cast(short8_t, h);
+        out[1] = __builtin_bit_cast(short8_t, l);
+    }
+    __device__ static __forceinline__ floatx16_t mfma(short8_t a, short8_t b, floatx16_t c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    }
+};
+
+// A tile of a block of keys in LDS: rows of CH chunks of 8 channels, K and V each with the chunks
+// of a row moved about so that the reads below meet no bank twice: K's by ds_read_b128 down 32 rows
+// of one chunk, V's by the transposing read, 4 rows of two chunks for 16 lanes.
+template <int CH>
+__device__ __forceinline__ int k_slot(int row, int c)
+{
+    return row * CH + (c ^ (CH == 8 ? (row >> 1) & 7 : row & 15));
+}
+template <int CH>
+__device__ __forceinline__ int v_turn(int row)
+{
+    return CH == 8 ? ((row >> 1) & 1) << 1 | ((row >> 2) & 1) << 2 : (row & 3) << 1 | ((row >> 2) & 1) << 3;
+}
+
+// Four waves of 32 rows each take blocks of BN keys through LDS, the next block's loads in flight
+// meanwhile. S^T = K Q^T (keys M, rows N) leaves lane l with scores of row l % 32 at keys 8 (v / 4)
+// + 4 (l / 32) + v % 4, and O^T += V^T P^T numbers its k-slots the same way, so the weights never
+// leave their lane and a row's statistics are its lane's own; V^T comes from ds_read_b64_tr_b16, which
+// hands 16 lanes four keys of one channel each. The online softmax runs in base 2 and moves
+// its maximum only in steps above 2^4, so that the accumulators are seldom rescaled.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(PagedAttnArgs p)
+{
+    typedef PagedSplit<T> S;
+    constexpr int DPL = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;   // channels of a row in LDS
+    constexpr int BN = DP <= 128 ? 64 : 32;
+    constexpr int CH = DPL / 8, KS = DP / 16, NT = DP / 32, KT = BN / 32;
+    constexpr int UN = BN * CH / 256;   // 8-channel units a thread moves of K, and of V
+    constexpr int TILE = BN * CH;       // 16-byte slots of a plane
+    __shared__ short8_t lds[2][2][TILE];
+
+    const int g = blockIdx.x % p.kvH, rest = blockIdx.x / p.kvH;
+    const int sp = rest % p.splits;
+    PagedTile t;
+    if (!paged_tile<128>(p, rest / p.splits, t)) return;
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const PagedRange kr = paged_range(p, t.past + p.grp.quot(t.row0), t.past + p.grp.quot(t.row0 + t.rows - 1), t.klast,
+                                      sp, BN);
+    const int row = t.row0 + min(32 * wave + l32, t.rows - 1), tok = p.grp.quot(row);
+    const int head = g * p.grp.div + row - tok * p.grp.div, pos = t.past + tok;
+    const int k_lo = max(kr.klo, p.window >= 0 ? max(0, pos - p.window + 1) : 0), k_hi = min(kr.khi, pos);
+    // the wave's rows: positions pos_a .. pos_b, and what all of them or some of them see
+    const int pos_a = t.past + p.grp.quot(t.row0 + min(32 * wave, t.rows - 1));
+    const int pos_b = t.past + p.grp.quot(t.row0 + min(32 * wave + 31, t.rows - 1));
+    const int all_lo = max(kr.klo, p.window >= 0 ? pos_b - p.window + 1 : 0), all_hi = min(kr.khi, pos_a);
+    const int any_lo = max(kr.klo, p.window >= 0 ? pos_a - p.window + 1 : 0), any_hi = min(kr.khi, pos_b);
+
+    short8_t qx[KS][S::kParts];
+    float fac = fabsf(p.scale2);
+    {
+        const float* const q = p.q + (int64_t)(t.t0 + tok) * p.q_stride + (int64_t)head * p.D;
+        const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;
+        float x[KS][8], mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int c = 16 * s + 8 * hf;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const floatx4_t v = c < p.D ? floatx4_t(*reinterpret_cast<const f4u_t*>(q + c + 4 * i)) : floatx4_t{};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[s][4 * i + e] = v[e] * sign;
+                    mx = fmaxf(mx, fabsf(v[e]));
+                }
+            }
+        }
+        mx = fmaxf(mx, xor32_value(mx));
+        const int e = mx > 0.0f && mx < __builtin_inff() ? __builtin_amdgcn_frexp_expf(mx) - 15 : 0;
+        fac = __builtin_amdgcn_ldexpf(fac, e);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[s][i] = __builtin_amdgcn_ldexpf(x[s][i], -e);
+            S::part(x[s], qx[s]);
+        }
+    }
+
+    // a thread's units of a block: unit u is chunk u % CH of row u / CH
+    const int64_t hs = (int64_t)p.kvH * p.D;
+    const T* const kc = static_cast<const T*>(p.kc) + (int64_t)g * p.D;
+    const T* const vc = static_cast<const T*>(p.vc) + (int64_t)g * p.D;
+    const int32_t* const table = p.b.table + (int64_t)t.r * p.b.max_pages;
+    const int chunk = tid % CH, urow = tid / CH;
+    const int ch = 8 * chunk < p.D ? 8 * chunk : 0;
+    int page[UN], slot[UN];
+    short8_t kx[UN], vx[UN];
+    auto look = [&](int k0) {   // keys past the request's last read that one; they are masked
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const int key = min(k0 + urow + 256 / CH * i, t.klast), pg = p.b.page.quot(key);
+            page[i] = table[pg];
+            slot[i] = key - pg * p.b.page.div;
+        }
+    };
+    auto fetch = [&]() {
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const bool there = (unsigned)page[i] < (unsigned)p.b.num_pages;
+            const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : 0) * hs + ch;
+            kx[i] = *reinterpret_cast<const short8_t*>(kc + at);
+            vx[i] = *reinterpret_cast<const short8_t*>(vc + at);
+            if (!there) kx[i] = short8_t{0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff};   // NaN: see below
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const int r = urow + 256 / CH * i;
+            lds[buf][0][k_slot<CH>(r, chunk)] = kx[i];
+            lds[buf][1][r * CH + (chunk ^ v_turn<CH>(r))] = vx[i];
+        }
+    };
+
+    floatx16_t acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n] = floatx16_t{};
+    float m = -__builtin_inff(), l = 0.0f;
+
+    const int first = kr.klo / BN * BN;
+    if (kr.khi >= kr.klo) {
+        look(first);
+        fetch();
+        look(first + BN);
+        store(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int k0 = first; k0 <= kr.khi; k0 += BN, buf ^= 1) {
+        const bool more = k0 + BN <= kr.khi;
+        if (more) {
+            fetch();
+            look(k0 + 2 * BN);
+        }
+        if (k0 <= any_hi && k0 + BN > any_lo) {
+            floatx16_t st[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) st[kt] = floatx16_t{};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                short8_t a[KT];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) a[kt] = lds[buf][0][k_slot<CH>(32 * kt + l32, 2 * s + hf)];
+#pragma unroll
+                for (int j = 0; j < S::kProducts; ++j)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) st[kt] = S::mfma(a[kt], qx[s][S::pair[j][1]], st[kt]);
+            }
+            if (k0 < all_lo || k0 + BN - 1 > all_hi)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) {
+                        const int key = k0 + 32 * kt + 8 * (v >> 2) + 4 * hf + (v & 3);
+                        st[kt][v] = key >= k_lo && key <= k_hi ? st[kt][v] : -__builtin_inff();
+                    }
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) mx = fmaxf(mx, st[kt][v]);
+            mx = fmaxf(mx, xor32_value(mx)) * fac;
+            if (__ballot(mx > m + kGrow)) {
+                const float mn = mx > m + kGrow ? mx : m;
+                const float al = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[n] *= al;
+            }
+            const float off = m == -__builtin_inff() ? 0.0f : (float)kWeightExp - m;
+#pragma unroll
+            for (int s = 0; s < 2 * KT; ++s) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + j], fac, off));
+                    l += w[j];
+                }
+                short8_t px[S::kParts];
+                S::part(w, px);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    // rows 16 s + 8 e + 4 hf + i / 4, 16 channels of 8-byte quarters of two chunks
+                    const int i = lane & 15;
+                    short8_t a;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = 16 * s + 8 * e + 4 * hf + (i >> 2), c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                        const short4_t h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_short4_t*)((short4_t*)&lds[buf][1][r * CH + (c ^ v_turn<CH>(r))] + (i & 1)));
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) a[4 * e + x] = h[x];
+                    }
+#pragma unroll
+                    for (int j = 0; j < S::kProducts; ++j) acc[n] = S::mfma(a, px[S::pair[j][1]], acc[n]);
+                }
+            }
+        }
+        if (more) store(buf ^ 1);
+        __syncthreads();
+    }
+
+    l += xor32_value(l);
+    const float f = l != 0.0f ? 1.0f / l : 0.0f;
+    const int64_t orow = (int64_t)(t.t0 + tok) * p.H + head;
+    float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
+    const bool mine = 32 * wave + l32 < t.rows;
+    bool odd = mine && m == -__builtin_inff() && k_hi >= k_lo;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const floatx4_t v = floatx4_t{acc[n][4 * b], acc[n][4 * b + 1], acc[n][4 * b + 2], acc[n][4 * b + 3]} * f;
+            const int c = 32 * n + 8 * b + 4 * hf;
+            if (mine && c < p.D) {
+                *reinterpret_cast<f4u_t*>(o + c) = v;
+                odd |= !finite4(v);
+            }
+        }
+    if (p.splits > 1 && mine && hf == 0) {
+        paged_part_ml(p, sp, orow)[0] = m;
+        paged_part_ml(p, sp, orow)[1] = l * (1.0f / (1 << kWeightExp));
+    }
+    // rows that met an infinity, a NaN or a page that is not there
+    uint64_t redo = __ballot(odd);
+    for (uint32_t rows = (uint32_t)(redo | redo >> 32); rows; rows &= rows - 1)
+        paged_exact_row<T>(p, t, 32 * wave + __ffs(rows) - 1, sp, kr);
 }
 
 // The splits' records of one output row, joined in the splits' order. A wave per row.

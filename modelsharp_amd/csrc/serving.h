@@ -108,12 +108,14 @@ struct PagedAttnArgs {
     float* out;       // [tokens, H * D]
     float* part;      // splits > 1: [splits][tokens * H] of (max, sum), then [splits][tokens * H][D]
     int H, kvH, D, window, f16, splits;
+    int rows_min, rows_max;   // the launch takes requests of that many rows (new tokens * group)
     int64_t q_stride;
     FastDiv grp;      // query heads per kv head
     float scale2;     // scale * log2(e)
 };
 struct PagedAttnPlan {
-    int splits = 1, grid = 0;
+    int splits = 1;
+    int64_t rows_grid = 0, blocks_grid = 0;   // 0: that kernel is not launched
     int64_t ws_bytes = 0;
 };
 MS_INTERNAL PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new, int64_t max_total, int H,
