@@ -3234,10 +3234,12 @@ PagedBatch paged_batch(const ms_hip_paged_desc& d, const int32_t* cu, const int3
 
 PagedAttnPlan paged_plan(const ms_hip_paged_desc& d, int64_t ws_avail)
 {
-    const int64_t reach = std::min<int64_t>((int64_t)d.max_pages * d.page_size, INT_MAX);
-    return paged_attention_plan(d.tokens, d.requests, d.max_new > 0 ? std::min(d.max_new, d.tokens) : d.tokens,
-                                d.max_total > 0 ? std::min<int64_t>(d.max_total, reach) : reach, d.num_heads,
-                                d.kv_num_heads, d.head_dim, d.cache_type == MS_HIP_DTYPE_F16, ws_avail, device_cus());
+    const int64_t max_new = d.max_new > 0 ? std::min(d.max_new, d.tokens) : d.tokens;
+    int64_t keys = std::min<int64_t>((int64_t)d.max_pages * d.page_size, INT_MAX);   // a tile's at the most
+    if (d.max_total > 0) keys = std::min<int64_t>(keys, d.max_total);
+    if (d.local_window_size >= 0) keys = std::min<int64_t>(keys, (int64_t)d.local_window_size + max_new);
+    return paged_attention_plan(d.tokens, d.requests, max_new, keys, d.num_heads, d.kv_num_heads, d.head_dim,
+                                d.cache_type == MS_HIP_DTYPE_F16, ws_avail, device_cus());
 }
 
 // What append and qk_norm_rotary share; the strides are in place.
@@ -3419,6 +3421,7 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const in
     p.window = d->local_window_size;
     p.f16 = d->cache_type == MS_HIP_DTYPE_F16;
     p.splits = plan.splits;
+    p.split_min = plan.split_min;
     const int64_t qw = (int64_t)p.H * p.D, T = d->tokens, f = sizeof(float);
     p.q_stride = d->q_stride ? d->q_stride : qw;
     p.grp = FastDiv(p.H / p.kvH);

@@ -37,7 +37,7 @@ constexpr int kFewRows = 32;
 bool blocks_fit(int D, int f16) { return f16 && D > 0; }
 }  // namespace
 
-PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new, int64_t max_total, int H, int kvH,
+PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new, int64_t keys, int H, int kvH,
                                    int D, int f16, int64_t ws_avail, int cus)
 {
     PagedAttnPlan pl;
@@ -51,10 +51,11 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new
                                : (int64_t)std::min<int64_t>(requests, tokens) * ((kFewRows + 15) / 16);
     const int64_t likely = few ? std::max<int64_t>(1, std::min(rows, (max_new * grp + 15) / 16 * requests)) : blocks;
     int64_t splits = std::max<int64_t>(1, (few ? 4 : 2) * (int64_t)cus / (likely * kvH));
-    splits = std::min<int64_t>({splits, std::max<int64_t>(1, max_total / (few ? 128 : 256)), 64});
+    splits = std::min<int64_t>({splits, std::max<int64_t>(1, keys / (few ? 128 : 256)), 64});
     const int64_t ws = splits > 1 ? splits * tokens * H * (D + 2) * (int64_t)sizeof(float) : 0;
     if (ws_avail >= 0 && ws > ws_avail) splits = 1;
     pl.splits = (int)splits;
+    pl.split_min = (int)((keys + splits - 1) / splits);
     pl.ws_bytes = splits > 1 ? ws : 0;
     pl.rows_grid = rows * splits * kvH;
     pl.blocks_grid = blocks * splits * kvH;
@@ -66,11 +67,11 @@ template <typename T>
 void launch_rows(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
 {
     if (p.D <= 64)
-        hipLaunchKernelGGL((paged_rows_kernel<T, 64, 2>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_rows_kernel<T, 64>), dim3(grid), dim3(256), 0, s, p);
     else if (p.D <= 128)
-        hipLaunchKernelGGL((paged_rows_kernel<T, 128, 2>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_rows_kernel<T, 128>), dim3(grid), dim3(256), 0, s, p);
     else
-        hipLaunchKernelGGL((paged_rows_kernel<T, 256, 1>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_rows_kernel<T, 256>), dim3(grid), dim3(256), 0, s, p);
 }
 
 template <typename T>

@@ -44,7 +44,7 @@ __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, Page
     const int lane = threadIdx.x & (kWave - 1);
     for (int base = 0; base < b.requests; base += kWave) {
         const int i = min(base + lane, b.requests - 1);
-        const int c0 = max(b.cu[i], 0), c1 = min(b.cu[i + 1], b.tokens);
+        const int c0 = max(b.cu[i], 0), c1 = min(b.cu[i + 1], b.tokens), past = b.past[i];
         const int n = base + lane < b.requests ? max(c1 - c0, 0) : 0;
         const int nr = n * p.grp.div;
         const int tiles = nr >= p.rows_min && nr <= p.rows_max ? (nr + BM - 1) / BM : 0;
@@ -59,7 +59,7 @@ __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, Page
             t.t0 = __builtin_amdgcn_readlane(c0, l);
             t.row0 = (nt - 1 - within) * BM;
             t.rows = min(BM, nl * p.grp.div - t.row0);
-            t.past = min(max(__builtin_amdgcn_readfirstlane(b.past[t.r]), 0), 0x3fffffff);
+            t.past = min(max(__builtin_amdgcn_readlane(past, l), 0), 0x3fffffff);
             t.klast = min((int64_t)t.past + nl, (int64_t)b.max_pages * b.page.div) - 1;
             return true;
         }
@@ -69,7 +69,8 @@ __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, Page
 }
 
 // Positions [lo, hi] that some row of the tile sees; split `sp` takes [klo, khi] of them, in
-// whole steps of `step`. Empty where khi < klo.
+// whole steps of `step`, all splits alike and split_min keys or more (so that short requests take
+// fewer splits, not smaller ones). Empty where khi < klo.
 struct PagedRange {
     int klo, khi;
 };
@@ -77,20 +78,21 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttnArgs& p, int po
 {
     const int lo = p.window >= 0 ? max(0, pos0 - p.window + 1) : 0, hi = min(pos1, klast);
     const int first = lo / step, n = hi >= lo ? hi / step - first + 1 : 0;
-    const int per = (n + p.splits - 1) / p.splits;
+    const int per = max((n + p.splits - 1) / p.splits, p.split_min / step);
+    if ((int64_t)sp * per >= n) return {0, -1};
     const int a = sp * per, e = min(n, a + per);
-    if (a >= e) return {0, -1};
     return {max(lo, (first + a) * step), min(hi, (first + e) * step - 1)};
 }
 
-__device__ __forceinline__ float* paged_part_ml(const PagedAttnArgs& p, int sp, int64_t row)
-{
-    return p.part + ((int64_t)sp * p.b.tokens * p.H + row) * 2;
-}
+// A split's record of an output row: its normed output, and (max, sum).
 __device__ __forceinline__ float* paged_part_o(const PagedAttnArgs& p, int sp, int64_t row)
 {
+    return p.part + ((int64_t)sp * p.b.tokens * p.H + row) * p.D;
+}
+__device__ __forceinline__ float* paged_part_ml(const PagedAttnArgs& p, int sp, int64_t row)
+{
     const int64_t n = (int64_t)p.b.tokens * p.H;
-    return p.part + (int64_t)p.splits * n * 2 + (sp * n + row) * p.D;
+    return p.part + p.splits * n * p.D + (sp * n + row) * 2;
 }
 
 __device__ __forceinline__ bool finite4(floatx4_t v)
@@ -184,8 +186,9 @@ template <> struct PagedElem<float> {
     typedef floatx4_t vec_t;
 };
 
-// Tiles of 16 rows: single tokens and short chunks. Four waves take every fourth step of 16 U
-// keys each with their own running maximum and sums, and meet in LDS at the end.
+// Tiles of 16 rows: single tokens and short chunks. Four waves take every fourth step of 16
+// keys each, the next step's loads in flight meanwhile, with their own running maximum and sums,
+// and meet in LDS at the end.
 //
 // S^T = K Q^T (keys M, rows N) leaves lane l with the scores of row l % 16 at keys 4 (l / 16) + i,
 // which is where the fp32 matrix product O^T += V^T P^T over four keys wants its weights: step i
@@ -195,8 +198,8 @@ template <> struct PagedElem<float> {
 // (22 bits; e by row, so that any fp32 query fits), K in fp32 in fp32.
 // The cache's bytes bound it: per 16 keys of fp16, D = 128, 8 KB against 1152 cycles of the
 // matrix cores, 17 TB/s over the card.
-template <typename T, int DP, int U>
-__global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs p)
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(PagedAttnArgs p)
 {
     constexpr bool F16 = sizeof(T) == 2;
     constexpr int VEC = F16 && DP >= 128 ? 8 : 4;   // channels of one lane's load of V
@@ -221,47 +224,29 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs p)
     const int head = g * p.grp.div + row - tok * p.grp.div;
     const int pos = t.past + tok;
     const PagedRange kr = paged_range(p, t.past + p.grp.quot(t.row0), t.past + p.grp.quot(t.row0 + t.rows - 1), t.klast,
-                                      sp, 16 * U);
+                                      sp, 16);
+    const int64_t orow = (int64_t)(t.t0 + tok) * p.H + head;
+    const bool mine = l16 < t.rows;
+    if (p.splits > 1 && kr.khi < kr.klo) {   // nothing for this split: its record's sum is 0
+        if (mine && threadIdx.x < 16) {
+            paged_part_ml(p, sp, orow)[0] = -__builtin_inff();
+            paged_part_ml(p, sp, orow)[1] = 0.0f;
+        }
+        return;
+    }
     const int k_lo = max(kr.klo, p.window >= 0 ? max(0, pos - p.window + 1) : 0), k_hi = min(kr.khi, pos);
 
-    // the queries, once
+    // the queries' loads, then the first keys', before either is waited for
     const float* const q = p.q + (int64_t)(t.t0 + tok) * p.q_stride + (int64_t)head * p.D;
-    kvec_t qh[KS], ql[F16 ? KS : 1];
-    float fac = p.scale2;
-    {
-        float x[KS][KV];
-        float mx = 0.0f;
+    float x[KS][KV];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int c = KV * grp + PagedElem<T>::kStep * s;
+    for (int s = 0; s < KS; ++s) {
+        const int c = KV * grp + PagedElem<T>::kStep * s;
 #pragma unroll
-            for (int i = 0; i < KV / 4; ++i) {
-                const floatx4_t v = c < p.D ? floatx4_t(*reinterpret_cast<const f4u_t*>(q + c + 4 * i)) : floatx4_t{};
+        for (int i = 0; i < KV / 4; ++i) {
+            const floatx4_t v = c < p.D ? floatx4_t(*reinterpret_cast<const f4u_t*>(q + c + 4 * i)) : floatx4_t{};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[s][4 * i + e] = v[e];
-                    mx = fmaxf(mx, fabsf(v[e]));
-                }
-            }
-        }
-        if constexpr (F16) {
-            mx = fmaxf(mx, xor16_value(mx));
-            mx = fmaxf(mx, xor32_value(mx));
-            const int e = mx > 0.0f && mx < __builtin_inff() ? __builtin_amdgcn_frexp_expf(mx) - 15 : 0;
-            fac = __builtin_amdgcn_ldexpf(p.scale2, e);
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < KV; ++i) {
-                    const float v = __builtin_amdgcn_ldexpf(x[s][i], -e);
-                    qh[s][i] = (_Float16)v;
-                    ql[s][i] = (_Float16)(v - (float)qh[s][i]);
-                }
-        } else {
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < KV; ++i) qh[s][i] = x[s][i];
+            for (int e = 0; e < 4; ++e) x[s][4 * i + e] = v[e];
         }
     }
 
@@ -269,6 +254,76 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs p)
     const T* const kc = static_cast<const T*>(p.kc) + (int64_t)g * p.D;
     const T* const vc = static_cast<const T*>(p.vc) + (int64_t)g * p.D;
     const bool whole = (p.b.page.div & 15) == 0;   // 16 aligned keys lie in one page
+    struct Keys {
+        kvec_t k[KS];
+        vvec_t v[4][NC];
+        bool there[4];
+    };
+    // keys past the request's last read that one, pages that are not there read the cache's
+    // first row, and both are masked
+    auto load = [&](int key, Keys& x) {
+        int krow, vrow[4];
+        if (whole) {
+            const int st = min(key, t.klast & ~15);
+            const int base = paged_row(p.b, t.r, st);
+            krow = base < 0 ? 0 : base + min(key + l16, t.klast) - st;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                vrow[i] = base < 0 ? 0 : base + min(key + 4 * grp + i, t.klast) - st;
+                x.there[i] = base >= 0;
+            }
+        } else {
+            krow = max(paged_row(p.b, t.r, min(key + l16, t.klast)), 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                vrow[i] = paged_row(p.b, t.r, min(key + 4 * grp + i, t.klast));
+                x.there[i] = vrow[i] >= 0;
+                vrow[i] = max(vrow[i], 0);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int c = KV * grp + PagedElem<T>::kStep * s;
+            x.k[s] = *reinterpret_cast<const kvec_t*>(kc + krow * hs + (c < p.D ? c : 0));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int ch = VEC * (l16 + 16 * c);
+                x.v[i][c] = *reinterpret_cast<const vvec_t*>(vc + vrow[i] * hs + (ch < p.D ? ch : 0));
+            }
+    };
+    int k0 = (kr.klo & ~15) + 16 * wave;
+    Keys ka, kb;
+    if (k0 <= kr.khi) load(k0, ka);
+
+    kvec_t qh[KS], ql[F16 ? KS : 1];
+    float fac = p.scale2;
+    if constexpr (F16) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < KV; ++i) mx = fmaxf(mx, fabsf(x[s][i]));
+        mx = fmaxf(mx, xor16_value(mx));
+        mx = fmaxf(mx, xor32_value(mx));
+        const int e = mx > 0.0f && mx < __builtin_inff() ? __builtin_amdgcn_frexp_expf(mx) - 15 : 0;
+        fac = __builtin_amdgcn_ldexpf(p.scale2, e);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < KV; ++i) {
+                const float v = __builtin_amdgcn_ldexpf(x[s][i], -e);
+                qh[s][i] = (_Float16)v;
+                ql[s][i] = (_Float16)(v - (float)qh[s][i]);
+            }
+    } else {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < KV; ++i) qh[s][i] = x[s][i];
+    }
 
     floatx4_t acc[NC][VEC];
 #pragma unroll
@@ -277,97 +332,64 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs p)
         for (int j = 0; j < VEC; ++j) acc[c][j] = floatx4_t{};
     float m = -__builtin_inff(), l = 0.0f;
 
-    for (int k0 = kr.klo / (16 * U) * (16 * U) + 16 * U * wave; k0 <= kr.khi; k0 += 64 * U) {
-        // every load first; keys past the request's last read that one, pages that are not
-        // there read the cache's first row, and both are masked
-        kvec_t kx[U][KS];
-        vvec_t vx[U][4][NC];
-        bool there[U][4];
+    auto add = [&](int key, const Keys& x) {
+        floatx4_t s4{};
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int key = k0 + 16 * u;
-            int krow, vrow[4];
-            if (whole) {
-                const int st = min(key, t.klast & ~15);
-                const int base = paged_row(p.b, t.r, st);
-                krow = base < 0 ? 0 : base + min(key + l16, t.klast) - st;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    vrow[i] = base < 0 ? 0 : base + min(key + 4 * grp + i, t.klast) - st;
-                    there[u][i] = base >= 0;
-                }
+        for (int s = 0; s < KS; ++s) {
+            if constexpr (F16) {
+                s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[s], qh[s], s4, 0, 0, 0);
+                s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[s], ql[s], s4, 0, 0, 0);
             } else {
-                krow = max(paged_row(p.b, t.r, min(key + l16, t.klast)), 0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    vrow[i] = paged_row(p.b, t.r, min(key + 4 * grp + i, t.klast));
-                    there[u][i] = vrow[i] >= 0;
-                    vrow[i] = max(vrow[i], 0);
-                }
+                for (int e = 0; e < 4; ++e) s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[s][e], qh[s][e], s4, 0, 0, 0);
             }
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int c = KV * grp + PagedElem<T>::kStep * s;
-                kx[u][s] = *reinterpret_cast<const kvec_t*>(kc + krow * hs + (c < p.D ? c : 0));
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const int ch = VEC * (l16 + 16 * c);
-                    vx[u][i][c] = *reinterpret_cast<const vvec_t*>(vc + vrow[i] * hs + (ch < p.D ? ch : 0));
-                }
         }
-        float sc[U][4];
-        float mt = -__builtin_inff();
+        float w[4], mt = -__builtin_inff();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            floatx4_t s4{};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                if constexpr (F16) {
-                    s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx[u][s], qh[s], s4, 0, 0, 0);
-                    s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx[u][s], ql[s], s4, 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[u][s][e], qh[s][e], s4, 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = k0 + 16 * u + 4 * grp + i;
-                sc[u][i] = there[u][i] && key >= k_lo && key <= k_hi ? s4[i] * fac : -__builtin_inff();
-                mt = fmaxf(mt, sc[u][i]);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const int k = key + 4 * grp + i;
+            w[i] = x.there[i] && k >= k_lo && k <= k_hi ? s4[i] * fac : -__builtin_inff();
+            mt = fmaxf(mt, w[i]);
         }
         mt = fmaxf(mt, xor16_value(mt));
         mt = fmaxf(mt, xor32_value(mt));
-        const float mn = fmaxf(m, mt), ms = mn == -__builtin_inff() ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m - ms);
-        m = mn;
-        l *= al;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sc[u][i] = __builtin_amdgcn_exp2f(sc[u][i] - ms);
-                l += sc[u][i];
-            }
-        if (__ballot(al != 1.0f))
+        if (__ballot(mt > m)) {
+            const float mn = fmaxf(m, mt);
+            const float al = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.0f : mn));
+            m = mn;
+            l *= al;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) acc[c][j] *= al;
+        }
+        const float ms = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int i = 0; i < 4; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(w[i] - ms);
+            l += w[i];
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)vx[u][i][c][j], sc[u][i], acc[c][j], 0, 0, 0);
+                for (int j = 0; j < VEC; ++j)
+                    acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[i][c][j], w[i], acc[c][j], 0, 0, 0);
+    };
+    constexpr bool kAhead = F16 || DP <= 128;   // two sets of 16 keys fit the registers
+    while (kAhead && k0 <= kr.khi) {
+        if (k0 + 64 <= kr.khi) load(k0 + 64, kb);
+        add(k0, ka);
+        k0 += 64;
+        if (k0 > kr.khi) break;
+        if (k0 + 64 <= kr.khi) load(k0 + 64, ka);
+        add(k0, kb);
+        k0 += 64;
+    }
+    for (; k0 <= kr.khi; k0 += 64) {
+        add(k0, ka);
+        if (k0 + 64 <= kr.khi) load(k0 + 64, ka);
     }
 
     // the waves' sums meet: statistics, then four quads of channels at a time
@@ -385,9 +407,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(PagedAttnArgs p)
 #pragma unroll
     for (int w = 0; w < 4; ++w) ll += stat[1][w][l16] * __builtin_amdgcn_exp2f(stat[0][w][l16] - ms);
     const float f = ll != 0.0f ? __builtin_amdgcn_exp2f(m - ms) / ll : 0.0f;
-    const int64_t orow = (int64_t)(t.t0 + tok) * p.H + head;
     float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
-    const bool mine = l16 < t.rows;
     bool odd = mine && mm == -__builtin_inff() && k_hi >= k_lo;
     // quad n of a lane's channels: chunk c, row i of the product, channels 4 b .. 4 b + 3 of VEC
     constexpr int QUADS = DP / 16;
@@ -494,6 +514,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
                                       sp, BN);
     const int row = t.row0 + min(32 * wave + l32, t.rows - 1), tok = p.grp.quot(row);
     const int head = g * p.grp.div + row - tok * p.grp.div, pos = t.past + tok;
+    const int64_t orow = (int64_t)(t.t0 + tok) * p.H + head;
+    const bool mine = 32 * wave + l32 < t.rows;
+    if (p.splits > 1 && kr.khi < kr.klo) {   // nothing for this split: its record's sum is 0
+        if (mine && hf == 0) {
+            paged_part_ml(p, sp, orow)[0] = -__builtin_inff();
+            paged_part_ml(p, sp, orow)[1] = 0.0f;
+        }
+        return;
+    }
     const int k_lo = max(kr.klo, p.window >= 0 ? max(0, pos - p.window + 1) : 0), k_hi = min(kr.khi, pos);
     // the wave's rows: positions pos_a .. pos_b, and what all of them or some of them see
     const int pos_a = t.past + p.grp.quot(t.row0 + min(32 * wave, t.rows - 1));
@@ -658,9 +687,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
 
     l += xor32_value(l);
     const float f = l != 0.0f ? 1.0f / l : 0.0f;
-    const int64_t orow = (int64_t)(t.t0 + tok) * p.H + head;
     float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
-    const bool mine = 32 * wave + l32 < t.rows;
     bool odd = mine && m == -__builtin_inff() && k_hi >= k_lo;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -683,39 +710,45 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
         paged_exact_row<T>(p, t, 32 * wave + __ffs(rows) - 1, sp, kr);
 }
 
-// The splits' records of one output row, joined in the splits' order. A wave per row.
+// The splits' records of one output row, joined in the splits' order. A wave per row: lane s holds
+// split s's weight, and the outputs' loads do not wait for them (what a split of weight zero left
+// is not used).
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs p)
 {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= (int64_t)p.b.tokens * p.H) return;
     const int tok = (int)(row / p.H);
-    if (tok < p.b.cu[0] || tok >= p.b.cu[p.b.requests]) return;   // rows of no request stay as they were
-    float m = -__builtin_inff();
-    bool low = false;
-    for (int s = 0; s < p.splits; ++s) {
-        const float* const ml = paged_part_ml(p, s, row);
-        if (ml[1] != 0.0f) {
-            m = fmaxf(m, ml[0]);
-            low = true;
+    const int c0 = p.b.cu[0], c1 = p.b.cu[p.b.requests];
+    const float* const ml = paged_part_ml(p, min(lane, p.splits - 1), row);
+    float m = ml[0], l = lane < p.splits ? ml[1] : 0.0f;
+    constexpr int kAtOnce = 8;
+    const float* const part = paged_part_o(p, 0, row);
+    const int64_t step = (int64_t)p.b.tokens * p.H * p.D;
+    if (l == 0.0f) m = -__builtin_inff();
+    float mx = row16_max_all(m);
+    mx = fmaxf(mx, xor16_value(mx));
+    mx = fmaxf(mx, xor32_value(mx));
+    // every score -infinity wherever there was a key: the definition's NaN
+    const bool low = mx == -__builtin_inff() && __ballot(l != 0.0f);
+    float w = m == -__builtin_inff() ? 0.0f : l * __builtin_amdgcn_exp2f(m - mx);
+    const float sum = group_sum_all<64>(w);
+    w = sum != 0.0f ? w / sum : 0.0f;   // NaN stays
+    for (int cw = 0; cw < p.D; cw += 4 * kWave) {   // uniform: the weights are read across lanes
+        const int c = min(cw + 4 * lane, p.D - 4);
+        floatx4_t o{};
+        for (int s0 = 0; s0 < p.splits; s0 += kAtOnce) {
+            floatx4_t v[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                v[i] = *reinterpret_cast<const floatx4_t*>(part + min(s0 + i, p.splits - 1) * step + c);
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                if (const float ws = s0 + i < p.splits ? lane_value(w, s0 + i) : 0.0f; ws != 0.0f) o += ws * v[i];
         }
-    }
-    const bool all_low = low && m == -__builtin_inff();
-    const float ms = m == -__builtin_inff() ? 0.0f : m;
-    float l = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float* const ml = paged_part_ml(p, s, row);
-        if (ml[1] != 0.0f) l += ml[1] * __builtin_amdgcn_exp2f(ml[0] - ms);
-    }
-    for (int c = lane; c < p.D; c += 64) {
-        float o = all_low ? __builtin_nanf("") : 0.0f;
-        if (!all_low)
-            for (int s = 0; s < p.splits; ++s) {
-                const float* const ml = paged_part_ml(p, s, row);
-                if (ml[1] != 0.0f && !(ml[0] == -__builtin_inff()))
-                    o += (ml[1] * __builtin_amdgcn_exp2f(ml[0] - ms) / l) * paged_part_o(p, s, row)[c];
-            }
-        p.out[row * p.D + c] = o;
+        if (low) o = floatx4_t{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        if (cw + 4 * lane < p.D && tok >= c0 && tok < c1)   // rows of no request stay
+            *reinterpret_cast<f4u_t*>(p.out + row * p.D + c) = o;
     }
 }
 

@@ -106,19 +106,20 @@ struct PagedAttnArgs {
     const void* kc;
     const void* vc;
     float* out;       // [tokens, H * D]
-    float* part;      // splits > 1: [splits][tokens * H] of (max, sum), then [splits][tokens * H][D]
+    float* part;      // splits > 1: [splits][tokens * H][D], then [splits][tokens * H] of (max, sum)
     int H, kvH, D, window, f16, splits;
+    int split_min;    // keys of a split at the least
     int rows_min, rows_max;   // the launch takes requests of that many rows (new tokens * group)
     int64_t q_stride;
     FastDiv grp;      // query heads per kv head
     float scale2;     // scale * log2(e)
 };
 struct PagedAttnPlan {
-    int splits = 1;
+    int splits = 1, split_min = 0;
     int64_t rows_grid = 0, blocks_grid = 0;   // 0: that kernel is not launched
     int64_t ws_bytes = 0;
 };
-MS_INTERNAL PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new, int64_t max_total, int H,
+MS_INTERNAL PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new, int64_t keys, int H,
                                                int kvH, int D, int f16, int64_t ws_avail, int cus);
 MS_INTERNAL hipError_t launch_paged_attention(const PagedAttnArgs& p, const PagedAttnPlan& plan, hipStream_t s);
 
