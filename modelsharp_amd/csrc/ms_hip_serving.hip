@@ -50,7 +50,7 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new
                          : few ? tokens * grp / 16 + requests
                                : (int64_t)std::min<int64_t>(requests, tokens) * ((kFewRows + 15) / 16);
     const int64_t likely = few ? std::max<int64_t>(1, std::min(rows, (max_new * grp + 15) / 16 * requests)) : blocks;
-    int64_t splits = std::max<int64_t>(1, (few ? 4 : 2) * (int64_t)cus / (likely * kvH));
+    int64_t splits = std::max<int64_t>(1, 2 * (int64_t)cus / (likely * kvH));
     splits = std::min<int64_t>({splits, std::max<int64_t>(1, keys / (few ? 128 : 256)), 64});
     const int64_t ws = splits > 1 ? splits * tokens * H * (D + 2) * (int64_t)sizeof(float) : 0;
     if (ws_avail >= 0 && ws > ws_avail) splits = 1;
@@ -63,15 +63,15 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new
 }
 
 namespace {
-template <typename T>
+template <typename T, bool WHOLE>
 void launch_rows(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
 {
     if (p.D <= 64)
-        hipLaunchKernelGGL((paged_rows_kernel<T, 64>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_rows_kernel<T, 64, WHOLE>), dim3(grid), dim3(256), 0, s, p);
     else if (p.D <= 128)
-        hipLaunchKernelGGL((paged_rows_kernel<T, 128>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_rows_kernel<T, 128, WHOLE>), dim3(grid), dim3(256), 0, s, p);
     else
-        hipLaunchKernelGGL((paged_rows_kernel<T, 256>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_rows_kernel<T, 256, WHOLE>), dim3(grid), dim3(256), 0, s, p);
 }
 
 template <typename T>
@@ -100,10 +100,10 @@ hipError_t launch_paged_attention(const PagedAttnArgs& args, const PagedAttnPlan
     if (plan.rows_grid) {
         p.rows_min = 0;
         p.rows_max = plan.blocks_grid ? kFewRows : INT32_MAX;
-        if (p.f16)
-            launch_rows<_Float16>(p, (unsigned)plan.rows_grid, s);
-        else
-            launch_rows<float>(p, (unsigned)plan.rows_grid, s);
+        const bool whole = p.b.page.div % 16 == 0;
+        const auto launch = p.f16 ? (whole ? launch_rows<_Float16, true> : launch_rows<_Float16, false>)
+                                  : (whole ? launch_rows<float, true> : launch_rows<float, false>);
+        launch(p, (unsigned)plan.rows_grid, s);
         if (hipError_t e = hipGetLastError()) return e;
     }
     if (p.splits > 1) {

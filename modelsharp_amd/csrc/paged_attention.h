@@ -186,19 +186,26 @@ template <> struct PagedElem<float> {
     typedef floatx4_t vec_t;
 };
 
+constexpr float kGrow = 4.0f;     // the running maximum moves in steps above 2^4
+constexpr int kWeightExp = 11;    // weights times 2^11: at most 2^15 in fp16
+
+// Steps of 16 keys in a wave's registers: the one in use and those on their way.
+constexpr int paged_ring(int DP, bool f16) { return f16 ? (DP <= 128 ? 3 : 2) : (DP <= 64 ? 3 : DP <= 128 ? 2 : 1); }
+
 // Tiles of 16 rows: single tokens and short chunks. Four waves take every fourth step of 16
-// keys each, the next step's loads in flight meanwhile, with their own running maximum and sums,
-// and meet in LDS at the end.
+// keys each, the next steps' loads in flight meanwhile, with their own running maximum (moved in
+// steps above 2^4, so that the sums are seldom rescaled) and sums, and meet in LDS at the end.
 //
 // S^T = K Q^T (keys M, rows N) leaves lane l with the scores of row l % 16 at keys 4 (l / 16) + i,
-// which is where the fp32 matrix product O^T += V^T P^T over four keys wants its weights: step i
-// takes keys 4 g + i of the four lane groups g, and lane l gives V[key 4 (l / 16) + i] from its
-// own 16-byte load. So neither the weights nor V pass through LDS, V's rows come in as whole
-// lines, and the weights stay fp32. K in fp16 meets the queries as two halves, q = 2^e (qh + ql)
-// (22 bits; e by row, so that any fp32 query fits), K in fp32 in fp32.
-// The cache's bytes bound it: per 16 keys of fp16, D = 128, 8 KB against 1152 cycles of the
-// matrix cores, 17 TB/s over the card.
-template <typename T, int DP>
+// i = 0 .. 3, and the same lane loads V's rows of those four keys, 8 (fp32: 4) channels of each:
+// O^T += V^T P^T over 16 keys then has both operands where they are, the weights as they come and
+// V's by packing the four keys of a channel (fp32: one key of each lane group per product). Neither
+// passes through LDS, and V's rows come in as whole lines. K in fp16 meets the queries as two
+// halves, q = 2^e (qh + ql) (22 bits; e by row, so that any fp32 query fits), V in fp16 the weights
+// as two halves; an fp32 cache is multiplied in fp32.
+// WHOLE: pages of a multiple of 16 rows, so that a step lies in one page: one lookup a step, and a
+// page that is not there is a step left out.
+template <typename T, int DP, bool WHOLE>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(PagedAttnArgs p)
 {
     constexpr bool F16 = sizeof(T) == 2;
@@ -208,6 +215,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
     constexpr int KV = F16 ? 8 : 4;                 // channels of one lane's load of K
     typedef typename PagedElem<T>::vec_t kvec_t;
     typedef T vvec_t __attribute__((ext_vector_type(VEC)));
+    constexpr int kRing = paged_ring(DP, F16);
     __shared__ float stat[2][4][16];
     __shared__ floatx4_t merge[4][4][kWave];
     __shared__ int flag;
@@ -253,50 +261,74 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
     const int64_t hs = (int64_t)p.kvH * p.D;   // a cache row
     const T* const kc = static_cast<const T*>(p.kc) + (int64_t)g * p.D;
     const T* const vc = static_cast<const T*>(p.vc) + (int64_t)g * p.D;
-    const bool whole = (p.b.page.div & 15) == 0;   // 16 aligned keys lie in one page
+    // where 16 keys lie: looked up a step before their loads. Keys past the request's last stand for
+    // that one, and pages that are not there for the cache's first row; both are masked.
+    struct Rows {
+        int first;     // WHOLE: the row of the step's first key, -1: not there
+        int k, v[4];   // else: this lane's rows of K and V, -1: not there
+    };
+    auto look = [&](int key, Rows& r) {
+        if constexpr (WHOLE) {
+            r.first = paged_row(p.b, t.r, min(key, t.klast & ~15));
+        } else {
+            r.k = paged_row(p.b, t.r, min(key + l16, t.klast));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.v[i] = paged_row(p.b, t.r, min(key + 4 * grp + i, t.klast));
+        }
+    };
     struct Keys {
         kvec_t k[KS];
         vvec_t v[4][NC];
         bool there[4];
     };
-    // keys past the request's last read that one, pages that are not there read the cache's
-    // first row, and both are masked
-    auto load = [&](int key, Keys& x) {
-        int krow, vrow[4];
-        if (whole) {
-            const int st = min(key, t.klast & ~15);
-            const int base = paged_row(p.b, t.r, st);
-            krow = base < 0 ? 0 : base + min(key + l16, t.klast) - st;
+    auto load = [&](int key, const Rows& r, Keys& x) {
+        if constexpr (WHOLE) {
+            // one base for the step, 32-bit offsets within its 16 rows (65535 heads of 256: 1 GB)
+            const char* const kb = reinterpret_cast<const char*>(kc + (int64_t)max(r.first, 0) * hs);
+            const char* const vb = reinterpret_cast<const char*>(vc + (int64_t)max(r.first, 0) * hs);
+            const uint32_t last = min(15, t.klast - key), w = (uint32_t)hs * sizeof(T);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int c = KV * grp + PagedElem<T>::kStep * s;
+                x.k[s] = *reinterpret_cast<const kvec_t*>(kb + (min((uint32_t)l16, last) * w + (c < p.D ? c : 0) * (uint32_t)sizeof(T)));
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                vrow[i] = base < 0 ? 0 : base + min(key + 4 * grp + i, t.klast) - st;
-                x.there[i] = base >= 0;
+                x.there[i] = r.first >= 0;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int ch = VEC * (l16 + 16 * c);
+                    x.v[i][c] = *reinterpret_cast<const vvec_t*>(
+                        vb + (min((uint32_t)(4 * grp + i), last) * w + (ch < p.D ? ch : 0) * (uint32_t)sizeof(T)));
+                }
             }
         } else {
-            krow = max(paged_row(p.b, t.r, min(key + l16, t.klast)), 0);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int c = KV * grp + PagedElem<T>::kStep * s;
+                x.k[s] = *reinterpret_cast<const kvec_t*>(kc + max(r.k, 0) * hs + (c < p.D ? c : 0));
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                vrow[i] = paged_row(p.b, t.r, min(key + 4 * grp + i, t.klast));
-                x.there[i] = vrow[i] >= 0;
-                vrow[i] = max(vrow[i], 0);
+                x.there[i] = r.v[i] >= 0;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int ch = VEC * (l16 + 16 * c);
+                    x.v[i][c] = *reinterpret_cast<const vvec_t*>(vc + max(r.v[i], 0) * hs + (ch < p.D ? ch : 0));
+                }
             }
         }
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int c = KV * grp + PagedElem<T>::kStep * s;
-            x.k[s] = *reinterpret_cast<const kvec_t*>(kc + krow * hs + (c < p.D ? c : 0));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int ch = VEC * (l16 + 16 * c);
-                x.v[i][c] = *reinterpret_cast<const vvec_t*>(vc + vrow[i] * hs + (ch < p.D ? ch : 0));
-            }
     };
     int k0 = (kr.klo & ~15) + 16 * wave;
-    Keys ka, kb;
-    if (k0 <= kr.khi) load(k0, ka);
+    Keys ring[kRing];
+    Rows next;
+    if (k0 <= kr.khi) look(k0, next);
+#pragma unroll
+    for (int n = 0; n + 1 < kRing; ++n)
+        if (k0 + 64 * n <= kr.khi) {
+            load(k0 + 64 * n, next, ring[n]);
+            look(k0 + 64 * (n + 1), next);
+        }
 
     kvec_t qh[KS], ql[F16 ? KS : 1];
     float fac = p.scale2;
@@ -332,7 +364,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
         for (int j = 0; j < VEC; ++j) acc[c][j] = floatx4_t{};
     float m = -__builtin_inff(), l = 0.0f;
 
+    // the keys that every row of the tile sees need no mask
+    const int all_lo = max(kr.klo, p.window >= 0 ? t.past + p.grp.quot(t.row0 + t.rows - 1) - p.window + 1 : 0);
+    const int all_hi = min(kr.khi, t.past + p.grp.quot(t.row0));
     auto add = [&](int key, const Keys& x) {
+        if (WHOLE && !x.there[0]) return;
         floatx4_t s4{};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -344,18 +380,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
                 for (int e = 0; e < 4; ++e) s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[s][e], qh[s][e], s4, 0, 0, 0);
             }
         }
-        float w[4], mt = -__builtin_inff();
+        float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = key + 4 * grp + i;
-            w[i] = x.there[i] && k >= k_lo && k <= k_hi ? s4[i] * fac : -__builtin_inff();
-            mt = fmaxf(mt, w[i]);
-        }
+        for (int i = 0; i < 4; ++i) w[i] = s4[i] * fac;
+        if (!WHOLE || key < all_lo || key + 15 > all_hi)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = key + 4 * grp + i;
+                w[i] = x.there[i] && k >= k_lo && k <= k_hi ? w[i] : -__builtin_inff();
+            }
+        float mt = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
         mt = fmaxf(mt, xor16_value(mt));
         mt = fmaxf(mt, xor32_value(mt));
-        if (__ballot(mt > m)) {
-            const float mn = fmaxf(m, mt);
-            const float al = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.0f : mn));
+        if (__ballot(mt > m + kGrow)) {
+            const float mn = mt > m + kGrow ? mt : m;
+            const float al = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= al;
 #pragma unroll
@@ -363,38 +402,60 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) acc[c][j] *= al;
         }
-        const float ms = m == -__builtin_inff() ? 0.0f : m;
+        const float off = (F16 ? (float)kWeightExp : 0.0f) - (m == -__builtin_inff() ? 0.0f : m);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(w[i] - ms);
+            w[i] = __builtin_amdgcn_exp2f(w[i] + off);
             l += w[i];
         }
+        if constexpr (F16) {
+            half4_t ph, pl;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) ph[i] = (_Float16)w[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pl[i] = (_Float16)__builtin_fmaf((float)ph[i], -1.0f, w[i]);
+            typedef uint32_t dwords_t __attribute__((ext_vector_type(VEC / 2)));
+            typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[i][c][j], w[i], acc[c][j], 0, 0, 0);
+                for (int j = 0; j < VEC; ++j) {
+                    uint32_t d[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) d[i] = __builtin_bit_cast(dwords_t, x.v[i][c])[j / 2];
+                    const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;   // the high or the low halves of two dwords
+                    const half4_t a = __builtin_bit_cast(half4_t, u32x2_t{__builtin_amdgcn_perm(d[1], d[0], sel),
+                                                                          __builtin_amdgcn_perm(d[3], d[2], sel)});
+                    acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, ph, acc[c][j], 0, 0, 0);
+                    acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, pl, acc[c][j], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[i][c][j], w[i], acc[c][j], 0, 0, 0);
+        }
     };
-    constexpr bool kAhead = F16 || DP <= 128;   // two sets of 16 keys fit the registers
-    while (kAhead && k0 <= kr.khi) {
-        if (k0 + 64 <= kr.khi) load(k0 + 64, kb);
-        add(k0, ka);
-        k0 += 64;
-        if (k0 > kr.khi) break;
-        if (k0 + 64 <= kr.khi) load(k0 + 64, ka);
-        add(k0, kb);
-        k0 += 64;
-    }
-    for (; k0 <= kr.khi; k0 += 64) {
-        add(k0, ka);
-        if (k0 + 64 <= kr.khi) load(k0 + 64, ka);
+    while (k0 <= kr.khi) {
+#pragma unroll
+        for (int n = 0; n < kRing; ++n) {
+            if (k0 > kr.khi) break;
+            if (k0 + 64 * (kRing - 1) <= kr.khi) {
+                load(k0 + 64 * (kRing - 1), next, ring[(n + kRing - 1) % kRing]);
+                look(k0 + 64 * kRing, next);
+            }
+            add(k0, ring[n]);
+            k0 += 64;
+        }
     }
 
     // the waves' sums meet: statistics, then four quads of channels at a time
     l += xor16_value(l);
     l += xor32_value(l);
+    if (F16) l *= 1.0f / (1 << kWeightExp);
     if (lane < 16) {
         stat[0][wave][lane] = m;
         stat[1][wave][lane] = l;
@@ -406,7 +467,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
     const float ms = mm == -__builtin_inff() ? 0.0f : mm;
 #pragma unroll
     for (int w = 0; w < 4; ++w) ll += stat[1][w][l16] * __builtin_amdgcn_exp2f(stat[0][w][l16] - ms);
-    const float f = ll != 0.0f ? __builtin_amdgcn_exp2f(m - ms) / ll : 0.0f;
+    // (a wave without a key that any row sees has m = -infinity: a factor of 0)
+    const float f = ll != 0.0f ? __builtin_amdgcn_exp2f(m - ms) / (F16 ? ll * (1 << kWeightExp) : ll) : 0.0f;
     float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
     bool odd = mine && mm == -__builtin_inff() && k_hi >= k_lo;
     // quad n of a lane's channels: chunk c, row i of the product, channels 4 b .. 4 b + 3 of VEC
@@ -445,9 +507,6 @@ typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef short short8_t __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) short4_t lds_short4_t;
-
-constexpr float kGrow = 4.0f;     // the running maximum moves in steps above 2^4
-constexpr int kWeightExp = 11;    // weights times 2^11: at most 2^15 in fp16
 
 // How an operand's fp32 values are held for the 16-bit matrix cores.
 //   fp16 cache: K and V are fp16 already; queries and weights are two fp16 halves (22 bits), two
