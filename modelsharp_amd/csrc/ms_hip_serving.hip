@@ -33,8 +33,8 @@ hipError_t launch_append(const AppendArgs& p, hipStream_t s)
 namespace {
 // Requests of up to this many rows go to paged_rows_kernel (16 rows a tile).
 constexpr int kFewRows = 32;
-// Which cases paged_blocks_kernel takes.
-bool blocks_fit(int D, int f16) { return f16 && D > 0; }
+// Which cases paged_blocks_kernel takes: an fp32 block's three parts fit LDS up to 128 channels.
+bool blocks_fit(int D, int f16) { return f16 || D <= 128; }
 }  // namespace
 
 PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new, int64_t keys, int H, int kvH,
@@ -83,7 +83,7 @@ void launch_blocks(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
         hipLaunchKernelGGL((paged_blocks_kernel<T, 96>), dim3(grid), dim3(256), 0, s, p);
     else if (p.D <= 128)
         hipLaunchKernelGGL((paged_blocks_kernel<T, 128>), dim3(grid), dim3(256), 0, s, p);
-    else
+    else if constexpr (sizeof(T) == 2)
         hipLaunchKernelGGL((paged_blocks_kernel<T, 256>), dim3(grid), dim3(256), 0, s, p);
 }
 }  // namespace
@@ -94,7 +94,10 @@ hipError_t launch_paged_attention(const PagedAttnArgs& args, const PagedAttnPlan
     if (plan.blocks_grid) {
         p.rows_min = plan.rows_grid ? kFewRows + 1 : 0;
         p.rows_max = INT32_MAX;
-        launch_blocks<_Float16>(p, (unsigned)plan.blocks_grid, s);
+        if (p.f16)
+            launch_blocks<_Float16>(p, (unsigned)plan.blocks_grid, s);
+        else
+            launch_blocks<float>(p, (unsigned)plan.blocks_grid, s);
         if (hipError_t e = hipGetLastError()) return e;
     }
     if (plan.rows_grid) {

@@ -532,6 +532,40 @@ template <> struct PagedSplit<_Float16> {
     }
 };
 
+//   fp32 cache: everything is three bf16 parts, x = x0 + x1 + x2 exactly (cut, not rounded: 8 bits
+//   each, and bf16 has fp32's range, so that any finite value fits), and the products of a pair
+//   whose terms are 2^-16 or more of the whole: six of nine, what is left out is below 2^-22.
+template <> struct PagedSplit<float> {
+    static constexpr int kPlanes = 3, kParts = 3;
+    static constexpr int kProducts = 6;
+    static constexpr int pair[kProducts][2] = {{2, 0}, {1, 1}, {0, 2}, {1, 0}, {0, 1}, {0, 0}};   // small terms first
+    __device__ static __forceinline__ void part(const float (&x)[8], short8_t (&out)[3])
+    {
+        typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+        u32x4_t o[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t b[2][3];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float v = x[2 * i + e];
+                b[e][0] = __float_as_uint(v);
+                const float r1 = v - __uint_as_float(b[e][0] & 0xffff0000u);
+                b[e][1] = __float_as_uint(r1);
+                b[e][2] = __float_as_uint(r1 - __uint_as_float(b[e][1] & 0xffff0000u));
+            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k) o[k][i] = __builtin_amdgcn_perm(b[1][k], b[0][k], 0x07060302u);   // the high halves
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) out[k] = __builtin_bit_cast(short8_t, o[k]);
+    }
+    __device__ static __forceinline__ floatx16_t mfma(short8_t a, short8_t b, floatx16_t c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0, 0);
+    }
+};
+
 // A tile of a block of keys in LDS: rows of CH chunks of 8 channels, K and V each with the chunks
 // of a row moved about so that the reads below meet no bank twice: K's by ds_read_b128 down 32 rows
 // of one chunk, V's by the transposing read, 4 rows of two chunks for 16 lanes.
@@ -557,11 +591,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
 {
     typedef PagedSplit<T> S;
     constexpr int DPL = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;   // channels of a row in LDS
-    constexpr int BN = DP <= 128 ? 64 : 32;
+    constexpr bool F16 = sizeof(T) == 2;
+    constexpr int BN = F16 && DP <= 128 ? 64 : 32;
+    constexpr int BUFS = F16 ? 2 : 1;   // fp32's parts leave room for one block
     constexpr int CH = DPL / 8, KS = DP / 16, NT = DP / 32, KT = BN / 32;
     constexpr int UN = BN * CH / 256;   // 8-channel units a thread moves of K, and of V
     constexpr int TILE = BN * CH;       // 16-byte slots of a plane
-    __shared__ short8_t lds[2][2][TILE];
+    __shared__ short8_t lds[BUFS][2][S::kPlanes][TILE];
 
     const int g = blockIdx.x % p.kvH, rest = blockIdx.x / p.kvH;
     const int sp = rest % p.splits;
@@ -608,15 +644,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
                 }
             }
         }
-        mx = fmaxf(mx, xor32_value(mx));
-        const int e = mx > 0.0f && mx < __builtin_inff() ? __builtin_amdgcn_frexp_expf(mx) - 15 : 0;
-        fac = __builtin_amdgcn_ldexpf(fac, e);
+        if constexpr (F16) {   // every row's largest value into [2^14, 2^15)
+            mx = fmaxf(mx, xor32_value(mx));
+            const int e = mx > 0.0f && mx < __builtin_inff() ? __builtin_amdgcn_frexp_expf(mx) - 15 : 0;
+            fac = __builtin_amdgcn_ldexpf(fac, e);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[s][i] = __builtin_amdgcn_ldexpf(x[s][i], -e);
-            S::part(x[s], qx[s]);
+                for (int i = 0; i < 8; ++i) x[s][i] = __builtin_amdgcn_ldexpf(x[s][i], -e);
         }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) S::part(x[s], qx[s]);
     }
 
     // a thread's units of a block: unit u is chunk u % CH of row u / CH
@@ -627,7 +665,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
     const int chunk = tid % CH, urow = tid / CH;
     const int ch = 8 * chunk < p.D ? 8 * chunk : 0;
     int page[UN], slot[UN];
-    short8_t kx[UN], vx[UN];
+    typedef T unit_t __attribute__((ext_vector_type(8)));
+    unit_t kx[UN], vx[UN];
     auto look = [&](int k0) {   // keys past the request's last read that one; they are masked
 #pragma unroll
         for (int i = 0; i < UN; ++i) {
@@ -641,17 +680,33 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
         for (int i = 0; i < UN; ++i) {
             const bool there = (unsigned)page[i] < (unsigned)p.b.num_pages;
             const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : 0) * hs + ch;
-            kx[i] = *reinterpret_cast<const short8_t*>(kc + at);
-            vx[i] = *reinterpret_cast<const short8_t*>(vc + at);
-            if (!there) kx[i] = short8_t{0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff, 0x7fff};   // NaN: see below
+            kx[i] = *reinterpret_cast<const unit_t*>(kc + at);
+            vx[i] = *reinterpret_cast<const unit_t*>(vc + at);
+            if (!there) kx[i] = unit_t((T)__builtin_nanf(""));   // such rows are done over, below
+        }
+    };
+    auto planes = [](const unit_t& x, short8_t (&out)[S::kPlanes]) {
+        if constexpr (F16) {
+            out[0] = __builtin_bit_cast(short8_t, x);
+        } else {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = x[i];
+            S::part(f, out);
         }
     };
     auto store = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < UN; ++i) {
             const int r = urow + 256 / CH * i;
-            lds[buf][0][k_slot<CH>(r, chunk)] = kx[i];
-            lds[buf][1][r * CH + (chunk ^ v_turn<CH>(r))] = vx[i];
+            short8_t kp[S::kPlanes], vp[S::kPlanes];
+            planes(kx[i], kp);
+            planes(vx[i], vp);
+#pragma unroll
+            for (int pl = 0; pl < S::kPlanes; ++pl) {
+                lds[buf][0][pl][k_slot<CH>(r, chunk)] = kp[pl];
+                lds[buf][1][pl][r * CH + (chunk ^ v_turn<CH>(r))] = vp[pl];
+            }
         }
     };
 
@@ -669,7 +724,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
     }
     __syncthreads();
     int buf = 0;
-    for (int k0 = first; k0 <= kr.khi; k0 += BN, buf ^= 1) {
+    for (int k0 = first; k0 <= kr.khi; k0 += BN) {
         const bool more = k0 + BN <= kr.khi;
         if (more) {
             fetch();
@@ -681,13 +736,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
             for (int kt = 0; kt < KT; ++kt) st[kt] = floatx16_t{};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                short8_t a[KT];
+                short8_t a[S::kPlanes][KT];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) a[kt] = lds[buf][0][k_slot<CH>(32 * kt + l32, 2 * s + hf)];
+                for (int pl = 0; pl < S::kPlanes; ++pl)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) a[pl][kt] = lds[buf][0][pl][k_slot<CH>(32 * kt + l32, 2 * s + hf)];
 #pragma unroll
                 for (int j = 0; j < S::kProducts; ++j)
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) st[kt] = S::mfma(a[kt], qx[s][S::pair[j][1]], st[kt]);
+                    for (int kt = 0; kt < KT; ++kt) st[kt] = S::mfma(a[S::pair[j][0]][kt], qx[s][S::pair[j][1]], st[kt]);
             }
             if (k0 < all_lo || k0 + BN - 1 > all_hi)
 #pragma unroll
@@ -711,7 +768,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
 #pragma unroll
                 for (int n = 0; n < NT; ++n) acc[n] *= al;
             }
-            const float off = m == -__builtin_inff() ? 0.0f : (float)kWeightExp - m;
+            const float off = m == -__builtin_inff() ? 0.0f : (F16 ? (float)kWeightExp : 0.0f) - m;
 #pragma unroll
             for (int s = 0; s < 2 * KT; ++s) {
                 float w[8];
@@ -726,21 +783,28 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
                 for (int n = 0; n < NT; ++n) {
                     // rows 16 s + 8 e + 4 hf + i / 4, 16 channels of 8-byte quarters of two chunks
                     const int i = lane & 15;
-                    short8_t a;
+                    short8_t a[S::kPlanes];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int r = 16 * s + 8 * e + 4 * hf + (i >> 2), c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-                        const short4_t h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_short4_t*)((short4_t*)&lds[buf][1][r * CH + (c ^ v_turn<CH>(r))] + (i & 1)));
+                    for (int pl = 0; pl < S::kPlanes; ++pl)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) a[4 * e + x] = h[x];
-                    }
+                        for (int e = 0; e < 2; ++e) {
+                            const int r = 16 * s + 8 * e + 4 * hf + (i >> 2);
+                            const int c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                            const short4_t h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (lds_short4_t*)((short4_t*)&lds[buf][1][pl][r * CH + (c ^ v_turn<CH>(r))] + (i & 1)));
 #pragma unroll
-                    for (int j = 0; j < S::kProducts; ++j) acc[n] = S::mfma(a, px[S::pair[j][1]], acc[n]);
+                            for (int x = 0; x < 4; ++x) a[pl][4 * e + x] = h[x];
+                        }
+#pragma unroll
+                    for (int j = 0; j < S::kProducts; ++j) acc[n] = S::mfma(a[S::pair[j][0]], px[S::pair[j][1]], acc[n]);
                 }
             }
         }
-        if (more) store(buf ^ 1);
+        if constexpr (BUFS == 2)
+            buf ^= 1;
+        else
+            __syncthreads();
+        if (more) store(buf);
         __syncthreads();
     }
 
@@ -761,7 +825,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
         }
     if (p.splits > 1 && mine && hf == 0) {
         paged_part_ml(p, sp, orow)[0] = m;
-        paged_part_ml(p, sp, orow)[1] = l * (1.0f / (1 << kWeightExp));
+        paged_part_ml(p, sp, orow)[1] = F16 ? l * (1.0f / (1 << kWeightExp)) : l;
     }
     // rows that met an infinity, a NaN or a page that is not there
     uint64_t redo = __ballot(odd);
