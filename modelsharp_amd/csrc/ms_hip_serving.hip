@@ -74,17 +74,17 @@ void launch_rows(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
         hipLaunchKernelGGL((paged_rows_kernel<T, 256, WHOLE>), dim3(grid), dim3(256), 0, s, p);
 }
 
-template <typename T>
+template <typename T, bool WHOLE>
 void launch_blocks(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
 {
     if (p.D <= 64)
-        hipLaunchKernelGGL((paged_blocks_kernel<T, 64>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_blocks_kernel<T, 64, WHOLE>), dim3(grid), dim3(256), 0, s, p);
     else if (p.D <= 96)
-        hipLaunchKernelGGL((paged_blocks_kernel<T, 96>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_blocks_kernel<T, 96, WHOLE>), dim3(grid), dim3(256), 0, s, p);
     else if (p.D <= 128)
-        hipLaunchKernelGGL((paged_blocks_kernel<T, 128>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_blocks_kernel<T, 128, WHOLE>), dim3(grid), dim3(256), 0, s, p);
     else if constexpr (sizeof(T) == 2)
-        hipLaunchKernelGGL((paged_blocks_kernel<T, 256>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_blocks_kernel<T, 256, WHOLE>), dim3(grid), dim3(256), 0, s, p);
 }
 }  // namespace
 
@@ -94,10 +94,10 @@ hipError_t launch_paged_attention(const PagedAttnArgs& args, const PagedAttnPlan
     if (plan.blocks_grid) {
         p.rows_min = plan.rows_grid ? kFewRows + 1 : 0;
         p.rows_max = INT32_MAX;
-        if (p.f16)
-            launch_blocks<_Float16>(p, (unsigned)plan.blocks_grid, s);
-        else
-            launch_blocks<float>(p, (unsigned)plan.blocks_grid, s);
+        const bool whole = p.b.page.div % 8 == 0;
+        const auto launch = p.f16 ? (whole ? launch_blocks<_Float16, true> : launch_blocks<_Float16, false>)
+                                  : (whole ? launch_blocks<float, true> : launch_blocks<float, false>);
+        launch(p, (unsigned)plan.blocks_grid, s);
         if (hipError_t e = hipGetLastError()) return e;
     }
     if (plan.rows_grid) {

@@ -518,13 +518,25 @@ template <> struct PagedSplit<_Float16> {
     static constexpr int pair[kProducts][2] = {{0, 0}, {0, 1}};   // (plane, part)
     __device__ static __forceinline__ void part(const float (&x)[8], short8_t (&out)[2])
     {
-        half8_t h, l;
+        typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+        u32x4_t h, l;
+        float minus = -1.0f;   // opaque, so that x - h is one v_fma_mix_f32 on the packed half
+        asm("" : "+s"(minus));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) l[i] = (_Float16)__builtin_fmaf((float)h[i], -1.0f, x[i]);
+        for (int i = 0; i < 4; ++i) {
+            h[i] = pack(x[2 * i], x[2 * i + 1]);
+            l[i] = pack(fmac_lo(h[i], minus, x[2 * i]), fmac_hi(h[i], minus, x[2 * i + 1]));
+        }
         out[0] = __builtin_bit_cast(short8_t, h);
         out[1] = __builtin_bit_cast(short8_t, l);
+    }
+    // both rounded to nearest, in one v_cvt_pk_f16_f32 (kept whole by the opaque result)
+    __device__ static __forceinline__ uint32_t pack(float a, float b)
+    {
+        typedef float f2_t __attribute__((ext_vector_type(2)));
+        uint32_t r = as_u32(__builtin_convertvector(f2_t{a, b}, h2_t));
+        asm("" : "+v"(r));
+        return r;
     }
     __device__ static __forceinline__ floatx16_t mfma(short8_t a, short8_t b, floatx16_t c)
     {
@@ -586,7 +598,9 @@ __device__ __forceinline__ int v_turn(int row)
 // leave their lane and a row's statistics are its lane's own; V^T comes from ds_read_b64_tr_b16, which
 // hands 16 lanes four keys of one channel each. The online softmax runs in base 2 and moves
 // its maximum only in steps above 2^4, so that the accumulators are seldom rescaled.
-template <typename T, int DP>
+// WHOLE: pages of a multiple of 8 rows, so that a wave's rows of a load lie in one page: its lookups
+// are the scalar unit's.
+template <typename T, int DP, bool WHOLE>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(PagedAttnArgs p)
 {
     typedef PagedSplit<T> S;
@@ -663,25 +677,36 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
     const T* const vc = static_cast<const T*>(p.vc) + (int64_t)g * p.D;
     const int32_t* const table = p.b.table + (int64_t)t.r * p.b.max_pages;
     const int chunk = tid % CH, urow = tid / CH;
+    constexpr int RU = 256 / CH, RW = 64 / CH;   // rows of a unit step over the workgroup and over a wave
     const int ch = 8 * chunk < p.D ? 8 * chunk : 0;
-    int page[UN], slot[UN];
     typedef T unit_t __attribute__((ext_vector_type(8)));
     unit_t kx[UN], vx[UN];
-    auto look = [&](int k0) {   // keys past the request's last read that one; they are masked
+    // keys past the request's last stand for that one; they are masked
+    int page[UN], slot[UN], ahead[UN];   // WHOLE: of the wave's first row, and how many rows follow up to the last key
+    auto look = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < UN; ++i) {
-            const int key = min(k0 + urow + 256 / CH * i, t.klast), pg = p.b.page.quot(key);
+            const int r = RU * i + (WHOLE ? RW * wave : urow);
+            const int key = min(k0 + r, WHOLE ? t.klast & ~(RW - 1) : t.klast), pg = p.b.page.quot(key);
             page[i] = table[pg];
             slot[i] = key - pg * p.b.page.div;
+            ahead[i] = t.klast - key;
         }
     };
     auto fetch = [&]() {
 #pragma unroll
         for (int i = 0; i < UN; ++i) {
             const bool there = (unsigned)page[i] < (unsigned)p.b.num_pages;
-            const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : 0) * hs + ch;
-            kx[i] = *reinterpret_cast<const unit_t*>(kc + at);
-            vx[i] = *reinterpret_cast<const unit_t*>(vc + at);
+            const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : 0) * hs;
+            if constexpr (WHOLE) {   // a scalar base and 32-bit offsets
+                const uint32_t off =
+                    (min(lane / CH, there ? ahead[i] : 0) * (uint32_t)hs + (uint32_t)ch) * (uint32_t)sizeof(T);
+                kx[i] = *reinterpret_cast<const unit_t*>(reinterpret_cast<const char*>(kc + at) + off);
+                vx[i] = *reinterpret_cast<const unit_t*>(reinterpret_cast<const char*>(vc + at) + off);
+            } else {
+                kx[i] = *reinterpret_cast<const unit_t*>(kc + at + ch);
+                vx[i] = *reinterpret_cast<const unit_t*>(vc + at + ch);
+            }
             if (!there) kx[i] = unit_t((T)__builtin_nanf(""));   // such rows are done over, below
         }
     };
