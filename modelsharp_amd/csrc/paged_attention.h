@@ -7,11 +7,11 @@
 // The query heads of a kv head and the tokens of a request are rows of one matrix, row = token
 // * group + head in group, so that a tile of K and V serves every row that reads it.
 #pragma once
+#include "mfma_device.h"
 #include "serving.h"
 
 namespace msnb {
 
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));   // rows are 4-byte aligned
 
@@ -502,7 +502,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
 }
 
 // ---- chunks: tiles of 128 rows -----------------------------------------------------------------
-typedef float floatx16_t __attribute__((ext_vector_type(16)));
 typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef short short8_t __attribute__((ext_vector_type(8)));
@@ -582,9 +581,14 @@ template <> struct PagedSplit<float> {
 // of a row moved about so that the reads below meet no bank twice: K's by ds_read_b128 down 32 rows
 // of one chunk, V's by the transposing read, 4 rows of two chunks for 16 lanes.
 template <int CH>
+__device__ __forceinline__ int k_turn(int row)
+{
+    return CH == 8 ? (row >> 1) & 7 : row & 15;
+}
+template <int CH>
 __device__ __forceinline__ int k_slot(int row, int c)
 {
-    return row * CH + (c ^ (CH == 8 ? (row >> 1) & 7 : row & 15));
+    return row * CH + (c ^ k_turn<CH>(row));
 }
 template <int CH>
 __device__ __forceinline__ int v_turn(int row)
@@ -639,6 +643,94 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
     const int all_lo = max(kr.klo, p.window >= 0 ? pos_b - p.window + 1 : 0), all_hi = min(kr.khi, pos_a);
     const int any_lo = max(kr.klo, p.window >= 0 ? pos_a - p.window + 1 : 0), any_hi = min(kr.khi, pos_b);
 
+    // a thread's units of a block: unit u is chunk u % CH of row u / CH
+    const int64_t hs = (int64_t)p.kvH * p.D;
+    const T* const kc = static_cast<const T*>(p.kc) + (int64_t)g * p.D;
+    const T* const vc = static_cast<const T*>(p.vc) + (int64_t)g * p.D;
+    const int32_t* const table = p.b.table + (int64_t)t.r * p.b.max_pages;
+    const int chunk = tid % CH, urow = tid / CH;
+    constexpr int RU = 256 / CH, RW = 64 / CH;   // rows of a unit step over the workgroup and over a wave
+    constexpr bool DIRECT = WHOLE && F16;        // straight from memory to LDS: fp16 needs no conversion
+    const int ch = 8 * chunk < p.D ? 8 * chunk : 0;
+    typedef T unit_t __attribute__((ext_vector_type(8)));
+    unit_t kx[DIRECT ? 1 : UN], vx[DIRECT ? 1 : UN];
+    // keys past the request's last stand for that one; they are masked
+    int page[UN], slot[UN], ahead[UN];   // WHOLE: of the wave's first row, and how many rows follow up to the last key
+    auto look = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const int r = RU * i + (WHOLE ? RW * wave : urow);
+            const int key = min(k0 + r, WHOLE ? t.klast & ~(RW - 1) : t.klast), pg = p.b.page.quot(key);
+            page[i] = table[pg];
+            slot[i] = key - pg * p.b.page.div;
+            ahead[i] = t.klast - key;
+        }
+    };
+    bool missing = false;   // a page that is not there
+    // the next block's loads: into registers, or into LDS buffer `buf`, where lane i of a load
+    // fills slot i of its 64, so that the lanes fetch the chunks that belong there. Rows of a
+    // page that is not there are any row's, and the tile is done over, below.
+    auto fetch = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const bool there = (unsigned)page[i] < (unsigned)p.b.num_pages;
+            const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : 0) * hs;
+            missing |= !there;
+            if constexpr (WHOLE) {   // a scalar base and 32-bit offsets
+                const int last = there ? ahead[i] : 0;
+                const uint32_t off = min(lane / CH, last) * (uint32_t)hs * (uint32_t)sizeof(T);
+                if constexpr (DIRECT) {
+                    const int bytes = (min(RW - 1, last) + 1) * (int)hs * (int)sizeof(T), r = RU * i + urow;
+                    const int ck = 8 * (chunk ^ k_turn<CH>(r)), cv = 8 * (chunk ^ v_turn<CH>(r));
+                    const uint32_t m0 = RU * CH * 16 * i + 1024 * wave;
+                    lds_load16(buffer_rsrc(kc + at, bytes), off + 2 * (ck < p.D ? ck : 0), 0, lds_address(&lds[buf][0][0][0]) + m0);
+                    lds_load16(buffer_rsrc(vc + at, bytes), off + 2 * (cv < p.D ? cv : 0), 0, lds_address(&lds[buf][1][0][0]) + m0);
+                } else {
+                    kx[i] = *reinterpret_cast<const unit_t*>(reinterpret_cast<const char*>(kc + at + ch) + off);
+                    vx[i] = *reinterpret_cast<const unit_t*>(reinterpret_cast<const char*>(vc + at + ch) + off);
+                }
+            } else {
+                kx[i] = *reinterpret_cast<const unit_t*>(kc + at + ch);
+                vx[i] = *reinterpret_cast<const unit_t*>(vc + at + ch);
+            }
+        }
+    };
+    auto planes = [](const unit_t& x, short8_t (&out)[S::kPlanes]) {
+        if constexpr (F16) {
+            out[0] = __builtin_bit_cast(short8_t, x);
+        } else {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = x[i];
+            S::part(f, out);
+        }
+    };
+    auto store = [&](int buf) {   // what fetch() brought is in LDS for every wave behind the next barrier
+        if constexpr (DIRECT) {
+            wait_vmcnt<0>();
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const int r = urow + 256 / CH * i;
+            short8_t kp[S::kPlanes], vp[S::kPlanes];
+            planes(kx[i], kp);
+            planes(vx[i], vp);
+#pragma unroll
+            for (int pl = 0; pl < S::kPlanes; ++pl) {
+                lds[buf][0][pl][k_slot<CH>(r, chunk)] = kp[pl];
+                lds[buf][1][pl][r * CH + (chunk ^ v_turn<CH>(r))] = vp[pl];
+            }
+        }
+    };
+
+    const int first = kr.klo / BN * BN;
+    const bool any = kr.khi >= kr.klo;
+    if (any) {
+        look(first);
+        fetch(0);
+        look(first + BN);
+    }
     short8_t qx[KS][S::kParts];
     float fac = fabsf(p.scale2);
     {
@@ -671,88 +763,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
         for (int s = 0; s < KS; ++s) S::part(x[s], qx[s]);
     }
 
-    // a thread's units of a block: unit u is chunk u % CH of row u / CH
-    const int64_t hs = (int64_t)p.kvH * p.D;
-    const T* const kc = static_cast<const T*>(p.kc) + (int64_t)g * p.D;
-    const T* const vc = static_cast<const T*>(p.vc) + (int64_t)g * p.D;
-    const int32_t* const table = p.b.table + (int64_t)t.r * p.b.max_pages;
-    const int chunk = tid % CH, urow = tid / CH;
-    constexpr int RU = 256 / CH, RW = 64 / CH;   // rows of a unit step over the workgroup and over a wave
-    const int ch = 8 * chunk < p.D ? 8 * chunk : 0;
-    typedef T unit_t __attribute__((ext_vector_type(8)));
-    unit_t kx[UN], vx[UN];
-    // keys past the request's last stand for that one; they are masked
-    int page[UN], slot[UN], ahead[UN];   // WHOLE: of the wave's first row, and how many rows follow up to the last key
-    auto look = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < UN; ++i) {
-            const int r = RU * i + (WHOLE ? RW * wave : urow);
-            const int key = min(k0 + r, WHOLE ? t.klast & ~(RW - 1) : t.klast), pg = p.b.page.quot(key);
-            page[i] = table[pg];
-            slot[i] = key - pg * p.b.page.div;
-            ahead[i] = t.klast - key;
-        }
-    };
-    auto fetch = [&]() {
-#pragma unroll
-        for (int i = 0; i < UN; ++i) {
-            const bool there = (unsigned)page[i] < (unsigned)p.b.num_pages;
-            const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : 0) * hs;
-            if constexpr (WHOLE) {   // a scalar base and 32-bit offsets
-                const uint32_t off =
-                    (min(lane / CH, there ? ahead[i] : 0) * (uint32_t)hs + (uint32_t)ch) * (uint32_t)sizeof(T);
-                kx[i] = *reinterpret_cast<const unit_t*>(reinterpret_cast<const char*>(kc + at) + off);
-                vx[i] = *reinterpret_cast<const unit_t*>(reinterpret_cast<const char*>(vc + at) + off);
-            } else {
-                kx[i] = *reinterpret_cast<const unit_t*>(kc + at + ch);
-                vx[i] = *reinterpret_cast<const unit_t*>(vc + at + ch);
-            }
-            if (!there) kx[i] = unit_t((T)__builtin_nanf(""));   // such rows are done over, below
-        }
-    };
-    auto planes = [](const unit_t& x, short8_t (&out)[S::kPlanes]) {
-        if constexpr (F16) {
-            out[0] = __builtin_bit_cast(short8_t, x);
-        } else {
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = x[i];
-            S::part(f, out);
-        }
-    };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < UN; ++i) {
-            const int r = urow + 256 / CH * i;
-            short8_t kp[S::kPlanes], vp[S::kPlanes];
-            planes(kx[i], kp);
-            planes(vx[i], vp);
-#pragma unroll
-            for (int pl = 0; pl < S::kPlanes; ++pl) {
-                lds[buf][0][pl][k_slot<CH>(r, chunk)] = kp[pl];
-                lds[buf][1][pl][r * CH + (chunk ^ v_turn<CH>(r))] = vp[pl];
-            }
-        }
-    };
 
     floatx16_t acc[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = floatx16_t{};
     float m = -__builtin_inff(), l = 0.0f;
 
-    const int first = kr.klo / BN * BN;
-    if (kr.khi >= kr.klo) {
-        look(first);
-        fetch();
-        look(first + BN);
-        store(0);
-    }
+    if (any) store(0);
     __syncthreads();
     int buf = 0;
     for (int k0 = first; k0 <= kr.khi; k0 += BN) {
         const bool more = k0 + BN <= kr.khi;
         if (more) {
-            fetch();
+            fetch(buf ^ (BUFS - 1));
             look(k0 + 2 * BN);
         }
         if (k0 <= any_hi && k0 + BN > any_lo) {
@@ -833,10 +856,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
         __syncthreads();
     }
 
+    int* const said = reinterpret_cast<int*>(lds);   // the blocks are done with
+    if (const bool any_missing = __ballot(missing); lane == 0) said[wave] = any_missing;
+    __syncthreads();
+    missing = said[0] | said[1] | said[2] | said[3];
+
     l += xor32_value(l);
     const float f = l != 0.0f ? 1.0f / l : 0.0f;
     float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
-    bool odd = mine && m == -__builtin_inff() && k_hi >= k_lo;
+    bool odd = mine && (missing || (m == -__builtin_inff() && k_hi >= k_lo));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
