@@ -3405,7 +3405,7 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const in
     if (misaligned16(dKCache) || misaligned16(dVCache))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the cache must be 16-byte aligned");
     const PagedAttnPlan plan = paged_plan(*d, dWorkspace && !misaligned16(dWorkspace) ? workspace_bytes : 0);
-    if (plan.rows_grid > INT_MAX || plan.blocks_grid > INT_MAX)
+    if (plan.rows_grid + plan.blocks_grid > INT_MAX)
         return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_attention: %d tokens of %d requests need too many workgroups",
                     d->tokens, d->requests);
     PagedAttnArgs p{};

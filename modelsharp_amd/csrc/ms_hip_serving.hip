@@ -31,9 +31,7 @@ hipError_t launch_append(const AppendArgs& p, hipStream_t s)
 
 // ---- attention over pages ----------------------------------------------------------------------
 namespace {
-// Requests of up to this many rows go to paged_rows_kernel (16 rows a tile).
-constexpr int kFewRows = 32;
-// Which cases paged_blocks_kernel takes: an fp32 block's three parts fit LDS up to 128 channels.
+// Which cases paged_blocks() takes: an fp32 block's three parts fit LDS up to 128 channels.
 bool blocks_fit(int D, int f16) { return f16 || D <= 128; }
 }  // namespace
 
@@ -49,7 +47,8 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new
     const int64_t rows = one   ? 0
                          : few ? tokens * grp / 16 + requests
                                : (int64_t)std::min<int64_t>(requests, tokens) * ((kFewRows + 15) / 16);
-    const int64_t likely = few ? std::max<int64_t>(1, std::min(rows, (max_new * grp + 15) / 16 * requests)) : blocks;
+    const int64_t likely = few ? std::max<int64_t>(1, std::min(rows, (max_new * grp + 15) / 16 * requests))
+                               : tokens * grp / 128 + 1 + (one ? 0 : std::min<int64_t>(requests, tokens));
     int64_t splits = std::max<int64_t>(1, 2 * (int64_t)cus / (likely * kvH));
     splits = std::min<int64_t>({splits, std::max<int64_t>(1, keys / (few ? 128 : 256)), 64});
     const int64_t ws = splits > 1 ? splits * tokens * H * (D + 2) * (int64_t)sizeof(float) : 0;
@@ -63,52 +62,42 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new
 }
 
 namespace {
-template <typename T, bool WHOLE>
-void launch_rows(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
+template <typename T, bool WHOLE, PagedMode MODE>
+void launch_paged_t(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
 {
+    constexpr bool kWide = sizeof(T) == 2 || MODE == kPagedRows;   // blocks_fit()
     if (p.D <= 64)
-        hipLaunchKernelGGL((paged_rows_kernel<T, 64, WHOLE>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_attention_kernel<T, 64, WHOLE, MODE>), dim3(grid), dim3(256), 0, s, p);
+    else if (MODE != kPagedRows && p.D <= 96)
+        hipLaunchKernelGGL((paged_attention_kernel<T, MODE == kPagedRows ? 64 : 96, WHOLE, MODE>), dim3(grid), dim3(256), 0, s, p);
     else if (p.D <= 128)
-        hipLaunchKernelGGL((paged_rows_kernel<T, 128, WHOLE>), dim3(grid), dim3(256), 0, s, p);
-    else
-        hipLaunchKernelGGL((paged_rows_kernel<T, 256, WHOLE>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_attention_kernel<T, 128, WHOLE, MODE>), dim3(grid), dim3(256), 0, s, p);
+    else if constexpr (kWide)
+        hipLaunchKernelGGL((paged_attention_kernel<T, 256, WHOLE, MODE>), dim3(grid), dim3(256), 0, s, p);
 }
 
 template <typename T, bool WHOLE>
-void launch_blocks(const PagedAttnArgs& p, unsigned grid, hipStream_t s)
+void launch_paged(const PagedAttnArgs& p, const PagedAttnPlan& plan, hipStream_t s)
 {
-    if (p.D <= 64)
-        hipLaunchKernelGGL((paged_blocks_kernel<T, 64, WHOLE>), dim3(grid), dim3(256), 0, s, p);
-    else if (p.D <= 96)
-        hipLaunchKernelGGL((paged_blocks_kernel<T, 96, WHOLE>), dim3(grid), dim3(256), 0, s, p);
-    else if (p.D <= 128)
-        hipLaunchKernelGGL((paged_blocks_kernel<T, 128, WHOLE>), dim3(grid), dim3(256), 0, s, p);
-    else if constexpr (sizeof(T) == 2)
-        hipLaunchKernelGGL((paged_blocks_kernel<T, 256, WHOLE>), dim3(grid), dim3(256), 0, s, p);
+    const unsigned grid = (unsigned)(plan.blocks_grid + plan.rows_grid);
+    if (!plan.blocks_grid)
+        launch_paged_t<T, WHOLE, kPagedRows>(p, grid, s);
+    else if (!plan.rows_grid)
+        launch_paged_t<T, WHOLE, kPagedBlocks>(p, grid, s);
+    else
+        launch_paged_t<T, WHOLE, kPagedBoth>(p, grid, s);
 }
 }  // namespace
 
 hipError_t launch_paged_attention(const PagedAttnArgs& args, const PagedAttnPlan& plan, hipStream_t s)
 {
     PagedAttnArgs p = args;
-    if (plan.blocks_grid) {
-        p.rows_min = plan.rows_grid ? kFewRows + 1 : 0;
-        p.rows_max = INT32_MAX;
-        const bool whole = p.b.page.div % 8 == 0;
-        const auto launch = p.f16 ? (whole ? launch_blocks<_Float16, true> : launch_blocks<_Float16, false>)
-                                  : (whole ? launch_blocks<float, true> : launch_blocks<float, false>);
-        launch(p, (unsigned)plan.blocks_grid, s);
-        if (hipError_t e = hipGetLastError()) return e;
-    }
-    if (plan.rows_grid) {
-        p.rows_min = 0;
-        p.rows_max = plan.blocks_grid ? kFewRows : INT32_MAX;
-        const bool whole = p.b.page.div % 16 == 0;
-        const auto launch = p.f16 ? (whole ? launch_rows<_Float16, true> : launch_rows<_Float16, false>)
-                                  : (whole ? launch_rows<float, true> : launch_rows<float, false>);
-        launch(p, (unsigned)plan.rows_grid, s);
-        if (hipError_t e = hipGetLastError()) return e;
-    }
+    p.blocks_grid = (int)plan.blocks_grid;
+    const bool whole = p.b.page.div % 16 == 0;
+    const auto launch = p.f16 ? (whole ? launch_paged<_Float16, true> : launch_paged<_Float16, false>)
+                              : (whole ? launch_paged<float, true> : launch_paged<float, false>);
+    launch(p, plan, s);
+    if (hipError_t e = hipGetLastError()) return e;
     if (p.splits > 1) {
         const int64_t rows = (int64_t)p.b.tokens * p.H;
         hipLaunchKernelGGL(paged_merge_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);

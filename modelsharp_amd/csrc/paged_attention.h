@@ -34,11 +34,11 @@ __device__ __forceinline__ int wave_scan(int x)
     return x;
 }
 
-// Tile `idx` of the launch's requests (those of rows_min to rows_max rows) in order, each one's tiles
+// Tile `idx` of the requests of rows_min to rows_max rows in order, each one's tiles
 // from its last (the longest range of keys) to its first; false past the end. Every wave by
 // itself, with a uniform idx.
 template <int BM>
-__device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, PagedTile& t)
+__device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, int rows_min, int rows_max, PagedTile& t)
 {
     const PagedBatch& b = p.b;
     const int lane = threadIdx.x & (kWave - 1);
@@ -47,7 +47,7 @@ __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, Page
         const int c0 = max(b.cu[i], 0), c1 = min(b.cu[i + 1], b.tokens), past = b.past[i];
         const int n = base + lane < b.requests ? max(c1 - c0, 0) : 0;
         const int nr = n * p.grp.div;
-        const int tiles = nr >= p.rows_min && nr <= p.rows_max ? (nr + BM - 1) / BM : 0;
+        const int tiles = nr >= rows_min && nr <= rows_max ? (nr + BM - 1) / BM : 0;
         const int sum = wave_scan(tiles);
         const uint64_t past_idx = __ballot(sum > idx);
         if (past_idx) {
@@ -109,11 +109,11 @@ __device__ __forceinline__ bool finite4(floatx4_t v)
 // that are not there. A split's record is (max, sum) with its normed output; no visible key: sum
 // 0; every score -infinity: max -infinity, sum 1; a score that is NaN or +infinity: NaN.
 template <typename T>
-__device__ __forceinline__ void paged_exact_row(const PagedAttnArgs& p, const PagedTile& t, int lr, int sp, PagedRange kr)
+__device__ __forceinline__ void paged_exact_row(const PagedAttnArgs& p, const PagedTile& t, int g, int lr, int sp, PagedRange kr)
 {
     const int lane = threadIdx.x & (kWave - 1);
     const int row = t.row0 + lr, tok = p.grp.quot(row);
-    const int g = blockIdx.x % p.kvH, head = g * p.grp.div + row - tok * p.grp.div;
+    const int head = g * p.grp.div + row - tok * p.grp.div;
     const int pos = t.past + tok;
     const int lo = max(kr.klo, p.window >= 0 ? max(0, pos - p.window + 1) : 0), hi = min(kr.khi, pos);
     const float* const q = p.q + (int64_t)(t.t0 + tok) * p.q_stride + (int64_t)head * p.D;
@@ -205,8 +205,9 @@ constexpr int paged_ring(int DP, bool f16) { return f16 ? (DP <= 128 ? 3 : 2) : 
 // as two halves; an fp32 cache is multiplied in fp32.
 // WHOLE: pages of a multiple of 16 rows, so that a step lies in one page: one lookup a step, and a
 // page that is not there is a step left out.
+constexpr int kRowsLds = 4 * 4 * kWave * 16 + 2 * 4 * 16 * 4 + 16;
 template <typename T, int DP, bool WHOLE>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(PagedAttnArgs p)
+__device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int rows_max, uint8_t* lds)
 {
     constexpr bool F16 = sizeof(T) == 2;
     constexpr int VEC = F16 && DP >= 128 ? 8 : 4;   // channels of one lane's load of V
@@ -216,14 +217,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
     typedef typename PagedElem<T>::vec_t kvec_t;
     typedef T vvec_t __attribute__((ext_vector_type(VEC)));
     constexpr int kRing = paged_ring(DP, F16);
-    __shared__ float stat[2][4][16];
-    __shared__ floatx4_t merge[4][4][kWave];
-    __shared__ int flag;
+    auto& merge = *reinterpret_cast<floatx4_t(*)[4][4][kWave]>(lds);
+    auto& stat = *reinterpret_cast<float(*)[2][4][16]>(lds + sizeof(merge));
+    int& flag = *reinterpret_cast<int*>(lds + sizeof(merge) + sizeof(stat));
 
-    const int g = blockIdx.x % p.kvH, rest = blockIdx.x / p.kvH;
+    const int g = bid % p.kvH, rest = bid / p.kvH;
     const int sp = rest % p.splits;
     PagedTile t;
-    if (!paged_tile<16>(p, rest / p.splits, t)) return;
+    if (!paged_tile<16>(p, rest / p.splits, 0, rows_max, t)) return;
     const int lane = threadIdx.x & 63, grp = lane >> 4, l16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (threadIdx.x == 0) flag = 0;
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_rows_kernel(Page
     if (odd) flag = 1;
     __syncthreads();
     if (flag)
-        for (int lr = wave; lr < t.rows; lr += 4) paged_exact_row<T>(p, t, lr, sp, kr);
+        for (int lr = wave; lr < t.rows; lr += 4) paged_exact_row<T>(p, t, g, lr, sp, kr);
 }
 
 // ---- chunks: tiles of 128 rows -----------------------------------------------------------------
@@ -602,25 +603,32 @@ __device__ __forceinline__ int v_turn(int row)
 // leave their lane and a row's statistics are its lane's own; V^T comes from ds_read_b64_tr_b16, which
 // hands 16 lanes four keys of one channel each. The online softmax runs in base 2 and moves
 // its maximum only in steps above 2^4, so that the accumulators are seldom rescaled.
-// WHOLE: pages of a multiple of 8 rows, so that a wave's rows of a load lie in one page: its lookups
+// WHOLE: pages of a multiple of 16 rows, so that a wave's rows of a load lie in one page: its lookups
 // are the scalar unit's.
+template <typename T, int DP>
+struct PagedBlock {
+    static constexpr bool F16 = sizeof(T) == 2;
+    static constexpr int DPL = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;   // channels of a row in LDS
+    static constexpr int BN = F16 && DP <= 128 ? 64 : 32;               // keys
+    static constexpr int BUFS = F16 ? 2 : 1;                            // fp32's parts leave room for one block
+    static constexpr int CH = DPL / 8, TILE = BN * CH;                  // 16-byte slots of a row, of a plane
+    typedef short8_t lds_t[BUFS][2][PagedSplit<T>::kPlanes][TILE];
+};
 template <typename T, int DP, bool WHOLE>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(PagedAttnArgs p)
+__device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, int rows_min, uint8_t* lds_bytes)
 {
     typedef PagedSplit<T> S;
-    constexpr int DPL = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;   // channels of a row in LDS
-    constexpr bool F16 = sizeof(T) == 2;
-    constexpr int BN = F16 && DP <= 128 ? 64 : 32;
-    constexpr int BUFS = F16 ? 2 : 1;   // fp32's parts leave room for one block
-    constexpr int CH = DPL / 8, KS = DP / 16, NT = DP / 32, KT = BN / 32;
+    typedef PagedBlock<T, DP> B;
+    constexpr bool F16 = B::F16;
+    constexpr int BN = B::BN, BUFS = B::BUFS, CH = B::CH;
+    constexpr int KS = DP / 16, NT = DP / 32, KT = BN / 32;
     constexpr int UN = BN * CH / 256;   // 8-channel units a thread moves of K, and of V
-    constexpr int TILE = BN * CH;       // 16-byte slots of a plane
-    __shared__ short8_t lds[BUFS][2][S::kPlanes][TILE];
+    auto& lds = *reinterpret_cast<typename B::lds_t*>(lds_bytes);
 
-    const int g = blockIdx.x % p.kvH, rest = blockIdx.x / p.kvH;
+    const int g = bid % p.kvH, rest = bid / p.kvH;
     const int sp = rest % p.splits;
     PagedTile t;
-    if (!paged_tile<128>(p, rest / p.splits, t)) return;
+    if (!paged_tile<128>(p, rest / p.splits, rows_min, INT32_MAX, t)) return;
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const PagedRange kr = paged_range(p, t.past + p.grp.quot(t.row0), t.past + p.grp.quot(t.row0 + t.rows - 1), t.klast,
@@ -883,7 +891,31 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_blocks_kernel(Pa
     // rows that met an infinity, a NaN or a page that is not there
     uint64_t redo = __ballot(odd);
     for (uint32_t rows = (uint32_t)(redo | redo >> 32); rows; rows &= rows - 1)
-        paged_exact_row<T>(p, t, 32 * wave + __ffs(rows) - 1, sp, kr);
+        paged_exact_row<T>(p, t, g, 32 * wave + __ffs(rows) - 1, sp, kr);
+}
+
+// A launch's workgroups: the first p.blocks_grid take tiles of 128 rows of the requests of more than
+// kFewRows rows (the longest work first), the others tiles of 16 rows of the rest, beside them:
+// one is bound by the matrix cores, the other by memory. Without the one or the other kind the
+// kind that is there takes every request.
+constexpr int kFewRows = 32;
+enum PagedMode { kPagedRows, kPagedBlocks, kPagedBoth };
+template <typename T, int DP, bool WHOLE, PagedMode MODE>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttnArgs p)
+{
+    constexpr int DPR = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;
+    constexpr int kBlocksLds = MODE == kPagedRows ? 0 : (int)sizeof(typename PagedBlock<T, DP>::lds_t);
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBlocksLds > kRowsLds ? kBlocksLds : kRowsLds];
+    if constexpr (MODE == kPagedRows) {
+        paged_rows<T, DPR, WHOLE>(p, blockIdx.x, INT32_MAX, lds);
+    } else if constexpr (MODE == kPagedBlocks) {
+        paged_blocks<T, DP, WHOLE>(p, blockIdx.x, 0, lds);
+    } else {
+        if ((int)blockIdx.x < p.blocks_grid)
+            paged_blocks<T, DP, WHOLE>(p, blockIdx.x, kFewRows + 1, lds);
+        else
+            paged_rows<T, DPR, WHOLE>(p, blockIdx.x - p.blocks_grid, kFewRows, lds);
+    }
 }
 
 // The splits' records of one output row, joined in the splits' order. A wave per row: lane s holds

@@ -109,7 +109,7 @@ struct PagedAttnArgs {
     float* part;      // splits > 1: [splits][tokens * H][D], then [splits][tokens * H] of (max, sum)
     int H, kvH, D, window, f16, splits;
     int split_min;    // keys of a split at the least
-    int rows_min, rows_max;   // the launch takes requests of that many rows (new tokens * group)
+    int blocks_grid;  // workgroups of paged_blocks()
     int64_t q_stride;
     FastDiv grp;      // query heads per kv head
     float scale2;     // scale * log2(e)
