@@ -20,7 +20,7 @@ struct AppendPlace {
 __device__ __forceinline__ bool append_place(const AppendArgs& p, int t, AppendPlace& at)
 {
     if (!p.b.cu) {
-        at.pos = max(p.positions[t], 0);
+        at.pos = p.positions ? max(p.positions[t], 0) : 0;   // null: nothing turns
         at.row = t;
         return true;
     }

@@ -369,6 +369,27 @@ def test_qk_norm_rotary(gpu, T, H, G, D, cols, inter, in_place):
         assert np.abs(got.cpu().numpy().reshape(T, n, D) - want).max() <= tol
 
 
+@pytest.mark.parametrize("D", [64, 50])
+@pytest.mark.parametrize("norm", [False, True])
+def test_qk_norm_without_rotation_reads_no_positions_and_no_caches(gpu, D, norm):
+    """do_rotary = 0: positions, cos and sin may be null, and so may either norm's weights."""
+    import torch
+    T, H, G = 5, 4, 2
+    rng = np.random.default_rng(33)
+    q, k = (rng.standard_normal((T, n * D)).astype(F32) for n in (H, G))
+    gk = (rng.random(D) + 0.5).astype(F32) if norm else None
+    d = native.QkNormDesc(tokens=T, num_heads=H, kv_num_heads=G, head_dim=D, eps=1e-6)
+    log(f"qk_norm without rotation D={D} norm={norm}")
+    qd, kd, gd = dev(q), dev(k), dev(gk)
+    qo, ko = torch.empty_like(qd), torch.empty_like(kd)
+    native.qk_norm_rotary(d, ptr(qd), ptr(kd), None, ptr(gd), None, None, None, ptr(qo), ptr(ko), stream())
+    torch.cuda.synchronize()
+    assert np.array_equal(qo.cpu().numpy(), q)
+    want = np.stack([ref.normed_rotated(k[t].reshape(G, D), gk, 0, None, None, False, 1e-6) for t in range(T)])
+    tol = ref.norm_tolerance(D, gk, 1.5 * np.sqrt(D), False)
+    assert np.abs(ko.cpu().numpy().reshape(T, G, D) - want).max() <= tol
+
+
 # ---- low-rank adapters -----------------------------------------------------------------------------
 
 # T, K, N, adapters, max_rank, pattern of adapters, with ranks / scales, base ("new", "same", None)
