@@ -110,25 +110,56 @@ LoraPlan lora_plan(int T, int K, int N, int adapters, int rank, int cus)
 {
     LoraPlan pl;
     const int tiles = (T + kLoraTokens - 1) / kLoraTokens;
-    pl.slots = T <= 64 ? std::min(kLoraTokens, adapters + 1) : 1;
-    pl.splits = std::max(1, std::min({2 * cus / (tiles * pl.slots), (K + 255) / 256, 16}));
+    // Many tiles: a tile's classes one after another, one workgroup of 16 waves for all of K, and as many
+    // tiles of tokens to an expand workgroup, which keeps B in registers across them, as leave two
+    // workgroups to a CU.
+    pl.many = tiles >= cus / 4;
+    if (pl.many) {
+        const int nb = (N + kLoraRows - 1) / kLoraRows;
+        while (pl.subs < tiles && (int64_t)((tiles + pl.subs - 1) / pl.subs) * nb > 2 * cus) ++pl.subs;
+    } else {   // few: the classes side by side, and K over workgroups
+        pl.slots = std::max(1, std::min({kLoraTokens, adapters + 1, 2 * cus / tiles}));
+        pl.splits = std::max(1, std::min({2 * cus / (tiles * pl.slots), (K + 255) / 256, 16}));
+    }
     pl.ws_bytes = (int64_t)pl.splits * T * ((rank + 15) / 16 * 16) * (int64_t)sizeof(float);
     return pl;
 }
 
 namespace {
+template <typename T, int C, int CH, bool ONE>
+void launch_expand(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
+{
+    const int tokens = kLoraTokens * plan.subs;
+    const dim3 grid((p.T + tokens - 1) / tokens * plan.slots * ((p.N + kLoraRows - 1) / kLoraRows));
+    hipLaunchKernelGGL((lora_expand_kernel<T, C, CH, ONE>), grid, dim3(256), 0, s, p, plan.slots, plan.subs);
+}
+
+template <typename T, int RT, int WAVES>
+void launch_shrink(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
+{
+    const int groups = (p.rank16 + 16 * RT - 1) / (16 * RT);
+    const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * groups * plan.slots * plan.splits);
+    hipLaunchKernelGGL((lora_shrink_kernel<T, RT, WAVES>), grid, dim3(64 * WAVES), 0, s, p, plan.slots);
+}
+
+template <typename T, int C, int CH>
+void launch_lora_c(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
+{
+    constexpr int RT = C / 16;
+    if (plan.many) {
+        launch_shrink<T, RT, 16>(p, plan, s);
+        launch_expand<T, C, CH, true>(p, plan, s);
+    } else {
+        launch_shrink<T, RT * CH, 4>(p, plan, s);
+        launch_expand<T, C, CH, false>(p, plan, s);
+    }
+}
+
 template <typename T>
 void launch_lora_t(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
-    const int tiles = (p.T + kLoraTokens - 1) / kLoraTokens;
-    const dim3 shrink(tiles * plan.slots * plan.splits), expand(tiles * plan.slots * ((p.N + kLoraRows - 1) / kLoraRows));
-    if (p.rank16 == 16)
-        hipLaunchKernelGGL((lora_shrink_kernel<T, 1>), shrink, dim3(256), 0, s, p, plan.slots);
-    else if (p.rank16 == 32)
-        hipLaunchKernelGGL((lora_shrink_kernel<T, 2>), shrink, dim3(256), 0, s, p, plan.slots);
-    else
-        hipLaunchKernelGGL((lora_shrink_kernel<T, 4>), shrink, dim3(256), 0, s, p, plan.slots);
-    hipLaunchKernelGGL(lora_expand_kernel<T>, expand, dim3(256), 0, s, p, plan.slots);
+    const auto launch = p.rank16 == 16 ? launch_lora_c<T, 16, 1> : p.rank16 == 32 ? launch_lora_c<T, 32, 1> : launch_lora_c<T, 32, 2>;
+    launch(p, plan, s);
 }
 }  // namespace
 

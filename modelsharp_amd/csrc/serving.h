@@ -136,7 +136,8 @@ struct LoraArgs {
     int T, K, N, adapters, rank, rank16, f16, splits, vec;
 };
 struct LoraPlan {
-    int splits = 1, slots = 1;
+    int splits = 1, slots = 1, subs = 1;   // subs: tiles of tokens to an expand workgroup
+    bool many = false;
     int64_t ws_bytes = 0;
 };
 MS_INTERNAL LoraPlan lora_plan(int T, int K, int N, int adapters, int rank, int cus);

@@ -406,6 +406,12 @@ LORA = [
     (200, 3000, 72, 7, 32, "mixed", False, None),
     (20, 128, 64, 2, 8, "none", True, "new"),             # no token has an adapter
     (20, 128, 64, 2, 8, "none", True, None),
+    (1100, 96, 300, 5, 20, "mixed", True, "new"),         # many tiles
+    (1040, 1024, 264, 4, 64, "runs", True, "same"),
+    (1033, 100, 52, 3, 5, "mixed", True, "new"),
+    (1030, 64, 520, 3, 130, "mixed", True, None),
+    (2100, 160, 2056, 6, 16, "runs", True, "new"),
+    (1029, 64, 64, 2, 8, "none", True, "same"),
 ]
 
 
