@@ -44,27 +44,39 @@ __device__ __forceinline__ int lora_rank(const LoraArgs& p, int a)
     return p.ranks ? min(max(p.ranks[a], 0), p.rank) : p.rank;
 }
 
-// E consecutive values from base + at, those from `n` on zero; vec: one load, then n is at most 0 or
-// at least E wherever E divides the row.
-template <int E, typename T>
-__device__ __forceinline__ auto lora_load(const T* base, int64_t at, int n, int vec)
+// E consecutive values from base + at, of which n are there (VEC: all E, or none: then the last E,
+// so that the load needs no branch). The others are zero without VEC, anything with it.
+template <int E, bool VEC, typename T>
+__device__ __forceinline__ auto lora_load(const T* base, int64_t at, int n)
 {
     typedef T tv __attribute__((ext_vector_type(E)));
-    tv x{};
-    if (vec && n >= E) {
-        x = *reinterpret_cast<const tv*>(base + at);
+    if constexpr (VEC) {
+        return *reinterpret_cast<const tv*>(base + (at + min(n - E, 0)));
     } else {
+        tv x{};
 #pragma unroll
         for (int i = 0; i < E; ++i)
             if (i < n) x[i] = base[at + i];
+        return x;
     }
-    return x;
+}
+
+// The first n of v's E values, zeros after them: by whole dwords, whatever the others hold.
+template <int E, typename T>
+__device__ __forceinline__ void lora_keep(T __attribute__((ext_vector_type(E))) & v, int n)
+{
+    typedef uint32_t dwords_t __attribute__((ext_vector_type(E * sizeof(T) / 4)));
+    constexpr int P = 4 / sizeof(T);   // values of a dword
+    dwords_t d = __builtin_bit_cast(dwords_t, v);
+#pragma unroll
+    for (int i = 0; i < E / P; ++i) d[i] &= n >= P * (i + 1) ? ~0u : n > P * i ? 0xffffu : 0u;
+    v = __builtin_bit_cast(T __attribute__((ext_vector_type(E))), d);
 }
 
 // grid: tiles * rank groups * slots * splits; slot s takes the tile's classes s, s + slots, ... The
 // waves take every WAVES'th step of 32 of the split's K, the next steps' loads in flight meanwhile,
 // and meet in LDS. RT: rank tiles of 16 in a group.
-template <typename T, int RT, int WAVES>
+template <typename T, int RT, int WAVES, bool VEC>
 __global__ __launch_bounds__(64 * WAVES) void lora_shrink_kernel(LoraArgs p, int slots)
 {
     __shared__ floatx4_t sums[WAVES][RT][kWave];
@@ -80,27 +92,31 @@ __global__ __launch_bounds__(64 * WAVES) void lora_shrink_kernel(LoraArgs p, int
     for (int c = 0; cls.left; ++c) {
         const int a = cls.next();
         if (c % slots != slot || a < 0) continue;
-        const int rank = lora_rank(p, a);
-        if (r0 >= rank) continue;
+        const int rank = lora_rank(p, a);   // 0: nothing to add up, h is written as zeros
         const T* const A = static_cast<const T*>(p.a) + (int64_t)a * p.rank * p.K;
         struct Step {
             floatx4_t x[2];
             T __attribute__((ext_vector_type(8))) a[RT];
         };
         auto load = [&](int s, Step& v) {
+            // rows of A past the rank stand for its last: their sums are not used
             const int k = 32 * s + 8 * grp;
-            v.x[0] = lora_load<4>(x, k, p.K - k, p.vec);
-            v.x[1] = lora_load<4>(x, k + 4, p.K - k - 4, p.vec);
+            v.x[0] = lora_load<4, VEC>(x, k, p.K - k);
+            v.x[1] = lora_load<4, VEC>(x, k + 4, p.K - k - 4);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const int r = r0 + 16 * rt + l16;
-                v.a[rt] = lora_load<8>(A, (int64_t)min(r, rank - 1) * p.K + k, r < rank ? p.K - k : 0, p.vec);
-            }
+            for (int rt = 0; rt < RT; ++rt)
+                v.a[rt] = lora_load<8, VEC>(A, (int64_t)min(r0 + 16 * rt + l16, rank - 1) * p.K + k, p.K - k);
         };
+        const bool any = r0 < rank;
         floatx4_t acc[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt] = floatx4_t{};
-        auto add = [&](const Step& v) {
+        auto add = [&](int s, Step& v) {
+            if (VEC && 32 * s + 32 > p.K && 32 * s + 8 * grp >= p.K) {   // the last step's lanes past K
+                v.x[0] = v.x[1] = floatx4_t{};
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) v.a[rt] = decltype(v.a[rt] + v.a[rt]){};
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -109,17 +125,20 @@ __global__ __launch_bounds__(64 * WAVES) void lora_shrink_kernel(LoraArgs p, int
         };
         constexpr int kRing = 3;
         Step ring[kRing];
+        // every load is made, past the last step that one's again: behind a load under a condition the
+        // compiler could only wait for all that is under way
         int s = s0 + wave;
+        if (any && s < s1) {
 #pragma unroll
-        for (int n = 0; n + 1 < kRing; ++n)
-            if (s + WAVES * n < s1) load(s + WAVES * n, ring[n]);
-        while (s < s1) {
+            for (int n = 0; n + 1 < kRing; ++n) load(min(s + WAVES * n, s1 - 1), ring[n]);
+            for (bool more = true; more;) {
 #pragma unroll
-            for (int n = 0; n < kRing; ++n) {
-                if (s >= s1) break;
-                if (s + WAVES * (kRing - 1) < s1) load(s + WAVES * (kRing - 1), ring[(n + kRing - 1) % kRing]);
-                add(ring[n]);
-                s += WAVES;
+                for (int n = 0; n < kRing; ++n) {
+                    load(min(s + WAVES * (kRing - 1), s1 - 1), ring[(n + kRing - 1) % kRing]);
+                    add(s, ring[n]);
+                    s += WAVES;
+                    if (!(more = s < s1)) break;
+                }
             }
         }
 #pragma unroll
@@ -130,6 +149,8 @@ __global__ __launch_bounds__(64 * WAVES) void lora_shrink_kernel(LoraArgs p, int
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) v += sums[w][wave][lane];
             const int r = r0 + 16 * wave + 4 * grp;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = r + i < rank ? v[i] : 0.0f;
             if (cls.mine == a && r < p.rank16)
                 *reinterpret_cast<floatx4_t*>(p.h + ((int64_t)sp * p.T + t) * p.rank16 + r) = v;
         }
@@ -137,174 +158,189 @@ __global__ __launch_bounds__(64 * WAVES) void lora_shrink_kernel(LoraArgs p, int
     }
 }
 
-// The products of a chunk of C = 16 or 32 ranks: B's rows n (lane % 16) and the tokens' h (lane % 16),
-// E = C / 4 ranks in a row a lane. fp16 weights go to the fp16 matrix cores as they are, h as two
-// halves of h 2^-e (22 bits, e by token: any fp32 h fits); fp32 weights to the fp32 ones.
-template <int E>
-struct LoraHalves {
-    _Float16 __attribute__((ext_vector_type(E))) hi, lo;
-    __device__ __forceinline__ void set(const float (&x)[E], int e)
-    {
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const float v = __builtin_amdgcn_ldexpf(x[j], -e);
-            hi[j] = (_Float16)v;
-            lo[j] = (_Float16)(v - (float)hi[j]);
-        }
-    }
-};
-
-// grid: tiles of 16 `sub` tokens * slots * ceil(N / 256); a wave takes 64 outputs of 16 tokens after 16, B_a
-// staying in its registers as long as the class does, CH chunks of C ranks at a time. What does not
-// depend on the class (the base, h) is on its way before the class is known, the next 16 tokens'
-// while these are worked on. ONE: h has one split.
+// grid: tiles of 16 `subs` tokens * slots * ceil(N / 256). For 16 tokens after 16:
+//   the threads take h (4 ranks of a token each, the splits added in their order) to LDS: for fp16
+//     weights as two halves of h 2^-e (22 bits, e by token, so that any fp32 h fits);
+//   each wave multiplies 64 rows of B_a, in its registers as long as the class does not change, with
+//     each class's tokens, and leaves scale * sum in LDS;
+//   the threads add it to the base and store, whole rows of 1 KB at a time.
+// (A wave's sums lie 16 tokens by 16 outputs: stored from there, every instruction touches 16 lines,
+// and the launch took 65 us in place of @@ at 2048 tokens of N = 11008.)
+// R ranks at a time, in chunks of C; more come in further passes over the sums in LDS. ONE: h has
+// one split, and the base and h of the next 16 tokens are on their way meanwhile. No load or store of
+// that loop is under a condition, behind which the compiler could only wait for all that is under way:
+// what is not wanted goes to an offset that the buffer does not have.
 // Memory bounds it: base and y once, 8 bytes an output against 2 ranks flops.
-template <typename T, int C, int CH, bool ONE>
+template <typename T, int C, int CH, bool ONE, bool VEC>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots, int subs)
 {
     constexpr bool F16 = sizeof(T) == 2;
-    constexpr int E = C / 4;
+    constexpr int E = C / 4, R = C * CH, LPT = R / 4;   // ranks of a lane's operand; lanes that take a token's h
+    constexpr int HS = R + (F16 ? 8 : 4), YS = kLoraRows + 4;   // strides off the powers of two
+    typedef T bvec_t __attribute__((ext_vector_type(E)));
+    __shared__ floatx4_t ys[kLoraTokens * YS / 4];
+    __shared__ floatx4_t hs[(F16 ? 2 * 2 : 4) * kLoraTokens * HS / 16];
+    __shared__ int exps[kLoraTokens];
+    T* const h0 = reinterpret_cast<T*>(hs);   // [token][HS], fp16: the high halves, then the low ones
+    float* const yl = reinterpret_cast<float*>(ys);
+
     const int nb = (p.N + kLoraRows - 1) / kLoraRows;
     const int rest = blockIdx.x / nb, slot = rest % slots, t00 = rest / slots * (kLoraTokens * subs);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, grp = lane >> 4;
-    const int n0 = blockIdx.x % nb * kLoraRows + 64 * wave;
-    typedef T bvec_t __attribute__((ext_vector_type(E)));
+    const int n0 = blockIdx.x % nb * kLoraRows;
+    const int ht = tid / LPT, hr = 4 * (tid % LPT);   // this thread's token and ranks of h (if ht < 16)
     bvec_t bv[CH][4];
-    int held = -1;   // whose ranks 0 .. C CH - 1 those are
+    int held = -1;   // whose ranks 0 .. R - 1 those are
+
     struct Ahead {
         int adapter;
-        floatx4_t base[4], h[ONE ? CH : 1][ONE ? E / 4 : 1];
+        floatx4_t base[4], h;
     };
     auto fetch = [&](int t0, Ahead& x) {
-        const int t = t0 + l16;
-        const bool in = t < p.T;
-        x.adapter = lora_adapter(p, t);
+        x.adapter = lora_adapter(p, t0 + l16);
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-            const int n = n0 + 16 * nt + 4 * grp;
-            x.base[nt] = p.base && in ? lora_load<4>(p.base, (int64_t)t * p.N + n, p.N - n, p.vec) : floatx4_t{};
+        for (int i = 0; i < 4; ++i) {   // token 4 wave + i, outputs 4 lane ..
+            const int t = min(t0 + 4 * wave + i, p.T - 1), n = n0 + 4 * lane;
+            x.base[i] = p.base ? lora_load<4, VEC>(p.base, (int64_t)t * p.N + n, p.N - n) : floatx4_t{};
         }
         if constexpr (ONE)
-#pragma unroll
-            for (int q = 0; q < CH; ++q)
-#pragma unroll
-                for (int e = 0; e < E / 4; ++e) {
-                    const int r = min(C * q + E * grp + 4 * e, p.rank16 - 4);
-                    x.h[q][e] = *reinterpret_cast<const floatx4_t*>(p.h + (int64_t)min(t, p.T - 1) * p.rank16 + r);
-                }
+            x.h = *reinterpret_cast<const floatx4_t*>(p.h + (int64_t)min(t0 + min(ht, 15), p.T - 1) * p.rank16 +
+                                                      min(hr, p.rank16 - 4));
     };
     Ahead next;
     fetch(t00, next);
 #pragma unroll 1
     for (int sub = 0; sub < subs; ++sub) {
-        const int t0 = t00 + kLoraTokens * sub, t = t0 + l16;
+        const int t0 = t00 + kLoraTokens * sub;
         if (t0 >= p.T) return;
+        const __amdgpu_buffer_rsrc_t rows = buffer_rsrc(p.y + (int64_t)t0 * p.N, 64 * p.N);   // these tokens' of y
         const Ahead now = next;
-        if (sub + 1 < subs) fetch(t0 + kLoraTokens, next);
-        LoraClasses cls(now.adapter);
-        for (int c = 0; cls.left; ++c) {
-            const int a = cls.next();
-            if (c % slots != slot || (a < 0 && p.base == p.y)) continue;
-            const int rank = a < 0 ? 0 : lora_rank(p, a);
-            const float scale = a < 0 || !p.scales ? 1.0f : p.scales[a];
-            const T* const B = static_cast<const T*>(p.b) + (int64_t)max(a, 0) * p.N * p.rank;
-            const bool mine = cls.mine == a;
-            floatx4_t sum[4];
+        if (subs > 1) fetch(min(t0 + kLoraTokens, p.T - 1), next);   // past the last: not used
+        uint32_t done = 0, adds = 0;   // tokens of this workgroup's classes, and those with an adapter
+        for (int r0 = 0; r0 < p.rank16; r0 += R) {
+            if (ht < kLoraTokens) {
+                floatx4_t h = now.h;
+                const int r = r0 + hr;
+                if (!ONE || r0 > 0) {
+                    constexpr int kAtOnce = ONE ? 1 : 8;
+                    const float* const src = p.h + (int64_t)min(t0 + ht, p.T - 1) * p.rank16 + min(r, p.rank16 - 4);
+                    const int64_t step = (int64_t)p.T * p.rank16;
+                    h = floatx4_t{};
+                    for (int s0 = 0; s0 < p.splits; s0 += kAtOnce) {
+                        floatx4_t v[kAtOnce];
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) sum[nt] = floatx4_t{};
-            for (int r0 = 0; r0 < rank; r0 += C * CH) {
-                if (held != a || r0 > 0 || rank > C * CH) {
+                        for (int i = 0; i < kAtOnce; ++i)
+                            v[i] = *reinterpret_cast<const floatx4_t*>(src + min(s0 + i, p.splits - 1) * step);
 #pragma unroll
-                    for (int q = 0; q < CH; ++q)
+                        for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-                        for (int nt = 0; nt < 4; ++nt) {
-                            const int n = min(n0 + 16 * nt + l16, p.N - 1), r = r0 + C * q + E * grp;
-                            bv[q][nt] = lora_load<E>(B, (int64_t)n * p.rank + r, rank - r, p.vec);
-                        }
-                    held = r0 == 0 ? a : -1;
-                }
-                float h[CH][E], mx = 0.0f;
-#pragma unroll
-                for (int q = 0; q < CH; ++q) {
-                    const int r = r0 + C * q + E * grp;
-#pragma unroll
-                    for (int j = 0; j < E; ++j) h[q][j] = 0.0f;
-                    if (ONE && r0 == 0) {
-#pragma unroll
-                        for (int j = 0; j < E; ++j) h[q][j] = now.h[ONE ? q : 0][ONE ? j >> 2 : 0][j & 3];
-                    } else if (mine && r < p.rank16) {
-                        constexpr int kAtOnce = ONE ? 1 : 8;   // splits, added in their order
-                        const float* const src = p.h + (int64_t)t * p.rank16 + r;
-                        const int64_t step = (int64_t)p.T * p.rank16;
-                        for (int s0 = 0; s0 < p.splits; s0 += kAtOnce) {
-                            floatx4_t v[kAtOnce][E / 4];
-#pragma unroll
-                            for (int i = 0; i < kAtOnce; ++i)
-#pragma unroll
-                                for (int e = 0; e < E / 4; ++e)
-                                    v[i][e] = *reinterpret_cast<const floatx4_t*>(src + min(s0 + i, p.splits - 1) * step + 4 * e);
-#pragma unroll
-                            for (int i = 0; i < kAtOnce; ++i)
-#pragma unroll
-                                for (int j = 0; j < E; ++j) h[q][j] += s0 + i < p.splits ? v[i][j >> 2][j & 3] : 0.0f;
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < E; ++j) {   // other tokens' and other ranks' were not written
-                        h[q][j] = mine && r + j < rank ? h[q][j] : 0.0f;
-                        mx = fmaxf(mx, fabsf(h[q][j]));
+                            for (int j = 0; j < 4; ++j) h[j] += s0 + i < p.splits ? v[i][j] : 0.0f;
                     }
                 }
+                if (r >= p.rank16) h = floatx4_t{};
                 if constexpr (F16) {
-                    mx = fmaxf(mx, xor16_value(mx));
-                    mx = fmaxf(mx, xor32_value(mx));
+                    float mx = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
+                    mx = fmaxf(mx, dpp_read<0xB1>(mx));
+                    mx = fmaxf(mx, dpp_read<0x4E>(mx));
+                    if constexpr (LPT >= 8) mx = fmaxf(mx, dpp_read<0x141>(mx));
+                    if constexpr (LPT >= 16) mx = fmaxf(mx, dpp_read<0x140>(mx));
                     const int e = mx > 0.0f && mx < __builtin_inff() ? __builtin_amdgcn_frexp_expf(mx) - 15 : 0;
-                    floatx4_t acc[4];
+                    _Float16 __attribute__((ext_vector_type(4))) hi, lo;
 #pragma unroll
-                    for (int nt = 0; nt < 4; ++nt) acc[nt] = floatx4_t{};
-#pragma unroll
-                    for (int q = 0; q < CH; ++q) {
-                        LoraHalves<E> x;
-                        x.set(h[q], e);
-#pragma unroll
-                        for (int nt = 0; nt < 4; ++nt) {
-                            if constexpr (C == 32) {
-                                acc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[q][nt], x.lo, acc[nt], 0, 0, 0);
-                                acc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[q][nt], x.hi, acc[nt], 0, 0, 0);
-                            } else {
-                                acc[nt] = __builtin_amdgcn_mfma_f32_16x16x16f16(bv[q][nt], x.lo, acc[nt], 0, 0, 0);
-                                acc[nt] = __builtin_amdgcn_mfma_f32_16x16x16f16(bv[q][nt], x.hi, acc[nt], 0, 0, 0);
-                            }
-                        }
+                    for (int j = 0; j < 4; ++j) {
+                        const float v = __builtin_amdgcn_ldexpf(h[j], -e);
+                        hi[j] = (_Float16)v;
+                        lo[j] = (_Float16)(v - (float)hi[j]);
                     }
-#pragma unroll
-                    for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sum[nt][i] += __builtin_amdgcn_ldexpf(acc[nt][i], e);
+                    *reinterpret_cast<decltype(hi)*>(h0 + ht * HS + hr) = hi;
+                    *reinterpret_cast<decltype(lo)*>(h0 + (kLoraTokens + ht) * HS + hr) = lo;
+                    if (hr == 0) exps[ht] = e;
                 } else {
-#pragma unroll
-                    for (int q = 0; q < CH; ++q)
-#pragma unroll
-                        for (int j = 0; j < E; ++j)
-#pragma unroll
-                            for (int nt = 0; nt < 4; ++nt)
-                                sum[nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[q][nt][j], h[q][j], sum[nt], 0, 0, 0);
+                    *reinterpret_cast<floatx4_t*>(h0 + ht * HS + hr) = h;
                 }
             }
+            __syncthreads();
+            LoraClasses cls(now.adapter);
+            bvec_t hv[F16 ? 2 : 1][CH];   // this lane's token's
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                const int n = n0 + 16 * nt + 4 * grp;
-                const int64_t at = (int64_t)t * p.N + n;
-                const floatx4_t y = a < 0 ? now.base[nt] : now.base[nt] + scale * sum[nt];
-                if (!mine) continue;
-                if (p.vec && n < p.N) {
-                    *reinterpret_cast<floatx4_t*>(p.y + at) = y;
-                } else {
+            for (int q = 0; q < CH; ++q)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (n + i < p.N) p.y[at + i] = y[i];
+                for (int k = 0; k < (F16 ? 2 : 1); ++k)
+                    hv[k][q] = *reinterpret_cast<const bvec_t*>(h0 + (kLoraTokens * k + l16) * HS + C * q + E * grp);
+            const int e = F16 ? exps[l16] : 0;
+            for (int c = 0; cls.left; ++c) {
+                const uint32_t before = cls.left;
+                const int a = cls.next();
+                if (c % slots != slot) continue;
+                done |= before & ~cls.left;
+                if (a < 0) continue;
+                adds |= before & ~cls.left;
+                const int rank = lora_rank(p, a);
+                const float scale = p.scales ? p.scales[a] : 1.0f;
+                const T* const B = static_cast<const T*>(p.b) + (int64_t)a * p.N * p.rank;
+                if (held != a || p.rank16 > R) {
+#pragma unroll
+                    for (int q = 0; q < CH; ++q)
+#pragma unroll
+                        for (int nt = 0; nt < 4; ++nt) {
+                            const int n = min(n0 + 64 * wave + 16 * nt + l16, p.N - 1), r = r0 + C * q + E * grp;
+                            bv[q][nt] = lora_load<E, VEC>(B, (int64_t)n * p.rank + r, p.rank - r);
+                        }
+                    if (rank < r0 + R)   // columns past the adapter's own rank are not its values
+#pragma unroll
+                        for (int q = 0; q < CH; ++q)
+#pragma unroll
+                            for (int nt = 0; nt < 4; ++nt) lora_keep<E, T>(bv[q][nt], rank - (r0 + C * q + E * grp));
+                    held = a;
                 }
+                floatx4_t acc[4];
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt) acc[nt] = floatx4_t{};
+#pragma unroll
+                for (int q = 0; q < CH; ++q)
+#pragma unroll
+                    for (int nt = 0; nt < 4; ++nt) {
+                        if constexpr (F16) {
+#pragma unroll
+                            for (int k = 1; k >= 0; --k) {
+                                if constexpr (C == 32)
+                                    acc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[q][nt], hv[k][q], acc[nt], 0, 0, 0);
+                                else
+                                    acc[nt] = __builtin_amdgcn_mfma_f32_16x16x16f16(bv[q][nt], hv[k][q], acc[nt], 0, 0, 0);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < E; ++j)
+                                acc[nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[q][nt][j], hv[0][q][j], acc[nt], 0, 0, 0);
+                        }
+                    }
+                if (cls.mine == a)
+#pragma unroll
+                    for (int nt = 0; nt < 4; ++nt) {
+                        floatx4_t* const y = reinterpret_cast<floatx4_t*>(yl + l16 * YS + 64 * wave + 16 * nt + 4 * grp);
+                        floatx4_t v;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = scale * (F16 ? __builtin_amdgcn_ldexpf(acc[nt][i], e) : acc[nt][i]);
+                        *y = r0 == 0 ? v : *y + v;
+                    }
+            }
+            __syncthreads();
+        }
+        if (p.base == p.y) done &= adds;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int tok = 4 * wave + i, n = n0 + 4 * lane;
+            const floatx4_t sum = *reinterpret_cast<const floatx4_t*>(yl + tok * YS + 4 * lane);
+            const floatx4_t y = adds >> tok & 1 ? now.base[i] + sum : now.base[i];
+            const bool mine = done >> tok & 1;
+            if constexpr (VEC) {
+                const int off = mine && n < p.N ? (int)((uint32_t)(tok * p.N + n) * 4u) : kOOB;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, y), rows, off, 0, 0);
+            } else if (mine) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (n + k < p.N) p.y[(int64_t)(t0 + tok) * p.N + n + k] = y[k];
             }
         }
     }

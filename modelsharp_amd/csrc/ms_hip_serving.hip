@@ -126,49 +126,50 @@ LoraPlan lora_plan(int T, int K, int N, int adapters, int rank, int cus)
 }
 
 namespace {
-template <typename T, int C, int CH, bool ONE>
+template <typename T, int C, int CH, bool ONE, bool VEC>
 void launch_expand(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     const int tokens = kLoraTokens * plan.subs;
     const dim3 grid((p.T + tokens - 1) / tokens * plan.slots * ((p.N + kLoraRows - 1) / kLoraRows));
-    hipLaunchKernelGGL((lora_expand_kernel<T, C, CH, ONE>), grid, dim3(256), 0, s, p, plan.slots, plan.subs);
+    hipLaunchKernelGGL((lora_expand_kernel<T, C, CH, ONE, VEC>), grid, dim3(256), 0, s, p, plan.slots, plan.subs);
 }
 
-template <typename T, int RT, int WAVES>
+template <typename T, int RT, int WAVES, bool VEC>
 void launch_shrink(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     const int groups = (p.rank16 + 16 * RT - 1) / (16 * RT);
     const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * groups * plan.slots * plan.splits);
-    hipLaunchKernelGGL((lora_shrink_kernel<T, RT, WAVES>), grid, dim3(64 * WAVES), 0, s, p, plan.slots);
+    hipLaunchKernelGGL((lora_shrink_kernel<T, RT, WAVES, VEC>), grid, dim3(64 * WAVES), 0, s, p, plan.slots);
 }
 
-template <typename T, int C, int CH>
+template <typename T, int C, int CH, bool VEC>
 void launch_lora_c(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     constexpr int RT = C / 16;
     if (plan.many) {
-        launch_shrink<T, RT, 16>(p, plan, s);
-        launch_expand<T, C, CH, true>(p, plan, s);
+        launch_shrink<T, RT, 16, VEC>(p, plan, s);
+        launch_expand<T, C, CH, true, VEC>(p, plan, s);
     } else {
-        launch_shrink<T, RT * CH, 4>(p, plan, s);
-        launch_expand<T, C, CH, false>(p, plan, s);
+        launch_shrink<T, RT * CH, 4, VEC>(p, plan, s);
+        launch_expand<T, C, CH, false, VEC>(p, plan, s);
     }
 }
 
-template <typename T>
+template <typename T, bool VEC>
 void launch_lora_t(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
-    const auto launch = p.rank16 == 16 ? launch_lora_c<T, 16, 1> : p.rank16 == 32 ? launch_lora_c<T, 32, 1> : launch_lora_c<T, 32, 2>;
+    const auto launch = p.rank16 == 16   ? launch_lora_c<T, 16, 1, VEC>
+                        : p.rank16 == 32 ? launch_lora_c<T, 32, 1, VEC>
+                                         : launch_lora_c<T, 32, 2, VEC>;
     launch(p, plan, s);
 }
 }  // namespace
 
 hipError_t launch_lora(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
-    if (p.f16)
-        launch_lora_t<_Float16>(p, plan, s);
-    else
-        launch_lora_t<float>(p, plan, s);
+    const auto launch = p.f16 ? (p.vec ? launch_lora_t<_Float16, true> : launch_lora_t<_Float16, false>)
+                              : (p.vec ? launch_lora_t<float, true> : launch_lora_t<float, false>);
+    launch(p, plan, s);
     return hipGetLastError();
 }
 
