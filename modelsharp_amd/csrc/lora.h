@@ -10,6 +10,7 @@
 //   lora_shrink_kernel   h[split][t] = A_a x[t] over the split's part of K
 //   lora_expand_kernel   y[t] = base[t] + scale[a] (B_a (sum of the splits' h[t]))
 #pragma once
+#include "mfma_device.h"
 #include "serving.h"
 
 namespace msnb {
@@ -153,6 +154,128 @@ __global__ __launch_bounds__(64 * WAVES) void lora_shrink_kernel(LoraArgs p, int
             for (int i = 0; i < 4; ++i) v[i] = r + i < rank ? v[i] : 0.0f;
             if (cls.mine == a && r < p.rank16)
                 *reinterpret_cast<floatx4_t*>(p.h + ((int64_t)sp * p.T + t) * p.rank16 + r) = v;
+        }
+        __syncthreads();
+    }
+}
+
+// The same for many tiles (one split, a tile's classes one after another): grid tiles * rank groups. A
+// wave's steps go straight from memory to its own part of LDS, three under way, and no wave waits
+// for another before the end. The products' operands want 16 rows side by side, and loaded that
+// way every lane touches a line of its own, 64 cycles an instruction: with 2048 tokens, K = 4096
+// and rank 64 those loads alone took 15.6 us of 24. Here 8 (fp16: 4) lanes take a row's part in a
+// line, and the chunks of a row are turned by its number, so that the reads meet no bank twice.
+constexpr int kLoraLdsWaves = 8, kLoraLdsRing = 3;
+template <typename T, int RT>
+constexpr int lora_lds_stage() { return 2048 + RT * 16 * 32 * (int)sizeof(T); }   // x, then A's rank tiles
+template <typename T, int RT>
+constexpr int lora_lds_bytes() { return kLoraLdsWaves * kLoraLdsRing * lora_lds_stage<T, RT>(); }
+template <typename T, int RT>
+__global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(LoraArgs p)
+{
+    constexpr bool F16 = sizeof(T) == 2;
+    constexpr int STAGE = lora_lds_stage<T, RT>(), LOADS = 2 + RT * (F16 ? 1 : 2);
+    constexpr int AC = F16 ? 4 : 8;   // 16-byte chunks of a row of A's step
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int groups = (p.rank16 + 16 * RT - 1) / (16 * RT);
+    const int r0 = blockIdx.x % groups * (16 * RT), t0 = blockIdx.x / groups * kLoraTokens;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, grp = lane >> 4, t = t0 + l16;
+    const int steps = (p.K + 31) / 32;
+    uint8_t* const mine = lds + wave * kLoraLdsRing * STAGE;
+    const uint32_t base = lds_address(mine);
+    // what is past the last token, the adapter's rank or K reads as zero
+    const __amdgpu_buffer_rsrc_t rx = buffer_rsrc(p.x + (int64_t)t0 * p.K, min(kLoraTokens, p.T - t0) * p.K * 4);
+    int xoff[2], aoff[F16 ? 1 : 2];   // of step 0; and the first k of each
+    const int xk = 4 * ((lane & 7) ^ (lane >> 3 & 7));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xoff[i] = ((8 * i + (lane >> 3)) * p.K + xk) * 4;
+    const int arow = lane / AC, ak = F16 ? 8 * ((lane & 3) ^ (arow >> 1 & 3)) : xk;
+#pragma unroll
+    for (int i = 0; i < (F16 ? 1 : 2); ++i) aoff[i] = ((8 * i + arow) * p.K + ak) * (int)sizeof(T);
+    LoraClasses cls(lora_adapter(p, t));
+    while (cls.left) {
+        const int a = cls.next();
+        if (a < 0) continue;
+        const int rank = __builtin_amdgcn_readfirstlane(lora_rank(p, a));
+        const T* const A = static_cast<const T*>(p.a) + ((int64_t)a * p.rank + r0) * p.K;
+        // (uniform, which the compiler does not see of a value read across lanes in a loop)
+        const uint64_t at = (uint64_t)__builtin_amdgcn_readfirstlane((int)((uintptr_t)A >> 32)) << 32 |
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)(uintptr_t)A);
+        const __amdgpu_buffer_rsrc_t ra =
+            buffer_rsrc(reinterpret_cast<const void*>(at),
+                        __builtin_amdgcn_readfirstlane(max(0, min(16 * RT, rank - r0)) * p.K * (int)sizeof(T)));
+        auto issue = [&](int s, int slot) {   // past the last step: zeros, so that the waits' counts hold
+            const uint32_t m0 = __builtin_amdgcn_readfirstlane(base) + slot * STAGE;
+            const bool in = s < steps;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                lds_load16(rx, in && 32 * s + xk < p.K ? xoff[i] + 128 * s : kOOB, 0, m0 + 1024 * i);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < (F16 ? 1 : 2); ++i)
+                    lds_load16(ra, in && 32 * s + ak < p.K ? aoff[i] + (16 * rt * p.K + 32 * s) * (int)sizeof(T) : kOOB, 0,
+                               m0 + 2048 + 1024 * (rt * (F16 ? 1 : 2) + i));
+        };
+        floatx4_t acc[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt] = floatx4_t{};
+        auto add = [&](int slot) {
+            const uint8_t* const st = mine + slot * STAGE;
+            floatx4_t x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                x[e] = *reinterpret_cast<const floatx4_t*>(st + l16 * 128 + ((2 * grp + e) ^ (l16 & 7)) * 16);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float av[8];
+                const uint8_t* const ar = st + 2048 + rt * 16 * 32 * sizeof(T);
+                if constexpr (F16) {
+                    const auto v = *reinterpret_cast<const _Float16 __attribute__((ext_vector_type(8)))*>(
+                        ar + l16 * 64 + (grp ^ (l16 >> 1 & 3)) * 16);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) av[j] = (float)v[j];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const floatx4_t v =
+                            *reinterpret_cast<const floatx4_t*>(ar + l16 * 128 + ((2 * grp + e) ^ (l16 & 7)) * 16);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) av[4 * e + j] = v[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    acc[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[j], x[j >> 2][j & 3], acc[rt], 0, 0, 0);
+            }
+        };
+        if (r0 < rank) {
+#pragma unroll
+            for (int n = 0; n + 1 < kLoraLdsRing; ++n) issue(wave + kLoraLdsWaves * n, n);
+            for (int s = wave, slot = 0; s < steps; s += kLoraLdsWaves) {
+                const int free_slot = slot == 0 ? kLoraLdsRing - 1 : slot - 1;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // that slot's reads are done
+                issue(s + kLoraLdsWaves * (kLoraLdsRing - 1), free_slot);
+                wait_vmcnt<(kLoraLdsRing - 1) * LOADS>();
+                add(slot);
+                slot = slot + 1 == kLoraLdsRing ? 0 : slot + 1;
+            }
+            wait_vmcnt<0>();
+        }
+        __syncthreads();
+        floatx4_t* const sums = reinterpret_cast<floatx4_t*>(lds);   // [wave][RT][lane]
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sums[(wave * RT + rt) * kWave + lane] = acc[rt];
+        __syncthreads();
+        if (wave < RT) {
+            floatx4_t v = sums[wave * kWave + lane];
+#pragma unroll
+            for (int w = 1; w < kLoraLdsWaves; ++w) v += sums[(w * RT + wave) * kWave + lane];
+            const int r = r0 + 16 * wave + 4 * grp;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = r + i < rank ? v[i] : 0.0f;
+            if (cls.mine == a && r < p.rank16) *reinterpret_cast<floatx4_t*>(p.h + (int64_t)t * p.rank16 + r) = v;
         }
         __syncthreads();
     }

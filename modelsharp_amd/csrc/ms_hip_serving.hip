@@ -143,25 +143,36 @@ void launch_shrink(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 }
 
 template <typename T, int C, int CH, bool VEC>
-void launch_lora_c(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
+hipError_t launch_lora_c(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     constexpr int RT = C / 16;
-    if (plan.many) {
-        launch_shrink<T, RT, 16, VEC>(p, plan, s);
-        launch_expand<T, C, CH, true, VEC>(p, plan, s);
-    } else {
+    if (!plan.many) {
         launch_shrink<T, RT * CH, 4, VEC>(p, plan, s);
         launch_expand<T, C, CH, false, VEC>(p, plan, s);
+        return hipGetLastError();
     }
+    if constexpr (VEC) {
+        constexpr int lds = lora_lds_bytes<T, RT>();
+        const auto fn = lora_shrink_lds_kernel<T, RT>;
+        if (lds > 64 * 1024)
+            if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, lds))
+                return e;
+        const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * ((p.rank16 + 16 * RT - 1) / (16 * RT)));
+        hipLaunchKernelGGL(fn, grid, dim3(64 * kLoraLdsWaves), lds, s, p);
+    } else {
+        launch_shrink<T, RT, 16, VEC>(p, plan, s);
+    }
+    launch_expand<T, C, CH, true, VEC>(p, plan, s);
+    return hipGetLastError();
 }
 
 template <typename T, bool VEC>
-void launch_lora_t(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
+hipError_t launch_lora_t(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     const auto launch = p.rank16 == 16   ? launch_lora_c<T, 16, 1, VEC>
                         : p.rank16 == 32 ? launch_lora_c<T, 32, 1, VEC>
                                          : launch_lora_c<T, 32, 2, VEC>;
-    launch(p, plan, s);
+    return launch(p, plan, s);
 }
 }  // namespace
 
@@ -169,8 +180,7 @@ hipError_t launch_lora(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     const auto launch = p.f16 ? (p.vec ? launch_lora_t<_Float16, true> : launch_lora_t<_Float16, false>)
                               : (p.vec ? launch_lora_t<float, true> : launch_lora_t<float, false>);
-    launch(p, plan, s);
-    return hipGetLastError();
+    return launch(p, plan, s);
 }
 
 }  // namespace msnb
