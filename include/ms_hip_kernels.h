@@ -459,7 +459,8 @@ int ms_hip_paged_check(const ms_hip_paged_desc* desc);
 /* Norms, rotation and append: queries and keys are normed per head, x * inv * gamma with inv =
  * 1 / sqrt(mean(x^2) + eps) (dQGamma / dKGamma [head_dim], null: that one is not normed),
  * rotated by their positions (do_rotary), the queries written to dQOut [tokens,
- * num_heads * head_dim] and the keys and the values to the cache. head_dim up to 1024. dQOut
+ * num_heads * head_dim] and the keys and the values to the cache (rounded to its type: past
+ * fp16's range to an infinity). head_dim up to 1024. dQOut
  * may be dQ where its rows lie back to back; no other output may overlap an input
  * (MS_HIP_ERR_INVALID). Two requests must not share a page that either appends to. */
 int ms_hip_paged_append(const ms_hip_paged_desc* desc, const float* dQ, const float* dK, const float* dV,
@@ -497,7 +498,8 @@ int ms_hip_qk_norm_rotary(const ms_hip_qk_norm_desc* desc, const float* dQ, cons
  * may be dBase; dBase null: zero); dA [adapters, max_rank, K], dB [adapters, N, max_rank],
  * fp32 or fp16 (weight_type); dRanks int32 [adapters] (null: max_rank; rows of A and columns of
  * B from an adapter's rank on are not used), dScales fp32 [adapters] (null: 1). max_rank up to
- * 1024. fp32 accuracy, no atomics. The workspace is needed, 16-byte aligned (a smaller or
+ * 1024. fp32 accuracy, no atomics; a token with a value that is not finite has outputs that are not
+ * finite, the others none of it. The workspace is needed, 16-byte aligned (a smaller or
  * misaligned one: MS_HIP_ERR_INVALID); calls that may overlap need one each. */
 typedef struct ms_hip_lora_desc {
     int tokens, K, N, adapters, max_rank, weight_type;

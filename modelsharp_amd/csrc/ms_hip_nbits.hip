@@ -3430,6 +3430,9 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const in
     if (overlap(dOut, ob, dQ, span(T, p.q_stride, qw) * f) || overlap(dOut, ob, dKCache, cb) || overlap(dOut, ob, dVCache, cb) ||
         overlap(dOut, ob, dWorkspace, plan.ws_bytes))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the output overlaps an input or the workspace");
+    if (overlap(dWorkspace, plan.ws_bytes, dQ, span(T, p.q_stride, qw) * f) || overlap(dWorkspace, plan.ws_bytes, dKCache, cb) ||
+        overlap(dWorkspace, plan.ws_bytes, dVCache, cb))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the workspace overlaps an input");
     MS_HIP_CHECK(launch_paged_attention(p, plan, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;
 }
@@ -3500,8 +3503,9 @@ int ms_hip_lora(const ms_hip_lora_desc* d, const float* dX, const void* dA, cons
     if (overlap(dY, yb, dX, xb) || overlap(dY, yb, dA, ab) || overlap(dY, yb, dB, bb) ||
         (dBase != dY && overlap(dY, yb, dBase, yb)))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: the output overlaps an input");
-    for (const void* x : {(const void*)dX, (const void*)dBase, (const void*)dY})
-        if (overlap(dWorkspace, plan.ws_bytes, x, x == dX ? xb : yb))
+    const std::pair<const void*, int64_t> others[] = {{dX, xb}, {dBase, yb}, {dY, yb}, {dA, ab}, {dB, bb}};
+    for (const auto& [x, bytes] : others)
+        if (overlap(dWorkspace, plan.ws_bytes, x, bytes))
             return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: the workspace overlaps a buffer of the call");
     MS_HIP_CHECK(launch_lora(p, plan, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;

@@ -117,32 +117,40 @@ __device__ __forceinline__ void paged_exact_row(const PagedAttnArgs& p, const Pa
     const int pos = t.past + tok;
     const int lo = max(kr.klo, p.window >= 0 ? max(0, pos - p.window + 1) : 0), hi = min(kr.khi, pos);
     const float* const q = p.q + (int64_t)(t.t0 + tok) * p.q_stride + (int64_t)head * p.D;
-    const T* const kc = static_cast<const T*>(p.kc);
-    const T* const vc = static_cast<const T*>(p.vc);
+    const T* const kc = static_cast<const T*>(p.kc) + (int64_t)g * p.D;
+    const T* const vc = static_cast<const T*>(p.vc) + (int64_t)g * p.D;
+    const int64_t hs = (int64_t)p.kvH * p.D;
     auto score = [&](int rw) {
-        const T* const k = kc + ((int64_t)rw * p.kvH + g) * p.D;
+        typedef T unit_t __attribute__((ext_vector_type(8)));
+        const T* const k = kc + rw * hs;
         float s = 0.0f;
-        for (int d = 0; d < p.D; ++d) s = __builtin_fmaf(q[d], (float)k[d], s);
+        for (int d = 0; d < p.D; d += 8) {
+            const unit_t x = *reinterpret_cast<const unit_t*>(k + d);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s = __builtin_fmaf(q[d + i], (float)x[i], s);
+        }
         return s * p.scale2;
     };
     float m = -__builtin_inff();
     bool seen = false, bad = false;
-    for (int k = lo + lane; k <= hi; k += kWave) {
-        const int rw = paged_row(p.b, t.r, k);
-        if (rw < 0) continue;
-        const float s = score(rw);
-        seen = true;
-        bad |= !(s < __builtin_inff());
-        m = fmaxf(m, s);
+    for (int k0 = lo; k0 <= hi && !bad; k0 += kWave) {   // a score that is NaN or +infinity decides
+        const int k = k0 + lane, rw = k <= hi ? paged_row(p.b, t.r, k) : -1;
+        if (rw >= 0) {
+            const float s = score(rw);
+            seen = true;
+            bad = !(s < __builtin_inff());
+            m = fmaxf(m, s);
+        }
+        bad = __ballot(bad) != 0;
     }
     m = row16_max_all(m);
     m = fmaxf(m, xor16_value(m));
     m = fmaxf(m, xor32_value(m));
     seen = __ballot(seen) != 0;
-    bad = __ballot(bad) != 0;
     const bool all_low = seen && !bad && m == -__builtin_inff();
+    const bool sums = seen && !bad && !all_low;
     float l = 0.0f;
-    if (seen && !bad && !all_low)
+    if (sums)
         for (int k = lo + lane; k <= hi; k += kWave) {
             const int rw = paged_row(p.b, t.r, k);
             if (rw >= 0) l += __builtin_amdgcn_exp2f(score(rw) - m);
@@ -155,21 +163,31 @@ __device__ __forceinline__ void paged_exact_row(const PagedAttnArgs& p, const Pa
     if (all_low) l = 1.0f;
     const int64_t orow = (int64_t)(t.t0 + tok) * p.H + head;
     float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
-    for (int c0 = 0; c0 < p.D; c0 += kWave) {
-        const int c = min(c0 + lane, p.D - 1);
-        float acc = bad || (all_low && p.splits == 1) ? __builtin_nanf("") : 0.0f;
-        if (seen && !bad && !all_low)
-            for (int k0 = lo; k0 <= hi; k0 += kWave) {
-                const int k = k0 + lane, rw = k <= hi ? paged_row(p.b, t.r, k) : -1;
-                const float w = rw >= 0 ? __builtin_amdgcn_exp2f(score(rw) - m) / l : 0.0f;
-                for (int j = 0; j < min(kWave, hi - k0 + 1); ++j) {
-                    const int rj = __builtin_amdgcn_readlane(rw, j);
-                    const float wj = lane_value(w, j);
-                    if (rj >= 0) acc = __builtin_fmaf(wj, (float)vc[((int64_t)rj * p.kvH + g) * p.D + c], acc);
-                }
+    constexpr int kParts = 4, kAtOnce = 4;   // 64 channels each, up to 256; keys
+    float acc[kParts];
+#pragma unroll
+    for (int c = 0; c < kParts; ++c) acc[c] = bad || (all_low && p.splits == 1) ? __builtin_nanf("") : 0.0f;
+    if (sums)
+        for (int k0 = lo; k0 <= hi; k0 += kWave) {
+            const int k = k0 + lane, rw = k <= hi ? paged_row(p.b, t.r, k) : -1;
+            const float w = rw >= 0 ? __builtin_amdgcn_exp2f(score(rw) - m) / l : 0.0f;
+            for (int j0 = 0; j0 < min(kWave, hi - k0 + 1); j0 += kAtOnce) {
+                float v[kAtOnce][kParts];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+                    for (int c = 0; c < kParts; ++c)
+                        v[j][c] = (float)vc[max(__builtin_amdgcn_readlane(rw, j0 + j), 0) * hs + min(64 * c + lane, p.D - 1)];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j)
+                    if (__builtin_amdgcn_readlane(rw, j0 + j) >= 0)
+#pragma unroll
+                        for (int c = 0; c < kParts; ++c) acc[c] = __builtin_fmaf(lane_value(w, j0 + j), v[j][c], acc[c]);
             }
-        if (c0 + lane < p.D) o[c0 + lane] = acc;
-    }
+        }
+#pragma unroll
+    for (int c = 0; c < kParts; ++c)
+        if (64 * c + lane < p.D) o[64 * c + lane] = acc[c];
     if (p.splits > 1 && lane == 0) {
         paged_part_ml(p, sp, orow)[0] = m;
         paged_part_ml(p, sp, orow)[1] = l;

@@ -39,8 +39,22 @@ def _heads(node: GraphNode, op: str) -> tuple[int, int]:
 
 
 class _Serving(IKernel):
+    """A kernel that runs on its first input's device, whatever the current one is."""
+
     def __init__(self):
         self._dev = _DeviceInputs()
+
+    def execute(self, node: GraphNode, ctx: GraphContext) -> None:
+        self._check(node)
+        t = ctx.get_tensor(node.inputs[0])
+        if isinstance(t, np.ndarray):
+            self._run(node, ctx)
+        else:
+            with _torch().cuda.device(t.device):
+                self._run(node, ctx)
+
+    def _check(self, node):
+        """What the attributes alone decide."""
 
     def _gamma(self, ctx, name, D):
         if not name:
@@ -76,11 +90,14 @@ class HipPagedAttentionKernel(_Serving):
     attribute epsilon). Rows past the last request's of the output are zeros."""
     op_type = "PagedAttention"
 
-    def execute(self, node: GraphNode, ctx: GraphContext) -> None:
-        torch = _torch()
-        H, G = _heads(node, self.op_type)
+    def _check(self, node):
+        _heads(node, self.op_type)
         if _attr_float(node, "softcap", 0.0) != 0.0:
             raise ModelSharpException("PagedAttention softcap is not supported.")
+
+    def _run(self, node: GraphNode, ctx: GraphContext) -> None:
+        torch = _torch()
+        H, G = _heads(node, self.op_type)
         q = self._dev.input(ctx, node.inputs[0])
         if q.dim() != 2:
             raise ModelSharpException(f"PagedAttention supports only 2-D query [tokens, hidden]; got rank {q.dim()}.")
@@ -153,7 +170,10 @@ class HipQkNormRotaryKernel(_Serving):
     attributes num_heads, kv_num_heads, epsilon, do_rotary (1 unless given), rotary_interleaved."""
     op_type = "QkNormRotary"
 
-    def execute(self, node: GraphNode, ctx: GraphContext) -> None:
+    def _check(self, node):
+        _heads(node, self.op_type)
+
+    def _run(self, node: GraphNode, ctx: GraphContext) -> None:
         torch = _torch()
         H, G = _heads(node, self.op_type)
         q, k = self._dev.input(ctx, node.inputs[0]), self._dev.input(ctx, node.inputs[1])
@@ -222,7 +242,7 @@ class HipLoraMatMulNBitsKernel(_Serving):
             raise ModelSharpException(f"LoraMatMulNBits '{name}' must be a 3-D fp32 or fp16 tensor.")
         return t.contiguous()
 
-    def execute(self, node: GraphNode, ctx: GraphContext) -> None:
+    def _run(self, node: GraphNode, ctx: GraphContext) -> None:
         torch = _torch()
         x = self._dev.input(ctx, node.inputs[0])
         mine = GraphContext({**ctx.values, node.inputs[0]: x}, ctx.constants)

@@ -704,3 +704,134 @@ def test_results_do_not_depend_on_the_hints_within_tolerance_and_repeat_exactly(
         o = torch.full((b.tokens, H * D), float("nan"), device="cuda")
         native.paged_attention(d, *map(ptr, bufs), ptr(o), ptr(ws), n, stream())
         check_attention(host(o), b, q, H)
+
+
+# ---- alignment, offsets, small numbers -----------------------------------------------------------------
+
+def shifted(x):
+    """A device copy that starts 4 bytes into its allocation."""
+    import torch
+    t = torch.empty(x.size + 1, dtype=torch.from_numpy(x).dtype, device="cuda")
+    v = t[1:].view(x.shape)
+    v.copy_(dev(x))
+    return v
+
+
+@pytest.mark.parametrize("news", [[1, 2], [60]], ids=["tokens", "chunk"])
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+def test_rows_aligned_to_four_bytes(gpu, dtype, news):
+    import torch
+    H, G, D = 8, 2, 128
+    pasts = [200] * len(news)
+    b = ref.Batch(81, news, pasts, G, D, 16, dtype)
+    q, k, v = (b.rng.standard_normal((b.tokens, n * D)).astype(F32) for n in (H, G, G))
+    gq, gk = ((b.rng.random(D) + 0.5).astype(F32) for _ in range(2))
+    cos, sin = rotary_caches(300, D // 2)
+    d = desc_of(b, H, eps=1e-6, do_rotary=1, cos_rows=300, cos_cols=D // 2)
+    outs = []
+    for put in (dev, shifted):
+        src = [put(x) for x in (q, k, v, gq, gk)]
+        lens = [dev(x) for x in (b.cu, b.past, b.table)]
+        rot = [put(x) for x in (cos, sin)]
+        o, kc, vc = put(np.zeros_like(q)), dev(b.k), dev(b.v)
+        native.paged_append(d, *map(ptr, src), *map(ptr, lens), *map(ptr, rot), ptr(o), ptr(kc), ptr(vc), stream())
+        n = native.paged_attention_workspace_size(d)
+        ws, out = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda"), put(np.zeros_like(q))
+        native.paged_attention(d, ptr(o), *map(ptr, lens), ptr(kc), ptr(vc), ptr(out), ptr(ws), n, stream())
+        outs.append([host(x) for x in (o, kc, out)])
+    # two orders of the norm's sum of squares: the chunks' queries and keys differ in a few last bits
+    tol = 2 * ref.norm_tolerance(D, gq, 1.5 * np.sqrt(D), True)
+    assert np.abs(outs[0][0] - outs[1][0]).max() <= tol
+    assert (np.abs(outs[0][1].astype(F32) - outs[1][1]) <= tol + np.abs(outs[0][1].astype(F32)) * (2.0 ** -10 if dtype == F16 else 0)).all()
+    for o, kc, out in outs:
+        b.k, b.v = kc, host(vc)
+        check_attention(out, b, o, H)
+
+
+@pytest.mark.parametrize("T", [5, 1040])
+def test_lora_rows_aligned_to_their_type(gpu, T):
+    import torch
+    case = (T, 96, 68, 2, 20, "mixed", True, "new")
+    x, a, b, ranks, scales, which, y0 = lora_inputs(case, F16, 83)
+    want, terms = ref.lora(x, a, b, ranks, scales, which, y0)
+    d = native.LoraDesc(tokens=T, K=96, N=68, adapters=2, max_rank=20, weight_type=native.MS_HIP_DTYPE_F16)
+    n = native.lora_workspace_size(d)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    half = torch.empty(a.size + b.size + 2, dtype=torch.float16, device="cuda")
+    half[1:1 + a.size], half[2 + a.size:] = dev(a).reshape(-1), dev(b).reshape(-1)
+    y = shifted(np.zeros_like(y0))
+    keep = [shifted(v) for v in (x, ranks, scales, which, y0)]
+    native.lora(d, ptr(keep[0]), half.data_ptr() + 2, half.data_ptr() + 2 * (2 + a.size), *map(ptr, keep[1:]), ptr(y), ptr(ws),
+                n, stream())
+    assert (np.abs(host(y) - want) <= ref.lora_tolerance(want, terms, 96, 20)).all()
+
+
+@pytest.mark.parametrize("news", [[1], [40]], ids=["token", "chunk"])
+def test_pages_past_two_to_the_31_elements(gpu, news):
+    """The same pages in a small cache and behind 2^31 elements of a large one: the same bits."""
+    import torch
+    H, G, D, page = 16, 8, 256, 64
+    b = ref.Batch(85, news, [130], G, D, page, F16)
+    far = 2 ** 31 // (page * G * D) + 1          # the first page behind
+    q, k, v = (b.rng.standard_normal((b.tokens, n * D)).astype(F32) for n in (H, G, G))
+    outs = []
+    for shift in (0, far):
+        kc, vc = (torch.zeros(b.num_pages + shift, page, G, D, dtype=torch.float16, device="cuda") for _ in range(2))
+        kc[shift:], vc[shift:] = dev(b.k), dev(b.v)
+        d = desc_of(b, H, eps=1e-6)
+        d.num_pages = b.num_pages + shift
+        lens = [dev(x) for x in (b.cu, b.past, np.where(b.table >= 0, b.table + shift, -1).astype(np.int32))]
+        src, qo = [dev(x) for x in (q, k, v)], torch.zeros(b.tokens, H * D, device="cuda")
+        native.paged_append(d, *map(ptr, src), None, None, *map(ptr, lens), None, None, ptr(qo), ptr(kc), ptr(vc), stream())
+        n = native.paged_attention_workspace_size(d)
+        ws, out = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda"), torch.zeros_like(qo)
+        native.paged_attention(d, ptr(qo), *map(ptr, lens), ptr(kc), ptr(vc), ptr(out), ptr(ws), n, stream())
+        outs.append([host(out), host(kc[shift:]), host(vc[shift:])])
+        del kc, vc
+    for x, y in zip(*outs):
+        assert np.array_equal(x, y)
+    b.k, b.v = outs[0][1:]
+    check_attention(outs[0][0], b, q, H)
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("news", [[2], [66]], ids=["tokens", "chunk"])
+def test_attention_subnormal_fp16_values(gpu, news, where):
+    H, G, D = 4, 2, 128
+    b = ref.Batch(87, news, [77], G, D, 16, F16)
+    x = (b.rng.standard_normal(b.k.shape) * 2e-6).astype(F16)   # most below fp16's smallest normal value
+    if where == "k":
+        b.k = x
+    else:
+        b.v = x
+    q = b.rng.standard_normal((b.tokens, H * D)).astype(F32)
+    scale = 5e4 if where == "k" else 0.0
+    check_attention(run_attention(b, q, H, scale=scale), b, q, H, scale=scale)
+
+
+def test_many_tiles_of_adapters_captured(gpu):
+    import torch
+    case = (1100, 256, 132, 3, 64, "runs", True, "new")
+    x, a, b, ranks, scales, which, y0 = lora_inputs(case, F16, 89)
+    want, terms = ref.lora(x, a, b, ranks, scales, which, y0)
+    d = native.LoraDesc(tokens=1100, K=256, N=132, adapters=3, max_rank=64, weight_type=native.MS_HIP_DTYPE_F16)
+    n = native.lora_workspace_size(d)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    keep = [dev(v) for v in (x, a, b, ranks, scales, which, y0)]
+    y = torch.empty_like(keep[-1])
+    g = torch.cuda.CUDAGraph()
+    call = lambda: native.lora(d, *map(ptr, keep), ptr(y), ptr(ws), n, stream())   # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        call()
+    for replay in range(4):
+        y.fill_(float("nan"))
+        ws.fill_(255)
+        torch.cuda.synchronize()
+        g.replay()
+        got = host(y)
+        assert (np.abs(got - want) <= ref.lora_tolerance(want, terms, 256, 64)).all()
+        y.fill_(float("nan"))
+        call()
+        assert np.array_equal(host(y), got)
