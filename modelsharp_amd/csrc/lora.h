@@ -7,8 +7,14 @@
 // matrix cores of which the class's own columns are kept: no sorting, no copies, and every output
 // has one writer, so that results do not depend on the order of anything.
 //
-//   lora_shrink_kernel   h[split][t] = A_a x[t] over the split's part of K
-//   lora_expand_kernel   y[t] = base[t] + scale[a] (B_a (sum of the splits' h[t]))
+//   lora_shrink_kernel,      h[split][t] = A_a x[t] over the split's part of K, zeros past the
+//   lora_shrink_lds_kernel   adapter's rank (the second one: many tiles)
+//   lora_expand_kernel       y[t] = base[t] + scale[a] (B_a (sum of the splits' h[t]))
+//
+// x and the sums are fp32; beside fp16 weights h is two fp16 halves (22 bits), as they are otherwise.
+// 32 tokens, 16 adapters of rank 16, K = N = 3584: 6.2 and 6.0 us, two launches each of a few round
+// trips to memory. 2048 tokens, rank 64, K = 4096, N = 11008: 19.3 us (1.7 TB/s of x, the fp32 matrix
+// cores busy 40% of the cycles) and 44 us (4.1 TB/s of base and y).
 #pragma once
 #include "mfma_device.h"
 #include "serving.h"
@@ -159,11 +165,11 @@ __global__ __launch_bounds__(64 * WAVES) void lora_shrink_kernel(LoraArgs p, int
     }
 }
 
-// The same for many tiles (one split, a tile's classes one after another): grid tiles * rank groups. A
+// The same for many tiles (one split): grid tiles * rank groups * slots. A
 // wave's steps go straight from memory to its own part of LDS, three under way, and no wave waits
 // for another before the end. The products' operands want 16 rows side by side, and loaded that
 // way every lane touches a line of its own, 64 cycles an instruction: with 2048 tokens, K = 4096
-// and rank 64 those loads alone took 15.6 us of 24. Here 8 (fp16: 4) lanes take a row's part in a
+// and rank 64 that is 15.6 us by count, of the 24 that the launch took. Here 8 (fp16: 4) lanes take a row's part in a
 // line, and the chunks of a row are turned by its number, so that the reads meet no bank twice.
 constexpr int kLoraLdsWaves = 8, kLoraLdsRing = 3;
 template <typename T, int RT>
@@ -171,14 +177,15 @@ constexpr int lora_lds_stage() { return 2048 + RT * 16 * 32 * (int)sizeof(T); } 
 template <typename T, int RT>
 constexpr int lora_lds_bytes() { return kLoraLdsWaves * kLoraLdsRing * lora_lds_stage<T, RT>(); }
 template <typename T, int RT>
-__global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(LoraArgs p)
+__global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(LoraArgs p, int slots)
 {
     constexpr bool F16 = sizeof(T) == 2;
     constexpr int STAGE = lora_lds_stage<T, RT>(), LOADS = 2 + RT * (F16 ? 1 : 2);
     constexpr int AC = F16 ? 4 : 8;   // 16-byte chunks of a row of A's step
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int groups = (p.rank16 + 16 * RT - 1) / (16 * RT);
-    const int r0 = blockIdx.x % groups * (16 * RT), t0 = blockIdx.x / groups * kLoraTokens;
+    const int slot = blockIdx.x % slots, rest = blockIdx.x / slots;
+    const int r0 = rest % groups * (16 * RT), t0 = rest / groups * kLoraTokens;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, grp = lane >> 4, t = t0 + l16;
     const int steps = (p.K + 31) / 32;
@@ -194,9 +201,9 @@ __global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(Lor
 #pragma unroll
     for (int i = 0; i < (F16 ? 1 : 2); ++i) aoff[i] = ((8 * i + arow) * p.K + ak) * (int)sizeof(T);
     LoraClasses cls(lora_adapter(p, t));
-    while (cls.left) {
+    for (int c = 0; cls.left; ++c) {
         const int a = cls.next();
-        if (a < 0) continue;
+        if (c % slots != slot || a < 0) continue;
         const int rank = __builtin_amdgcn_readfirstlane(lora_rank(p, a));
         const T* const A = static_cast<const T*>(p.a) + ((int64_t)a * p.rank + r0) * p.K;
         // (uniform, which the compiler does not see of a value read across lanes in a loop)
@@ -288,7 +295,7 @@ __global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(Lor
 //     each class's tokens, and leaves scale * sum in LDS;
 //   the threads add it to the base and store, whole rows of 1 KB at a time.
 // (A wave's sums lie 16 tokens by 16 outputs: stored from there, every instruction touches 16 lines,
-// and the launch took 65 us in place of @@ at 2048 tokens of N = 11008.)
+// and the launch took 65 us in place of 44 at 2048 tokens of N = 11008.)
 // R ranks at a time, in chunks of C; more come in further passes over the sums in LDS. ONE: h has
 // one split, and the base and h of the next 16 tokens are on their way meanwhile. No load or store of
 // that loop is under a condition, behind which the compiler could only wait for all that is under way:

@@ -40,17 +40,29 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new
 {
     PagedAttnPlan pl;
     const int64_t grp = H / kvH;
-    const bool few = max_new * grp <= kFewRows || !blocks_fit(D, f16);   // as far as is known
+    // Rows of a request up to which tiles of 16 rows take it, though each reads its keys. At 2000 cached
+    // tokens of 28 / 4 heads of 128, fp16: 8 requests of 42 rows 19 us against 24 in tiles of 128, 32 of
+    // 63 46 against 57; 32 of 126 80 against 64. An fp32 cache (32 / 8 heads), whose larger
+    // tiles do six products a pair: 8 of 128 rows 72 against 94, 8 of 192 119 against 116. Where all tiles of
+    // 16 leave CUs idle, further: one request of 126 rows 15.3 against 21.8, of 252 17.2 against 23.5.
+    pl.few_rows = tokens * H <= 4 * (int64_t)cus ? 256 : f16 ? 64 : 128;
+    const bool few = max_new * grp <= pl.few_rows || !blocks_fit(D, f16);   // as far as is known
     const bool one = requests == 1 && !few;
     // tiles at the most, and as many as the bounds make likely
-    const int64_t blocks = few ? 0 : tokens * grp / 128 + std::min<int64_t>(requests, tokens * grp / (kFewRows + 1) + 1);
-    const int64_t rows = one   ? 0
-                         : few ? tokens * grp / 16 + requests
-                               : (int64_t)std::min<int64_t>(requests, tokens) * ((kFewRows + 15) / 16);
+    const int64_t blocks =
+        few ? 0 : tokens * grp / 128 + std::min<int64_t>(requests, tokens * grp / (pl.few_rows + 1) + 1);
+    const int64_t rows16 = tokens * grp / 16 + requests;
+    const int64_t rows = one ? 0 : few ? rows16 : std::min<int64_t>(rows16, (int64_t)requests * (pl.few_rows / 16));
     const int64_t likely = few ? std::max<int64_t>(1, std::min(rows, (max_new * grp + 15) / 16 * requests))
                                : tokens * grp / 128 + 1 + (one ? 0 : std::min<int64_t>(requests, tokens));
-    int64_t splits = std::max<int64_t>(1, 2 * (int64_t)cus / (likely * kvH));
-    splits = std::min<int64_t>({splits, std::max<int64_t>(1, keys / (few ? 128 : 256)), 64});
+    // Two workgroups to a CU, and as many splits of a tile's keys as pay for their join: of 32 KB of keys
+    // up to 16, more only of 128 KB. One token of 28 / 4 heads of 128, fp16: 1000 cached ones in 7 splits
+    // 10.8 us, in 3 12.1; 8000 in 16 13.0, in 31 13.6, in 62 15.8. fp32 (8 kv heads): 1000 in 15 12.5, in 7
+    // 13.3; 4000 in 15 18.2, in 62 22.8; 64 tokens after 500 (96 channels) in 8 19.3, in 2 32.5. Up to 128 KB
+    // a tile of 16 rows keeps its keys together, without the merge: 500 in one 9.8, in 3 10.8.
+    const int64_t bytes = keys * D * (f16 ? 2 : 4);
+    const int64_t most = few && bytes <= (128 << 10) ? 1 : std::max(std::min<int64_t>(bytes >> 15, 16), bytes >> 17);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)cus / (likely * kvH), most, 64}));
     const int64_t ws = splits > 1 ? splits * tokens * H * (D + 2) * (int64_t)sizeof(float) : 0;
     if (ws_avail >= 0 && ws > ws_avail) splits = 1;
     pl.splits = (int)splits;
@@ -93,6 +105,7 @@ hipError_t launch_paged_attention(const PagedAttnArgs& args, const PagedAttnPlan
 {
     PagedAttnArgs p = args;
     p.blocks_grid = (int)plan.blocks_grid;
+    p.few_rows = plan.few_rows;
     const bool whole = p.b.page.div % 16 == 0;
     const auto launch = p.f16 ? (whole ? launch_paged<_Float16, true> : launch_paged<_Float16, false>)
                               : (whole ? launch_paged<float, true> : launch_paged<float, false>);
@@ -110,16 +123,21 @@ LoraPlan lora_plan(int T, int K, int N, int adapters, int rank, int cus)
 {
     LoraPlan pl;
     const int tiles = (T + kLoraTokens - 1) / kLoraTokens;
-    // Many tiles: a tile's classes one after another, one workgroup of 16 waves for all of K, and as many
-    // tiles of tokens to an expand workgroup, which keeps B in registers across them, as leave two
-    // workgroups to a CU.
-    pl.many = tiles >= cus / 4;
+    // Many tiles: all of K in one workgroup, a tile's classes over workgroups only where CUs would be idle,
+    // and as many tiles of tokens to an expand workgroup, which keeps B in registers across them, as leave
+    // two workgroups to a CU. K = N = 4096, us, the other way first: 4 adapters of rank 64, 128 tokens 16.6
+    // against 20.6, 160 21.3 against 22.1, 256 22.0 against 21.3, 512 40 against 24.5; 16 of rank 16, a token each
+    // its own, 128 tokens 22.3 against 21.6, 160 27.4 against 22.1, 512 65 against 36.
+    pl.many = tiles > cus / 32;
     if (pl.many) {
         const int nb = (N + kLoraRows - 1) / kLoraRows;
         while (pl.subs < tiles && (int64_t)((tiles + pl.subs - 1) / pl.subs) * nb > 2 * cus) ++pl.subs;
+        const int groups = (rank + 31) / 32;
+        pl.shrink_slots = std::max(1, std::min({kLoraTokens, adapters, cus / (tiles * groups)}));
     } else {   // few: the classes side by side, and K over workgroups
         pl.slots = std::max(1, std::min({kLoraTokens, adapters + 1, 2 * cus / tiles}));
         pl.splits = std::max(1, std::min({2 * cus / (tiles * pl.slots), (K + 255) / 256, 16}));
+        pl.shrink_slots = pl.slots;
     }
     pl.ws_bytes = (int64_t)pl.splits * T * ((rank + 15) / 16 * 16) * (int64_t)sizeof(float);
     return pl;
@@ -138,8 +156,8 @@ template <typename T, int RT, int WAVES, bool VEC>
 void launch_shrink(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     const int groups = (p.rank16 + 16 * RT - 1) / (16 * RT);
-    const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * groups * plan.slots * plan.splits);
-    hipLaunchKernelGGL((lora_shrink_kernel<T, RT, WAVES, VEC>), grid, dim3(64 * WAVES), 0, s, p, plan.slots);
+    const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * groups * plan.shrink_slots * plan.splits);
+    hipLaunchKernelGGL((lora_shrink_kernel<T, RT, WAVES, VEC>), grid, dim3(64 * WAVES), 0, s, p, plan.shrink_slots);
 }
 
 template <typename T, int C, int CH, bool VEC>
@@ -157,8 +175,8 @@ hipError_t launch_lora_c(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
         if (lds > 64 * 1024)
             if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, lds))
                 return e;
-        const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * ((p.rank16 + 16 * RT - 1) / (16 * RT)));
-        hipLaunchKernelGGL(fn, grid, dim3(64 * kLoraLdsWaves), lds, s, p);
+        const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * ((p.rank16 + 16 * RT - 1) / (16 * RT)) * plan.shrink_slots);
+        hipLaunchKernelGGL(fn, grid, dim3(64 * kLoraLdsWaves), lds, s, p, plan.shrink_slots);
     } else {
         launch_shrink<T, RT, 16, VEC>(p, plan, s);
     }

@@ -224,6 +224,12 @@ constexpr int paged_ring(int DP, bool f16) { return f16 ? 2 : (DP <= 64 ? 3 : DP
 // as two halves; an fp32 cache is multiplied in fp32.
 // WHOLE: pages of a multiple of 16 rows, so that a step lies in one page: one lookup a step, and a
 // page that is not there is a step left out.
+//
+// The cache's bytes bound it (16 keys of fp16, D = 128: 8 KB against 384 cycles of the matrix cores).
+// 32 tokens over 1000-4000 keys of 4 heads of 128 in fp16, 171 MB: 42.7 us (4.0 TB/s), and 4.7 of merge;
+// 8 over 2000-8000 of 8 heads in fp32, 340 MB: 68 us (5.0 TB/s) and 4.6. Between the two 169 MB cost
+// 26 us: what does not grow with the keys is the larger part of a call of a few of them (the chain cu,
+// past -> table -> keys, the join in LDS, the merge's launch).
 constexpr int kRowsLds = 4 * 4 * kWave * 16 + 2 * 4 * 16 * 4 + 16;
 template <typename T, int DP, bool WHOLE>
 __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int rows_max, uint8_t* lds)
@@ -569,6 +575,7 @@ template <> struct PagedSplit<_Float16> {
 //   fp32 cache: everything is three bf16 parts, x = x0 + x1 + x2 exactly (cut, not rounded: 8 bits
 //   each, and bf16 has fp32's range, so that any finite value fits), and the products of a pair
 //   whose terms are 2^-16 or more of the whole: six of nine, what is left out is below 2^-22.
+//   (The matrix cores take bf16 below 2^-126 as zero: values below 2^-110 keep fewer bits.)
 template <> struct PagedSplit<float> {
     static constexpr int kPlanes = 3, kParts = 3;
     static constexpr int kProducts = 6;
@@ -625,6 +632,13 @@ __device__ __forceinline__ int v_turn(int row)
 // leave their lane and a row's statistics are its lane's own; V^T comes from ds_read_b64_tr_b16, which
 // hands 16 lanes four keys of one channel each. The online softmax runs in base 2 and moves
 // its maximum only in steps above 2^4, so that the accumulators are seldom rescaled.
+//
+// 128 rows, since two such workgroups fill a CU's LDS (64 KB each at D = 128: two blocks of 64 keys) and
+// registers, and each block of keys is then read from L2 once for 128 rows. The matrix cores bound a
+// long chunk: 512 tokens of 28 / 4 heads over 16000 keys take 236-241 us with the merge, 500 TFLOP/s of
+// attention and twice that of products (a library product of 8192 reaches 1063). Fresh prompts of 200-650
+// tokens (44 us for five) are bound by the longest tile's chain of blocks. An fp32 cache, with six
+// products a pair: two chunks of 300 tokens of 32 / 8 heads of 96, 1024 keys visible: 62 + 9 us.
 // WHOLE: pages of a multiple of 16 rows, so that a wave's rows of a load lie in one page: its lookups
 // are the scalar unit's.
 template <typename T, int DP>
@@ -917,10 +931,9 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
 }
 
 // A launch's workgroups: the first p.blocks_grid take tiles of 128 rows of the requests of more than
-// kFewRows rows (the longest work first), the others tiles of 16 rows of the rest, beside them:
+// p.few_rows rows (the longest work first), the others tiles of 16 rows of the rest, beside them:
 // one is bound by the matrix cores, the other by memory. Without the one or the other kind the
 // kind that is there takes every request.
-constexpr int kFewRows = 32;
 enum PagedMode { kPagedRows, kPagedBlocks, kPagedBoth };
 template <typename T, int DP, bool WHOLE, PagedMode MODE>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_attention_kernel(PagedAttnArgs p)
@@ -934,9 +947,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_attention_kernel
         paged_blocks<T, DP, WHOLE>(p, blockIdx.x, 0, lds);
     } else {
         if ((int)blockIdx.x < p.blocks_grid)
-            paged_blocks<T, DP, WHOLE>(p, blockIdx.x, kFewRows + 1, lds);
+            paged_blocks<T, DP, WHOLE>(p, blockIdx.x, p.few_rows + 1, lds);
         else
-            paged_rows<T, DPR, WHOLE>(p, blockIdx.x - p.blocks_grid, kFewRows, lds);
+            paged_rows<T, DPR, WHOLE>(p, blockIdx.x - p.blocks_grid, p.few_rows, lds);
     }
 }
 

@@ -110,12 +110,13 @@ struct PagedAttnArgs {
     int H, kvH, D, window, f16, splits;
     int split_min;    // keys of a split at the least
     int blocks_grid;  // workgroups of paged_blocks()
+    int few_rows;     // rows of a request that paged_rows() takes where both kinds are launched
     int64_t q_stride;
     FastDiv grp;      // query heads per kv head
     float scale2;     // scale * log2(e)
 };
 struct PagedAttnPlan {
-    int splits = 1, split_min = 0;
+    int splits = 1, split_min = 0, few_rows = 0;
     int64_t rows_grid = 0, blocks_grid = 0;   // 0: that kernel is not launched
     int64_t ws_bytes = 0;
 };
@@ -136,7 +137,9 @@ struct LoraArgs {
     int T, K, N, adapters, rank, rank16, f16, splits, vec;
 };
 struct LoraPlan {
-    int splits = 1, slots = 1, subs = 1;   // subs: tiles of tokens to an expand workgroup
+    int splits = 1;
+    int slots = 1, shrink_slots = 1;   // workgroups that share out a tile's classes
+    int subs = 1;                      // tiles of tokens to an expand workgroup
     bool many = false;
     int64_t ws_bytes = 0;
 };

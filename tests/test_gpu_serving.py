@@ -835,3 +835,61 @@ def test_many_tiles_of_adapters_captured(gpu):
         y.fill_(float("nan"))
         call()
         assert np.array_equal(host(y), got)
+
+
+# Around the borders of the launch rules: rows of a request in tiles of 16 or of 128, keys kept together or
+# split.
+BORDERS = [
+    ([9, 10, 18, 19], [300, 40, 0, 700], 28, 4, 128, 16, -1),   # 63 to 133 rows
+    ([1, 9], [600, 500], 28, 4, 128, 16, -1),
+    ([36], [513], 28, 4, 128, 16, -1),                  # 252 rows, few tokens: tiles of 16
+    ([37], [513], 28, 4, 128, 24, -1),
+    ([128], [30], 8, 1, 64, 16, -1),                    # 1024 rows of few tokens
+    ([30, 2, 96], [100, 5, 0], 8, 1, 64, 10, -1),       # 240, 16 and 768 of them
+    ([1], [511], 4, 4, 128, 16, -1),
+    ([1], [512], 4, 4, 128, 16, -1),
+    ([1, 0, 1], [0, 9000, 9000], 2, 1, 64, 64, -1),     # a request of one key beside one of many splits
+    ([16, 17], [800, 20], 32, 8, 128, 32, -1),
+    ([32, 33, 1], [50, 400, 3], 32, 8, 96, 16, -1),     # 128 and 132 rows
+    ([48, 1], [2000, 2000], 8, 1, 96, 10, 700),
+]
+
+
+@pytest.mark.parametrize("hints", [True, False], ids=["bounds", "no-bounds"])
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("case", range(len(BORDERS)))
+def test_paged_attention_around_the_launch_rules(gpu, case, dtype, hints):
+    news, pasts, H, G, D, page, window = BORDERS[case]
+    log(f"attention {BORDERS[case]} {dtype.__name__} bounds={hints}")
+    b = ref.Batch(2000 + case, news, pasts, G, D, page, dtype, spare_rows=case % 2)
+    q = b.rng.standard_normal((b.tokens, H * D)).astype(F32) * F32(1.5)
+    check_attention(run_attention(b, q, H, window, hints=hints), b, q, H, window)
+
+
+def test_bounds_that_are_too_small_cost_no_result(gpu):
+    """max_new and max_total choose the launch only."""
+    import torch
+    b = ref.Batch(91, [1, 150, 9], [700, 20, 300], 2, 64, 16, F16)
+    q = b.rng.standard_normal((b.tokens, 8 * 64)).astype(F32)
+    for new, total in [(1, 1), (1, 10 ** 6), (200, 8), (2 ** 31 - 1, 2 ** 31 - 1)]:
+        d = desc_of(b, 8, max_new=new, max_total=total)
+        n = native.paged_attention_workspace_size(d)
+        ws = torch.full((n // 4 + 64,), float("nan"), device="cuda")
+        o = torch.full((b.tokens, 8 * 64), float("nan"), device="cuda")
+        bufs = [dev(x) for x in (q, b.cu, b.past, b.table, b.k, b.v)]
+        native.paged_attention(d, *map(ptr, bufs), ptr(o), ptr(ws), n, stream())
+        check_attention(host(o), b, q, 8)
+        assert torch.isnan(ws[n // 4:]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("case", [
+    (128, 256, 264, 20, 16, "each", True, "new"),        # the last of few tiles
+    (129, 256, 264, 20, 16, "each", True, "new"),        # classes over workgroups
+    (144, 520, 300, 16, 16, "each", True, "same"),
+    (160, 264, 264, 5, 64, "mixed", True, "new"),
+    (400, 96, 72, 30, 130, "each", True, None),
+    (513, 100, 52, 20, 20, "each", True, "new"),
+], ids=lambda c: "-".join(map(str, c)))
+def test_lora_around_the_launch_rules(gpu, case, dtype):
+    test_lora(gpu, case, dtype)
