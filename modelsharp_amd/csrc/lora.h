@@ -165,7 +165,7 @@ __global__ __launch_bounds__(64 * WAVES) void lora_shrink_kernel(LoraArgs p, int
     }
 }
 
-// The same for many tiles (one split): grid tiles * rank groups * slots. A
+// The same for many tiles: grid tiles * rank groups * slots * splits. A
 // wave's steps go straight from memory to its own part of LDS, three under way, and no wave waits
 // for another before the end. The products' operands want 16 rows side by side, and loaded that
 // way every lane touches a line of its own, 64 cycles an instruction: with 2048 tokens, K = 4096
@@ -184,11 +184,12 @@ __global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(Lor
     constexpr int AC = F16 ? 4 : 8;   // 16-byte chunks of a row of A's step
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int groups = (p.rank16 + 16 * RT - 1) / (16 * RT);
-    const int slot = blockIdx.x % slots, rest = blockIdx.x / slots;
-    const int r0 = rest % groups * (16 * RT), t0 = rest / groups * kLoraTokens;
+    const int sp = blockIdx.x % p.splits, rest = blockIdx.x / p.splits, slot = rest % slots;
+    const int r0 = rest / slots % groups * (16 * RT), t0 = rest / slots / groups * kLoraTokens;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, grp = lane >> 4, t = t0 + l16;
-    const int steps = (p.K + 31) / 32;
+    const int all = (p.K + 31) / 32, per = (all + p.splits - 1) / p.splits;
+    const int first = sp * per, steps = min(all, first + per);
     uint8_t* const mine = lds + wave * kLoraLdsRing * STAGE;
     const uint32_t base = lds_address(mine);
     // what is past the last token, the adapter's rank or K reads as zero
@@ -259,8 +260,8 @@ __global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(Lor
         };
         if (r0 < rank) {
 #pragma unroll
-            for (int n = 0; n + 1 < kLoraLdsRing; ++n) issue(wave + kLoraLdsWaves * n, n);
-            for (int s = wave, slot = 0; s < steps; s += kLoraLdsWaves) {
+            for (int n = 0; n + 1 < kLoraLdsRing; ++n) issue(first + wave + kLoraLdsWaves * n, n);
+            for (int s = first + wave, slot = 0; s < steps; s += kLoraLdsWaves) {
                 const int free_slot = slot == 0 ? kLoraLdsRing - 1 : slot - 1;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // that slot's reads are done
                 issue(s + kLoraLdsWaves * (kLoraLdsRing - 1), free_slot);
@@ -282,7 +283,8 @@ __global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(Lor
             const int r = r0 + 16 * wave + 4 * grp;
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = r + i < rank ? v[i] : 0.0f;
-            if (cls.mine == a && r < p.rank16) *reinterpret_cast<floatx4_t*>(p.h + (int64_t)t * p.rank16 + r) = v;
+            if (cls.mine == a && r < p.rank16)
+                *reinterpret_cast<floatx4_t*>(p.h + ((int64_t)sp * p.T + t) * p.rank16 + r) = v;
         }
         __syncthreads();
     }
@@ -299,9 +301,11 @@ __global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(Lor
 // R ranks at a time, in chunks of C; more come in further passes over the sums in LDS. ONE: h has
 // one split, and the base and h of the next 16 tokens are on their way meanwhile. No load or store of
 // that loop is under a condition, behind which the compiler could only wait for all that is under way:
-// what is not wanted goes to an offset that the buffer does not have.
+// what is not wanted goes to an offset that the buffer does not have. VEC: B's ranks are read by
+// fours or eights, base and y by fours; 0: value by value. (64 tokens of rank 64: eights 25.1 us, fours
+// 28.1; 40 of rank 20: fours 12.7, value by value 29.9.)
 // Memory bounds it: base and y once, 8 bytes an output against 2 ranks flops.
-template <typename T, int C, int CH, bool ONE, bool VEC>
+template <typename T, int C, int CH, bool ONE, int VEC>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots, int subs)
 {
     constexpr bool F16 = sizeof(T) == 2;
@@ -332,7 +336,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots,
 #pragma unroll
         for (int i = 0; i < 4; ++i) {   // token 4 wave + i, outputs 4 lane ..
             const int t = min(t0 + 4 * wave + i, p.T - 1), n = n0 + 4 * lane;
-            x.base[i] = p.base ? lora_load<4, VEC>(p.base, (int64_t)t * p.N + n, p.N - n) : floatx4_t{};
+            x.base[i] = p.base ? lora_load<4, (VEC > 0)>(p.base, (int64_t)t * p.N + n, p.N - n) : floatx4_t{};
         }
         if constexpr (ONE)
             x.h = *reinterpret_cast<const floatx4_t*>(p.h + (int64_t)min(t0 + min(ht, 15), p.T - 1) * p.rank16 +
@@ -415,7 +419,13 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots,
 #pragma unroll
                         for (int nt = 0; nt < 4; ++nt) {
                             const int n = min(n0 + 64 * wave + 16 * nt + l16, p.N - 1), r = r0 + C * q + E * grp;
-                            bv[q][nt] = lora_load<E, VEC>(B, (int64_t)n * p.rank + r, p.rank - r);
+                            const int64_t at = (int64_t)n * p.rank + r;
+                            if constexpr (E == 8 && VEC == 4)
+                                bv[q][nt] = __builtin_shufflevector(lora_load<4, true>(B, at, p.rank - r),
+                                                                    lora_load<4, true>(B, at + 4, p.rank - r - 4), 0, 1, 2,
+                                                                    3, 4, 5, 6, 7);
+                            else
+                                bv[q][nt] = lora_load<E, (VEC > 0)>(B, at, p.rank - r);
                         }
                     if (rank < r0 + R)   // columns past the adapter's own rank are not its values
 #pragma unroll
@@ -464,7 +474,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots,
             const floatx4_t sum = *reinterpret_cast<const floatx4_t*>(yl + tok * YS + 4 * lane);
             const floatx4_t y = adds >> tok & 1 ? now.base[i] + sum : now.base[i];
             const bool mine = done >> tok & 1;
-            if constexpr (VEC) {
+            if constexpr (VEC > 0) {
                 const int off = mine && n < p.N ? (int)((uint32_t)(tok * p.N + n) * 4u) : kOOB;
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, y), rows, off, 0, 0);
             } else if (mine) {

@@ -3495,9 +3495,10 @@ int ms_hip_lora(const ms_hip_lora_desc* d, const float* dX, const void* dA, cons
     p.rank16 = (d->max_rank + 15) / 16 * 16;
     p.f16 = f16;
     p.splits = plan.splits;
-    p.vec = p.N <= (1 << 24) && p.K <= (1 << 22) && (p.K & 7) == 0 && (p.N & 3) == 0 && (p.rank & (p.rank > 16 ? 7 : 3)) == 0;
-    for (const void* x : {(const void*)dX, dA, dB, (const void*)dBase, (const void*)dY})
-        if (misaligned16(x)) p.vec = 0;
+    p.vec_x = p.K <= (1 << 22) && (p.K & 7) == 0 && !misaligned16(dX) && !misaligned16(dA);
+    const bool whole = p.N <= (1 << 24) && (p.N & 3) == 0 && (p.rank & 3) == 0 && !misaligned16(dB) &&
+                       !misaligned16(dBase) && !misaligned16(dY);
+    p.vec_y = !whole ? 0 : p.rank & 7 ? 4 : 8;
     const int64_t f = sizeof(float), yb = (int64_t)p.T * p.N * f, xb = (int64_t)p.T * p.K * f, e = f16 ? 2 : 4;
     const int64_t ab = (int64_t)p.adapters * p.rank * p.K * e, bb = (int64_t)p.adapters * p.rank * p.N * e;
     if (overlap(dY, yb, dX, xb) || overlap(dY, yb, dA, ab) || overlap(dY, yb, dB, bb) ||

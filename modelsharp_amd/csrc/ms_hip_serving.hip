@@ -123,17 +123,19 @@ LoraPlan lora_plan(int T, int K, int N, int adapters, int rank, int cus)
 {
     LoraPlan pl;
     const int tiles = (T + kLoraTokens - 1) / kLoraTokens;
-    // Many tiles: all of K in one workgroup, a tile's classes over workgroups only where CUs would be idle,
-    // and as many tiles of tokens to an expand workgroup, which keeps B in registers across them, as leave
-    // two workgroups to a CU. K = N = 4096, us, the other way first: 4 adapters of rank 64, 128 tokens 16.6
-    // against 20.6, 160 21.3 against 22.1, 256 22.0 against 21.3, 512 40 against 24.5; 16 of rank 16, a token each
-    // its own, 128 tokens 22.3 against 21.6, 160 27.4 against 22.1, 512 65 against 36.
+    // Many tiles: x and A through LDS, a tile's classes and then K over workgroups only as long as CUs
+    // would be idle, and as many tiles of tokens to an expand workgroup, which keeps B in registers across
+    // them, as leave two workgroups to a CU. us, the other way first: K = N = 4096, 3 adapters of rank 16,
+    // 200 tokens 14.4 against 11.3, 512 20.1 against 14.0, 1024 33 against 22; 16 of rank 16, a token each its
+    // own, 64 tokens 15.7 against 18.0, 128 22.4 against 19.2, 512 65 against 36; 8 of rank 64 likewise, 64
+    // 21.7 against 24.5, 128 28.9 against 32.2, 200 38 against 44.
     pl.many = tiles > cus / 32;
     if (pl.many) {
         const int nb = (N + kLoraRows - 1) / kLoraRows;
         while (pl.subs < tiles && (int64_t)((tiles + pl.subs - 1) / pl.subs) * nb > 2 * cus) ++pl.subs;
         const int groups = (rank + 31) / 32;
         pl.shrink_slots = std::max(1, std::min({kLoraTokens, adapters, cus / (tiles * groups)}));
+        pl.splits = std::max(1, std::min({cus / (tiles * groups * pl.shrink_slots), (K + 511) / 512, 16}));
     } else {   // few: the classes side by side, and K over workgroups
         pl.slots = std::max(1, std::min({kLoraTokens, adapters + 1, 2 * cus / tiles}));
         pl.splits = std::max(1, std::min({2 * cus / (tiles * pl.slots), (K + 255) / 256, 16}));
@@ -144,12 +146,15 @@ LoraPlan lora_plan(int T, int K, int N, int adapters, int rank, int cus)
 }
 
 namespace {
-template <typename T, int C, int CH, bool ONE, bool VEC>
+template <typename T, int C, int CH, bool ONE>
 void launch_expand(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     const int tokens = kLoraTokens * plan.subs;
     const dim3 grid((p.T + tokens - 1) / tokens * plan.slots * ((p.N + kLoraRows - 1) / kLoraRows));
-    hipLaunchKernelGGL((lora_expand_kernel<T, C, CH, ONE, VEC>), grid, dim3(256), 0, s, p, plan.slots, plan.subs);
+    const auto fn = !p.vec_y                  ? lora_expand_kernel<T, C, CH, ONE, 0>
+                    : C == 16 || p.vec_y == 4 ? lora_expand_kernel<T, C, CH, ONE, 4>
+                                              : lora_expand_kernel<T, C, CH, ONE, C == 16 ? 4 : 8>;
+    hipLaunchKernelGGL(fn, grid, dim3(256), 0, s, p, plan.slots, plan.subs);
 }
 
 template <typename T, int RT, int WAVES, bool VEC>
@@ -160,45 +165,51 @@ void launch_shrink(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
     hipLaunchKernelGGL((lora_shrink_kernel<T, RT, WAVES, VEC>), grid, dim3(64 * WAVES), 0, s, p, plan.shrink_slots);
 }
 
-template <typename T, int C, int CH, bool VEC>
+template <typename T, int RT>
+hipError_t launch_shrink_lds(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
+{
+    constexpr int lds = lora_lds_bytes<T, RT>();
+    const auto fn = lora_shrink_lds_kernel<T, RT>;
+    if (lds > 64 * 1024)
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds))
+            return e;
+    const int groups = (p.rank16 + 16 * RT - 1) / (16 * RT);
+    const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * groups * plan.shrink_slots * plan.splits);
+    hipLaunchKernelGGL(fn, grid, dim3(64 * kLoraLdsWaves), lds, s, p, plan.shrink_slots);
+    return hipSuccess;
+}
+
+template <typename T, int C, int CH>
 hipError_t launch_lora_c(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
     constexpr int RT = C / 16;
     if (!plan.many) {
-        launch_shrink<T, RT * CH, 4, VEC>(p, plan, s);
-        launch_expand<T, C, CH, false, VEC>(p, plan, s);
+        (p.vec_x ? launch_shrink<T, RT * CH, 4, true> : launch_shrink<T, RT * CH, 4, false>)(p, plan, s);
+        launch_expand<T, C, CH, false>(p, plan, s);
         return hipGetLastError();
     }
-    if constexpr (VEC) {
-        constexpr int lds = lora_lds_bytes<T, RT>();
-        const auto fn = lora_shrink_lds_kernel<T, RT>;
-        if (lds > 64 * 1024)
-            if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, lds))
-                return e;
-        const dim3 grid((p.T + kLoraTokens - 1) / kLoraTokens * ((p.rank16 + 16 * RT - 1) / (16 * RT)) * plan.shrink_slots);
-        hipLaunchKernelGGL(fn, grid, dim3(64 * kLoraLdsWaves), lds, s, p, plan.shrink_slots);
-    } else {
-        launch_shrink<T, RT, 16, VEC>(p, plan, s);
-    }
-    launch_expand<T, C, CH, true, VEC>(p, plan, s);
+    if (!p.vec_x)
+        launch_shrink<T, RT, 16, false>(p, plan, s);
+    else if (hipError_t e = launch_shrink_lds<T, RT>(p, plan, s))
+        return e;
+    (plan.splits == 1 ? launch_expand<T, C, CH, true> : launch_expand<T, C, CH, false>)(p, plan, s);
     return hipGetLastError();
 }
 
-template <typename T, bool VEC>
+template <typename T>
 hipError_t launch_lora_t(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
-    const auto launch = p.rank16 == 16   ? launch_lora_c<T, 16, 1, VEC>
-                        : p.rank16 == 32 ? launch_lora_c<T, 32, 1, VEC>
-                                         : launch_lora_c<T, 32, 2, VEC>;
+    const auto launch = p.rank16 == 16   ? launch_lora_c<T, 16, 1>
+                        : p.rank16 == 32 ? launch_lora_c<T, 32, 1>
+                                         : launch_lora_c<T, 32, 2>;
     return launch(p, plan, s);
 }
 }  // namespace
 
 hipError_t launch_lora(const LoraArgs& p, const LoraPlan& plan, hipStream_t s)
 {
-    const auto launch = p.f16 ? (p.vec ? launch_lora_t<_Float16, true> : launch_lora_t<_Float16, false>)
-                              : (p.vec ? launch_lora_t<float, true> : launch_lora_t<float, false>);
-    return launch(p, plan, s);
+    return p.f16 ? launch_lora_t<_Float16>(p, plan, s) : launch_lora_t<float>(p, plan, s);
 }
 
 }  // namespace msnb

@@ -134,7 +134,8 @@ struct LoraArgs {
     const float* base;        // [T, N], or null: zero
     float* y;                 // [T, N]
     float* h;                 // [splits][T][rank16]
-    int T, K, N, adapters, rank, rank16, f16, splits, vec;
+    int T, K, N, adapters, rank, rank16, f16, splits;
+    int vec_x, vec_y;         // whole chunks of x and A; of B, base and y (fours, or eights of B)
 };
 struct LoraPlan {
     int splits = 1;

@@ -893,3 +893,17 @@ def test_bounds_that_are_too_small_cost_no_result(gpu):
 ], ids=lambda c: "-".join(map(str, c)))
 def test_lora_around_the_launch_rules(gpu, case, dtype):
     test_lora(gpu, case, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("case", [
+    (40, 264, 132, 5, 20, "mixed", True, "new"),         # ranks of whole fours
+    (40, 100, 132, 5, 20, "mixed", True, "same"),        # x in single values, y in chunks
+    (40, 264, 131, 5, 20, "mixed", True, "new"),         # and the other way
+    (40, 264, 132, 5, 19, "mixed", True, "new"),
+    (640, 264, 132, 5, 100, "runs", True, "new"),
+    (640, 100, 132, 5, 36, "mixed", True, "new"),
+    (640, 264, 130, 5, 4, "mixed", True, None),
+], ids=lambda c: "-".join(map(str, c)))
+def test_lora_in_whole_chunks_on_either_side(gpu, case, dtype):
+    test_lora(gpu, case, dtype)
