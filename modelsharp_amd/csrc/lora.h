@@ -12,8 +12,8 @@
 //   lora_expand_kernel       y[t] = base[t] + scale[a] (B_a (sum of the splits' h[t]))
 //
 // x and the sums are fp32; beside fp16 weights h is two fp16 halves (22 bits), as they are otherwise.
-// 32 tokens, 16 adapters of rank 16, K = N = 3584: 6.2 and 6.0 us, two launches each of a few round
-// trips to memory. 2048 tokens, rank 64, K = 4096, N = 11008: 19.3 us (1.7 TB/s of x, the fp32 matrix
+// 32 tokens, 16 adapters of rank 16, K = N = 3584: 6.0 and 5.9 us, two launches each of a few round
+// trips to memory. 2048 tokens, rank 64, K = 4096, N = 11008: 19.5 us (1.7 TB/s of x, the fp32 matrix
 // cores busy 40% of the cycles) and 44 us (4.1 TB/s of base and y).
 #pragma once
 #include "mfma_device.h"
