@@ -49,6 +49,9 @@ class _Serving(IKernel):
         t = ctx.get_tensor(node.inputs[0])
         if isinstance(t, np.ndarray):
             self._run(node, ctx)
+        elif t.device.type != "cuda":
+            raise ModelSharpException(f"{self.op_type} '{node.inputs[0]}' is a tensor on {t.device}; expected a host "
+                                      "array or a device tensor.")
         else:
             with _torch().cuda.device(t.device):
                 self._run(node, ctx)
@@ -56,20 +59,24 @@ class _Serving(IKernel):
     def _check(self, node):
         """What the attributes alone decide."""
 
-    def _gamma(self, ctx, name, D):
+    def _input(self, ctx, name, device):
+        """A further fp32 input, on the first one's device wherever it lies."""
+        return self._dev.input(ctx, name).to(device)
+
+    def _gamma(self, ctx, name, D, device):
         if not name:
             return None
-        g = self._dev.input(ctx, name)
+        g = self._input(ctx, name, device)
         if g.numel() != D:
             raise ModelSharpException(f"{self.op_type} norm weight has {g.numel()} elements; expected head_dim={D}.")
         return g.reshape(-1)
 
-    def _rotary(self, node, ctx, i):
+    def _rotary(self, node, ctx, i, device):
         """The cos and sin caches at inputs i and i + 1."""
         if not _optional(node, i) or not _optional(node, i + 1):
             raise ModelSharpException(f"{self.op_type} do_rotary=1 requires cos_cache (input {i}) and sin_cache "
                                       f"(input {i + 1}).")
-        cos, sin = self._dev.input(ctx, node.inputs[i]), self._dev.input(ctx, node.inputs[i + 1])
+        cos, sin = (self._input(ctx, node.inputs[j], device) for j in (i, i + 1))
         if cos.dim() != 2 or cos.shape != sin.shape:
             raise ModelSharpException(f"{self.op_type} cos_cache and sin_cache must be equal 2-D shapes.")
         return cos, sin
@@ -139,15 +146,15 @@ class HipPagedAttentionKernel(_Serving):
             d.q_stride = d.k_stride = d.v_stride = hidden
             pq, pk, pv = q.data_ptr(), q.data_ptr() + 4 * H * D, q.data_ptr() + 4 * (H + G) * D
         else:
-            k, v = self._dev.input(ctx, node.inputs[1]), self._dev.input(ctx, node.inputs[2])
+            k, v = (self._input(ctx, node.inputs[i], q.device) for i in (1, 2))
             if tuple(k.shape) != (T, G * D) or tuple(v.shape) != (T, G * D):
                 raise ModelSharpException(f"PagedAttention key and value must be [{T}, {G * D}].")
             pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
         cos = sin = None
         if d.do_rotary:
-            cos, sin = self._rotary(node, ctx, 8)
+            cos, sin = self._rotary(node, ctx, 8, q.device)
             d.cos_rows, d.cos_cols = int(cos.shape[0]), int(cos.shape[1])
-        gq, gk = (self._gamma(ctx, _optional(node, i), D) for i in (10, 11))
+        gq, gk = (self._gamma(ctx, _optional(node, i), D, q.device) for i in (10, 11))
         turned = torch.empty((T, H * D), dtype=torch.float32, device=q.device)
         out = torch.zeros_like(turned)
         st = _stream(q)
@@ -176,7 +183,8 @@ class HipQkNormRotaryKernel(_Serving):
     def _run(self, node: GraphNode, ctx: GraphContext) -> None:
         torch = _torch()
         H, G = _heads(node, self.op_type)
-        q, k = self._dev.input(ctx, node.inputs[0]), self._dev.input(ctx, node.inputs[1])
+        q = self._dev.input(ctx, node.inputs[0])
+        k = self._input(ctx, node.inputs[1], q.device)
         T = int(np.prod(q.shape[:-1]))
         D = int(q.shape[-1]) // H
         if int(q.shape[-1]) != H * D or tuple(k.shape) != tuple(q.shape[:-1]) + (G * D,):
@@ -189,9 +197,9 @@ class HipQkNormRotaryKernel(_Serving):
             if not _optional(node, 4):
                 raise ModelSharpException("QkNormRotary do_rotary=1 requires position_ids (input 4).")
             pos = self._lengths(ctx, node.inputs[4], T, q.device)
-            cos, sin = self._rotary(node, ctx, 5)
+            cos, sin = self._rotary(node, ctx, 5, q.device)
             d.cos_rows, d.cos_cols = int(cos.shape[0]), int(cos.shape[1])
-        gq, gk = (self._gamma(ctx, _optional(node, i), D) for i in (2, 3))
+        gq, gk = (self._gamma(ctx, _optional(node, i), D, q.device) for i in (2, 3))
         qo, ko = torch.empty_like(q), torch.empty_like(k)
         native.qk_norm_rotary(d, q.data_ptr(), k.data_ptr(), _ptr(gq), _ptr(gk), _ptr(pos), _ptr(cos), _ptr(sin),
                               qo.data_ptr(), ko.data_ptr(), _stream(q))
@@ -214,6 +222,7 @@ class HipLoraMatMulNBitsKernel(_Serving):
 
     def close(self):
         self._mm.close()
+        self._weights.clear()
 
     @staticmethod
     def _projection(node: GraphNode, a: str, y: str) -> GraphNode:
@@ -233,14 +242,14 @@ class HipLoraMatMulNBitsKernel(_Serving):
         if isinstance(t, np.ndarray):
             hit = self._weights.get(id(t)) if ctx.is_constant(name) else None
             if hit is not None and hit[0] is t:
-                return hit[1]
+                return hit[1].to(device)
             d = torch.from_numpy(np.ascontiguousarray(t)).to(device)
             if ctx.is_constant(name):
                 self._weights[id(t)] = (t, d)
             t = d
         if t.dim() != 3 or t.dtype not in (torch.float32, torch.float16):
             raise ModelSharpException(f"LoraMatMulNBits '{name}' must be a 3-D fp32 or fp16 tensor.")
-        return t.contiguous()
+        return t.to(device).contiguous()
 
     def _run(self, node: GraphNode, ctx: GraphContext) -> None:
         torch = _torch()
@@ -256,7 +265,7 @@ class HipLoraMatMulNBitsKernel(_Serving):
             raise ModelSharpException(f"LoraMatMulNBits lora_a must be [adapters, rank, {K}] and lora_b [adapters, {N}, "
                                       "rank] of one type.")
         ranks = self._lengths(ctx, node.inputs[6], A, x.device) if _optional(node, 6) else None
-        scales = self._dev.input(ctx, node.inputs[7]).reshape(-1) if _optional(node, 7) else None
+        scales = self._input(ctx, node.inputs[7], x.device).reshape(-1) if _optional(node, 7) else None
         if scales is not None and scales.numel() != A:
             raise ModelSharpException(f"LoraMatMulNBits lora_scales has {scales.numel()} elements; expected {A}.")
         which = self._lengths(ctx, node.inputs[8], T, x.device)

@@ -907,3 +907,30 @@ def test_lora_around_the_launch_rules(gpu, case, dtype):
 ], ids=lambda c: "-".join(map(str, c)))
 def test_lora_in_whole_chunks_on_either_side(gpu, case, dtype):
     test_lora(gpu, case, dtype)
+
+
+def test_node_inputs_on_the_host_follow_the_first_ones_device(gpu):
+    import torch
+    from modelsharp_amd import workloads
+    from modelsharp_amd.graph import GraphContext, GraphNode
+    from modelsharp_amd.serving_kernels import HipLoraMatMulNBitsKernel, HipQkNormRotaryKernel
+    rng = np.random.default_rng(6)
+    w, s, z = workloads.make_weights(workloads.Op("p", 64, 96, 32, True), seed=1)
+    cos, sin = rotary_caches(32, 32)
+    values = {"q": rng.standard_normal((5, 256)).astype(F32), "k": rng.standard_normal((5, 128)).astype(F32),
+              "g": (rng.random(64) + 0.5).astype(F32), "pos": np.arange(5, dtype=np.int32), "cos": cos, "sin": sin,
+              "x": rng.standard_normal((5, 64)).astype(F32), "la": rng.standard_normal((2, 8, 64)).astype(F16),
+              "lb": rng.standard_normal((2, 96, 8)).astype(F16), "r": np.array([8, 3], np.int32),
+              "ls": np.array([1.0, 0.5], F32), "which": np.array([0, 1, -1, 1, 0], np.int32)}
+    results = []
+    for place in (dev, torch.from_numpy):
+        ctx = GraphContext({"b": w, "s": s, "z": z,
+                            **{n: (dev if n in "qx" else place)(v) for n, v in values.items()}})
+        HipQkNormRotaryKernel().execute(GraphNode("QkNormRotary", "r", ["q", "k", "g", "g", "pos", "cos", "sin"],
+                                                  ["q2", "k2"], {"num_heads": 4, "kv_num_heads": 2}), ctx)
+        k = HipLoraMatMulNBitsKernel()
+        k.execute(GraphNode("LoraMatMulNBits", "l", ["x", "b", "s", "z", "la", "lb", "r", "ls", "which"], ["y"],
+                            {"K": 64, "N": 96, "bits": 4, "block_size": 32}), ctx)
+        results.append([host(ctx.get_tensor(n)) for n in ("q2", "k2", "y")])
+        k.close()
+    assert all(np.array_equal(a, b) and np.isfinite(a).all() for a, b in zip(*results))

@@ -172,6 +172,29 @@ def test_registration_and_node_checks():
         HipQkNormRotaryKernel().execute(GraphNode("QkNormRotary", "r", ["q", "k"], ["a", "b"]), GraphContext({}))
 
 
+def test_nodes_take_their_inputs_to_the_first_ones_device():
+    """A tensor on another device, the host among them, never reaches a kernel by its address."""
+    import torch
+    x = torch.zeros(2, 64)
+    for k, node in (
+            (HipPagedAttentionKernel(), GraphNode("PagedAttention", "a", ["x"] + [""] * 7, ["o"],
+                                                  {"num_heads": 1, "kv_num_heads": 1})),
+            (HipQkNormRotaryKernel(), GraphNode("QkNormRotary", "r", ["x", "x"], ["a", "b"],
+                                                {"num_heads": 1, "kv_num_heads": 1})),
+            (HipLoraMatMulNBitsKernel(), GraphNode("LoraMatMulNBits", "l", ["x"] * 9, ["o"], {}))):
+        with pytest.raises(ModelSharpException, match="is a tensor on cpu"):
+            k.execute(node, GraphContext({"x": x}))
+    meta = torch.device("meta")
+    ctx = GraphContext({"g": torch.ones(8), "c": torch.ones(4, 4), "a": torch.zeros(1, 2, 8), "n": torch.zeros(3)})
+    k = HipLoraMatMulNBitsKernel()
+    assert k._gamma(ctx, "g", 8, meta).device == meta
+    assert all(t.device == meta for t in k._rotary(GraphNode("", "", ["c", "c"], []), ctx, 0, meta))
+    assert k._adapter(ctx, "a", meta).device == meta and k._lengths(ctx, "n", 3, meta).device == meta
+    w = np.zeros((1, 2, 8), np.float16)   # an initializer, kept from its first use on another device
+    k._weights[id(w)] = (w, torch.zeros(1, 2, 8, dtype=torch.float16))
+    assert k._adapter(GraphContext({"w": w}, ["w"]), "w", meta).device == meta
+
+
 # ---- the plain forms themselves ---------------------------------------------------------------------
 
 def test_plain_attention_against_a_hand_worked_case():
