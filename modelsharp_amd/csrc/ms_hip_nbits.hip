@@ -3404,7 +3404,9 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const in
         if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: buffers must be 4-byte aligned");
     if (misaligned16(dKCache) || misaligned16(dVCache))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the cache must be 16-byte aligned");
-    const PagedAttnPlan plan = paged_plan(*d, dWorkspace && !misaligned16(dWorkspace) ? workspace_bytes : 0);
+    // (a negative limit is the plan's "no limit")
+    const PagedAttnPlan plan =
+        paged_plan(*d, dWorkspace && !misaligned16(dWorkspace) ? std::max<int64_t>(workspace_bytes, 0) : 0);
     if (plan.rows_grid + plan.blocks_grid > INT_MAX)
         return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_attention: %d tokens of %d requests need too many workgroups",
                     d->tokens, d->requests);
