@@ -3099,9 +3099,9 @@ int ms_hip_gqa(const ms_hip_gqa_desc* d, const float* dQ, const float* dK, const
         hipLaunchKernelGGL(gqa_copy_past_kernel, dim3(elementwise_grid(n)), dim3(256), 0, s, p);
         MS_HIP_CHECK(hipGetLastError());
     }
-    const GqaPlan plan = p.Sq > 0 ? gqa_plan(*d, dWorkspace && !misaligned4(dWorkspace) ? workspace_bytes : 0,
-                                             (reinterpret_cast<uintptr_t>(dWorkspace) & 15) == 0)
-                                  : GqaPlan{};
+    // (a negative limit is the plan's "no limit")
+    const int64_t avail = dWorkspace && !misaligned4(dWorkspace) ? std::max<int64_t>(workspace_bytes, 0) : 0;
+    const GqaPlan plan = p.Sq > 0 ? gqa_plan(*d, avail, (reinterpret_cast<uintptr_t>(dWorkspace) & 15) == 0) : GqaPlan{};
     if (plan.split_waves) {
         MS_HIP_CHECK(launch_gqa_split(p, plan.split_waves, dWorkspace, s));
         return MS_HIP_OK;

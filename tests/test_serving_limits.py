@@ -33,3 +33,15 @@ def test_a_negative_workspace_size_is_no_workspace(size):
     q, cu, past, table, out, kc, vc = (P + i * 64 * MB for i in range(7))
     refused(lambda: native.paged_attention(d, q, cu, past, table, kc, vc, out, kc, n), 1, "workspace overlaps")
     refused(lambda: native.paged_attention(d, q, cu, past, table, kc, vc, out, kc, size), 3, "launch_paged_attention")
+
+
+@pytest.mark.parametrize("size", [-1, -2 ** 40])
+def test_group_query_attention_takes_a_negative_workspace_size_as_none(size):
+    """A history whose scores do not fit one workgroup is refused without a workspace."""
+    d = native.GqaDesc(batch=1, q_seq=1, kv_seq=0, past_seq=100000, past_in_present=1, num_heads=2, kv_num_heads=1,
+                       head_dim=32, present_capacity=100000, local_window_size=-1)
+    n = native.gqa_workspace_size(d)
+    assert n > 0
+    args = [P + i * 64 * MB for i in range(3)] + [None] * 5 + [P + (8 + i) * 1024 * MB for i in range(4)]
+    refused(lambda: native.gqa(d, *args, 0), 4, "history too long")
+    refused(lambda: native.gqa(d, *args, size), 4, "history too long")
