@@ -44,10 +44,10 @@ __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, int 
     const int lane = threadIdx.x & (kWave - 1);
     for (int base = 0; base < b.requests; base += kWave) {
         const int i = min(base + lane, b.requests - 1);
-        const int c0 = max(b.cu[i], 0), c1 = min(b.cu[i + 1], b.tokens), past = b.past[i];
-        const int n = base + lane < b.requests ? max(c1 - c0, 0) : 0;
+        const PagedSpan span = paged_span(b.cu[i], b.cu[i + 1], b.tokens);
+        const int c0 = span.first, past = b.past[i], n = base + lane < b.requests ? span.count : 0;
         const int nr = n * p.grp.div;
-        const int tiles = nr >= rows_min && nr <= rows_max ? (nr + BM - 1) / BM : 0;
+        const int tiles = nr >= rows_min && nr <= rows_max ? paged_tiles(nr, BM) : 0;
         const int sum = wave_scan(tiles);
         const uint64_t past_idx = __ballot(sum > idx);
         if (past_idx) {

@@ -32,7 +32,7 @@ struct FastDiv {
 // [cu[r], cu[r + 1]) of the step's tensors, its position p lies in row table[r][p / page] * page
 // + p % page of the cache. Entries outside [0, num_pages) hold nothing: their keys are masked
 // and appends to them dropped. Lengths that make no sense (below zero, past the tensors' rows
-// or the table) are cut to what is there.
+// or the table) are cut to what is there (paged_span).
 struct PagedBatch {
     const int32_t* cu;
     const int32_t* past;
@@ -40,6 +40,24 @@ struct PagedBatch {
     int tokens, requests, num_pages, max_pages;
     FastDiv page;
 };
+
+// A request's rows of the step's tensors from cu[r] and cu[r + 1], whatever those hold.
+struct PagedSpan {
+    int first, count;
+};
+__host__ __device__ inline PagedSpan paged_span(int c0, int c1, int tokens)
+{
+    const int first = c0 < 0 ? 0 : c0 > tokens ? tokens : c0, end = c1 < first ? first : c1 > tokens ? tokens : c1;
+    return {first, end - first};
+}
+
+// Tiles of bm rows of `rows` rows; at most 2^24, as many workgroups as a launch can have (2^32
+// threads), so that those of 64 requests add up in 32 bits even where senseless lengths overlap.
+__host__ __device__ inline int paged_tiles(int rows, int bm)
+{
+    const uint32_t n = ((uint32_t)rows + bm - 1) / bm;
+    return n < (1u << 24) ? (int)n : 1 << 24;
+}
 
 // The request that row t belongs to, or `requests` for a row behind the last: how many end at or
 // before t, counted 64 at a time. Called by whole waves with a uniform t.

@@ -2,10 +2,16 @@
 borders of what the entries take."""
 from __future__ import annotations
 
+import os
+import pathlib
+import shutil
+import subprocess
+
 import pytest
 
 from modelsharp_amd import native
 
+CSRC = pathlib.Path(__file__).resolve().parents[1] / "modelsharp_amd" / "csrc"
 P, MB = 1 << 20, 1 << 20   # addresses that are never followed
 
 
@@ -45,3 +51,46 @@ def test_group_query_attention_takes_a_negative_workspace_size_as_none(size):
     args = [P + i * 64 * MB for i in range(3)] + [None] * 5 + [P + (8 + i) * 1024 * MB for i in range(4)]
     refused(lambda: native.gqa(d, *args, 0), 4, "history too long")
     refused(lambda: native.gqa(d, *args, size), 4, "history too long")
+
+
+@pytest.fixture(scope="module")
+def lengths(tmp_path_factory):
+    """paged_span and paged_tiles of the kernels' own header, compiled for the host: lines of cu[r],
+    cu[r + 1], tokens, query heads of a kv head and a tile's rows in; first, count and tiles out."""
+    hipcc = shutil.which("hipcc", path="/opt/rocm/bin:" + os.environ.get("PATH", ""))
+    if not hipcc:
+        pytest.skip("no hipcc")
+    at = tmp_path_factory.mktemp("lengths")
+    (at / "lengths.hip").write_text("""
+#include <cstdio>
+#include "serving.h"
+int main()
+{
+    int c0, c1, tokens, grp, bm;
+    while (std::scanf("%d %d %d %d %d", &c0, &c1, &tokens, &grp, &bm) == 5) {
+        const msnb::PagedSpan s = msnb::paged_span(c0, c1, tokens);
+        std::printf("%d %d %d\\n", s.first, s.count, msnb::paged_tiles(s.count * grp, bm));
+    }
+}
+""")
+    subprocess.run([hipcc, "--offload-arch=gfx950", "--offload-host-only", "-std=c++17", "-I", str(CSRC), "-o",
+                    str(at / "lengths"), str(at / "lengths.hip")], check=True, capture_output=True)
+
+    def run(rows):
+        out = subprocess.run([str(at / "lengths")], input="\n".join(" ".join(map(str, r)) for r in rows), check=True,
+                             capture_output=True, text=True).stdout
+        return [tuple(map(int, line.split())) for line in out.splitlines()]
+    return run
+
+
+def test_lengths_that_make_no_sense_are_cut_to_the_tensors_rows(lengths):
+    lo, hi = -2 ** 31, 2 ** 31 - 1
+    some = [lo, lo + 1, -5, -1, 0, 1, 7, 30, 31, 100, hi - 1, hi]
+    rows = [(c0, c1, tokens, 4, bm) for c0 in some for c1 in some for tokens in (1, 30, 2 ** 29) for bm in (16, 128)]
+    for (c0, c1, tokens, grp, bm), (first, count, tiles) in zip(rows, lengths(rows)):
+        begin = min(max(c0, 0), tokens)
+        assert first == begin and count == max(min(c1, tokens) - begin, 0), (c0, c1, tokens)
+        assert 0 <= first <= first + count <= tokens
+        assert tiles == min(-(-count * grp // bm), 2 ** 24)
+    # the most rows that a call may have
+    assert lengths([(0, 1, 1, hi, 16), (0, 1, 1, hi, 128)]) == [(0, 1, 2 ** 24), (0, 1, 2 ** 24)]
