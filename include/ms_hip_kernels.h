@@ -434,7 +434,8 @@ int ms_hip_gqa(const ms_hip_gqa_desc* desc, const float* dQ, const float* dK, co
  * int32 [requests]); its position p lies in page table[r][p / page_size] (dTable int32
  * [requests, max_pages]). A request may have no new token. Rows behind the last request's are
  * left as they were, in every output. A table entry outside [0, num_pages), or a position past
- * the table, is a page that is not there: its keys are masked, appends to it dropped. The lengths
+ * the table or from 2^31 - 4096 on, is a page that is not there: its keys are masked, appends to it
+ * dropped. The lengths
  * and the table are read on the device, so a captured step is replayed with new ones.
  *   max_new, max_total   bounds of any request's new tokens and of past + new tokens (0: not
  *                        known). They choose the launch; results do not depend on them.

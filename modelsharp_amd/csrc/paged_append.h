@@ -29,8 +29,8 @@ __device__ __forceinline__ bool append_place(const AppendArgs& p, int t, AppendP
     if (r >= p.b.requests) return false;   // a row behind the last request's
     const int i = t - p.b.cu[r];
     if (i < 0) return false;
-    at.pos = (int)min((int64_t)max(p.b.past[r], 0) + i, (int64_t)INT32_MAX);
-    at.row = paged_row(p.b, r, at.pos);
+    at.pos = (int)min((int64_t)max(p.b.past[r], 0) + i, (int64_t)kPagedPositions);
+    at.row = at.pos < kPagedPositions ? paged_row(p.b, r, at.pos) : -1;
     return true;
 }
 

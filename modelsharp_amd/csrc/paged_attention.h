@@ -59,7 +59,7 @@ __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, int 
             t.t0 = __builtin_amdgcn_readlane(c0, l);
             t.row0 = (nt - 1 - within) * BM;
             t.rows = min(BM, nl * p.grp.div - t.row0);
-            t.past = min(max(__builtin_amdgcn_readlane(past, l), 0), 0x3fffffff);
+            t.past = min(max(__builtin_amdgcn_readlane(past, l), 0), kPagedPositions - nl);
             t.klast = min((int64_t)t.past + nl, (int64_t)b.max_pages * b.page.div) - 1;
             return true;
         }

@@ -28,6 +28,10 @@ struct FastDiv {
     }
 };
 
+// Positions from here on have no page: 2^31 with a margin, so that a position and a few blocks of
+// keys add up in 32 bits.
+constexpr int kPagedPositions = 0x7ffff000;
+
 // A batch of `requests` requests over one paged cache: request r's new tokens are rows
 // [cu[r], cu[r + 1]) of the step's tensors, its position p lies in row table[r][p / page] * page
 // + p % page of the cache. Entries outside [0, num_pages) hold nothing: their keys are masked

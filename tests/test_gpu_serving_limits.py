@@ -49,3 +49,53 @@ def test_lengths_that_wrap_stay_inside(gpu, cu):
         native.paged_attention(d, *map(ptr, bufs), ptr(o), ptr(ws), n, stream())
         torch.cuda.synchronize()
         assert (o[b.tokens:] == 0).all() and (ws[n // 4:] == 0).all()
+
+
+@pytest.mark.parametrize("first", [2 ** 30 - 20, 2 ** 30 + 70000, 2 ** 31 - 4096 - 90], ids=["2^30", "past-2^30", "last"])
+@pytest.mark.parametrize("news", [[2], [90]], ids=["tokens", "chunk"])
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+def test_positions_of_a_very_long_history(gpu, dtype, news, first):
+    """Appends and attention under a window agree about positions past 2^30, where only the last pages
+    are there."""
+    import torch
+    H, G, D, page, window = 4, 1, 64, 1 << 16, 70
+    b = ref.Batch(105, news, [1], G, D, page, dtype, spare_pages=1)
+    b.pasts, b.past = [first], np.array([first], np.int32)
+    b.max_pages = (first + news[0] - 1) // page + 1
+    b.table = np.full((1, b.max_pages), -1, np.int32)
+    b.table[0, -2:] = [1, 0]
+    q, k, v = (b.rng.standard_normal((b.tokens, n * D)).astype(F32) for n in (H, G, G))
+    log(f"positions from {first} {news} {dtype.__name__}")
+    d = desc_of(b, H, local_window_size=window)
+    lens = [dev(x) for x in (b.cu, b.past, b.table)]
+    src, qo, kc, vc = [dev(x) for x in (q, k, v)], torch.empty(b.tokens, H * D, device="cuda"), dev(b.k), dev(b.v)
+    native.paged_append(d, *map(ptr, src), None, None, *map(ptr, lens), None, None, ptr(qo), ptr(kc), ptr(vc), stream())
+    want = b.k.copy(), b.v.copy()
+    for t, r, pos in b.each_token():
+        for w, x in zip(want, (k, v)):
+            w.reshape(-1, G, D)[b.row(r, pos)] = x[t].reshape(G, D)
+    assert np.array_equal(host(kc), want[0]) and np.array_equal(host(vc), want[1])
+    b.k, b.v = want
+    n = native.paged_attention_workspace_size(d)
+    ws, out = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda"), torch.empty_like(qo)
+    native.paged_attention(d, ptr(qo), *map(ptr, lens), ptr(kc), ptr(vc), ptr(out), ptr(ws), n, stream())
+    check_attention(host(out), b, q, H, window)
+
+
+def test_positions_without_a_page_are_dropped(gpu):
+    """From 2^31 - 4096 on there is no page, whatever the table holds."""
+    import torch
+    H, G, D, page, first = 2, 1, 64, 1 << 16, 2 ** 31 - 4096 - 3
+    b = ref.Batch(107, [8], [1], G, D, page, F32)
+    b.max_pages = 1 << 15
+    b.table = np.zeros((1, b.max_pages), np.int32)
+    d = desc_of(b, H)
+    q, k, v = (dev(b.rng.standard_normal((8, n * D)).astype(F32)) for n in (H, G, G))
+    kc, vc = dev(b.k), dev(b.v)
+    lens = [dev(x) for x in (b.cu, np.array([first], np.int32), b.table)]
+    log("positions past the last")
+    native.paged_append(d, ptr(q), ptr(k), ptr(v), None, None, *map(ptr, lens), None, None, ptr(torch.empty_like(q)), ptr(kc),
+                        ptr(vc), stream())
+    want = b.k.copy()
+    want.reshape(-1, G, D)[first % page:first % page + 3] = host(k)[:3].reshape(3, G, D)
+    assert np.array_equal(host(kc), want)
