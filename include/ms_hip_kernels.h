@@ -470,9 +470,11 @@ int ms_hip_paged_append(const ms_hip_paged_desc* desc, const float* dQ, const fl
                         void* dKCache, void* dVCache, void* stream);
 /* Attention of the new tokens (their keys and values appended) over each request's positions
  * [max(0, pos - window + 1), pos]: dOut [tokens, num_heads * head_dim]. head_dim a multiple
- * of 8 up to 256 (else MS_HIP_ERR_UNSUPPORTED). A row that sees no key is zero. fp32 accuracy
- * for both cache types (values of an fp32 cache below 2^-110 may count with an error of up to
- * 2^-126); what a query does not see does not reach it, infinities and NaN included. The
+ * of 8 up to 256 (else MS_HIP_ERR_UNSUPPORTED). A row that sees no key is zero. Accuracy: that
+ * of a plain fp32 evaluation, to a factor of about 3, for either cache type. Over an fp16 cache queries
+ * and softmax weights count with 22 bits, those below 2^-28 of their row's largest query or 2^-25 of
+ * its largest weight with an error of up to 2^-51 or 2^-48 of it; over an fp32 cache requests of
+ * many rows take products to 2^-21, and values below 2^-110 may count with an error of up to 2^-126. What a query does not see does not reach it, infinities and NaN included. The
  * workspace is optional (a smaller, misaligned or NULL one: the keys of a tile of queries are not
  * shared out); calls that may overlap need one each. */
 int64_t ms_hip_paged_attention_workspace_size(const ms_hip_paged_desc* desc);

@@ -206,6 +206,17 @@ template <> struct PagedElem<float> {
 
 constexpr float kGrow = 4.0f;     // the running maximum moves in steps above 2^4
 constexpr int kWeightExp = 11;    // weights times 2^11: at most 2^15 in fp16
+// The low halves of weights and queries are held times 2^12 and summed apart: a half ulp of the high
+// half becomes at most 2^15, and what is left of a value so small that its high half is subnormal
+// keeps its bits: 22 bits down to 2^-25 of a row's largest weight (2^-28 of its largest query), then an
+// error of 2^-48 (2^-51) of the largest. With one scale for both, they went from 2^-14 on: 1.4e-3 of a row where weights of 2^-30
+// met values 2^25 larger. The join of the sums costs single tokens 0 to 3%, and chunks, which the
+// vector unit's share of a block of keys slows down, 7 to 14% (512 tokens of 28 / 4 heads of 128 over 16000
+// keys: 235 us before, 257 now), at 256 channels 27%. Kept over all blocks instead, the low halves'
+// sums spilled (64 registers more at 128 channels), and left out for queries without small values, by a
+// branch, they cost the products their order: 286 us.
+constexpr int kLowExp = 12;
+constexpr float kLow = 1.0f / (1 << kLowExp);
 
 // Steps of 16 keys in a wave's registers: the one in use and those on their way. A third for fp16 at
 // D = 128 made no difference (47.1 against 46.2 us for 32 tokens over 1000-4000 keys).
@@ -379,7 +390,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
             for (int i = 0; i < KV; ++i) {
                 const float v = __builtin_amdgcn_ldexpf(x[s][i], -e);
                 qh[s][i] = (_Float16)v;
-                ql[s][i] = (_Float16)(v - (float)qh[s][i]);
+                ql[s][i] = (_Float16)((v - (float)qh[s][i]) * (1 << kLowExp));
             }
     } else {
 #pragma unroll
@@ -388,11 +399,14 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
             for (int i = 0; i < KV; ++i) qh[s][i] = x[s][i];
     }
 
-    floatx4_t acc[NC][VEC];
+    floatx4_t acc[NC][VEC], low[F16 ? NC : 1][F16 ? VEC : 1];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[c][j] = floatx4_t{};
+        for (int j = 0; j < VEC; ++j) {
+            acc[c][j] = floatx4_t{};
+            if constexpr (F16) low[c][j] = floatx4_t{};
+        }
     float m = -__builtin_inff(), l = 0.0f;
 
     // the keys that every row of the tile sees need no mask
@@ -400,12 +414,12 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
     const int all_hi = min(kr.khi, t.past + p.grp.quot(t.row0));
     auto add = [&](int key, const Keys& x) {
         if (WHOLE && !x.there[0]) return;
-        floatx4_t s4{};
+        floatx4_t s4{}, s4l{};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             if constexpr (F16) {
                 s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[s], qh[s], s4, 0, 0, 0);
-                s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[s], ql[s], s4, 0, 0, 0);
+                s4l = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.k[s], ql[s], s4l, 0, 0, 0);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[s][e], qh[s][e], s4, 0, 0, 0);
@@ -413,7 +427,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
         }
         float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = s4[i] * fac;
+        for (int i = 0; i < 4; ++i) w[i] = (F16 ? __builtin_fmaf(s4l[i], kLow, s4[i]) : s4[i]) * fac;
         if (!WHOLE || key < all_lo || key + 15 > all_hi)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -431,20 +445,25 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) acc[c][j] *= al;
+                for (int j = 0; j < VEC; ++j) {
+                    acc[c][j] *= al;
+                    if constexpr (F16) low[c][j] *= al;
+                }
         }
-        const float off = (F16 ? (float)kWeightExp : 0.0f) - (m == -__builtin_inff() ? 0.0f : m);
+        // (scaled behind the exponential: an argument of 11 or more would be rounded to 2^-21)
+        const float off = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(w[i] + off);
+            w[i] = __builtin_amdgcn_exp2f(w[i] - off);
             l += w[i];
         }
         if constexpr (F16) {
             half4_t ph, pl;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ph[i] = (_Float16)w[i];
+            for (int i = 0; i < 4; ++i) ph[i] = (_Float16)(w[i] * (1 << kWeightExp));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pl[i] = (_Float16)__builtin_fmaf((float)ph[i], -1.0f, w[i]);
+            for (int i = 0; i < 4; ++i)
+                pl[i] = (_Float16)__builtin_fmaf((float)ph[i], -(float)(1 << kLowExp), w[i] * (1 << (kWeightExp + kLowExp)));
             typedef uint32_t dwords_t __attribute__((ext_vector_type(VEC / 2)));
             typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -458,7 +477,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
                     const half4_t a = __builtin_bit_cast(half4_t, u32x2_t{__builtin_amdgcn_perm(d[1], d[0], sel),
                                                                           __builtin_amdgcn_perm(d[3], d[2], sel)});
                     acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, ph, acc[c][j], 0, 0, 0);
-                    acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, pl, acc[c][j], 0, 0, 0);
+                    low[c][j] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, pl, low[c][j], 0, 0, 0);
                 }
         } else {
 #pragma unroll
@@ -484,7 +503,14 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
     // the waves' sums meet: statistics, then four quads of channels at a time
     l += xor16_value(l);
     l += xor32_value(l);
-    if (F16) l *= 1.0f / (1 << kWeightExp);
+    if constexpr (F16) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[c][j][i] = __builtin_fmaf(low[c][j][i], kLow, acc[c][j][i]);
+    }
     if (lane < 16) {
         stat[0][wave][lane] = m;
         stat[1][wave][lane] = l;
@@ -537,32 +563,34 @@ typedef short short8_t __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) short4_t lds_short4_t;
 
 // How an operand's fp32 values are held for the 16-bit matrix cores.
-//   fp16 cache: K and V are fp16 already; queries and weights are two fp16 halves (22 bits), two
-//   products an operand pair.
+//   fp16 cache: K and V are fp16 already; queries and weights, times 2^EXP, are two fp16 halves (22
+//   bits), the low one times 2^12 (kLowExp): two products an operand pair, each with a sum of its own.
 template <typename T> struct PagedSplit;
 template <> struct PagedSplit<_Float16> {
-    static constexpr int kPlanes = 1, kParts = 2;   // of the cache, of queries and weights
+    static constexpr int kPlanes = 1, kParts = 2, kSums = 2;   // of the cache; of queries and weights
     static constexpr int kProducts = 2;
-    static constexpr int pair[kProducts][2] = {{0, 0}, {0, 1}};   // (plane, part)
+    static constexpr int pair[kProducts][3] = {{0, 0, 0}, {0, 1, 1}};   // (plane, part, sum)
+    template <int EXP>
     __device__ static __forceinline__ void part(const float (&x)[8], short8_t (&out)[2])
     {
         typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+        constexpr float scale = 1 << EXP, low = 1 << (EXP + kLowExp);
         u32x4_t h, l;
-        float minus = -1.0f;   // opaque, so that x - h is one v_fma_mix_f32 on the packed half
-        asm("" : "+s"(minus));
+        // each half is one v_fma_mixlo_f16 or v_fma_mixhi_f16: scaled, subtracted, rounded
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            h[i] = pack(x[2 * i], x[2 * i + 1]);
-            l[i] = pack(fmac_lo(h[i], minus, x[2 * i]), fmac_hi(h[i], minus, x[2 * i + 1]));
+            h[i] = pack(__builtin_fmaf(x[2 * i], scale, 0.0f), __builtin_fmaf(x[2 * i + 1], scale, 0.0f));
+            const h2_t v = as_h2(h[i]);
+            l[i] = pack(__builtin_fmaf((float)v.x, -(float)(1 << kLowExp), x[2 * i] * low),
+                        __builtin_fmaf((float)v.y, -(float)(1 << kLowExp), x[2 * i + 1] * low));
         }
         out[0] = __builtin_bit_cast(short8_t, h);
         out[1] = __builtin_bit_cast(short8_t, l);
     }
-    // both rounded to nearest, in one v_cvt_pk_f16_f32 (kept whole by the opaque result)
+    // two fp16 of a dword, kept whole by the opaque result
     __device__ static __forceinline__ uint32_t pack(float a, float b)
     {
-        typedef float f2_t __attribute__((ext_vector_type(2)));
-        uint32_t r = as_u32(__builtin_convertvector(f2_t{a, b}, h2_t));
+        uint32_t r = as_u32(h2_t{(_Float16)a, (_Float16)b});
         asm("" : "+v"(r));
         return r;
     }
@@ -577,9 +605,10 @@ template <> struct PagedSplit<_Float16> {
 //   whose terms are 2^-16 or more of the whole: six of nine, what is left out is below 2^-22.
 //   (The matrix cores take bf16 below 2^-126 as zero: values below 2^-110 keep fewer bits.)
 template <> struct PagedSplit<float> {
-    static constexpr int kPlanes = 3, kParts = 3;
+    static constexpr int kPlanes = 3, kParts = 3, kSums = 1;
     static constexpr int kProducts = 6;
-    static constexpr int pair[kProducts][2] = {{2, 0}, {1, 1}, {0, 2}, {1, 0}, {0, 1}, {0, 0}};   // small terms first
+    static constexpr int pair[kProducts][3] = {{2, 0, 0}, {1, 1, 0}, {0, 2, 0}, {1, 0, 0}, {0, 1, 0}, {0, 0, 0}};   // small terms first
+    template <int EXP>
     __device__ static __forceinline__ void part(const float (&x)[8], short8_t (&out)[3])
     {
         typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
@@ -635,9 +664,9 @@ __device__ __forceinline__ int v_turn(int row)
 //
 // 128 rows, since two such workgroups fill a CU's LDS (64 KB each at D = 128: two blocks of 64 keys) and
 // registers, and each block of keys is then read from L2 once for 128 rows. The matrix cores bound a
-// long chunk: 512 tokens of 28 / 4 heads over 16000 keys take 236-241 us with the merge, 500 TFLOP/s of
-// attention and twice that of products (a library product of 8192 reaches 1063). Fresh prompts of 200-650
-// tokens (44 us for five) are bound by the longest tile's chain of blocks. An fp32 cache, with six
+// long chunk, and the vector unit, which the products hardly run beside: 512 tokens of 28 / 4 heads over
+// 16000 keys take 253-258 us with the merge, 470 TFLOP/s of attention and twice that of products (a library
+// product of 8192 reaches 1063). Fresh prompts of 200-650 tokens (46 us for five) are bound by the longest tile's chain of blocks. An fp32 cache, with six
 // products a pair: two chunks of 300 tokens of 32 / 8 heads of 96, 1024 keys visible: 62 + 9 us.
 // WHOLE: pages of a multiple of 16 rows, so that a wave's rows of a load lie in one page: its lookups
 // are the scalar unit's.
@@ -659,6 +688,10 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
     constexpr int BN = B::BN, BUFS = B::BUFS, CH = B::CH;
     constexpr int KS = DP / 16, NT = DP / 32, KT = BN / 32;
     constexpr int UN = BN * CH / 256;   // 8-channel units a thread moves of K, and of V
+    // Two sums: so many tiles of scores and of channels at a time that the low halves' sums fit the
+    // registers beside the rest (what is loaded ahead among it, unless it goes straight to LDS).
+    constexpr bool FEW = S::kSums == 2 && !WHOLE;
+    constexpr int KG = FEW ? 1 : KT, NG = S::kSums == 1 ? NT : FEW ? 1 : 2;
     auto& lds = *reinterpret_cast<typename B::lds_t*>(lds_bytes);
 
     const int g = bid % p.kvH, rest = bid / p.kvH;
@@ -746,7 +779,7 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
             float f[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = x[i];
-            S::part(f, out);
+            S::template part<0>(f, out);
         }
     };
     auto store = [&](int buf) {   // what fetch() brought is in LDS for every wave behind the next barrier
@@ -804,7 +837,7 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
                 for (int i = 0; i < 8; ++i) x[s][i] = __builtin_amdgcn_ldexpf(x[s][i], -e);
         }
 #pragma unroll
-        for (int s = 0; s < KS; ++s) S::part(x[s], qx[s]);
+        for (int s = 0; s < KS; ++s) S::template part<0>(x[s], qx[s]);
     }
 
 
@@ -823,20 +856,37 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
             look(k0 + 2 * BN);
         }
         if (k0 <= any_hi && k0 + BN > any_lo) {
+            // (two sums: this wave's products go before the CU's other waves' exponentials, 2% of a long chunk)
+            if constexpr (S::kSums == 2) __builtin_amdgcn_s_setprio(1);
             floatx16_t st[KT];
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) st[kt] = floatx16_t{};
+            for (int t0 = 0; t0 < KT; t0 += KG) {
+                floatx16_t low[KG];
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                short8_t a[S::kPlanes][KT];
+                for (int kt = 0; kt < KG; ++kt) st[t0 + kt] = low[kt] = floatx16_t{};
 #pragma unroll
-                for (int pl = 0; pl < S::kPlanes; ++pl)
+                for (int s = 0; s < KS; ++s) {
+                    short8_t a[S::kPlanes][KG];
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) a[pl][kt] = lds[buf][0][pl][k_slot<CH>(32 * kt + l32, 2 * s + hf)];
+                    for (int pl = 0; pl < S::kPlanes; ++pl)
 #pragma unroll
-                for (int j = 0; j < S::kProducts; ++j)
+                        for (int kt = 0; kt < KG; ++kt)
+                            a[pl][kt] = lds[buf][0][pl][k_slot<CH>(32 * (t0 + kt) + l32, 2 * s + hf)];
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) st[kt] = S::mfma(a[S::pair[j][0]][kt], qx[s][S::pair[j][1]], st[kt]);
+                    for (int j = 0; j < S::kProducts; ++j)
+#pragma unroll
+                        for (int kt = 0; kt < KG; ++kt) {
+                            floatx16_t& sum = S::pair[j][2] ? low[kt] : st[t0 + kt];
+                            sum = S::mfma(a[S::pair[j][0]][kt], qx[s][S::pair[j][1]], sum);
+                        }
+                }
+                if constexpr (S::kSums == 2) {
+                    if (t0 + KG == KT) __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+                    for (int kt = 0; kt < KG; ++kt)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) st[t0 + kt][v] = __builtin_fmaf(low[kt][v], kLow, st[t0 + kt][v]);
+                }
             }
             if (k0 < all_lo || k0 + BN - 1 > all_hi)
 #pragma unroll
@@ -860,36 +910,53 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
 #pragma unroll
                 for (int n = 0; n < NT; ++n) acc[n] *= al;
             }
-            const float off = m == -__builtin_inff() ? 0.0f : (F16 ? (float)kWeightExp : 0.0f) - m;
+            // (fp16's scale comes behind the exponential: an argument of 11 or more would be rounded to 2^-21)
+            const float off = m == -__builtin_inff() ? 0.0f : -m;
+            short8_t px[2 * KT][S::kParts];
 #pragma unroll
-            for (int s = 0; s < 2 * KT; ++s) {
-                float w[8];
+            for (int n0 = 0; n0 < NT; n0 += NG) {
+                floatx16_t low[NG];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + j], fac, off));
-                    l += w[j];
-                }
-                short8_t px[S::kParts];
-                S::part(w, px);
+                for (int n = 0; n < NG; ++n) low[n] = floatx16_t{};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    // rows 16 s + 8 e + 4 hf + i / 4, 16 channels of 8-byte quarters of two chunks
-                    const int i = lane & 15;
-                    short8_t a[S::kPlanes];
+                for (int s = 0; s < 2 * KT; ++s) {
+                    if (n0 == 0) {
+                        float w[8];
 #pragma unroll
-                    for (int pl = 0; pl < S::kPlanes; ++pl)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int r = 16 * s + 8 * e + 4 * hf + (i >> 2);
-                            const int c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-                            const short4_t h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (lds_short4_t*)((short4_t*)&lds[buf][1][pl][r * CH + (c ^ v_turn<CH>(r))] + (i & 1)));
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) a[pl][4 * e + x] = h[x];
+                        for (int j = 0; j < 8; ++j) {
+                            w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[s >> 1][8 * (s & 1) + j], fac, off));
+                            l += w[j];
                         }
+                        S::template part<kWeightExp>(w, px[s]);
+                    }
 #pragma unroll
-                    for (int j = 0; j < S::kProducts; ++j) acc[n] = S::mfma(a[S::pair[j][0]], px[S::pair[j][1]], acc[n]);
+                    for (int n = n0; n < min(n0 + NG, NT); ++n) {
+                        // rows 16 s + 8 e + 4 hf + i / 4, 16 channels of 8-byte quarters of two chunks
+                        const int i = lane & 15;
+                        short8_t a[S::kPlanes];
+#pragma unroll
+                        for (int pl = 0; pl < S::kPlanes; ++pl)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int r = 16 * s + 8 * e + 4 * hf + (i >> 2);
+                                const int c = 4 * n + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                                const short4_t h = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (lds_short4_t*)((short4_t*)&lds[buf][1][pl][r * CH + (c ^ v_turn<CH>(r))] + (i & 1)));
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) a[pl][4 * e + x] = h[x];
+                            }
+#pragma unroll
+                        for (int j = 0; j < S::kProducts; ++j) {
+                            floatx16_t& sum = S::pair[j][2] ? low[n - n0] : acc[n];
+                            sum = S::mfma(a[S::pair[j][0]], px[s][S::pair[j][1]], sum);
+                        }
+                    }
                 }
+                if constexpr (S::kSums == 2)
+#pragma unroll
+                    for (int n = n0; n < min(n0 + NG, NT); ++n)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) acc[n][v] = __builtin_fmaf(low[n - n0][v], kLow, acc[n][v]);
             }
         }
         if constexpr (BUFS == 2)
@@ -906,7 +973,7 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
     missing = said[0] | said[1] | said[2] | said[3];
 
     l += xor32_value(l);
-    const float f = l != 0.0f ? 1.0f / l : 0.0f;
+    const float f = l != 0.0f ? 1.0f / (F16 ? l * (1 << kWeightExp) : l) : 0.0f;
     float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
     bool odd = mine && (missing || (m == -__builtin_inff() && k_hi >= k_lo));
 #pragma unroll
@@ -922,7 +989,7 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
         }
     if (p.splits > 1 && mine && hf == 0) {
         paged_part_ml(p, sp, orow)[0] = m;
-        paged_part_ml(p, sp, orow)[1] = F16 ? l * (1.0f / (1 << kWeightExp)) : l;
+        paged_part_ml(p, sp, orow)[1] = l;
     }
     // rows that met an infinity, a NaN or a page that is not there
     uint64_t redo = __ballot(odd);

@@ -135,3 +135,100 @@ def lora_tolerance(y, terms, K, R):
     terms' magnitudes: the lanes' chains, the waves' and splits' joins), and the last sum with
     the base."""
     return terms * (K / 8 + R / 4 + 24) * EPS24 + (np.abs(y) + terms) * 2 * EPS24 + 1e-30
+
+
+# ---- bounds by a row's own size ----------------------------------------------------------------
+
+def attention_sums(b: Batch, q, H, window=-1, scale=0.0):
+    """(out, sums, mass, keys), 64 bits, [tokens, H, D] and [tokens, H]: out, the sum of w |v| of each
+    output, the largest sum |q| |k| scale of a row's visible keys, and how many it sees. Rows of no
+    request are NaN."""
+    G, D = b.G, b.D
+    scale = scale or 1.0 / math.sqrt(D)
+    k, v = b.k.reshape(-1, G, D).astype(np.float64), b.v.reshape(-1, G, D).astype(np.float64)
+    q = q.reshape(b.tokens, H, D).astype(np.float64)
+    out, sums = np.full((b.tokens, H, D), np.nan), np.full((b.tokens, H, D), np.nan)
+    mass, keys = np.zeros((b.tokens, H)), np.zeros((b.tokens, H))
+    for t, r, pos in b.each_token():
+        lo = max(0, pos - window + 1) if window >= 0 else 0
+        rows = np.array([x for x in (b.row(r, j) for j in range(lo, pos + 1)) if x >= 0], np.int64)
+        for h in range(H):
+            g = h // (H // G)
+            s = k[rows, g] @ q[t, h] * scale
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            out[t, h], sums[t, h] = w @ v[rows, g], w @ np.abs(v[rows, g])
+            mass[t, h] = (np.abs(k[rows, g]) @ np.abs(q[t, h])).max() * abs(scale)
+            keys[t, h] = len(rows)
+    return out, sums, mass, keys
+
+
+def attention_own_tolerance(sums, mass, keys, D, exact_scores=False):
+    """How far attention may be from 64 bits, output by output, relative to its own sum of w |v|. A
+    score's operands are held to 8 EPS24 (three bf16 parts with six products; fp16 halves 2), its D
+    products added in at most D / 4 + 8 roundings and scaled in 3. A weight is the exponential (2) of
+    that, held to 8, and counts in numerator and denominator, whose sums over the keys take at most
+    keys / 4 + 16 roundings each. Where operands are of so few bits that products and their sums are
+    exact (exact_scores), a score is rounded by its scaling alone."""
+    ds = mass * (3 if exact_scores else 8 + D / 4 + 8 + 3)
+    return sums * (2 * (ds + 2 + 8 + keys / 4 + 16) * EPS24)[..., None]
+
+
+def halves(x, exp, low):
+    """x as the high and low fp16 halves of x * 2^exp, the low one times 2^low, each in 64 bits and scaled
+    back: what the fp16 matrix cores are given."""
+    y = np.asarray(x, np.float32).astype(np.float64) * 2.0 ** exp
+    hi = y.astype(np.float16).astype(np.float64)
+    lo = ((y - hi) * 2.0 ** low).astype(np.float16).astype(np.float64)
+    return hi * 2.0 ** -exp, lo * 2.0 ** -(low + exp)
+
+
+def bf16_parts(x):
+    """x as three bf16 parts, each cut."""
+    out, rest = [], np.asarray(x, np.float32)
+    for _ in range(3):
+        p = (rest.view(np.uint32) & np.uint32(0xffff0000)).view(np.float32)
+        out.append(p.astype(np.float64))
+        rest = (rest - p).astype(np.float32)
+    return out
+
+
+def attention_form(b: Batch, q, H, form, window=-1, scale=0.0):
+    """Attention as a form of the kernels' products has it, everything else in 64 bits. form:
+    "f32"          plain: float32 throughout
+    "halves"       queries and weights as two fp16 halves, the low one times 2^12
+    "one scale"    the same with the low half unscaled
+    "no low q", "no low w"    without the one or the other low half
+    "six", "three"            three bf16 parts of everything, six products, three of them
+    [tokens, H, D]; rows of no request are NaN."""
+    G, D = b.G, b.D
+    scale = scale or 1.0 / math.sqrt(D)
+    f32 = form == "f32"
+    k, v = (x.reshape(-1, G, D).astype(np.float32) for x in (b.k, b.v))
+    q = q.reshape(b.tokens, H, D).astype(np.float32)
+    out = np.full((b.tokens, H, D), np.nan)
+    low = 0 if form == "one scale" else 12
+
+    def product(a, x, exp, drop):   # a [keys, D] and x: matrix by vector or vector by matrix, in a's order
+        if form in ("six", "three"):
+            pairs = [(2, 0), (1, 1), (0, 2), (1, 0), (0, 1), (0, 0)][0 if form == "six" else 3:]
+            pa, px = bf16_parts(a), bf16_parts(x)
+            return sum(pa[i] @ px[j] for i, j in pairs)
+        hi, lo = halves(x, exp, low)
+        return a.astype(np.float64) @ hi + (0.0 if drop else a.astype(np.float64) @ lo)
+
+    for t, r, pos in b.each_token():
+        lo_key = max(0, pos - window + 1) if window >= 0 else 0
+        rows = np.array([x for x in (b.row(r, j) for j in range(lo_key, pos + 1)) if x >= 0], np.int64)
+        for h in range(H):
+            kk, vv = k[rows, h // (H // G)], v[rows, h // (H // G)]
+            if f32:
+                s = (kk @ q[t, h]) * np.float32(scale)
+                w = np.exp(s - s.max())
+                out[t, h] = (w @ vv) / w.sum(dtype=np.float32)
+                continue
+            e = 15 - int(np.frexp(np.abs(q[t, h]).max())[1])
+            s = product(kk, q[t, h], e, form == "no low q") * scale
+            w = np.exp(s - s.max()).astype(np.float32)
+            out[t, h] = product(vv.T.copy(), w, 11, form == "no low w") / w.sum(dtype=np.float64)
+    return out
