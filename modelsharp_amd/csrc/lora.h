@@ -292,7 +292,8 @@ __global__ __launch_bounds__(64 * kLoraLdsWaves) void lora_shrink_lds_kernel(Lor
 
 // grid: tiles of 16 `subs` tokens * slots * ceil(N / 256). For 16 tokens after 16:
 //   the threads take h (4 ranks of a token each, the splits added in their order) to LDS: for fp16
-//     weights as two halves of h 2^-e (22 bits, e by token, so that any fp32 h fits);
+//     weights as two halves of h 2^-e (kLowExp: 22 bits down to 2^-28 of the token's largest, then an
+//     error of 2^-51 of that; e by token, so that any fp32 h fits);
 //   each wave multiplies 64 rows of B_a, in its registers as long as the class does not change, with
 //     each class's tokens, and leaves scale * sum in LDS;
 //   the threads add it to the base and store, whole rows of 1 KB at a time.
@@ -385,7 +386,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots,
                     for (int j = 0; j < 4; ++j) {
                         const float v = __builtin_amdgcn_ldexpf(h[j], -e);
                         hi[j] = (_Float16)v;
-                        lo[j] = (_Float16)(v - (float)hi[j]);
+                        lo[j] = (_Float16)((v - (float)hi[j]) * (1 << kLowExp));
                     }
                     *reinterpret_cast<decltype(hi)*>(h0 + ht * HS + hr) = hi;
                     *reinterpret_cast<decltype(lo)*>(h0 + (kLoraTokens + ht) * HS + hr) = lo;
@@ -434,9 +435,9 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots,
                             for (int nt = 0; nt < 4; ++nt) lora_keep<E, T>(bv[q][nt], rank - (r0 + C * q + E * grp));
                     held = a;
                 }
-                floatx4_t acc[4];
+                floatx4_t acc[4], low[4];
 #pragma unroll
-                for (int nt = 0; nt < 4; ++nt) acc[nt] = floatx4_t{};
+                for (int nt = 0; nt < 4; ++nt) acc[nt] = low[nt] = floatx4_t{};
 #pragma unroll
                 for (int q = 0; q < CH; ++q)
 #pragma unroll
@@ -444,10 +445,11 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots,
                         if constexpr (F16) {
 #pragma unroll
                             for (int k = 1; k >= 0; --k) {
+                                floatx4_t& sum = k ? low[nt] : acc[nt];
                                 if constexpr (C == 32)
-                                    acc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[q][nt], hv[k][q], acc[nt], 0, 0, 0);
+                                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[q][nt], hv[k][q], sum, 0, 0, 0);
                                 else
-                                    acc[nt] = __builtin_amdgcn_mfma_f32_16x16x16f16(bv[q][nt], hv[k][q], acc[nt], 0, 0, 0);
+                                    sum = __builtin_amdgcn_mfma_f32_16x16x16f16(bv[q][nt], hv[k][q], sum, 0, 0, 0);
                             }
                         } else {
 #pragma unroll
@@ -461,7 +463,9 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p, int slots,
                         floatx4_t* const y = reinterpret_cast<floatx4_t*>(yl + l16 * YS + 64 * wave + 16 * nt + 4 * grp);
                         floatx4_t v;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = scale * (F16 ? __builtin_amdgcn_ldexpf(acc[nt][i], e) : acc[nt][i]);
+                        for (int i = 0; i < 4; ++i)
+                            v[i] = scale * (F16 ? __builtin_amdgcn_ldexpf(__builtin_fmaf(low[nt][i], kLow, acc[nt][i]), e)
+                                                : acc[nt][i]);
                         *y = r0 == 0 ? v : *y + v;
                     }
             }

@@ -206,17 +206,14 @@ template <> struct PagedElem<float> {
 
 constexpr float kGrow = 4.0f;     // the running maximum moves in steps above 2^4
 constexpr int kWeightExp = 11;    // weights times 2^11: at most 2^15 in fp16
-// The low halves of weights and queries are held times 2^12 and summed apart: a half ulp of the high
-// half becomes at most 2^15, and what is left of a value so small that its high half is subnormal
-// keeps its bits: 22 bits down to 2^-25 of a row's largest weight (2^-28 of its largest query), then an
-// error of 2^-48 (2^-51) of the largest. With one scale for both, they went from 2^-14 on: 1.4e-3 of a row where weights of 2^-30
-// met values 2^25 larger. The join of the sums costs single tokens 0 to 3%, and chunks, which the
-// vector unit's share of a block of keys slows down, 7 to 14% (512 tokens of 28 / 4 heads of 128 over 16000
-// keys: 235 us before, 257 now), at 256 channels 27%. Kept over all blocks instead, the low halves'
-// sums spilled (64 registers more at 128 channels), and left out for queries without small values, by a
-// branch, they cost the products their order: 286 us.
-constexpr int kLowExp = 12;
-constexpr float kLow = 1.0f / (1 << kLowExp);
+// The low halves of weights and queries are summed apart (kLowExp): 22 bits down to 2^-25 of a row's
+// largest weight (2^-28 of its largest query), then an error of 2^-48 (2^-51) of the largest. With one
+// scale for both, bits went from 2^-14 on: 1.4e-3 of a row where weights of 2^-30 met values 2^25
+// larger. The join of the sums costs single tokens 0 to 3%, and chunks, which the vector unit's share of
+// a block of keys slows down, 7 to 14% (512 tokens of 28 / 4 heads of 128 over 16000 keys: 235 us before,
+// 257 now), at 256 channels 27%. Kept over all blocks instead, the low halves' sums spilled (64 registers
+// more at 128 channels), and left out for queries without small values, by a branch, they cost the
+// products their order: 286 us.
 
 // Steps of 16 keys in a wave's registers: the one in use and those on their way. A third for fp16 at
 // D = 128 made no difference (47.1 against 46.2 us for 32 tokens over 1000-4000 keys).

@@ -10,6 +10,12 @@
 
 namespace msnb {
 
+// An fp32 value as two fp16 halves, the low one times 2^12 with a sum of its own: a half ulp of a
+// high half below 2^15 becomes at most 2^15, and what is left of a value so small that its high
+// half is subnormal keeps its bits.
+constexpr int kLowExp = 12;
+constexpr float kLow = 1.0f / (1 << kLowExp);
+
 // n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery's round-up method):
 // with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(n, m) + n) >> s.
 struct FastDiv {
