@@ -475,8 +475,9 @@ int ms_hip_paged_append(const ms_hip_paged_desc* desc, const float* dQ, const fl
  * and softmax weights count with 22 bits, those below 2^-28 of their row's largest query or 2^-25 of
  * its largest weight with an error of up to 2^-51 or 2^-48 of it; over an fp32 cache requests of
  * many rows take products to 2^-21, and values below 2^-110 may count with an error of up to
- * 2^-126. What a query does not see does not reach it, infinities and NaN included. The workspace is optional (a smaller, misaligned or NULL one: the keys of a tile of queries are not
- * shared out); calls that may overlap need one each. */
+ * 2^-126. What a query does not see does not reach it, infinities and NaN included. The workspace is
+ * optional (a smaller, misaligned or NULL one: the keys of a tile of queries are not shared out);
+ * calls that may overlap need one each. */
 int64_t ms_hip_paged_attention_workspace_size(const ms_hip_paged_desc* desc);
 int ms_hip_paged_attention(const ms_hip_paged_desc* desc, const float* dQ, const int32_t* dCu,
                            const int32_t* dPast, const int32_t* dTable, const void* dKCache,

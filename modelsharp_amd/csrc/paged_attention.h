@@ -740,7 +740,7 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
             ahead[i] = t.klast - key;
         }
     };
-    bool missing = false;   // a page that is not there
+    bool missing = false;   // a page that some row of the tile sees and that is not there
     // the next block's loads: into registers, or into LDS buffer `buf`, where lane i of a load
     // fills slot i of its 64, so that the lanes fetch the chunks that belong there. Rows of a
     // page that is not there are any row's, and the tile is done over, below.
@@ -749,7 +749,8 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
         for (int i = 0; i < UN; ++i) {
             const bool there = (unsigned)page[i] < (unsigned)p.b.num_pages;
             const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : 0) * hs;
-            missing |= !there;
+            const int key = t.klast - ahead[i];   // a page that no row of the tile sees may be gone
+            missing |= !there && key + (WHOLE ? RW - 1 : 0) >= kr.klo && key <= kr.khi;
             if constexpr (WHOLE) {   // a scalar base and 32-bit offsets
                 const int last = there ? ahead[i] : 0;
                 const uint32_t off = min(lane / CH, last) * (uint32_t)hs * (uint32_t)sizeof(T);
