@@ -478,6 +478,7 @@ int ms_hip_paged_append(const ms_hip_paged_desc* desc, const float* dQ, const fl
  * 2^-126. What a query does not see does not reach it, infinities and NaN included. The workspace is
  * optional (a smaller, misaligned or NULL one: the keys of a tile of queries are not shared out);
  * calls that may overlap need one each. */
+int ms_hip_paged_attention_check(const ms_hip_paged_desc* desc);   /* before an append whose attention is to follow */
 int64_t ms_hip_paged_attention_workspace_size(const ms_hip_paged_desc* desc);
 int ms_hip_paged_attention(const ms_hip_paged_desc* desc, const float* dQ, const int32_t* dCu,
                            const int32_t* dPast, const int32_t* dTable, const void* dKCache,

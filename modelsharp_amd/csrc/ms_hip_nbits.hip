@@ -3383,6 +3383,19 @@ int ms_hip_qk_norm_rotary(const ms_hip_qk_norm_desc* d, const float* dQ, const f
     return MS_HIP_OK;
 }
 
+int ms_hip_paged_attention_check(const ms_hip_paged_desc* d)
+{
+    if (int st = ms_hip_paged_check(d)) return st;
+    if (d->head_dim % 8 != 0 || d->head_dim > 256)
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_attention: head_dim=%d is not a multiple of 8 up to 256",
+                    d->head_dim);
+    const PagedAttnPlan plan = paged_plan(*d, -1);
+    if (plan.rows_grid + plan.blocks_grid >= 1 << 24)   // a launch has fewer than 2^32 threads
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_attention: %d tokens of %d requests need too many workgroups",
+                    d->tokens, d->requests);
+    return MS_HIP_OK;
+}
+
 int64_t ms_hip_paged_attention_workspace_size(const ms_hip_paged_desc* d)
 {
     return d && ms_hip_paged_check(d) == MS_HIP_OK ? paged_plan(*d, -1).ws_bytes : 0;
@@ -3393,10 +3406,7 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const in
                            void* dWorkspace, int64_t workspace_bytes, void* stream)
 {
     if (int st = gate()) return st;
-    if (int st = ms_hip_paged_check(d)) return st;
-    if (d->head_dim % 8 != 0 || d->head_dim > 256)
-        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_attention: head_dim=%d is not a multiple of 8 up to 256",
-                    d->head_dim);
+    if (int st = ms_hip_paged_attention_check(d)) return st;
     if (d->tokens == 0 || d->requests == 0) return MS_HIP_OK;
     if (!dQ || !dCu || !dPast || (!dTable && d->max_pages > 0) || !dKCache || !dVCache || !dOut)
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: null query, lengths, table, cache or output");
@@ -3407,9 +3417,6 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const in
     // (a negative limit is the plan's "no limit")
     const PagedAttnPlan plan =
         paged_plan(*d, dWorkspace && !misaligned16(dWorkspace) ? std::max<int64_t>(workspace_bytes, 0) : 0);
-    if (plan.rows_grid + plan.blocks_grid > INT_MAX)
-        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_attention: %d tokens of %d requests need too many workgroups",
-                    d->tokens, d->requests);
     PagedAttnArgs p{};
     p.b = paged_batch(*d, dCu, dPast, dTable);
     p.q = dQ;

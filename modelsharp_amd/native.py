@@ -76,6 +76,7 @@ _PROTOTYPES = {
     "ms_hip_gqa_workspace_size": (_c_i64, [_vp]),
     "ms_hip_paged_check": (_c_int, [_vp]),
     "ms_hip_paged_append": (_c_int, [_vp] * 15),
+    "ms_hip_paged_attention_check": (_c_int, [_vp]),
     "ms_hip_paged_attention_workspace_size": (_c_i64, [_vp]),
     "ms_hip_paged_attention": (_c_int, [_vp] * 9 + [_c_i64, _vp]),
     "ms_hip_qk_norm_check": (_c_int, [_vp]),
@@ -506,6 +507,11 @@ def paged_append(desc: PagedDesc, dQ, dK, dV, dQGamma, dKGamma, dCu, dPast, dTab
     """Norms per head, rotation, and append of the new keys and values to their pages."""
     check(load().ms_hip_paged_append(ctypes.byref(desc), dQ, dK, dV, dQGamma, dKGamma, dCu, dPast, dTable, dCos, dSin,
                                      dQOut, dKCache, dVCache, stream))
+
+
+def paged_attention_check(desc: PagedDesc):
+    """Raises what paged_attention would refuse of the descriptor."""
+    check(load().ms_hip_paged_attention_check(ctypes.byref(desc)))
 
 
 def paged_attention_workspace_size(desc: PagedDesc) -> int:

@@ -155,6 +155,7 @@ class HipPagedAttentionKernel(_Serving):
             cos, sin = self._rotary(node, ctx, 8, q.device)
             d.cos_rows, d.cos_cols = int(cos.shape[0]), int(cos.shape[1])
         gq, gk = (self._gamma(ctx, _optional(node, i), D, q.device) for i in (10, 11))
+        native.paged_attention_check(d)   # before the caches are written
         turned = torch.empty((T, H * D), dtype=torch.float32, device=q.device)
         out = torch.zeros_like(turned)
         st = _stream(q)
