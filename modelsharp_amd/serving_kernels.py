@@ -109,7 +109,9 @@ class HipPagedAttentionKernel(_Serving):
         if q.dim() != 2:
             raise ModelSharpException(f"PagedAttention supports only 2-D query [tokens, hidden]; got rank {q.dim()}.")
         T, hidden = int(q.shape[0]), int(q.shape[1])
-        packed = not (_optional(node, 1) and _optional(node, 2))
+        packed = not _optional(node, 1)
+        if packed != (not _optional(node, 2)):
+            raise ModelSharpException("PagedAttention key and value must be given together, or neither with a packed query.")
         unit = H + 2 * G if packed else H
         if hidden % unit != 0:
             raise ModelSharpException(f"PagedAttention query hidden {hidden} not divisible by {unit} heads.")

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from modelsharp_amd import native, serving_kernels
-from modelsharp_amd.graph import GraphContext, GraphNode
+from modelsharp_amd.graph import GraphContext, GraphNode, ModelSharpException
 from modelsharp_amd.serving_kernels import HipPagedAttentionKernel
 
 
@@ -59,3 +59,13 @@ def test_descriptors_that_attention_refuses():
         with pytest.raises(native.HipError, match=words):
             native.paged_attention_check(native.PagedDesc(**{**d, **kw}))
     assert native.load().ms_hip_paged_attention_check(None) == native.MS_HIP_ERR_INVALID
+
+
+@pytest.mark.parametrize("there", [1, 2], ids=["key", "value"])
+def test_key_and_value_come_together(on_the_host, there):
+    """One without the other is refused; it was read as a packed query."""
+    node, ctx = step(64)
+    node.inputs[there] = "kv"[there - 1]
+    with pytest.raises(ModelSharpException, match="key and value must be given together"):
+        run(node, ctx)
+    assert on_the_host == []
