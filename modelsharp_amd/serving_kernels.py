@@ -242,6 +242,8 @@ class HipLoraMatMulNBitsKernel(_Serving):
         """A tensor of adapter weights in its own type; initializers are uploaded once and kept."""
         torch = _torch()
         t = ctx.get_tensor(name)
+        if t.ndim != 3 or t.dtype not in (torch.float32, torch.float16, np.float32, np.float16):
+            raise ModelSharpException(f"LoraMatMulNBits '{name}' must be a 3-D fp32 or fp16 tensor.")
         if isinstance(t, np.ndarray):
             hit = self._weights.get(id(t)) if ctx.is_constant(name) else None
             if hit is not None and hit[0] is t:
@@ -249,9 +251,7 @@ class HipLoraMatMulNBitsKernel(_Serving):
             d = torch.from_numpy(np.ascontiguousarray(t)).to(device)
             if ctx.is_constant(name):
                 self._weights[id(t)] = (t, d)
-            t = d
-        if t.dim() != 3 or t.dtype not in (torch.float32, torch.float16):
-            raise ModelSharpException(f"LoraMatMulNBits '{name}' must be a 3-D fp32 or fp16 tensor.")
+            return d
         return t.to(device).contiguous()
 
     def _run(self, node: GraphNode, ctx: GraphContext) -> None:

@@ -6,7 +6,7 @@ import pytest
 
 from modelsharp_amd import native, serving_kernels
 from modelsharp_amd.graph import GraphContext, GraphNode, ModelSharpException
-from modelsharp_amd.serving_kernels import HipPagedAttentionKernel
+from modelsharp_amd.serving_kernels import HipLoraMatMulNBitsKernel, HipPagedAttentionKernel
 
 
 @pytest.fixture
@@ -69,3 +69,20 @@ def test_key_and_value_come_together(on_the_host, there):
     with pytest.raises(ModelSharpException, match="key and value must be given together"):
         run(node, ctx)
     assert on_the_host == []
+
+
+@pytest.mark.parametrize("bad", [np.zeros((1, 2, 8), np.float64), np.zeros((2, 8), np.float16),
+                                 np.zeros((1, 2, 8), np.int32)], ids=["f64", "2-D", "i32"])
+def test_a_refused_adapter_initializer_is_refused_again(bad):
+    """(It was kept before it was looked at: the second call took 64-bit weights as 32-bit ones.)"""
+    import torch
+    k = HipLoraMatMulNBitsKernel()
+    ctx = GraphContext({"w": bad}, ["w"])
+    for _ in range(3):
+        with pytest.raises(ModelSharpException, match="3-D fp32 or fp16"):
+            k._adapter(ctx, "w", torch.device("cpu"))
+    assert not k._weights
+    good = np.zeros((1, 2, 8), np.float16)
+    ctx = GraphContext({"w": good}, ["w"])
+    first = k._adapter(ctx, "w", torch.device("cpu"))
+    assert k._adapter(ctx, "w", torch.device("cpu")).data_ptr() == first.data_ptr()   # uploaded once
