@@ -477,7 +477,8 @@ int ms_hip_paged_append(const ms_hip_paged_desc* desc, const float* dQ, const fl
  * many rows take products to 2^-21, and values below 2^-110 may count with an error of up to
  * 2^-126. What a query does not see does not reach it, infinities and NaN included. The workspace is
  * optional (a smaller, misaligned or NULL one: the keys of a tile of queries are not shared out);
- * calls that may overlap need one each. */
+ * calls that may overlap need one each. Neither it nor dOut may overlap an input, nor they each
+ * other (MS_HIP_ERR_INVALID). */
 int ms_hip_paged_attention_check(const ms_hip_paged_desc* desc);   /* before an append whose attention is to follow */
 int64_t ms_hip_paged_attention_workspace_size(const ms_hip_paged_desc* desc);
 int ms_hip_paged_attention(const ms_hip_paged_desc* desc, const float* dQ, const int32_t* dCu,
@@ -505,9 +506,10 @@ int ms_hip_qk_norm_rotary(const ms_hip_qk_norm_desc* desc, const float* dQ, cons
  * fp32 or fp16 (weight_type); dRanks int32 [adapters] (null: max_rank; rows of A and columns of
  * B from an adapter's rank on are not used), dScales fp32 [adapters] (null: 1). max_rank up to
  * 1024. fp32 accuracy (beside fp16 weights A_a x[t] counts with 22 bits, ranks below 2^-28 of the
- * token's largest with an error of up to 2^-51 of that), no atomics; a token with a value that is not finite has outputs that are not
- * finite, the others none of it. The workspace is needed, 16-byte aligned (a smaller or
- * misaligned one: MS_HIP_ERR_INVALID); calls that may overlap need one each. */
+ * token's largest with an error of up to 2^-51 of that), no atomics; a token with a value that is not
+ * finite has outputs that are not finite, the others none of it. The workspace is needed, 16-byte
+ * aligned (a smaller or misaligned one: MS_HIP_ERR_INVALID); calls that may overlap need one each.
+ * Neither it nor dY may overlap an input, but for dY on dBase (MS_HIP_ERR_INVALID). */
 typedef struct ms_hip_lora_desc {
     int tokens, K, N, adapters, max_rank, weight_type;
 } ms_hip_lora_desc;

@@ -3190,6 +3190,15 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb)
     return a && b && na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
 
+typedef std::pair<const void*, int64_t> Buffer;   // address (null: absent) and bytes
+
+bool overlap_any(const void* a, int64_t na, std::initializer_list<Buffer> others)
+{
+    for (const auto& [b, nb] : others)
+        if (overlap(a, na, b, nb)) return true;
+    return false;
+}
+
 int check_heads(const char* op, int tokens, int heads, int kv_heads, int head_dim)
 {
     if (heads <= 0 || kv_heads <= 0 || heads > 65535)
@@ -3322,11 +3331,14 @@ int ms_hip_paged_append(const ms_hip_paged_desc* d, const float* dQ, const float
     append_rotary(p, d->do_rotary, d->rotary_interleaved, d->cos_rows, d->cos_cols, dCos, dSin);
     const int64_t qs = span(T, p.q_stride, qw) * f, ks = span(T, p.k_stride, kw) * f, vs = span(T, p.v_stride, kw) * f;
     const int64_t cb = cache_bytes(*d), ob = T * qw * f;
+    const int64_t rb = p.rot_half ? (int64_t)p.cos_rows * p.half * f : 0, gb = p.D * f;
     bool clash = overlap(dQOut, ob, dQ, qs) && !(dQOut == dQ && p.q_stride == qw);
-    clash |= overlap(dQOut, ob, dK, ks) || overlap(dQOut, ob, dV, vs) || overlap(dQOut, ob, dKCache, cb) ||
-             overlap(dQOut, ob, dVCache, cb) || overlap(dKCache, cb, dVCache, cb);
-    for (const void* c : {(const void*)dKCache, (const void*)dVCache})
-        clash |= overlap(c, cb, dQ, qs) || overlap(c, cb, dK, ks) || overlap(c, cb, dV, vs);
+    clash |= overlap_any(dQOut, ob, {{dKCache, cb}, {dVCache, cb}}) || overlap(dKCache, cb, dVCache, cb);
+    for (const auto& [o, bytes] : {Buffer{dQOut, ob}, Buffer{dKCache, cb}, Buffer{dVCache, cb}})
+        clash |= (o != dQOut && overlap(o, bytes, dQ, qs)) ||
+                 overlap_any(o, bytes, {{dK, ks}, {dV, vs}, {dQGamma, gb}, {dKGamma, gb}, {dCu, (d->requests + 1ll) * 4},
+                                        {dPast, d->requests * 4ll}, {dTable, 4ll * d->requests * d->max_pages},
+                                        {dCos, rb}, {dSin, rb}});
     if (clash) return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_append: an output overlaps an input or another output");
     MS_HIP_CHECK(launch_append(p, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;
@@ -3375,9 +3387,13 @@ int ms_hip_qk_norm_rotary(const ms_hip_qk_norm_desc* d, const float* dQ, const f
     p.eps = d->eps;
     append_rotary(p, d->do_rotary, d->rotary_interleaved, d->cos_rows, d->cos_cols, dCos, dSin);
     const int64_t qs = span(T, p.q_stride, qw) * f, ks = span(T, p.k_stride, kw) * f, qb = T * qw * f, kb = T * kw * f;
-    if ((overlap(dQOut, qb, dQ, qs) && !(dQOut == dQ && p.q_stride == qw)) ||
-        (overlap(dKOut, kb, dK, ks) && !(dKOut == dK && p.k_stride == kw)) || overlap(dQOut, qb, dK, ks) ||
-        overlap(dKOut, kb, dQ, qs) || overlap(dQOut, qb, dKOut, kb))
+    const int64_t rb = p.rot_half ? (int64_t)p.cos_rows * p.half * f : 0, gb = p.D * f, pb = p.positions ? T * 4 : 0;
+    bool clash = (overlap(dQOut, qb, dQ, qs) && !(dQOut == dQ && p.q_stride == qw)) ||
+                 (overlap(dKOut, kb, dK, ks) && !(dKOut == dK && p.k_stride == kw)) || overlap(dQOut, qb, dK, ks) ||
+                 overlap(dKOut, kb, dQ, qs) || overlap(dQOut, qb, dKOut, kb);
+    for (const auto& [o, bytes] : {Buffer{dQOut, qb}, Buffer{dKOut, kb}})
+        clash |= overlap_any(o, bytes, {{dQGamma, gb}, {dKGamma, gb}, {dPositions, pb}, {dCos, rb}, {dSin, rb}});
+    if (clash)
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] qk_norm_rotary: an output overlaps an input or another output");
     MS_HIP_CHECK(launch_append(p, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;
@@ -3436,11 +3452,12 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const in
     p.grp = FastDiv(p.H / p.kvH);
     p.scale2 = (d->scale != 0.0f ? d->scale : 1.0f / std::sqrt((float)p.D)) * 1.44269504088896341f;
     const int64_t ob = T * qw * f, cb = cache_bytes(*d);
-    if (overlap(dOut, ob, dQ, span(T, p.q_stride, qw) * f) || overlap(dOut, ob, dKCache, cb) || overlap(dOut, ob, dVCache, cb) ||
-        overlap(dOut, ob, dWorkspace, plan.ws_bytes))
+    const std::initializer_list<Buffer> inputs = {{dQ, span(T, p.q_stride, qw) * f}, {dKCache, cb}, {dVCache, cb},
+                                                  {dCu, (d->requests + 1ll) * 4}, {dPast, d->requests * 4ll},
+                                                  {dTable, 4ll * d->requests * d->max_pages}};
+    if (overlap_any(dOut, ob, inputs) || overlap(dOut, ob, dWorkspace, plan.ws_bytes))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the output overlaps an input or the workspace");
-    if (overlap(dWorkspace, plan.ws_bytes, dQ, span(T, p.q_stride, qw) * f) || overlap(dWorkspace, plan.ws_bytes, dKCache, cb) ||
-        overlap(dWorkspace, plan.ws_bytes, dVCache, cb))
+    if (overlap_any(dWorkspace, plan.ws_bytes, inputs))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the workspace overlaps an input");
     MS_HIP_CHECK(launch_paged_attention(p, plan, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;
@@ -3510,13 +3527,12 @@ int ms_hip_lora(const ms_hip_lora_desc* d, const float* dX, const void* dA, cons
     p.vec_y = !whole ? 0 : p.rank & 7 ? 4 : 8;
     const int64_t f = sizeof(float), yb = (int64_t)p.T * p.N * f, xb = (int64_t)p.T * p.K * f, e = f16 ? 2 : 4;
     const int64_t ab = (int64_t)p.adapters * p.rank * p.K * e, bb = (int64_t)p.adapters * p.rank * p.N * e;
-    if (overlap(dY, yb, dX, xb) || overlap(dY, yb, dA, ab) || overlap(dY, yb, dB, bb) ||
-        (dBase != dY && overlap(dY, yb, dBase, yb)))
+    const std::initializer_list<Buffer> inputs = {{dX, xb}, {dA, ab}, {dB, bb}, {dRanks, p.adapters * f},
+                                                  {dScales, p.adapters * f}, {dAdapters, p.T * f}};
+    if (overlap_any(dY, yb, inputs) || (dBase != dY && overlap(dY, yb, dBase, yb)))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: the output overlaps an input");
-    const std::pair<const void*, int64_t> others[] = {{dX, xb}, {dBase, yb}, {dY, yb}, {dA, ab}, {dB, bb}};
-    for (const auto& [x, bytes] : others)
-        if (overlap(dWorkspace, plan.ws_bytes, x, bytes))
-            return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: the workspace overlaps a buffer of the call");
+    if (overlap_any(dWorkspace, plan.ws_bytes, inputs) || overlap_any(dWorkspace, plan.ws_bytes, {{dBase, yb}, {dY, yb}}))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: the workspace overlaps a buffer of the call");
     MS_HIP_CHECK(launch_lora(p, plan, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;
 }

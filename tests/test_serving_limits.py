@@ -94,3 +94,34 @@ def test_lengths_that_make_no_sense_are_cut_to_the_tensors_rows(lengths):
         assert tiles == min(-(-count * grp // bm), 2 ** 24)
     # the most rows that a call may have
     assert lengths([(0, 1, 1, hi, 16), (0, 1, 1, hi, 128)]) == [(0, 1, 2 ** 24), (0, 1, 2 ** 24)]
+
+
+def test_outputs_do_not_overlap_the_small_inputs():
+    """Lengths, tables, norm weights, rotary caches, positions, ranks and scales are inputs too: an output or a
+    workspace on them is refused before anything is launched."""
+    at = [P + i * 64 * MB for i in range(14)]
+    q, k, v, gq, gk, cu, past, table, cos, sin, out, kc, vc, ws = at
+    d = paged(do_rotary=1, cos_rows=64, cos_cols=32)
+    good = [q, k, v, gq, gk, cu, past, table, cos, sin, out, kc, vc]
+    last = {gq: 63, gk: 63, cu: 2, past: 1, table: 2 * 4 - 1, cos: 64 * 32 - 1, sin: 64 * 32 - 1}   # elements
+    for i in (10, 11, 12):
+        for j in (3, 4, 5, 6, 7, 8, 9):
+            for x in (good[j], good[j] + 4 * last[good[j]] & ~15):
+                refused(lambda: native.paged_append(d, *[x if n == i else y for n, y in enumerate(good)]), 1, "overlaps")
+    d = paged(tokens=1, requests=1, num_pages=4096, max_pages=4096)
+    n = native.paged_attention_workspace_size(d)
+    assert n > 0
+    for x in (cu, past, table, table + 4 * 4092):
+        refused(lambda: native.paged_attention(d, q, cu, past, table, kc, vc, x), 1, "overlaps")
+        refused(lambda: native.paged_attention(d, q, cu, past, table, kc, vc, out, x, n), 1, "overlaps")
+    d = native.QkNormDesc(tokens=4, num_heads=4, kv_num_heads=2, head_dim=64, do_rotary=1, cos_rows=8, cos_cols=32)
+    good = [q, k, gq, gk, past, cos, sin, out, kc]
+    for i in (7, 8):
+        for j in (2, 3, 4, 5, 6):
+            refused(lambda: native.qk_norm_rotary(d, *[good[j] if n == i else y for n, y in enumerate(good)]), 1, "overlaps")
+    d = native.LoraDesc(tokens=4, K=64, N=32, adapters=2, max_rank=8, weight_type=native.MS_HIP_DTYPE_F16)
+    n = native.lora_workspace_size(d)
+    good = [q, k, v, gq, gk, cu, past, out, ws]   # x, a, b, ranks, scales, which, base, y, workspace
+    for i in (7, 8):
+        for j in (3, 4, 5):
+            refused(lambda: native.lora(d, *[good[j] if m == i else y for m, y in enumerate(good)], n), 1, "overlaps")
