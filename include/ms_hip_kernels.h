@@ -438,7 +438,12 @@ int ms_hip_gqa(const ms_hip_gqa_desc* desc, const float* dQ, const float* dK, co
  * dropped. The lengths
  * and the table are read on the device, so a captured step is replayed with new ones.
  *   max_new, max_total   bounds of any request's new tokens and of past + new tokens (0: not
- *                        known). They choose the launch; results do not depend on them.
+ *                        known). They choose the launch, and with it the order and form of the
+ *                        sums: results are of the same accuracy whatever they are, and the same
+ *                        bits for the same descriptor, workspace (there or not) and kind of device.
+ *                        Roomy bounds cost time, since the keys are shared out in parts of
+ *                        max_total (0: of the table): 32 single tokens of up to 4096 keys take
+ *                        twice as long with a bound of 32768.
  *   q_stride, ...        floats from one token's row to the next (0: rows lie back to back);
  *                        packed QKV rows are three pointers with one stride.
  *   rotary               as ms_hip_gqa's: cos/sin [cos_rows, cos_cols], positions past the

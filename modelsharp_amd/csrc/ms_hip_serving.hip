@@ -62,7 +62,9 @@ PagedAttnPlan paged_attention_plan(int64_t tokens, int requests, int64_t max_new
     // a tile of 16 rows keeps its keys together, without the merge: 500 in one 9.8, in 3 10.8.
     const int64_t bytes = keys * D * (f16 ? 2 : 4);
     const int64_t most = few && bytes <= (128 << 10) ? 1 : std::max(std::min<int64_t>(bytes >> 15, 16), bytes >> 17);
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)cus / (likely * kvH), most, 64}));
+    // (no more workgroups than a launch can have, should the bounds be far too small)
+    const int64_t fit = ((1 << 24) - 1) / std::max<int64_t>(1, (rows + blocks) * kvH);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)cus / (likely * kvH), most, 64, fit}));
     const int64_t ws = splits > 1 ? splits * tokens * H * (D + 2) * (int64_t)sizeof(float) : 0;
     if (ws_avail >= 0 && ws > ws_avail) splits = 1;
     pl.splits = (int)splits;

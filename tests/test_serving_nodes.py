@@ -54,6 +54,9 @@ def test_descriptors_that_attention_refuses():
     d = dict(tokens=4, requests=2, num_heads=4, kv_num_heads=2, head_dim=64, page_size=16, num_pages=8, max_pages=4,
              cache_type=native.MS_HIP_DTYPE_F16, local_window_size=-1)
     native.paged_attention_check(native.PagedDesc(**d))
+    # a bound that is far too small splits the keys less rather than pass what a launch can have
+    native.paged_attention_check(native.PagedDesc(**{**d, "tokens": 2 ** 21, "requests": 1, "max_new": 1, "num_pages": 2 ** 20,
+                                                     "max_pages": 2 ** 20}))
     for kw, words in ((dict(head_dim=36), "multiple of 8"), (dict(num_heads=3), "multiple of kv_num_heads"),
                       (dict(tokens=2 ** 26, max_new=1, num_heads=8, kv_num_heads=8, head_dim=8), "too many workgroups")):
         with pytest.raises(native.HipError, match=words):
