@@ -209,11 +209,11 @@ constexpr int kWeightExp = 11;    // weights times 2^11: at most 2^15 in fp16
 // The low halves of weights and queries are summed apart (kLowExp): 22 bits down to 2^-25 of a row's
 // largest weight (2^-28 of its largest query), then an error of 2^-48 (2^-51) of the largest. With one
 // scale for both, bits went from 2^-14 on: 1.4e-3 of a row where weights of 2^-30 met values 2^25
-// larger. The join of the sums costs single tokens 0 to 3%, and chunks, which the vector unit's share of
-// a block of keys slows down, 7 to 14% (512 tokens of 28 / 4 heads of 128 over 16000 keys: 235 us before,
-// 257 now), at 256 channels 27%. Kept over all blocks instead, the low halves' sums spilled (64 registers
-// more at 128 channels), and left out for queries without small values, by a branch, they cost the
-// products their order: 286 us.
+// larger. The joins of the sums cost single tokens 0 to 5%, and chunks, whose products hardly run beside
+// the vector unit, 7 to 16% (512 tokens of 28 / 4 heads of 128 over 16000 keys: 230-240 us before, 253-263
+// now), at 256 channels 28%. Tried against it: the low halves' sums kept over all blocks spill (64 more
+// registers at 128 channels), half of them kept gain 1%; a branch for queries without small values
+// costs the products their order (286 us), scores that start from their low halves' sum 264.
 
 // Steps of 16 keys in a wave's registers: the one in use and those on their way. A third for fp16 at
 // D = 128 made no difference (47.1 against 46.2 us for 32 tokens over 1000-4000 keys).
@@ -662,8 +662,8 @@ __device__ __forceinline__ int v_turn(int row)
 // 128 rows, since two such workgroups fill a CU's LDS (64 KB each at D = 128: two blocks of 64 keys) and
 // registers, and each block of keys is then read from L2 once for 128 rows. The matrix cores bound a
 // long chunk, and the vector unit, which the products hardly run beside: 512 tokens of 28 / 4 heads over
-// 16000 keys take 253-258 us with the merge, 470 TFLOP/s of attention and twice that of products (a library
-// product of 8192 reaches 1063). Fresh prompts of 200-650 tokens (46 us for five) are bound by the longest tile's chain of blocks. An fp32 cache, with six
+// 16000 keys take 253-263 us with the merge, 460 TFLOP/s of attention and twice that of products (a library
+// product of 8192 reaches 1063). Fresh prompts of 200-650 tokens (46-47 us for five) are bound by the longest tile's chain of blocks. An fp32 cache, with six
 // products a pair: two chunks of 300 tokens of 32 / 8 heads of 96, 1024 keys visible: 62 + 9 us.
 // WHOLE: pages of a multiple of 16 rows, so that a wave's rows of a load lie in one page: its lookups
 // are the scalar unit's.
