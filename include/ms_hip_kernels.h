@@ -435,8 +435,9 @@ int ms_hip_gqa(const ms_hip_gqa_desc* desc, const float* dQ, const float* dK, co
  * [requests, max_pages]). A request may have no new token. Rows behind the last request's are
  * left as they were, in every output. A table entry outside [0, num_pages), or a position past
  * the table or from 2^31 - 4096 on, is a page that is not there: its keys are masked, appends to it
- * dropped. The lengths
- * and the table are read on the device, so a captured step is replayed with new ones.
+ * dropped. (Pages wholly behind a window may be gone; a visible one that is costs a request of many
+ * rows its speed.) The lengths and the table are read on the device, so a captured step is replayed
+ * with new ones.
  *   max_new, max_total   bounds of any request's new tokens and of past + new tokens (0: not
  *                        known). They choose the launch, and with it the order and form of the
  *                        sums: results are of the same accuracy whatever they are, and the same

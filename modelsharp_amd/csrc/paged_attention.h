@@ -68,6 +68,13 @@ __device__ __forceinline__ bool paged_tile(const PagedAttnArgs& p, int idx, int 
     return false;
 }
 
+// The row of the cache that keys without one stand for: the request's last key's, so that what
+// nobody has written does not come in; the first where that has none either.
+__device__ __forceinline__ int paged_stand(const PagedBatch& b, const PagedTile& t)
+{
+    return t.klast >= 0 ? max(paged_row(b, t.r, t.klast), 0) : 0;
+}
+
 // Positions [lo, hi] that some row of the tile sees; split `sp` takes [klo, khi] of them, in
 // whole steps of `step`, all splits alike and split_min keys or more (so that short requests take
 // fewer splits, not smaller ones). Empty where khi < klo.
@@ -295,8 +302,10 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
     const int64_t hs = (int64_t)p.kvH * p.D;   // a cache row
     const T* const kc = static_cast<const T*>(p.kc) + (int64_t)g * p.D;
     const T* const vc = static_cast<const T*>(p.vc) + (int64_t)g * p.D;
-    // where 16 keys lie: looked up a step before their loads. Keys past the request's last stand for
-    // that one, and pages that are not there for the cache's first row; both are masked.
+    // where 16 keys lie: looked up a step before their loads. Keys past the request's last, and keys of
+    // pages that are not there, stand for the last one; both are masked. (WHOLE: steps without a page
+    // are left out, their loads any row's.)
+    const int stand = WHOLE ? 0 : paged_stand(p.b, t);
     struct Rows {
         int first;     // WHOLE: the row of the step's first key, -1: not there
         int k, v[4];   // else: this lane's rows of K and V, -1: not there
@@ -340,7 +349,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const int c = KV * grp + PagedElem<T>::kStep * s;
-                x.k[s] = *reinterpret_cast<const kvec_t*>(kc + max(r.k, 0) * hs + (c < p.D ? c : 0));
+                x.k[s] = *reinterpret_cast<const kvec_t*>(kc + (r.k >= 0 ? r.k : stand) * hs + (c < p.D ? c : 0));
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -348,7 +357,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const int ch = VEC * (l16 + 16 * c);
-                    x.v[i][c] = *reinterpret_cast<const vvec_t*>(vc + max(r.v[i], 0) * hs + (ch < p.D ? ch : 0));
+                    x.v[i][c] = *reinterpret_cast<const vvec_t*>(vc + (r.v[i] >= 0 ? r.v[i] : stand) * hs + (ch < p.D ? ch : 0));
                 }
             }
         }
@@ -660,11 +669,12 @@ __device__ __forceinline__ int v_turn(int row)
 // its maximum only in steps above 2^4, so that the accumulators are seldom rescaled.
 //
 // 128 rows, since two such workgroups fill a CU's LDS (64 KB each at D = 128: two blocks of 64 keys) and
-// registers, and each block of keys is then read from L2 once for 128 rows. The matrix cores bound a
-// long chunk, and the vector unit, which the products hardly run beside: 512 tokens of 28 / 4 heads over
-// 16000 keys take 253-263 us with the merge, 460 TFLOP/s of attention and twice that of products (a library
-// product of 8192 reaches 1063). Fresh prompts of 200-650 tokens (46-47 us for five) are bound by the longest tile's chain of blocks. An fp32 cache, with six
-// products a pair: two chunks of 300 tokens of 32 / 8 heads of 96, 1024 keys visible: 62 + 9 us.
+// registers, and each block of keys is then read from L2 once for 128 rows. The matrix cores and the vector
+// unit, hardly beside each other, bound a long chunk: 512 tokens of 28 / 4 heads over 16000 keys take
+// 253-263 us with the merge, 460 TFLOP/s of attention and twice that of products (a library product of
+// 8192 reaches 1063). Fresh prompts of 200-650 tokens (46-47 us for five) are bound by the longest tile's
+// chain of blocks. An fp32 cache, with six products a pair: two chunks of 300 tokens of 32 / 8 heads of
+// 96, 1024 keys visible: 62 + 9 us.
 // WHOLE: pages of a multiple of 16 rows, so that a wave's rows of a load lie in one page: its lookups
 // are the scalar unit's.
 template <typename T, int DP>
@@ -743,12 +753,14 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
     bool missing = false;   // a page that some row of the tile sees and that is not there
     // the next block's loads: into registers, or into LDS buffer `buf`, where lane i of a load
     // fills slot i of its 64, so that the lanes fetch the chunks that belong there. Rows of a
-    // page that is not there are any row's, and the tile is done over, below.
+    // page that is not there are the last key's; where a row of the tile sees them, the tile is done over,
+    // below.
+    const int stand = paged_stand(p.b, t);
     auto fetch = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < UN; ++i) {
             const bool there = (unsigned)page[i] < (unsigned)p.b.num_pages;
-            const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : 0) * hs;
+            const int64_t at = (int64_t)(there ? page[i] * p.b.page.div + slot[i] : stand) * hs;
             const int key = t.klast - ahead[i];   // a page that no row of the tile sees may be gone
             missing |= !there && key + (WHOLE ? RW - 1 : 0) >= kr.klo && key <= kr.khi;
             if constexpr (WHOLE) {   // a scalar base and 32-bit offsets

@@ -128,3 +128,23 @@ def test_pages_behind_a_window_may_be_gone(gpu, case, dtype):
     gone = run_attention(b, q, H, window)
     check_attention(gone, b, q, H, window)
     assert np.array_equal(gone, there)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("case", range(len(GONE)))
+def test_pages_gone_beside_a_page_of_nans(gpu, case, dtype):
+    """What stands for a page that is gone is a row of the request itself, not whatever the cache's first
+    page holds (never written, say): the same bits again."""
+    news, pasts, H, G, D, page, window = GONE[case]
+    b = ref.Batch(500 + case, news, pasts, G, D, page, dtype)
+    b.table[b.table >= 0] += 1            # page 0 is nobody's
+    b.num_pages += 1
+    b.k, b.v = (np.concatenate([np.full_like(x[:1], np.nan), x]) for x in (b.k, b.v))
+    q = b.rng.standard_normal((b.tokens, H * D)).astype(F32)
+    log(f"pages gone beside NaN {GONE[case]} {dtype.__name__}")
+    there = run_attention(b, q, H, window)
+    for r, past in enumerate(pasts):
+        b.table[r, :max(0, past - window + 1) // page] = -1
+    gone = run_attention(b, q, H, window)
+    check_attention(gone, b, q, H, window)
+    assert np.array_equal(gone, there)
