@@ -217,8 +217,8 @@ constexpr int kWeightExp = 11;    // weights times 2^11: at most 2^15 in fp16
 // largest weight (2^-28 of its largest query), then an error of 2^-48 (2^-51) of the largest. With one
 // scale for both, bits went from 2^-14 on: 1.4e-3 of a row where weights of 2^-30 met values 2^25
 // larger. The joins of the sums cost single tokens 0 to 5%, and chunks, whose products hardly run beside
-// the vector unit, 7 to 16% (512 tokens of 28 / 4 heads of 128 over 16000 keys: 230-240 us before, 253-263
-// now), at 256 channels 28%. Tried against it: the low halves' sums kept over all blocks spill (64 more
+// the vector unit, 7 to 17% (512 tokens of 28 / 4 heads of 128 over 16000 keys: 230-240 us before, 253-263
+// now), at 256 channels 30%. Tried against it: the low halves' sums kept over all blocks spill (64 more
 // registers at 128 channels), half of them kept gain 1%; a branch for queries without small values
 // costs the products their order (286 us), scores that start from their low halves' sum 264.
 
