@@ -525,6 +525,70 @@ int ms_hip_lora(const ms_hip_lora_desc* desc, const float* dX, const void* dA, c
                 const int32_t* dRanks, const float* dScales, const int32_t* dAdapters,
                 const float* dBase, float* dY, void* dWorkspace, int64_t workspace_bytes, void* stream);
 
+/* ---- around a step: its plan and end, and the next tokens --------------------------
+ * What a server's loop needs beside the step itself, on device pointers and a stream, nothing
+ * allocated, only kernel launches: plan -> append, attention, adapters -> ... -> sample -> commit
+ * can be captured as one graph and replayed, without a copy to the host. The calling thread's
+ * current device must be the buffers'. No counterpart in the reference.
+ *
+ * A step's plan from what each request wants: dWant int32 [requests] new tokens (0 or less:
+ * none) after dPast int32 [requests] cached ones, and the free pages, a stack dFree int32
+ * [num_pages] of which [0, dFreeCount[0]) are free. A request is served as a whole or not at
+ * all: if its pages fit the table, the sum of what is wanted up to and with it is at most
+ * `tokens`, and it needs no new page or the sum of the pages needed up to and with it is at
+ * most the free ones (sums over the requests whose pages fit the table). Written:
+ *   dCu int32 [requests + 1]   the step's rows, cu of ms_hip_paged_append and _attention: request
+ *                              r is served where cu[r] < cu[r + 1]
+ *   dTable int32 [requests, max_pages]   the new pages of those served, from the top of the stack in
+ *                              order of requests and positions; all else stays
+ *   dUsed int32 [1]            how many pages those are
+ *   dRequests, dPositions, dSlots int32 [tokens]   of each row: its request (lora's adapters by
+ *                              request), its position (qk_norm_rotary's), and its row of the cache,
+ *                              page * page_size + position % page_size (-1: a page that is not
+ *                              there); all three -1 behind the last request's rows
+ * The stack and its count stay as they are, so that a plan can be made again; commit takes the
+ * pages. At most 8192 requests (else MS_HIP_ERR_UNSUPPORTED). No output may overlap an input or another
+ * output (MS_HIP_ERR_INVALID). */
+typedef struct ms_hip_step_desc {
+    int tokens, requests, page_size, num_pages, max_pages;
+} ms_hip_step_desc;
+int ms_hip_step_check(const ms_hip_step_desc* desc);
+int ms_hip_paged_plan(const ms_hip_step_desc* desc, const int32_t* dWant, const int32_t* dPast,
+                      const int32_t* dFree, const int32_t* dFreeCount, int32_t* dTable, int32_t* dCu,
+                      int32_t* dUsed, int32_t* dRequests, int32_t* dPositions, int32_t* dSlots, void* stream);
+/* The step's end: past[r] += cu[r + 1] - cu[r], and dUsed's pages leave the stack. Requests with dDone[r]
+ * not 0 (int32 [requests], null: none) have ended: their pages from table column dKeep[r] on (int32
+ * [requests], null: 0; the columns before it are a prefix that others share) go back on the
+ * stack in order of requests and positions, those entries become -1, past[r] 0. Entries outside
+ * [0, num_pages) are not pages and not returned. Once after each plan. */
+int ms_hip_paged_commit(const ms_hip_step_desc* desc, const int32_t* dCu, const int32_t* dUsed,
+                        const int32_t* dDone, const int32_t* dKeep, int32_t* dPast, int32_t* dTable,
+                        int32_t* dFree, int32_t* dFreeCount, void* stream);
+/* The next token of each row of logits (fp32 [rows, vocab], `stride` floats from row to row, 0: vocab)
+ * from given random numbers: w = exp((l - max l) / temperature); tokens in order of falling logits,
+ * equal ones by rising index; kept are the first top_k of them, of these the fewest whose w sum to
+ * at least top_p of theirs, of these the ones with w >= min_p (the first always). dTokens int32
+ * [rows]: the first token by index at which the kept w sum to more than random times all of
+ * theirs; dLogProbs fp32 [rows] (or null): the log of its share of them. Each setting is an array
+ * of its own value a row: dTemperature fp32 (null: 1; 0 or less or NaN: the likeliest token), dTopK
+ * int32 (null, 0 or less: all), dTopP fp32 (null, 1 or more or NaN: all; 0 or less: the
+ * likeliest), dMinP fp32 (null, 0 or less or NaN: none), dRandom fp32 in [0, 1) (what is outside counts
+ * as its nearest end). A NaN logit counts as -infinity; with one of +infinity only those are drawn;
+ * a row without a logit above -infinity has token -1 and log-probability NaN. Weights count in
+ * 64 bits, as multiples of 2^-44 (vocabularies above 2^18: of 2^-62 times the next power of two), so a
+ * token is that of the 64-bit definition but where that lies within such a step, and the same on
+ * every run. vocab up to 2^24. The workspace is needed, 16-byte aligned (a smaller or misaligned one:
+ * MS_HIP_ERR_INVALID; size 0: none); calls that may overlap need one each. No output may overlap an
+ * input, the workspace or the other output (MS_HIP_ERR_INVALID). */
+typedef struct ms_hip_sample_desc {
+    int rows, vocab, stride;
+} ms_hip_sample_desc;
+int ms_hip_sample_check(const ms_hip_sample_desc* desc);
+int64_t ms_hip_sample_workspace_size(const ms_hip_sample_desc* desc);
+int ms_hip_sample(const ms_hip_sample_desc* desc, const float* dLogits, const float* dTemperature,
+                  const int32_t* dTopK, const float* dTopP, const float* dMinP, const float* dRandom,
+                  int32_t* dTokens, float* dLogProbs, void* dWorkspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

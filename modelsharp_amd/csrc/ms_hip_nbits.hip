@@ -55,6 +55,7 @@
 #include "mfma_w4_pipe.h"
 #include "mfma_w4_rb.h"
 #include "serving.h"
+#include "serving_loop.h"
 #include "skinny_w4.h"
 
 using namespace msnb;
@@ -3534,6 +3535,168 @@ int ms_hip_lora(const ms_hip_lora_desc* d, const float* dX, const void* dA, cons
     if (overlap_any(dWorkspace, plan.ws_bytes, inputs) || overlap_any(dWorkspace, plan.ws_bytes, {{dBase, yb}, {dY, yb}}))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] lora: the workspace overlaps a buffer of the call");
     MS_HIP_CHECK(launch_lora(p, plan, static_cast<hipStream_t>(stream)));
+    return MS_HIP_OK;
+}
+
+}  // extern "C"
+
+// =========================================================================================
+// Around a step: its plan and end, and the next tokens (kernels in ms_hip_loop.hip).
+namespace {
+
+// Whether an output overlaps an input or another output.
+bool outputs_clash(std::initializer_list<Buffer> outputs, std::initializer_list<Buffer> inputs)
+{
+    for (auto o = outputs.begin(); o != outputs.end(); ++o) {
+        if (overlap_any(o->first, o->second, inputs)) return true;
+        for (auto q = outputs.begin(); q != o; ++q)
+            if (overlap(o->first, o->second, q->first, q->second)) return true;
+    }
+    return false;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ms_hip_step_check(const ms_hip_step_desc* d)
+{
+    if (!d) return fail(MS_HIP_ERR_INVALID, "[ms_hip] null step descriptor");
+    if (d->tokens < 0 || d->tokens > (1 << 29))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] step: %d tokens are out of range", d->tokens);
+    if (d->requests < 0 || d->max_pages < 0) return fail(MS_HIP_ERR_INVALID, "[ms_hip] step: negative sizes");
+    if (d->page_size <= 0 || d->num_pages <= 0)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] step: page_size and num_pages must be positive");
+    if ((int64_t)d->num_pages * d->page_size > INT_MAX)
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] step: the cache has more than 2^31-1 rows");
+    if (d->requests > kPlanRequests)
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] step: %d requests are more than %d", d->requests, kPlanRequests);
+    if ((int64_t)d->requests * d->max_pages > INT_MAX)
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] step: the table has more than 2^31-1 entries");
+    return MS_HIP_OK;
+}
+
+int ms_hip_paged_plan(const ms_hip_step_desc* d, const int32_t* dWant, const int32_t* dPast, const int32_t* dFree,
+                      const int32_t* dFreeCount, int32_t* dTable, int32_t* dCu, int32_t* dUsed, int32_t* dRequests,
+                      int32_t* dPositions, int32_t* dSlots, void* stream)
+{
+    if (int st = gate()) return st;
+    if (int st = ms_hip_step_check(d)) return st;
+    const int64_t R = d->requests, T = d->tokens, table = R * d->max_pages * 4;
+    if ((R && (!dWant || !dPast)) || !dFree || !dFreeCount || (!dTable && table) || !dCu || !dUsed ||
+        (T && (!dRequests || !dPositions || !dSlots)))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_plan: null lengths, free pages, table or output");
+    for (const void* x : {(const void*)dWant, (const void*)dPast, (const void*)dFree, (const void*)dFreeCount,
+                          (const void*)dTable, (const void*)dCu, (const void*)dUsed, (const void*)dRequests,
+                          (const void*)dPositions, (const void*)dSlots})
+        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_plan: buffers must be 4-byte aligned");
+    if (outputs_clash({{dTable, table}, {dCu, (R + 1) * 4}, {dUsed, 4}, {dRequests, T * 4}, {dPositions, T * 4}, {dSlots, T * 4}},
+                      {{dWant, R * 4}, {dPast, R * 4}, {dFree, d->num_pages * 4ll}, {dFreeCount, 4}}))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_plan: an output overlaps an input or another output");
+    PlanArgs p{};
+    p.want = dWant;
+    p.past = dPast;
+    p.free = dFree;
+    p.free_count = dFreeCount;
+    p.table = dTable;
+    p.cu = dCu;
+    p.used = dUsed;
+    p.request = dRequests;
+    p.position = dPositions;
+    p.slot = dSlots;
+    p.tokens = d->tokens;
+    p.requests = d->requests;
+    p.num_pages = d->num_pages;
+    p.max_pages = d->max_pages;
+    p.page = FastDiv(d->page_size);
+    MS_HIP_CHECK(launch_plan(p, device_cus(), static_cast<hipStream_t>(stream)));
+    return MS_HIP_OK;
+}
+
+int ms_hip_paged_commit(const ms_hip_step_desc* d, const int32_t* dCu, const int32_t* dUsed, const int32_t* dDone,
+                        const int32_t* dKeep, int32_t* dPast, int32_t* dTable, int32_t* dFree, int32_t* dFreeCount,
+                        void* stream)
+{
+    if (int st = gate()) return st;
+    if (int st = ms_hip_step_check(d)) return st;
+    const int64_t R = d->requests, table = R * d->max_pages * 4;
+    if (!dCu || !dUsed || (R && !dPast) || (!dTable && table) || !dFree || !dFreeCount)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_commit: null lengths, table or free pages");
+    for (const void* x : {(const void*)dCu, (const void*)dUsed, (const void*)dDone, (const void*)dKeep, (const void*)dPast,
+                          (const void*)dTable, (const void*)dFree, (const void*)dFreeCount})
+        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_commit: buffers must be 4-byte aligned");
+    if (outputs_clash({{dPast, R * 4}, {dTable, table}, {dFree, d->num_pages * 4ll}, {dFreeCount, 4}},
+                      {{dCu, (R + 1) * 4}, {dUsed, 4}, {dDone, R * 4}, {dKeep, R * 4}}))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_commit: an output overlaps an input or another output");
+    CommitArgs p{};
+    p.cu = dCu;
+    p.used = dUsed;
+    p.done = dDone;
+    p.keep = dKeep;
+    p.past = dPast;
+    p.table = dTable;
+    p.free = dFree;
+    p.free_count = dFreeCount;
+    p.requests = d->requests;
+    p.num_pages = d->num_pages;
+    p.max_pages = d->max_pages;
+    p.page = FastDiv(d->page_size);
+    MS_HIP_CHECK(launch_commit(p, static_cast<hipStream_t>(stream)));
+    return MS_HIP_OK;
+}
+
+int ms_hip_sample_check(const ms_hip_sample_desc* d)
+{
+    if (!d) return fail(MS_HIP_ERR_INVALID, "[ms_hip] null sample descriptor");
+    if (d->rows < 0 || d->vocab <= 0)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] sample: rows must be at least 0, vocab at least 1");
+    if (d->stride && d->stride < d->vocab)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] sample: the row stride %d is below the row's width %d", d->stride, d->vocab);
+    if (d->vocab > kSampleVocab || d->rows > kSampleRows)
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] sample: %d rows of %d tokens are out of range", d->rows, d->vocab);
+    return MS_HIP_OK;
+}
+
+int64_t ms_hip_sample_workspace_size(const ms_hip_sample_desc* d)
+{
+    if (!d || ms_hip_sample_check(d) != MS_HIP_OK || d->rows == 0) return 0;
+    return sample_plan(d->rows, d->vocab, device_cus()).ws_bytes;
+}
+
+int ms_hip_sample(const ms_hip_sample_desc* d, const float* dLogits, const float* dTemperature, const int32_t* dTopK,
+                  const float* dTopP, const float* dMinP, const float* dRandom, int32_t* dTokens, float* dLogProbs,
+                  void* dWorkspace, int64_t workspace_bytes, void* stream)
+{
+    if (int st = gate()) return st;
+    if (int st = ms_hip_sample_check(d)) return st;
+    if (d->rows == 0) return MS_HIP_OK;
+    if (!dLogits || !dRandom || !dTokens) return fail(MS_HIP_ERR_INVALID, "[ms_hip] sample: null logits, random numbers or output");
+    for (const void* x : {(const void*)dLogits, (const void*)dTemperature, (const void*)dTopK, (const void*)dTopP,
+                          (const void*)dMinP, (const void*)dRandom, (const void*)dTokens, (const void*)dLogProbs})
+        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] sample: buffers must be 4-byte aligned");
+    const SamplePlan plan = sample_plan(d->rows, d->vocab, device_cus());
+    if (plan.ws_bytes && (!dWorkspace || misaligned16(dWorkspace) || workspace_bytes < plan.ws_bytes))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] sample needs a 16-byte aligned workspace of %lld bytes (got %lld)",
+                    (long long)plan.ws_bytes, (long long)(dWorkspace ? workspace_bytes : 0));
+    SampleArgs p{};
+    p.logits = dLogits;
+    p.temperature = dTemperature;
+    p.top_k = dTopK;
+    p.top_p = dTopP;
+    p.min_p = dMinP;
+    p.random = dRandom;
+    p.token = dTokens;
+    p.logprob = dLogProbs;
+    p.rows = d->rows;
+    p.vocab = d->vocab;
+    p.stride = d->stride ? d->stride : d->vocab;
+    p.frac = sample_frac(d->vocab);
+    const int64_t n = p.rows * 4ll;
+    if (outputs_clash({{dTokens, n}, {dLogProbs, n}, {dWorkspace, plan.ws_bytes}},
+                      {{dLogits, span(p.rows, p.stride, p.vocab) * 4}, {dTemperature, n}, {dTopK, n}, {dTopP, n}, {dMinP, n},
+                       {dRandom, n}}))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] sample: an output or the workspace overlaps another buffer of the call");
+    MS_HIP_CHECK(launch_sample(p, plan, dWorkspace, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;
 }
 

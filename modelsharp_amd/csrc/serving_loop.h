@@ -1,0 +1,70 @@
+// serving_loop.h — what a server's loop needs around a serving step's attention, kernels of a
+// code object of their own (ms_hip_loop.hip; formats.h says why they are apart from the others):
+//
+//   paged_plan.h        page tables, lengths, positions and slot maps from what requests want, and
+//                       the step's end
+//   sample.h            the next tokens from logits
+#pragma once
+#include "serving.h"
+
+namespace msnb {
+
+constexpr int kPlanRequests = 8192;   // two cumulative lengths of each in LDS: 64 KB
+
+struct PlanArgs {
+    const int32_t* want;
+    const int32_t* past;
+    const int32_t* free;         // a stack of pages: [0, free_count)
+    const int32_t* free_count;
+    int32_t* table;
+    int32_t* cu;
+    int32_t* used;
+    int32_t* request;            // [tokens]
+    int32_t* position;
+    int32_t* slot;
+    int tokens, requests, num_pages, max_pages;
+    FastDiv page;
+};
+MS_INTERNAL hipError_t launch_plan(const PlanArgs& p, int cus, hipStream_t s);
+
+struct CommitArgs {
+    const int32_t* cu;
+    const int32_t* used;
+    const int32_t* done;         // or null: none
+    const int32_t* keep;         // or null: 0
+    int32_t* past;
+    int32_t* table;
+    int32_t* free;
+    int32_t* free_count;
+    int requests, num_pages, max_pages;
+    FastDiv page;
+};
+MS_INTERNAL hipError_t launch_commit(const CommitArgs& p, hipStream_t s);
+
+struct SampleArgs {
+    const float* logits;
+    const float* temperature;    // [rows], or null: 1
+    const int32_t* top_k;        // or null: all
+    const float* top_p;          // or null: 1
+    const float* min_p;          // or null: 0
+    const float* random;
+    int32_t* token;
+    float* logprob;              // or null
+    int rows, vocab, frac;       // weights are whole multiples of 2^-frac
+    int64_t stride;
+};
+struct SamplePlan {
+    int64_t ws_bytes = 0;
+};
+MS_INTERNAL SamplePlan sample_plan(int rows, int vocab, int cus);
+MS_INTERNAL hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* workspace, hipStream_t s);
+constexpr int kSampleVocab = 1 << 24, kSampleRows = 1 << 20;
+// Weights are at most 2^frac: no sum over the vocabulary passes 2^62.
+inline int sample_frac(int vocab)
+{
+    int bits = 0;
+    while ((1 << bits) < vocab) ++bits;
+    return bits < 18 ? 44 : 62 - bits;
+}
+
+}  // namespace msnb

@@ -84,6 +84,12 @@ _PROTOTYPES = {
     "ms_hip_lora_check": (_c_int, [_vp]),
     "ms_hip_lora_workspace_size": (_c_i64, [_vp]),
     "ms_hip_lora": (_c_int, [_vp] * 10 + [_c_i64, _vp]),
+    "ms_hip_step_check": (_c_int, [_vp]),
+    "ms_hip_paged_plan": (_c_int, [_vp] * 12),
+    "ms_hip_paged_commit": (_c_int, [_vp] * 10),
+    "ms_hip_sample_check": (_c_int, [_vp]),
+    "ms_hip_sample_workspace_size": (_c_i64, [_vp]),
+    "ms_hip_sample": (_c_int, [_vp] * 10 + [_c_i64, _vp]),
     "ms_hip_nbits_weights_create_from_files": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int,
                                                         ctypes.POINTER(_vp)]),
     "ms_hip_debug_force_failure": (_c_int, [_c_int]),
@@ -539,3 +545,37 @@ def lora(desc: LoraDesc, dX, dA, dB, dRanks, dScales, dAdapters, dBase, dY, dWor
     """y[t] = base[t] + scale[a] B_a (A_a x[t]) with a = adapters[t]."""
     check(load().ms_hip_lora(ctypes.byref(desc), dX, dA, dB, dRanks, dScales, dAdapters, dBase, dY, dWorkspace,
                              workspace_bytes, stream))
+
+
+# ---- around a step (device pointers; 0 / None for an absent optional buffer) ----
+class StepDesc(ctypes.Structure):
+    """ms_hip_step_desc."""
+    _fields_ = [(n, ctypes.c_int) for n in ("tokens", "requests", "page_size", "num_pages", "max_pages")]
+
+
+class SampleDesc(ctypes.Structure):
+    """ms_hip_sample_desc."""
+    _fields_ = [(n, ctypes.c_int) for n in ("rows", "vocab", "stride")]
+
+
+def paged_plan(desc: StepDesc, dWant, dPast, dFree, dFreeCount, dTable, dCu, dUsed, dRequests, dPositions, dSlots,
+               stream=None):
+    """A step's cumulative lengths, new pages and rows from what each request wants."""
+    check(load().ms_hip_paged_plan(ctypes.byref(desc), dWant, dPast, dFree, dFreeCount, dTable, dCu, dUsed, dRequests,
+                                   dPositions, dSlots, stream))
+
+
+def paged_commit(desc: StepDesc, dCu, dUsed, dDone, dKeep, dPast, dTable, dFree, dFreeCount, stream=None):
+    """The step's end: lengths advance, pages leave the free stack, those of requests that ended return."""
+    check(load().ms_hip_paged_commit(ctypes.byref(desc), dCu, dUsed, dDone, dKeep, dPast, dTable, dFree, dFreeCount, stream))
+
+
+def sample_workspace_size(desc: SampleDesc) -> int:
+    return int(load().ms_hip_sample_workspace_size(ctypes.byref(desc)))
+
+
+def sample(desc: SampleDesc, dLogits, dTemperature, dTopK, dTopP, dMinP, dRandom, dTokens, dLogProbs=None, dWorkspace=None,
+           workspace_bytes=0, stream=None):
+    """The next token of each row of logits by temperature, top-k, top-p and min-p."""
+    check(load().ms_hip_sample(ctypes.byref(desc), dLogits, dTemperature, dTopK, dTopP, dMinP, dRandom, dTokens, dLogProbs,
+                               dWorkspace, workspace_bytes, stream))
