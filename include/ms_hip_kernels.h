@@ -491,6 +491,28 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* desc, const float* dQ, const
                            const int32_t* dPast, const int32_t* dTable, const void* dKCache,
                            const void* dVCache, float* dOut, void* dWorkspace, int64_t workspace_bytes,
                            void* stream);
+/* The same attention where groups of requests share a prefix (a system prompt, a document, the
+ * samples of one prompt), whose keys are read once for all rows of a group: group i's requests are
+ * [dGroups[i], dGroups[i + 1]) (dGroups int32 [groups + 1], not decreasing, in [0, requests];
+ * requests before the first and behind the last are in none), and their first dShared[i] positions
+ * (int32 [groups]) hold the same keys and values, cached by each of them (past[r] >= dShared[i]), as a
+ * rule in the same pages. They are read from the pages of the group's first request; a prefix need not
+ * end with a page. The result is that of ms_hip_paged_attention, of the same accuracy; where a group's
+ * requests do not agree so, its rows are unspecified. A call with local_window_size >= 0, without groups or without the workspace
+ * shares nothing, and is ms_hip_paged_attention.
+ *   max_shared, max_rest   bounds of the shared positions of a group and of any request's positions
+ *                          behind its prefix, new tokens among them (0: not known). They choose the
+ *                          launch, as max_new and max_total do. */
+typedef struct ms_hip_shared_desc {
+    int groups, max_shared, max_rest;
+} ms_hip_shared_desc;
+int ms_hip_paged_shared_attention_check(const ms_hip_paged_desc* desc, const ms_hip_shared_desc* shared);
+int64_t ms_hip_paged_shared_attention_workspace_size(const ms_hip_paged_desc* desc, const ms_hip_shared_desc* shared);
+int ms_hip_paged_shared_attention(const ms_hip_paged_desc* desc, const ms_hip_shared_desc* shared, const float* dQ,
+                                  const int32_t* dCu, const int32_t* dPast, const int32_t* dTable,
+                                  const int32_t* dGroups, const int32_t* dShared, const void* dKCache,
+                                  const void* dVCache, float* dOut, void* dWorkspace, int64_t workspace_bytes,
+                                  void* stream);
 /* The norms and the rotation alone, for GroupQueryAttention with do_rotary = 0: dQ [tokens,
  * num_heads * head_dim] and dK [tokens, kv_num_heads * head_dim] to dQOut and dKOut of the
  * same shape (each may be its input where rows lie back to back), at dPositions int32 [tokens]

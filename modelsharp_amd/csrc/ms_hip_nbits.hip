@@ -3252,6 +3252,66 @@ PagedAttnPlan paged_plan(const ms_hip_paged_desc& d, int64_t ws_avail)
                                 d.cache_type == MS_HIP_DTYPE_F16, ws_avail, device_cus());
 }
 
+// What the attention entries refuse of their buffers, and what their kernels share.
+int paged_attention_buffers(const char* op, const ms_hip_paged_desc& d, const float* q, const int32_t* cu, const int32_t* past,
+                            const int32_t* table, const void* kc, const void* vc, const float* out)
+{
+    if (!q || !cu || !past || (!table && d.max_pages > 0) || !kc || !vc || !out)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: null query, lengths, table, cache or output", op);
+    for (const void* x : {(const void*)q, (const void*)cu, (const void*)past, (const void*)table, (const void*)out})
+        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: buffers must be 4-byte aligned", op);
+    if (misaligned16(kc) || misaligned16(vc))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: the cache must be 16-byte aligned", op);
+    return MS_HIP_OK;
+}
+
+void paged_attention_args(PagedAttnArgs& p, const ms_hip_paged_desc& d, const float* q, const int32_t* cu, const int32_t* past,
+                          const int32_t* table, const void* kc, const void* vc, float* out, void* workspace)
+{
+    p.b = paged_batch(d, cu, past, table);
+    p.q = q;
+    p.kc = kc;
+    p.vc = vc;
+    p.out = out;
+    p.part = static_cast<float*>(workspace);
+    p.H = d.num_heads;
+    p.kvH = d.kv_num_heads;
+    p.D = d.head_dim;
+    p.window = d.local_window_size;
+    p.f16 = d.cache_type == MS_HIP_DTYPE_F16;
+    p.q_stride = d.q_stride ? d.q_stride : (int64_t)p.H * p.D;
+    p.grp = FastDiv(p.H / p.kvH);
+    p.scale2 = (d.scale != 0.0f ? d.scale : 1.0f / std::sqrt((float)p.D)) * 1.44269504088896341f;
+}
+
+int paged_attention_overlaps(const char* op, const ms_hip_paged_desc& d, const PagedAttnArgs& p, const int32_t* bounds,
+                             const int32_t* shared, int64_t groups, int64_t ws_bytes)
+{
+    const int64_t qw = (int64_t)p.H * p.D, T = d.tokens, f = sizeof(float), ob = T * qw * f, cb = cache_bytes(d);
+    const std::initializer_list<Buffer> inputs = {{p.q, span(T, p.q_stride, qw) * f}, {p.kc, cb}, {p.vc, cb},
+                                                  {p.b.cu, (d.requests + 1ll) * 4}, {p.b.past, d.requests * 4ll},
+                                                  {p.b.table, 4ll * d.requests * d.max_pages},
+                                                  {bounds, (groups + 1) * 4}, {shared, groups * 4}};
+    if (overlap_any(p.out, ob, inputs) || overlap(p.out, ob, p.part, ws_bytes))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: the output overlaps an input or the workspace", op);
+    if (overlap_any(p.part, ws_bytes, inputs))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: the workspace overlaps an input", op);
+    return MS_HIP_OK;
+}
+
+// The plan behind shared prefixes; splits 0: as if nothing were shared.
+SharedPlan shared_plan(const ms_hip_paged_desc& d, const ms_hip_shared_desc& s)
+{
+    if (d.local_window_size >= 0 || s.groups == 0) return {};   // (a window has left a long prefix behind)
+    const int64_t max_new = d.max_new > 0 ? std::min(d.max_new, d.tokens) : d.tokens;
+    int64_t keys = std::min<int64_t>((int64_t)d.max_pages * d.page_size, INT_MAX);
+    if (d.max_total > 0) keys = std::min<int64_t>(keys, d.max_total);
+    const int64_t prefix = s.max_shared > 0 ? std::min<int64_t>(keys, s.max_shared) : keys;
+    const int64_t rest = s.max_rest > 0 ? std::min<int64_t>(keys, s.max_rest) : keys;
+    return shared_attention_plan(d.tokens, d.requests, max_new, s.groups, prefix, rest, d.num_heads, d.kv_num_heads, d.head_dim,
+                                 d.cache_type == MS_HIP_DTYPE_F16, device_cus());
+}
+
 // What append and qk_norm_rotary share; the strides are in place.
 void append_rotary(AppendArgs& p, int do_rotary, int interleaved, int cos_rows, int cos_cols, const float* cos,
                    const float* sin)
@@ -3425,42 +3485,70 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* d, const float* dQ, const in
     if (int st = gate()) return st;
     if (int st = ms_hip_paged_attention_check(d)) return st;
     if (d->tokens == 0 || d->requests == 0) return MS_HIP_OK;
-    if (!dQ || !dCu || !dPast || (!dTable && d->max_pages > 0) || !dKCache || !dVCache || !dOut)
-        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: null query, lengths, table, cache or output");
-    for (const void* x : {(const void*)dQ, (const void*)dCu, (const void*)dPast, (const void*)dTable, (const void*)dOut})
-        if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: buffers must be 4-byte aligned");
-    if (misaligned16(dKCache) || misaligned16(dVCache))
-        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the cache must be 16-byte aligned");
+    if (int st = paged_attention_buffers("paged_attention", *d, dQ, dCu, dPast, dTable, dKCache, dVCache, dOut)) return st;
     // (a negative limit is the plan's "no limit")
     const PagedAttnPlan plan =
         paged_plan(*d, dWorkspace && !misaligned16(dWorkspace) ? std::max<int64_t>(workspace_bytes, 0) : 0);
     PagedAttnArgs p{};
-    p.b = paged_batch(*d, dCu, dPast, dTable);
-    p.q = dQ;
-    p.kc = dKCache;
-    p.vc = dVCache;
-    p.out = dOut;
-    p.part = static_cast<float*>(dWorkspace);
-    p.H = d->num_heads;
-    p.kvH = d->kv_num_heads;
-    p.D = d->head_dim;
-    p.window = d->local_window_size;
-    p.f16 = d->cache_type == MS_HIP_DTYPE_F16;
+    paged_attention_args(p, *d, dQ, dCu, dPast, dTable, dKCache, dVCache, dOut, dWorkspace);
     p.splits = plan.splits;
     p.split_min = plan.split_min;
-    const int64_t qw = (int64_t)p.H * p.D, T = d->tokens, f = sizeof(float);
-    p.q_stride = d->q_stride ? d->q_stride : qw;
-    p.grp = FastDiv(p.H / p.kvH);
-    p.scale2 = (d->scale != 0.0f ? d->scale : 1.0f / std::sqrt((float)p.D)) * 1.44269504088896341f;
-    const int64_t ob = T * qw * f, cb = cache_bytes(*d);
-    const std::initializer_list<Buffer> inputs = {{dQ, span(T, p.q_stride, qw) * f}, {dKCache, cb}, {dVCache, cb},
-                                                  {dCu, (d->requests + 1ll) * 4}, {dPast, d->requests * 4ll},
-                                                  {dTable, 4ll * d->requests * d->max_pages}};
-    if (overlap_any(dOut, ob, inputs) || overlap(dOut, ob, dWorkspace, plan.ws_bytes))
-        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the output overlaps an input or the workspace");
-    if (overlap_any(dWorkspace, plan.ws_bytes, inputs))
-        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_attention: the workspace overlaps an input");
+    if (int st = paged_attention_overlaps("paged_attention", *d, p, nullptr, nullptr, 0, plan.ws_bytes)) return st;
     MS_HIP_CHECK(launch_paged_attention(p, plan, static_cast<hipStream_t>(stream)));
+    return MS_HIP_OK;
+}
+
+int ms_hip_paged_shared_attention_check(const ms_hip_paged_desc* d, const ms_hip_shared_desc* s)
+{
+    if (int st = ms_hip_paged_attention_check(d)) return st;
+    if (!s) return fail(MS_HIP_ERR_INVALID, "[ms_hip] null shared prefix descriptor");
+    if (s->groups < 0 || s->max_shared < 0 || s->max_rest < 0)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_shared_attention: negative sizes");
+    if (s->groups > d->requests)
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_shared_attention: %d groups of %d requests", s->groups, d->requests);
+    const SharedPlan plan = shared_plan(*d, *s);
+    if (plan.prefix_grid + plan.blocks_grid + plan.rows_grid >= 1 << 24)   // a launch has fewer than 2^32 threads
+        return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_shared_attention: %d tokens of %d requests need too many workgroups",
+                    d->tokens, d->requests);
+    return MS_HIP_OK;
+}
+
+int64_t ms_hip_paged_shared_attention_workspace_size(const ms_hip_paged_desc* d, const ms_hip_shared_desc* s)
+{
+    if (!d || !s || ms_hip_paged_shared_attention_check(d, s) != MS_HIP_OK) return 0;
+    return std::max(shared_plan(*d, *s).ws_bytes, paged_plan(*d, -1).ws_bytes);
+}
+
+int ms_hip_paged_shared_attention(const ms_hip_paged_desc* d, const ms_hip_shared_desc* s, const float* dQ,
+                                  const int32_t* dCu, const int32_t* dPast, const int32_t* dTable, const int32_t* dGroups,
+                                  const int32_t* dShared, const void* dKCache, const void* dVCache, float* dOut,
+                                  void* dWorkspace, int64_t workspace_bytes, void* stream)
+{
+    if (int st = gate()) return st;
+    if (int st = ms_hip_paged_shared_attention_check(d, s)) return st;
+    if (d->tokens == 0 || d->requests == 0) return MS_HIP_OK;
+    const char* const op = "paged_shared_attention";
+    if (int st = paged_attention_buffers(op, *d, dQ, dCu, dPast, dTable, dKCache, dVCache, dOut)) return st;
+    if (s->groups && (!dGroups || !dShared)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: null groups or shared lengths", op);
+    if (misaligned4(dGroups) || misaligned4(dShared))
+        return fail(MS_HIP_ERR_INVALID, "[ms_hip] %s: buffers must be 4-byte aligned", op);
+    const int64_t ws_avail = dWorkspace && !misaligned16(dWorkspace) ? std::max<int64_t>(workspace_bytes, 0) : 0;
+    const SharedPlan plan = shared_plan(*d, *s);
+    const bool share = plan.splits > 0 && plan.ws_bytes <= ws_avail;
+    const PagedAttnPlan alone = share ? PagedAttnPlan{} : paged_plan(*d, ws_avail);
+    SharedAttnArgs p{};
+    paged_attention_args(p, *d, dQ, dCu, dPast, dTable, dKCache, dVCache, dOut, dWorkspace);
+    if (int st = paged_attention_overlaps(op, *d, p, dGroups, dShared, s->groups, share ? plan.ws_bytes : alone.ws_bytes)) return st;
+    if (share) {
+        p.bounds = dGroups;
+        p.shared = dShared;
+        p.groups = s->groups;
+        MS_HIP_CHECK(launch_shared_attention(p, plan, static_cast<hipStream_t>(stream)));
+        return MS_HIP_OK;
+    }
+    p.splits = alone.splits;
+    p.split_min = alone.split_min;
+    MS_HIP_CHECK(launch_paged_attention(p, alone, static_cast<hipStream_t>(stream)));
     return MS_HIP_OK;
 }
 

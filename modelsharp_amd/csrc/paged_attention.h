@@ -7,6 +7,8 @@
 // The query heads of a kv head and the tokens of a request are rows of one matrix, row = token
 // * group + head in group, so that a tile of K and V serves every row that reads it.
 #pragma once
+#include <type_traits>
+
 #include "mfma_device.h"
 #include "serving.h"
 
@@ -81,14 +83,68 @@ __device__ __forceinline__ int paged_stand(const PagedBatch& b, const PagedTile&
 struct PagedRange {
     int klo, khi;
 };
-__device__ __forceinline__ PagedRange paged_range(const PagedAttnArgs& p, int pos0, int pos1, int klast, int sp, int step)
+// The keys that a tile's splits share out: positions from `lo` on, in records rec, rec + 1, ...
+struct PagedPart {
+    int splits, split_min, lo, rec;
+};
+__device__ __forceinline__ PagedRange paged_range(const PagedAttnArgs& p, const PagedPart& part, int pos0, int pos1, int klast,
+                                                  int sp, int step)
 {
-    const int lo = p.window >= 0 ? max(0, pos0 - p.window + 1) : 0, hi = min(pos1, klast);
+    const int lo = max(part.lo, p.window >= 0 ? max(0, pos0 - p.window + 1) : 0), hi = min(pos1, klast);
     const int first = lo / step, n = hi >= lo ? hi / step - first + 1 : 0;
-    const int per = max((n + p.splits - 1) / p.splits, p.split_min / step);
+    const int per = max((n + part.splits - 1) / part.splits, part.split_min / step);
     if ((int64_t)sp * per >= n) return {0, -1};
     const int a = sp * per, e = min(n, a + per);
     return {max(lo, (first + a) * step), min(hi, (first + e) * step - 1)};
+}
+
+// Attention behind a shared prefix (SharedAttnArgs): tile `idx` of the groups' rows, all new tokens of
+// a group's requests being rows of one matrix, each of which sees the whole prefix; or of the
+// requests' own keys, from the prefix's end on. part.lo is where the keys begin.
+template <int BM>
+__device__ __forceinline__ bool shared_tile(const SharedAttnArgs& p, bool prefix, int idx, int rows_min, int rows_max,
+                                            PagedTile& t, PagedPart& part)
+{
+    const PagedBatch& b = p.b;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t reach = min((int64_t)b.max_pages * b.page.div, (int64_t)kSharedPositions);
+    if (!prefix) {
+        if (!paged_tile<BM>(p, idx, rows_min, rows_max, t)) return false;
+        part.lo = 0;
+        for (int base = 0; base < p.groups; base += kWave) {
+            const int i = min(base + lane, p.groups - 1);
+            const bool mine = p.bounds[i] <= t.r && t.r < p.bounds[i + 1];
+            const int n = (int)min((int64_t)max(p.shared[i], 0), reach);
+            if (const uint64_t found = __ballot(mine && base + lane < p.groups)) {
+                part.lo = __builtin_amdgcn_readlane(n, __ffsll((unsigned long long)found) - 1);
+                break;
+            }
+        }
+        return true;
+    }
+    for (int base = 0; base < p.groups; base += kWave) {
+        const int i = min(base + lane, p.groups - 1);
+        const int r0 = min(max(p.bounds[i], 0), b.requests), r1 = min(max(p.bounds[i + 1], r0), b.requests);
+        const PagedSpan span = paged_span(b.cu[r0], b.cu[r1], b.tokens);
+        const int keys = (int)min((int64_t)max(p.shared[i], 0), reach);
+        const int c0 = span.first, n = base + lane < p.groups && keys > 0 ? span.count : 0;
+        const int tiles = paged_tiles(n * p.grp.div, BM);
+        const int sum = wave_scan(tiles);
+        if (const uint64_t past_idx = __ballot(sum > idx)) {
+            const int l = __ffsll((unsigned long long)past_idx) - 1;
+            const int nt = __builtin_amdgcn_readlane(tiles, l);
+            t.r = __builtin_amdgcn_readlane(r0, l);
+            t.t0 = __builtin_amdgcn_readlane(c0, l);
+            t.row0 = (idx - (__builtin_amdgcn_readlane(sum, l) - nt)) * BM;
+            t.rows = min(BM, __builtin_amdgcn_readlane(n, l) * p.grp.div - t.row0);
+            t.past = __builtin_amdgcn_readlane(keys, l);   // every row's position is past the prefix's last
+            t.klast = t.past - 1;
+            part.lo = 0;
+            return true;
+        }
+        idx -= __builtin_amdgcn_readlane(sum, kWave - 1);
+    }
+    return false;
 }
 
 // A split's record of an output row: its normed output, and (max, sum).
@@ -100,6 +156,15 @@ __device__ __forceinline__ float* paged_part_ml(const PagedAttnArgs& p, int sp, 
 {
     const int64_t n = (int64_t)p.b.tokens * p.H;
     return p.part + p.splits * n * p.D + (sp * n + row) * 2;
+}
+
+// The first `n` records of a row that has no keys there.
+__device__ __forceinline__ void paged_no_prefix(const PagedAttnArgs& p, int n, int64_t row)
+{
+    for (int i = 0; i < n; ++i) {
+        paged_part_ml(p, i, row)[0] = -__builtin_inff();
+        paged_part_ml(p, i, row)[1] = 0.0f;
+    }
 }
 
 __device__ __forceinline__ bool finite4(floatx4_t v)
@@ -246,9 +311,10 @@ constexpr int paged_ring(int DP, bool f16) { return f16 ? 2 : (DP <= 64 ? 3 : DP
 // 26 us: what does not grow with the keys is the larger part of a call of a few of them (the chain cu,
 // past -> table -> keys, the join in LDS, the merge's launch).
 constexpr int kRowsLds = 4 * 4 * kWave * 16 + 2 * 4 * 16 * 4 + 16;
-template <typename T, int DP, bool WHOLE>
-__device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int rows_max, uint8_t* lds)
+template <typename T, int DP, bool WHOLE, typename A>
+__device__ __forceinline__ void paged_rows(const A& p, PagedPart part, bool prefix, int bid, int rows_max, uint8_t* lds)
 {
+    constexpr bool SHARED = std::is_same<A, SharedAttnArgs>::value;
     constexpr bool F16 = sizeof(T) == 2;
     constexpr int VEC = F16 && DP >= 128 ? 8 : 4;   // channels of one lane's load of V
     constexpr int NC = DP / (16 * VEC);             // loads of a V row's part
@@ -262,9 +328,13 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
     int& flag = *reinterpret_cast<int*>(lds + sizeof(merge) + sizeof(stat));
 
     const int g = bid % p.kvH, rest = bid / p.kvH;
-    const int sp = rest % p.splits;
+    const int sp = rest % part.splits, rec = part.rec + sp;
     PagedTile t;
-    if (!paged_tile<16>(p, rest / p.splits, 0, rows_max, t)) return;
+    if constexpr (SHARED) {
+        if (!shared_tile<16>(p, prefix, rest / part.splits, 0, rows_max, t, part)) return;
+    } else {
+        if (!paged_tile<16>(p, rest / part.splits, 0, rows_max, t)) return;
+    }
     const int lane = threadIdx.x & 63, grp = lane >> 4, l16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (threadIdx.x == 0) flag = 0;
@@ -272,14 +342,16 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
     const int row = t.row0 + min(l16, t.rows - 1), tok = p.grp.quot(row);
     const int head = g * p.grp.div + row - tok * p.grp.div;
     const int pos = t.past + tok;
-    const PagedRange kr = paged_range(p, t.past + p.grp.quot(t.row0), t.past + p.grp.quot(t.row0 + t.rows - 1), t.klast,
+    const PagedRange kr = paged_range(p, part, t.past + p.grp.quot(t.row0), t.past + p.grp.quot(t.row0 + t.rows - 1), t.klast,
                                       sp, 16);
     const int64_t orow = (int64_t)(t.t0 + tok) * p.H + head;
     const bool mine = l16 < t.rows;
+    if constexpr (SHARED)
+        if (!prefix && sp == 0 && part.lo == 0 && mine && threadIdx.x < 16) paged_no_prefix(p, part.rec, orow);
     if (p.splits > 1 && kr.khi < kr.klo) {   // nothing for this split: its record's sum is 0
         if (mine && threadIdx.x < 16) {
-            paged_part_ml(p, sp, orow)[0] = -__builtin_inff();
-            paged_part_ml(p, sp, orow)[1] = 0.0f;
+            paged_part_ml(p, rec, orow)[0] = -__builtin_inff();
+            paged_part_ml(p, rec, orow)[1] = 0.0f;
         }
         return;
     }
@@ -530,7 +602,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
     for (int w = 0; w < 4; ++w) ll += stat[1][w][l16] * __builtin_amdgcn_exp2f(stat[0][w][l16] - ms);
     // (a wave without a key that any row sees has m = -infinity: a factor of 0)
     const float f = ll != 0.0f ? __builtin_amdgcn_exp2f(m - ms) / (F16 ? ll * (1 << kWeightExp) : ll) : 0.0f;
-    float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
+    float* const o = p.splits > 1 ? paged_part_o(p, rec, orow) : p.out + orow * p.D;
     bool odd = mine && mm == -__builtin_inff() && k_hi >= k_lo;
     // quad n of a lane's channels: chunk c, row i of the product, channels 4 b .. 4 b + 3 of VEC
     constexpr int QUADS = DP / 16;
@@ -553,13 +625,13 @@ __device__ __forceinline__ void paged_rows(const PagedAttnArgs& p, int bid, int 
         __syncthreads();
     }
     if (p.splits > 1 && mine && wave == 0 && grp == 0) {
-        paged_part_ml(p, sp, orow)[0] = mm;
-        paged_part_ml(p, sp, orow)[1] = ll;
+        paged_part_ml(p, rec, orow)[0] = mm;
+        paged_part_ml(p, rec, orow)[1] = ll;
     }
     if (odd) flag = 1;
     __syncthreads();
     if (flag)
-        for (int lr = wave; lr < t.rows; lr += 4) paged_exact_row<T>(p, t, g, lr, sp, kr);
+        for (int lr = wave; lr < t.rows; lr += 4) paged_exact_row<T>(p, t, g, lr, rec, kr);
 }
 
 // ---- chunks: tiles of 128 rows -----------------------------------------------------------------
@@ -686,9 +758,10 @@ struct PagedBlock {
     static constexpr int CH = DPL / 8, TILE = BN * CH;                  // 16-byte slots of a row, of a plane
     typedef short8_t lds_t[BUFS][2][PagedSplit<T>::kPlanes][TILE];
 };
-template <typename T, int DP, bool WHOLE>
-__device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, int rows_min, uint8_t* lds_bytes)
+template <typename T, int DP, bool WHOLE, typename A>
+__device__ __forceinline__ void paged_blocks(const A& p, PagedPart part, bool prefix, int bid, int rows_min, uint8_t* lds_bytes)
 {
+    constexpr bool SHARED = std::is_same<A, SharedAttnArgs>::value;
     typedef PagedSplit<T> S;
     typedef PagedBlock<T, DP> B;
     constexpr bool F16 = B::F16;
@@ -702,21 +775,27 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
     auto& lds = *reinterpret_cast<typename B::lds_t*>(lds_bytes);
 
     const int g = bid % p.kvH, rest = bid / p.kvH;
-    const int sp = rest % p.splits;
+    const int sp = rest % part.splits, rec = part.rec + sp;
     PagedTile t;
-    if (!paged_tile<128>(p, rest / p.splits, rows_min, INT32_MAX, t)) return;
+    if constexpr (SHARED) {
+        if (!shared_tile<128>(p, prefix, rest / part.splits, rows_min, INT32_MAX, t, part)) return;
+    } else {
+        if (!paged_tile<128>(p, rest / part.splits, rows_min, INT32_MAX, t)) return;
+    }
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const PagedRange kr = paged_range(p, t.past + p.grp.quot(t.row0), t.past + p.grp.quot(t.row0 + t.rows - 1), t.klast,
+    const PagedRange kr = paged_range(p, part, t.past + p.grp.quot(t.row0), t.past + p.grp.quot(t.row0 + t.rows - 1), t.klast,
                                       sp, BN);
     const int row = t.row0 + min(32 * wave + l32, t.rows - 1), tok = p.grp.quot(row);
     const int head = g * p.grp.div + row - tok * p.grp.div, pos = t.past + tok;
     const int64_t orow = (int64_t)(t.t0 + tok) * p.H + head;
     const bool mine = 32 * wave + l32 < t.rows;
+    if constexpr (SHARED)
+        if (!prefix && sp == 0 && part.lo == 0 && mine && hf == 0) paged_no_prefix(p, part.rec, orow);
     if (p.splits > 1 && kr.khi < kr.klo) {   // nothing for this split: its record's sum is 0
         if (mine && hf == 0) {
-            paged_part_ml(p, sp, orow)[0] = -__builtin_inff();
-            paged_part_ml(p, sp, orow)[1] = 0.0f;
+            paged_part_ml(p, rec, orow)[0] = -__builtin_inff();
+            paged_part_ml(p, rec, orow)[1] = 0.0f;
         }
         return;
     }
@@ -984,7 +1063,7 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
 
     l += xor32_value(l);
     const float f = l != 0.0f ? 1.0f / (F16 ? l * (1 << kWeightExp) : l) : 0.0f;
-    float* const o = p.splits > 1 ? paged_part_o(p, sp, orow) : p.out + orow * p.D;
+    float* const o = p.splits > 1 ? paged_part_o(p, rec, orow) : p.out + orow * p.D;
     bool odd = mine && (missing || (m == -__builtin_inff() && k_hi >= k_lo));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -998,13 +1077,13 @@ __device__ __forceinline__ void paged_blocks(const PagedAttnArgs& p, int bid, in
             }
         }
     if (p.splits > 1 && mine && hf == 0) {
-        paged_part_ml(p, sp, orow)[0] = m;
-        paged_part_ml(p, sp, orow)[1] = l;
+        paged_part_ml(p, rec, orow)[0] = m;
+        paged_part_ml(p, rec, orow)[1] = l;
     }
     // rows that met an infinity, a NaN or a page that is not there
     uint64_t redo = __ballot(odd);
     for (uint32_t rows = (uint32_t)(redo | redo >> 32); rows; rows &= rows - 1)
-        paged_exact_row<T>(p, t, g, 32 * wave + __ffs(rows) - 1, sp, kr);
+        paged_exact_row<T>(p, t, g, 32 * wave + __ffs(rows) - 1, rec, kr);
 }
 
 // A launch's workgroups: the first p.blocks_grid take tiles of 128 rows of the requests of more than
@@ -1018,22 +1097,45 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_attention_kernel
     constexpr int DPR = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;
     constexpr int kBlocksLds = MODE == kPagedRows ? 0 : (int)sizeof(typename PagedBlock<T, DP>::lds_t);
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBlocksLds > kRowsLds ? kBlocksLds : kRowsLds];
+    const PagedPart part{p.splits, p.split_min, 0, 0};
     if constexpr (MODE == kPagedRows) {
-        paged_rows<T, DPR, WHOLE>(p, blockIdx.x, INT32_MAX, lds);
+        paged_rows<T, DPR, WHOLE>(p, part, false, blockIdx.x, INT32_MAX, lds);
     } else if constexpr (MODE == kPagedBlocks) {
-        paged_blocks<T, DP, WHOLE>(p, blockIdx.x, 0, lds);
+        paged_blocks<T, DP, WHOLE>(p, part, false, blockIdx.x, 0, lds);
     } else {
         if ((int)blockIdx.x < p.blocks_grid)
-            paged_blocks<T, DP, WHOLE>(p, blockIdx.x, p.few_rows + 1, lds);
+            paged_blocks<T, DP, WHOLE>(p, part, false, blockIdx.x, p.few_rows + 1, lds);
         else
-            paged_rows<T, DPR, WHOLE>(p, blockIdx.x - p.blocks_grid, p.few_rows, lds);
+            paged_rows<T, DPR, WHOLE>(p, part, false, blockIdx.x - p.blocks_grid, p.few_rows, lds);
+    }
+}
+
+// Attention behind shared prefixes: the prefixes' tiles first (128 rows, or 16), then those of the requests'
+// own keys, all of a launch beside each other. MODE as above; both kinds where either has both.
+template <typename T, int DP, bool WHOLE, PagedMode MODE>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_attention_kernel(SharedAttnArgs p)
+{
+    constexpr int DPR = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;
+    constexpr int kBlocksLds = MODE == kPagedRows ? 0 : (int)sizeof(typename PagedBlock<T, DP>::lds_t);
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBlocksLds > kRowsLds ? kBlocksLds : kRowsLds];
+    const bool prefix = (int)blockIdx.x < p.prefix_grid;
+    const int bid = blockIdx.x - (prefix ? 0 : p.prefix_grid);
+    const PagedPart part = prefix ? PagedPart{p.prefix_splits, p.prefix_min, 0, 0}
+                                  : PagedPart{p.splits - p.prefix_splits, p.split_min, 0, p.prefix_splits};
+    if constexpr (MODE == kPagedRows) {
+        paged_rows<T, DPR, WHOLE>(p, part, prefix, bid, INT32_MAX, lds);
+    } else {
+        if (prefix ? p.prefix_blocks : bid < p.blocks_grid)
+            paged_blocks<T, DP, WHOLE>(p, part, prefix, bid, prefix ? 0 : p.few_rows + 1, lds);
+        else
+            paged_rows<T, DPR, WHOLE>(p, part, prefix, bid - (prefix ? 0 : p.blocks_grid), prefix ? INT32_MAX : p.few_rows, lds);
     }
 }
 
 // The splits' records of one output row, joined in the splits' order. A wave per row: lane s holds
 // split s's weight, and the outputs' loads do not wait for them (what a split of weight zero left
 // is not used).
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs p)
+static __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs p)
 {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;

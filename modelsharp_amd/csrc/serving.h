@@ -143,6 +143,15 @@ struct PagedAttnArgs {
     FastDiv grp;      // query heads per kv head
     float scale2;     // scale * log2(e)
 };
+// The same behind prefixes that groups of requests share: group i's requests are [bounds[i], bounds[i + 1])
+// and their first shared[i] positions lie in its first request's pages. `splits` records of a
+// row: the prefix's, then those of the request's own keys.
+struct SharedAttnArgs : PagedAttnArgs {
+    const int32_t* bounds;   // [groups + 1]
+    const int32_t* shared;   // [groups]
+    int groups, prefix_splits, prefix_min, prefix_grid, prefix_blocks;
+};
+constexpr int kSharedPositions = 1 << 30;   // a prefix's at the most: what lies behind counts as a request's own
 struct PagedAttnPlan {
     int splits = 1, split_min = 0, few_rows = 0;
     int64_t rows_grid = 0, blocks_grid = 0;   // 0: that kernel is not launched

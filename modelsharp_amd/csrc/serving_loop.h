@@ -3,6 +3,7 @@
 //
 //   paged_plan.h        page tables, lengths, positions and slot maps from what requests want, and
 //                       the step's end
+//   paged_attention.h   attention behind prefixes that requests share (shared_attention_kernel)
 //   sample.h            the next tokens from logits
 #pragma once
 #include "serving.h"
@@ -40,6 +41,17 @@ struct CommitArgs {
     FastDiv page;
 };
 MS_INTERNAL hipError_t launch_commit(const CommitArgs& p, hipStream_t s);
+
+struct SharedPlan {
+    int splits = 0, prefix_splits = 0;   // records of a row, and the prefix's among them; 0: not shared
+    int split_min = 0, prefix_min = 0, few_rows = 0;
+    bool prefix_blocks = false;
+    int64_t prefix_grid = 0, blocks_grid = 0, rows_grid = 0;
+    int64_t ws_bytes = 0;
+};
+MS_INTERNAL SharedPlan shared_attention_plan(int64_t tokens, int requests, int64_t max_new, int groups, int64_t prefix,
+                                             int64_t rest, int H, int kvH, int D, int f16, int cus);
+MS_INTERNAL hipError_t launch_shared_attention(const SharedAttnArgs& p, const SharedPlan& plan, hipStream_t s);
 
 struct SampleArgs {
     const float* logits;

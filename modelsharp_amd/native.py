@@ -79,6 +79,9 @@ _PROTOTYPES = {
     "ms_hip_paged_attention_check": (_c_int, [_vp]),
     "ms_hip_paged_attention_workspace_size": (_c_i64, [_vp]),
     "ms_hip_paged_attention": (_c_int, [_vp] * 9 + [_c_i64, _vp]),
+    "ms_hip_paged_shared_attention_check": (_c_int, [_vp] * 2),
+    "ms_hip_paged_shared_attention_workspace_size": (_c_i64, [_vp] * 2),
+    "ms_hip_paged_shared_attention": (_c_int, [_vp] * 12 + [_c_i64, _vp]),
     "ms_hip_qk_norm_check": (_c_int, [_vp]),
     "ms_hip_qk_norm_rotary": (_c_int, [_vp] * 11),
     "ms_hip_lora_check": (_c_int, [_vp]),
@@ -529,6 +532,27 @@ def paged_attention(desc: PagedDesc, dQ, dCu, dPast, dTable, dKCache, dVCache, d
     """Attention of each request's new tokens over its pages."""
     check(load().ms_hip_paged_attention(ctypes.byref(desc), dQ, dCu, dPast, dTable, dKCache, dVCache, dOut, dWorkspace,
                                         workspace_bytes, stream))
+
+
+class SharedDesc(ctypes.Structure):
+    """ms_hip_shared_desc."""
+    _fields_ = [(n, ctypes.c_int) for n in ("groups", "max_shared", "max_rest")]
+
+
+def paged_shared_attention_check(desc: PagedDesc, shared: SharedDesc):
+    """Raises what paged_shared_attention would refuse of the descriptors."""
+    check(load().ms_hip_paged_shared_attention_check(ctypes.byref(desc), ctypes.byref(shared)))
+
+
+def paged_shared_attention_workspace_size(desc: PagedDesc, shared: SharedDesc) -> int:
+    return int(load().ms_hip_paged_shared_attention_workspace_size(ctypes.byref(desc), ctypes.byref(shared)))
+
+
+def paged_shared_attention(desc: PagedDesc, shared: SharedDesc, dQ, dCu, dPast, dTable, dGroups, dShared, dKCache, dVCache,
+                           dOut, dWorkspace=None, workspace_bytes=0, stream=None):
+    """Attention of each request's new tokens over its pages, prefixes that groups of requests share read once."""
+    check(load().ms_hip_paged_shared_attention(ctypes.byref(desc), ctypes.byref(shared), dQ, dCu, dPast, dTable, dGroups,
+                                               dShared, dKCache, dVCache, dOut, dWorkspace, workspace_bytes, stream))
 
 
 def qk_norm_rotary(desc: QkNormDesc, dQ, dK, dQGamma, dKGamma, dPositions, dCos, dSin, dQOut, dKOut, stream=None):
