@@ -104,12 +104,52 @@ hipError_t launch_shared_attention(const SharedAttnArgs& args, const SharedPlan&
 }
 
 // ---- sampling ----------------------------------------------------------------------------------
-SamplePlan sample_plan(int, int, int) { return {}; }
-
-hipError_t launch_sample(const SampleArgs& p, const SamplePlan&, void*, hipStream_t s)
+namespace {
+int64_t sample_row_bytes(int64_t chunks)
 {
-    hipLaunchKernelGGL(sample_any_kernel, dim3(p.rows), dim3(kSampleThreads), 0, s, p);
-    return hipGetLastError();
+    return (chunks * (kSampleBins + kSampleTiles + 2) + kSampleList) * 8 + sizeof(SampleFound) + chunks * 8;
+}
+}  // namespace
+
+SamplePlan sample_plan(int rows, int vocab, int)
+{
+    SamplePlan pl;
+    pl.chunks = (vocab + kSampleChunk - 1) / kSampleChunk;
+    // rows at a time: what fits 64 MB, and 64 at the least
+    pl.batch = (int)std::min<int64_t>(rows, std::max<int64_t>(64, (64ll << 20) / sample_row_bytes(pl.chunks)));
+    pl.ws_bytes = (pl.batch * sample_row_bytes(pl.chunks) + 15) / 16 * 16;
+    return pl;
+}
+
+hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* workspace, hipStream_t s)
+{
+    static_assert(kSampleChunk == kSampleTile * kSampleTiles && kSampleChunk < 1 << 15, "a chunk's counts have 15 bits");
+    static_assert(sizeof(SampleFound) % 8 == 0, "the workspace's parts are aligned");
+    SampleWs ws{};
+    const int64_t n = plan.batch, c = n * plan.chunks;
+    ws.chunks = plan.chunks;
+    while ((1 << ws.index_bits) < p.vocab) ++ws.index_bits;
+    ws.hist = static_cast<unsigned long long*>(workspace);
+    ws.list = ws.hist + c * kSampleBins;
+    ws.tiles = ws.list + n * kSampleList;
+    ws.sums = ws.tiles + c * kSampleTiles;
+    ws.found = reinterpret_cast<SampleFound*>(ws.sums + c * 2);
+    ws.top = reinterpret_cast<float*>(ws.found + n);
+    ws.first = reinterpret_cast<int32_t*>(ws.top + c);
+    const bool vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.stride % 4 == 0;
+    const int lds = (int)(sizeof(SampleLds) + plan.chunks * kSampleTiles * 8);
+    if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sample_draw_kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds))
+        return e;
+    for (; ws.row0 < p.rows; ws.row0 += plan.batch) {
+        const int rows = std::min(plan.batch, p.rows - ws.row0);
+        const dim3 grid(plan.chunks, rows), block(kSampleThreads);
+        hipLaunchKernelGGL(vec ? sample_scan_kernel<true> : sample_scan_kernel<false>, grid, block, 0, s, p, ws);
+        hipLaunchKernelGGL(vec ? sample_sum_kernel<true> : sample_sum_kernel<false>, grid, block, 0, s, p, ws);
+        hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), block, lds, s, p, ws);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace msnb

@@ -65,7 +65,30 @@ struct SampleArgs {
     int rows, vocab, frac;       // weights are whole multiples of 2^-frac
     int64_t stride;
 };
+constexpr int kSampleBins = 512;                 // of logits, by which a border is first looked for
+constexpr int kSampleList = 8192;                // logits of the bins that a border lies in
+constexpr int kSampleChunk = 16384;              // tokens of a workgroup of the first two launches
+// What the second launch finds out about a row.
+struct SampleFound {
+    float top;
+    int lo, hi, bk;            // bins: where the last token kept may lie, and the k-th token's (kSampleBins: none)
+    int by_k, by_p;
+    uint32_t k_before;         // tokens before bin bk
+    uint32_t listed;           // 0: nothing, or more than the list holds
+};
+// The workspace of `batch` rows: rows are taken so many at a time.
+struct SampleWs {
+    unsigned long long* hist;  // [rows][chunks][kSampleBins]
+    unsigned long long* list;  // [rows][kSampleList]
+    unsigned long long* tiles; // [rows][chunks][4]: kept weights
+    unsigned long long* sums;  // [rows][chunks][2]
+    SampleFound* found;        // [rows]
+    float* top;                // [rows][chunks]: largest logit
+    int32_t* first;            // [rows][chunks]: its index
+    int row0, chunks, index_bits;
+};
 struct SamplePlan {
+    int chunks = 0, batch = 0;
     int64_t ws_bytes = 0;
 };
 MS_INTERNAL SamplePlan sample_plan(int rows, int vocab, int cus);
