@@ -107,7 +107,7 @@ hipError_t launch_shared_attention(const SharedAttnArgs& args, const SharedPlan&
 namespace {
 int64_t sample_row_bytes(int64_t chunks)
 {
-    return (chunks * (kSampleBins + kSampleTiles + 2) + kSampleList) * 8 + sizeof(SampleFound) + chunks * 8;
+    return (chunks * (kSampleBins + kSampleTiles + 3) + kSampleList) * 8 + sizeof(SampleFound) + chunks * 8;
 }
 }  // namespace
 
@@ -124,6 +124,7 @@ SamplePlan sample_plan(int rows, int vocab, int)
 hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* workspace, hipStream_t s)
 {
     static_assert(kSampleChunk == kSampleTile * kSampleTiles && kSampleChunk < 1 << 15, "a chunk's counts have 15 bits");
+    static_assert(kSampleChunks <= kSampleThreads, "a chunk of a row to a thread");
     static_assert(sizeof(SampleFound) % 8 == 0, "the workspace's parts are aligned");
     SampleWs ws{};
     const int64_t n = plan.batch, c = n * plan.chunks;
@@ -133,7 +134,8 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     ws.list = ws.hist + c * kSampleBins;
     ws.tiles = ws.list + n * kSampleList;
     ws.sums = ws.tiles + c * kSampleTiles;
-    ws.found = reinterpret_cast<SampleFound*>(ws.sums + c * 2);
+    ws.all = ws.sums + c * 2;
+    ws.found = reinterpret_cast<SampleFound*>(ws.all + c);
     ws.top = reinterpret_cast<float*>(ws.found + n);
     ws.first = reinterpret_cast<int32_t*>(ws.top + c);
     const bool vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.stride % 4 == 0;

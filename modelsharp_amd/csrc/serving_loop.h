@@ -82,6 +82,7 @@ struct SampleWs {
     unsigned long long* list;  // [rows][kSampleList]
     unsigned long long* tiles; // [rows][chunks][4]: kept weights
     unsigned long long* sums;  // [rows][chunks][2]
+    unsigned long long* all;   // [rows][chunks]: the sum of a chunk's bins
     SampleFound* found;        // [rows]
     float* top;                // [rows][chunks]: largest logit
     int32_t* first;            // [rows][chunks]: its index
@@ -93,7 +94,7 @@ struct SamplePlan {
 };
 MS_INTERNAL SamplePlan sample_plan(int rows, int vocab, int cus);
 MS_INTERNAL hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* workspace, hipStream_t s);
-constexpr int kSampleVocab = 1 << 24, kSampleRows = 1 << 20;
+constexpr int kSampleVocab = 1 << 24, kSampleRows = 1 << 20, kSampleChunks = kSampleVocab / kSampleChunk;
 // Weights are at most 2^frac: no sum over the vocabulary passes 2^62.
 inline int sample_frac(int vocab)
 {
