@@ -114,7 +114,7 @@ int64_t sample_row_bytes(int64_t chunks)
 SamplePlan sample_plan(int rows, int vocab, int)
 {
     SamplePlan pl;
-    pl.chunks = (vocab + kSampleChunk - 1) / kSampleChunk;
+    pl.chunks = (vocab + 3 + kSampleChunk - 1) / kSampleChunk;   // (rows that begin up to 3 floats behind 16 bytes)
     // rows at a time: what fits 64 MB, and 64 at the least
     pl.batch = (int)std::min<int64_t>(rows, std::max<int64_t>(64, (64ll << 20) / sample_row_bytes(pl.chunks)));
     pl.ws_bytes = (pl.batch * sample_row_bytes(pl.chunks) + 15) / 16 * 16;
@@ -124,7 +124,6 @@ SamplePlan sample_plan(int rows, int vocab, int)
 hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* workspace, hipStream_t s)
 {
     static_assert(kSampleChunk == kSampleTile * kSampleTiles && kSampleChunk < 1 << 15, "a chunk's counts have 15 bits");
-    static_assert(kSampleChunks <= kSampleThreads, "a chunk of a row to a thread");
     static_assert(sizeof(SampleFound) % 8 == 0, "the workspace's parts are aligned");
     SampleWs ws{};
     const int64_t n = plan.batch, c = n * plan.chunks;
@@ -138,7 +137,6 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     ws.found = reinterpret_cast<SampleFound*>(ws.all + c);
     ws.top = reinterpret_cast<float*>(ws.found + n);
     ws.first = reinterpret_cast<int32_t*>(ws.top + c);
-    const bool vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.stride % 4 == 0;
     const int lds = (int)(sizeof(SampleLds) + plan.chunks * kSampleTiles * 8);
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sample_draw_kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds))
@@ -146,8 +144,8 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     for (; ws.row0 < p.rows; ws.row0 += plan.batch) {
         const int rows = std::min(plan.batch, p.rows - ws.row0);
         const dim3 grid(plan.chunks, rows), block(kSampleThreads);
-        hipLaunchKernelGGL(vec ? sample_scan_kernel<true> : sample_scan_kernel<false>, grid, block, 0, s, p, ws);
-        hipLaunchKernelGGL(vec ? sample_sum_kernel<true> : sample_sum_kernel<false>, grid, block, 0, s, p, ws);
+        hipLaunchKernelGGL(sample_scan_kernel, grid, block, 0, s, p, ws);
+        hipLaunchKernelGGL(sample_sum_kernel, grid, block, 0, s, p, ws);
         hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), block, lds, s, p, ws);
         if (hipError_t e = hipGetLastError()) return e;
     }

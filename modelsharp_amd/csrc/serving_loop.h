@@ -75,6 +75,7 @@ struct SampleFound {
     int by_k, by_p;
     uint32_t k_before;         // tokens before bin bk
     uint32_t listed;           // 0: nothing, or more than the list holds
+    int answered, unused;      // the row's answer is there
 };
 // The workspace of `batch` rows: rows are taken so many at a time.
 struct SampleWs {
@@ -94,7 +95,7 @@ struct SamplePlan {
 };
 MS_INTERNAL SamplePlan sample_plan(int rows, int vocab, int cus);
 MS_INTERNAL hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* workspace, hipStream_t s);
-constexpr int kSampleVocab = 1 << 24, kSampleRows = 1 << 20, kSampleChunks = kSampleVocab / kSampleChunk;
+constexpr int kSampleVocab = 1 << 24, kSampleRows = 1 << 20;
 // Weights are at most 2^frac: no sum over the vocabulary passes 2^62.
 inline int sample_frac(int vocab)
 {
