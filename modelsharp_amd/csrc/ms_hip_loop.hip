@@ -107,7 +107,7 @@ hipError_t launch_shared_attention(const SharedAttnArgs& args, const SharedPlan&
 namespace {
 int64_t sample_row_bytes(int64_t chunks)
 {
-    return (chunks * (kSampleBins + kSampleTiles + 3) + kSampleList) * 8 + sizeof(SampleFound) + chunks * 8;
+    return chunks * ((kSampleBins + kSampleListChunk + kSampleTiles + 3) * 8 + 12) + sizeof(SampleFound);
 }
 }  // namespace
 
@@ -131,12 +131,13 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     while ((1 << ws.index_bits) < p.vocab) ++ws.index_bits;
     ws.hist = static_cast<unsigned long long*>(workspace);
     ws.list = ws.hist + c * kSampleBins;
-    ws.tiles = ws.list + n * kSampleList;
+    ws.tiles = ws.list + c * kSampleListChunk;
     ws.sums = ws.tiles + c * kSampleTiles;
     ws.all = ws.sums + c * 2;
     ws.found = reinterpret_cast<SampleFound*>(ws.all + c);
     ws.top = reinterpret_cast<float*>(ws.found + n);
     ws.first = reinterpret_cast<int32_t*>(ws.top + c);
+    ws.listed = reinterpret_cast<uint32_t*>(ws.first + c);
     const int lds = (int)(sizeof(SampleLds) + plan.chunks * kSampleTiles * 8);
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sample_draw_kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds))

@@ -17,13 +17,13 @@ namespace msnb {
 
 typedef unsigned long long u64;
 
-// A logit as the order has it: NaN as -infinity, -0 as 0.
-__device__ __forceinline__ float sample_logit(float l) { return l != l ? -__builtin_inff() : l + 0.0f; }
+// A logit as the order has it: NaN as -infinity, +infinity as the largest finite value.
+__device__ __forceinline__ float sample_logit(float l) { return fminf(fmaxf(l, -__builtin_inff()), 3.402823466e38f); }
 
-// Ascending in the order: falling logits, then rising indexes.
+// Ascending in the order: falling logits (-0 as 0), then rising indexes.
 __device__ __forceinline__ uint32_t sample_key(float l)
 {
-    const uint32_t b = __float_as_uint(l);
+    const uint32_t b = __float_as_uint(l + 0.0f);
     return ~(b ^ ((int32_t)b < 0 ? ~0u : 0x80000000u));
 }
 __device__ __forceinline__ float sample_unkey(uint32_t k)
@@ -34,31 +34,44 @@ __device__ __forceinline__ float sample_unkey(uint32_t k)
 // A logit and its index in one number, the index in the low `bits`.
 __device__ __forceinline__ u64 sample_place(float l, int i, int bits) { return (u64)sample_key(l) << bits | (uint32_t)i; }
 
-// 2^y by 2^k 2^f, k the nearest whole number, f in [-1/2, 1/2] by the series of e^(f ln 2) up to the
-// eleventh power (the next term is below 2^-46), in multiples of 2^-frac; 0 from y = -64 down and for NaN.
-__device__ __forceinline__ u64 sample_exp2(double y, int frac)
+// 2^y by 2^k 2^f, k the nearest whole number, f in [-1/2, 1/2] by a polynomial (through 2^f at the zeros of a
+// Chebyshev polynomial, 1 at 0; off by 2^-50), as a whole multiple of 2^-frac in the low bits of a double's (the sum
+// with 2^52 rounds it): kSampleBits above it. y from -64 on; below that, and for NaN, it is 0. A logit's 17 operations
+// in 64 bits are most of what bounds sampling by p, where every logit's weight counts.
+// Four at a time, so that the operations of one wait for nothing.
+constexpr u64 kSampleBits = 0x433ull << 52;
+template <int N>
+__device__ __forceinline__ void sample_raw(const double (&x)[N], int frac, u64 (&out)[N])
 {
-    constexpr double c[12] = {1.0,
-                              0.69314718055994530942,      // ln(2)^n / n!
-                              0.24022650695910071233,
-                              0.055504108664821579953,
-                              0.0096181291076284771620,
-                              0.0013333558146428443423,
-                              0.00015403530393381609954,
-                              1.5252733804059840280e-5,
-                              1.3215486790144309488e-6,
-                              1.0178086009239699728e-7,
-                              7.0549116208011233299e-9,
-                              4.4455382718708114976e-10};
-    const bool some = y > -64.0;
-    y = some ? y : 0.0;
-    const double k = __builtin_rint(y), f = y - k;
-    double s = c[11];
+    constexpr double c[11] = {1.0,
+                              0.6931471805599462,
+                              0.24022650695910075,
+                              0.05550410866465167,
+                              0.009618129107618665,
+                              0.0013333558200794592,
+                              0.00015403530424776529,
+                              1.5252672924850737e-05,
+                              1.3215451633221434e-06,
+                              1.0205905413765595e-07,
+                              7.070977866508138e-09};
+    double t[N], f[N], s[N];
 #pragma unroll
-    for (int n = 10; n >= 0; --n) s = __builtin_fma(s, f, c[n]);
-    // below 2^52 the sum's low bits are the whole number, rounded
-    const u64 w = __builtin_bit_cast(u64, __builtin_ldexp(s, (int)k + frac) + 0x1p52) & ((1ull << 52) - 1);
-    return some ? w : 0;
+    for (int i = 0; i < N; ++i) {
+        const double y = __builtin_fmax(x[i], -64.0);
+        t[i] = y + 0x1.8p52;   // y's whole part in t's low bits
+        f[i] = y - (t[i] - 0x1.8p52);
+        s[i] = c[10];
+    }
+#pragma unroll
+    for (int n = 9; n >= 0; --n)
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = __builtin_fma(s[i], f[i], c[n]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const u64 b = __builtin_bit_cast(u64, s[i]);
+        const uint32_t hi = (uint32_t)(b >> 32) + (((uint32_t)__builtin_bit_cast(u64, t[i]) + frac) << 20);
+        out[i] = __builtin_bit_cast(u64, __builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)b) + 0x1p52);
+    }
 }
 
 // What a row's settings say.
@@ -81,11 +94,18 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int r)
     s.u = a.random[r];
     return s;
 }
-__device__ __forceinline__ u64 sample_weight(float l, float top, const SampleRow& s, int frac)
+__device__ __forceinline__ void sample_weights(floatx4_t l, double top, const SampleRow& s, int frac, u64 (&raw)[4])
 {
-    // (a difference from an infinite largest is -infinity, and so is that from a logit of -infinity)
-    const u64 w = sample_exp2(((double)l - (double)top) * s.scale, frac);
-    return l == top ? 1ull << frac : w;
+    const double y[4] = {((double)l[0] - top) * s.scale, ((double)l[1] - top) * s.scale, ((double)l[2] - top) * s.scale,
+                         ((double)l[3] - top) * s.scale};
+    sample_raw<4>(y, frac, raw);
+}
+__device__ __forceinline__ u64 sample_weight(float l, double top, const SampleRow& s, int frac)
+{
+    const double y[1] = {((double)l - top) * s.scale};
+    u64 raw[1];
+    sample_raw<1>(y, frac, raw);
+    return raw[0] - kSampleBits;
 }
 // The least whole number a sum has to reach to be at least x of w, and the largest it must pass to be above it.
 __device__ __forceinline__ u64 sample_part(float x, u64 w, bool up)
@@ -102,9 +122,6 @@ __device__ __forceinline__ u64 sample_least(const SampleRow& s, int frac)
 {
     return s.m > 0.0f ? (u64)__builtin_rint(__builtin_ldexp((double)fminf(s.m, 1.0f), frac)) : 0;
 }
-
-// e^(d / t) in fp32, to 2^-17 of it where it counts; where d and t are infinite, 0
-__device__ __forceinline__ float sample_rough(float d, float scale) { return fmaxf(__builtin_amdgcn_exp2f(d * scale), 0.0f); }
 
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / kWave;
 constexpr int kSampleTile = 4 * kSampleThreads, kSampleTiles = 4;   // tokens of a tile; tiles of a chunk
@@ -216,19 +233,43 @@ struct SampleSums {
 // Where a row's tokens lie: four neighbours at 16 bytes to a load, so tile and chunk borders are `lead` tokens
 // before multiples of theirs, lead being how many floats the row begins behind 16 bytes.
 __device__ __forceinline__ int sample_lead(const float* x) { return (int)(reinterpret_cast<uintptr_t>(x) / 4 & 3); }
-__device__ __forceinline__ floatx4_t sample_load(const float* x, int i, int V)
+__device__ __forceinline__ floatx4_t sample_edge(const float* x, int i, int V)
 {
     floatx4_t v;
-    if (i >= 0 && i + 3 < V) {
-        v = *reinterpret_cast<const floatx4_t*>(x + i);
-    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < V ? x[i + e] : -__builtin_inff();
-    }
+    for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < V ? x[i + e] : -__builtin_inff();
+    return v;
+}
+__device__ __forceinline__ floatx4_t sample_logits(floatx4_t v)
+{
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = sample_logit(v[e]);
     return v;
 }
+// A thread's four tokens of each of a chunk's tiles. What follows goes from tile to tile in loops that are not
+// unrolled (a code of 23 KB run through once took 12 us for a row, most of it for the instructions), so the
+// tiles move down a place each time.
+struct SampleChunk {
+    floatx4_t v[kSampleTiles];
+    __device__ __forceinline__ void load(const float* x, int at, int V)
+    {
+        const int first = __builtin_amdgcn_readfirstlane(at - 4 * (int)threadIdx.x % (4 * kWave));
+        if (first >= 0 && first + kSampleTile * (kSampleTiles - 1) + 4 * kWave <= V) {   // all of the wave's
+#pragma unroll
+            for (int j = 0; j < kSampleTiles; ++j) v[j] = *reinterpret_cast<const floatx4_t*>(x + at + j * kSampleTile);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kSampleTiles; ++j) v[j] = sample_edge(x, at + j * kSampleTile, V);
+        }
+    }
+    __device__ __forceinline__ floatx4_t next()
+    {
+        const floatx4_t x = v[0];
+#pragma unroll
+        for (int j = 0; j + 1 < kSampleTiles; ++j) v[j] = v[j + 1];
+        return sample_logits(x);
+    }
+};
 
 // Bins of logits on a grid that does not depend on the row: of a sixteenth, or a sixteenth of t where t is
 // below 1, so that the 512 from the largest logit's down reach weights of e^-32 (t up to 1) or 32 below it; the last
@@ -242,13 +283,19 @@ __device__ __forceinline__ int sample_bin(float l, int top_grid, float step)
 {
     return min(top_grid - sample_grid(l, step), kSampleBins - 1);
 }
+// Where the grid's lines are no whole numbers in fp32, or t is next to infinity, the bins say nothing.
+__device__ __forceinline__ bool sample_wide(float top, float step, const SampleRow& s)
+{
+    return !(fabsf(top * step) < 0x1p22f) || !(s.t < 1e30f);
+}
+constexpr float kSampleNone = -46.0f;   // weights of 2^-46 and less are 0: such logits need not be counted
 
 // 1. Each chunk of a row: its largest logit (and that one's index, for the likeliest token), and, where k or p
 // is set, how many logits fall into each bin and, roughly, their weights relative to the chunk's largest: a count in
 // the low 15 bits (a chunk has 2^14), the weights in fp32 as multiples of 2^-31 above, in one whole number, so that an
 // addition in LDS does both and the order of additions does not matter. A bin's place is its grid line modulo
 // 512, the same in every chunk.
-__global__ __launch_bounds__(kSampleThreads) void sample_scan_kernel(SampleArgs a, SampleWs ws)
+__global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleArgs a, SampleWs ws)
 {
     __shared__ u64 hist[kSampleBins], all;
     __shared__ float tops[kSampleWaves];
@@ -257,9 +304,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_scan_kernel(SampleArgs 
     const float* const x = a.logits + (ws.row0 + r) * a.stride;
     const SampleRow s = sample_row(a, ws.row0 + r);
     const int at = c * kSampleTile * kSampleTiles + 4 * tid - sample_lead(x);
-    floatx4_t v[kSampleTiles];
-#pragma unroll
-    for (int j = 0; j < kSampleTiles; ++j) v[j] = sample_load(x, at + j * kSampleTile, a.vocab);
+    SampleChunk tiles;
+    tiles.load(x, at, a.vocab);
     if (tid < kSampleBins) hist[tid] = 0;
     if (tid == 0) {
         first = INT32_MAX;
@@ -269,8 +315,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_scan_kernel(SampleArgs 
 #pragma unroll
     for (int j = 0; j < kSampleTiles; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, v[j][e]);
-    top = wave_max_all(top);
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, tiles.v[j][e]);   // (NaN does not count)
+    top = wave_max_all(fminf(top, 3.402823466e38f));
     if ((tid & (kWave - 1)) == 0) tops[tid >> 6] = top;
     __syncthreads();
 #pragma unroll
@@ -279,10 +325,15 @@ __global__ __launch_bounds__(kSampleThreads) void sample_scan_kernel(SampleArgs 
     if (tid == 0) ws.top[chunk] = top;
     if (s.greedy) {
         int mine = INT32_MAX;
+#pragma unroll 1
+        for (int j = 0; j < kSampleTiles; ++j) {
+            const floatx4_t v = tiles.next();
 #pragma unroll
-        for (int j = kSampleTiles - 1; j >= 0; --j)
-#pragma unroll
-            for (int e = 3; e >= 0; --e) mine = v[j][e] == top && at + j * kSampleTile + e >= 0 ? at + j * kSampleTile + e : mine;
+            for (int e = 0; e < 4; ++e) {
+                const int i = at + j * kSampleTile + e;
+                mine = v[e] == top && i >= 0 ? min(mine, i) : mine;
+            }
+        }
         if (mine != INT32_MAX) atomicMin(&first, mine);
         __syncthreads();
         if (tid == 0) ws.first[chunk] = first;
@@ -290,20 +341,21 @@ __global__ __launch_bounds__(kSampleThreads) void sample_scan_kernel(SampleArgs 
     }
     if (s.k == a.vocab && !(s.p < 1.0f)) return;
     u64 sum = 0;
-    if (top > -__builtin_inff()) {
-        const float step = sample_step(s), scale = (float)s.scale;
-        const int grid = sample_grid(top, step);
-#pragma unroll
-        for (int j = 0; j < kSampleTiles; ++j)
+    const float step = sample_step(s), grid = floorf(top * step), shift = 31.0f - top * (float)s.scale;
+    if (fabsf(shift) < __builtin_inff()) {   // (else nothing here counts beside another chunk, or the row is wide)
+        const float scale = (float)s.scale;
+#pragma unroll 1
+        for (int j = 0; j < kSampleTiles; ++j) {
+            const floatx4_t v = tiles.next();
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float l = v[j][e];
-                const float w = l == top ? 1.0f : sample_rough(l - top, scale);
-                const u64 add = l > -__builtin_inff() ? (u64)(uint32_t)__builtin_fmaf(w, 0x1p31f, 0.5f) << 15 | 1 : 0;
-                const int g = sample_grid(l, step);
+                const float l = v[e], y = __builtin_fmaf(l, scale, shift), g = floorf(l * step);
+                const uint32_t w = (uint32_t)__builtin_amdgcn_exp2f(y);
+                const u64 add = (u64)w << 15 | (y >= 31.0f + kSampleNone ? 1 : 0);
                 sum += add;
-                if (add && grid - g < kSampleBins) atomicAdd(&hist[g & (kSampleBins - 1)], add);
+                if (grid - g < (float)kSampleBins) atomicAdd(&hist[(int)g & (kSampleBins - 1)], add);
             }
+        }
     }
     sum = wave_scan64(sum);
     if ((tid & (kWave - 1)) == kWave - 1) atomicAdd(&all, sum);
@@ -314,44 +366,33 @@ __global__ __launch_bounds__(kSampleThreads) void sample_scan_kernel(SampleArgs 
 
 // 2. Each chunk again, with the whole row's largest logit and bins. The bins that a border may lie in are known but
 // for the rough sums' error: [lo, hi] for the last token kept, and k's where p needs the sum of the first k. Their
-// logits go to the row's list (as places, in the chunks' order); what lies before them is kept and summed
-// exactly, tile by tile. Every workgroup adds up the chunks' bins for itself (4 KB each, from L2, a chunk to a wave), and
-// every wave finds the borders' bins for itself: what is waited for is one round of loads and three barriers. (With a
-// barrier at each step of the search this launch took 54 us for 64 x 151936 of mixed settings.)
+// logits go to the chunk's list (as places); what lies before them is kept and summed exactly, tile by tile. Every
+// workgroup adds up the chunks' bins for itself (4 KB each, from L2), two threads to a bin's place, and every wave
+// finds the borders' bins for itself: one round of loads and one barrier. (With a barrier at each step of the search
+// this launch took 54 us for 64 x 151936 of mixed settings, with additions in LDS 40.)
 __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
 {
-    __shared__ u64 mass[kSampleBins], all_mass, sums[kSampleTiles + 2];
-    __shared__ uint32_t counts[kSampleBins], all_count, place;
+    __shared__ float mass[2][kSampleBins];
+    __shared__ uint32_t counts[2][kSampleBins], place;
+    __shared__ u64 sums[kSampleTiles + 2];
     const int r = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t chunk0 = (int64_t)r * ws.chunks;
     const float* const x = a.logits + (ws.row0 + r) * a.stride;
     const SampleRow s = sample_row(a, ws.row0 + r);
     const int at = c * kSampleTile * kSampleTiles + 4 * tid - sample_lead(x);
-    floatx4_t v[kSampleTiles];
-#pragma unroll
-    for (int j = 0; j < kSampleTiles; ++j) v[j] = sample_load(x, at + j * kSampleTile, a.vocab);
-    if (tid < kSampleBins) {
-        mass[tid] = 0;
-        counts[tid] = 0;
-    }
+    SampleChunk chunk;
+    chunk.load(x, at, a.vocab);
     if (tid < kSampleTiles + 2) sums[tid] = 0;
-    if (tid == 0) {
-        all_mass = 0;
-        all_count = place = 0;
-    }
+    if (tid == 0) place = 0;
     float top = -__builtin_inff();
-    int which = 0;
-    for (int i = lane; i < ws.chunks; i += kWave) {
-        const float t = ws.top[chunk0 + i];
-        which = t > top ? i : which;
-        top = fmaxf(top, t);
-    }
-    const float mine = top;
+    for (int i = lane; i < ws.chunks; i += kWave) top = fmaxf(top, ws.top[chunk0 + i]);
     top = wave_max_all(top);
     if (s.greedy || top == -__builtin_inff()) {   // the first chunk that has it; nothing to draw from
         if (c == 0 && wave == 0) {
-            int i = top > -__builtin_inff() && mine == top ? which : INT32_MAX;
+            int i = INT32_MAX;
+            if (top > -__builtin_inff())
+                for (int j = lane; j < ws.chunks; j += kWave) i = ws.top[chunk0 + j] == top ? min(i, j) : i;
 #pragma unroll
             for (int o = 32; o; o >>= 1) i = min(i, __shfl_xor(i, o));
             if (lane == 0) {
@@ -362,128 +403,131 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
         }
         return;
     }
-    const float step = sample_step(s);
+    const float step = sample_step(s), scale = (float)s.scale;
     const int grid = sample_grid(top, step);
     bool by_k = s.k < a.vocab;
-    const bool by_p = s.p < 1.0f;
+    const bool by_p = s.p < 1.0f, borders = by_k || by_p, wide = borders && sample_wide(top, step, s);
     int lo = kSampleBins, hi = kSampleBins, bk = kSampleBins;
-    uint32_t k_before = 0, listed = 0;
-    __syncthreads();
-    if (by_k || by_p) {
-        // a lane has eight places of a chunk's bins; place q holds grid line grid - b with b = (grid - q) mod 512
-        const u64* const hists = ws.hist + chunk0 * kSampleBins;
-        for (int i = wave; i < ws.chunks; i += kSampleWaves) {
-            const float ti = ws.top[chunk0 + i];
-            if (ti == -__builtin_inff()) continue;
-            const float f = ti == top ? 1.0f : sample_rough(ti - top, (float)s.scale);
-            const int below = grid - sample_grid(ti, step);   // the chunk's bins begin so far below the row's
-            const u64 rest = ws.all[chunk0 + i];
-#pragma unroll
-            for (int e = 0; e < kSampleEach; ++e) {
-                const u64 h = hists[(int64_t)i * kSampleBins + kSampleEach * lane + e];
-                const int b = (grid - (kSampleEach * lane + e)) & (kSampleBins - 1);
-                if (h && b >= below && b < kSampleBins - 1) {
-                    atomicAdd(&mass[b], (u64)((double)(h >> 15) * f));
-                    atomicAdd(&counts[b], (uint32_t)(h & 0x7fff));
-                }
-            }
-            if (lane == 0) {
-                atomicAdd(&all_mass, (u64)((double)(rest >> 15) * f));
-                atomicAdd(&all_count, (uint32_t)(rest & 0x7fff));
+    uint32_t k_before = 0;
+    if (wide) {   // any bin
+        lo = 0;
+        hi = kSampleBins - 1;
+        bk = by_k ? 0 : kSampleBins;
+    } else if (borders) {
+        // place q of a chunk's bins holds grid line grid - b with b = (grid - q) mod 512, or one too far down
+        const int q = tid & (kSampleBins - 1), half = tid / kSampleBins, b0 = (grid - q) & (kSampleBins - 1);
+        const u64* const hists = ws.hist + chunk0 * kSampleBins + q;
+        float m = 0.0f;
+        uint32_t n = 0;
+#pragma unroll 4
+        for (int i = half; i < ws.chunks; i += 2) {
+            const u64 h = hists[(int64_t)i * kSampleBins];
+            const float t = ws.top[chunk0 + i];
+            const bool in = (float)b0 >= (float)grid - floorf(t * step);   // no higher than the chunk's largest
+            n += in ? (uint32_t)(h & 0x7fff) : 0;
+            m += in ? (float)(h >> 15) * __builtin_amdgcn_exp2f((t - top) * scale) : 0.0f;
+        }
+        const bool last = b0 == kSampleBins - 1;
+        mass[half][b0] = last ? 0.0f : m;
+        counts[half][b0] = last ? 0 : n;
+        float all_mass = 0.0f;
+        uint32_t all_count = 0;
+        for (int i = lane; i < ws.chunks; i += kWave) {
+            const float y = (ws.top[chunk0 + i] - top) * scale;
+            const u64 h = ws.all[chunk0 + i];
+            if (y >= kSampleNone) {
+                all_mass += (float)(h >> 15) * __builtin_amdgcn_exp2f(y);
+                all_count += (uint32_t)(h & 0x7fff);
             }
         }
+        all_mass = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_sums(all_mass)), kWave - 1));
+        all_count = (uint32_t)__builtin_amdgcn_readlane((int)wave_sums(all_count), kWave - 1);
         __syncthreads();
-        SampleSums<float> m;
-        SampleSums<uint32_t> n;
+        SampleSums<float> ms;
+        SampleSums<uint32_t> ns;
 #pragma unroll
         for (int e = 0; e < kSampleEach; ++e) {
-            m.up[e] = (float)mass[kSampleEach * lane + e];
-            n.up[e] = counts[kSampleEach * lane + e];
+            ms.up[e] = mass[0][kSampleEach * lane + e] + mass[1][kSampleEach * lane + e];
+            ns.up[e] = counts[0][kSampleEach * lane + e] + counts[1][kSampleEach * lane + e];
         }
-        m.scan();
-        n.scan();
+        ms.scan();
+        ns.scan();
         if (lane == kWave - 1) {   // the row's last bin: what none of the others holds
-            m.up[kSampleEach - 1] = (float)all_mass;
-            n.up[kSampleEach - 1] = all_count;
+            ms.up[kSampleEach - 1] = fmaxf(all_mass, ms.up[kSampleEach - 1]);
+            ns.up[kSampleEach - 1] = max(all_count, ns.up[kSampleEach - 1]);
         }
-        by_k = by_k && (uint32_t)s.k < all_count;
+        by_k = by_k && (uint32_t)s.k < ns.at(kSampleBins - 1);
         if (by_k) {
-            bk = n.reach(s.k);
-            k_before = n.at(bk - 1);
+            bk = ns.reach(s.k);
+            k_before = ns.at(bk - 1);
         }
         if (by_p) {
-            // two of fp32's exponentials, off by 2^-17 each (arguments up to 64, rounded twice), a sum in fp32, half a
-            // step for each logit and a step of each bin and chunk
-            const float off = 0x1p-14f * (float)all_mass + (float)all_count + (float)ws.chunks * kSampleBins;
-            const float w0 = m.at(by_k ? bk - 1 : kSampleBins - 1), w1 = m.at(by_k ? bk : kSampleBins - 1);
-            const float p = fmaxf(s.p, 0.0f);
-            hi = min(m.reach(p * w1 + off), by_k ? bk : kSampleBins - 1);
-            lo = min(m.reach(p * w0 - off), hi);
+            // two of fp32's exponentials: arguments of up to 64 with three roundings (2^-16 of it each) and a shift by the
+            // chunk's largest logit (half a step of that), sums in fp32, a step of 2^-31 each
+            const float all = ms.at(kSampleBins - 1);
+            const float off = (0x1p-13f + 0x1p-22f * fabsf(top * scale)) * all + (float)ns.at(kSampleBins - 1);
+            const float w0 = by_k ? ms.at(bk - 1) : all, w1 = by_k ? ms.at(bk) : all, p = fmaxf(s.p, 0.0f);
+            hi = min(ms.reach(p * w1 + off), by_k ? bk : kSampleBins - 1);
+            lo = min(ms.reach(p * w0 - off), hi);
         } else if (by_k) {
             lo = hi = bk;
         }
-        // how many are listed, and how many of them by the chunks before this one
-        if (lo < kSampleBins) {
-            const bool two = by_p && by_k && bk > hi;
-            listed = n.at(hi) - n.at(lo - 1) + (two ? n.at(bk) - n.at(bk - 1) : 0);
-            for (int i = wave; i < c; i += kSampleWaves) {
-                const float ti = ws.top[chunk0 + i];
-                if (ti == -__builtin_inff()) continue;
-                const int below = grid - sample_grid(ti, step);
-                u64 in = 0;      // listed, and in any bin but the last
-#pragma unroll
-                for (int e = 0; e < kSampleEach; ++e) {
-                    const u64 h = hists[(int64_t)i * kSampleBins + kSampleEach * lane + e] & 0x7fff;
-                    const int b = (grid - (kSampleEach * lane + e)) & (kSampleBins - 1);
-                    if (b >= below && b < kSampleBins - 1) in += h << 32 | ((b >= lo && b <= hi) || (two && b == bk) ? h : 0);
-                }
-                in = wave_scan64(in);
-                if (lane == kWave - 1) {
-                    const bool last = hi == kSampleBins - 1 || (two && bk == kSampleBins - 1);
-                    atomicAdd(&place, (uint32_t)in + (last ? (uint32_t)(ws.all[chunk0 + i] & 0x7fff) - (uint32_t)(in >> 32) : 0));
-                }
-            }
-            __syncthreads();
-        }
+    } else {
+        __syncthreads();   // the sums are zero
     }
-    const bool list = listed && listed <= kSampleList;
-    if (c == 0 && tid == 0) ws.found[r] = {top, lo, hi, bk, by_k, by_p, k_before, list ? listed : 0, 0, 0};
+    if (wide) __syncthreads();
+    if (c == 0 && tid == 0) ws.found[r] = {top, lo, hi, bk, by_k, by_p, k_before, 0};
 
     // sums: each tile's kept weights before `lo`; the weights before `lo`; all weights that p is a part of
     const u64 least = sample_least(s, a.frac);
-    const int whole = by_p ? by_k ? bk : kSampleBins : 0, bins = max(lo, whole);
-    u64* const out = ws.list + (int64_t)r * kSampleList;
+    const bool every = by_p && !by_k, two = by_p && by_k && bk > hi;
+    // Logits from which on a tile has something to keep or to list (on the grid), or, without borders, to keep.
+    const int deep = by_k ? max(hi, bk) : hi;
+    const float slack = 0.01f + 0x1p-21f * fabsf(top * scale);   // of the divisions and sums here
+    const float none = top + (kSampleNone - slack) / scale;
+    const float from = lo == kSampleBins && least ? top + (__builtin_amdgcn_logf(fminf(s.m, 1.0f)) - slack) / scale : none;
+    const float line = deep < kSampleBins - 1 ? (float)(grid - deep) : -__builtin_inff();
+    const float line_lo = lo < kSampleBins ? (float)(grid - lo + 1) : -__builtin_inff();   // in a bin before lo
+    const float line_hi = hi < kSampleBins - 1 ? (float)(grid - hi) : -__builtin_inff();
+    const float line_k = by_k ? (float)(grid - bk + 1) : __builtin_inff();   // in a bin before bk
+    const float line_k_end = bk < kSampleBins - 1 ? (float)(grid - bk) : -__builtin_inff();
+    u64* const out = ws.list + (chunk0 + c) * kSampleListChunk;
     u64 before_lo = 0, part = 0;
-#pragma unroll
+#pragma unroll 1
     for (int j = 0; j < kSampleTiles; ++j) {
-        int b[4];
-        bool any = false, some = false;
+        const floatx4_t v = chunk.next();
+        const float high = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        const bool some = __ballot(high >= from && high * step >= line) && !wide;
+        if (!some && !every) continue;
+        u64 raw[4];
+        sample_weights(v, (double)top, s, a.frac, raw);
+        if (every) part += (raw[0] + raw[1]) + (raw[2] + raw[3]) - 4 * kSampleBits;
+        if (!some) continue;
+        u64 tile = 0;
+        uint32_t listed = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            b[e] = lo < kSampleBins ? sample_bin(v[j][e], grid, step) : 0;
-            b[e] = v[j][e] == -__builtin_inff() ? kSampleBins : b[e];
-            any |= b[e] < bins;
-            some |= b[e] >= lo && (b[e] <= hi || b[e] == bk);
+            const float g = v[e] * step;
+            const u64 w = raw[e] - kSampleBits, before = g >= line_lo ? w : 0;
+            tile += before >= least ? before : 0;
+            before_lo += before;
+            if (!every) part += g >= line_k ? w : 0;
+            const bool in = g < line_lo && v[e] >= none && (g >= line_hi || (two && g < line_k && g >= line_k_end));
+            listed |= in ? 1u << e : 0;
         }
-        if (__ballot(any)) {
-            u64 tile = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const u64 w = sample_weight(v[j][e], top, s, a.frac);
-                const u64 before = b[e] < lo ? w : 0;
-                tile += before >= least ? before : 0;
-                before_lo += before;
-                part += b[e] < whole ? w : 0;
+        tile = wave_scan64(tile);
+        if (lane == kWave - 1) atomicAdd(&sums[j], tile);
+        while (const uint64_t ready = __ballot(listed != 0)) {   // (a lane's in order)
+            uint32_t to = 0;
+            if (lane == 0) to = atomicAdd(&place, __popcll(ready));
+            to = __builtin_amdgcn_readfirstlane(to) + __builtin_amdgcn_mbcnt_hi((uint32_t)(ready >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ready, 0));
+            if (listed) {
+                const int e = __ffs(listed) - 1;
+                const float l = e & 2 ? e & 1 ? v[3] : v[2] : e & 1 ? v[1] : v[0];
+                if (to < kSampleListChunk) out[to] = sample_place(l, at + j * kSampleTile + e, ws.index_bits);
+                listed &= listed - 1;
             }
-            tile = wave_scan64(tile);
-            if (lane == kWave - 1) atomicAdd(&sums[j], tile);
         }
-        if (list && some)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (b[e] < kSampleBins && ((b[e] >= lo && b[e] <= hi) || (by_p && b[e] == bk)))
-                    if (const uint32_t to = atomicAdd(&place, 1); to < kSampleList)   // (or the logits have changed since)
-                        out[to] = sample_place(v[j][e], at + j * kSampleTile + e, ws.index_bits);
     }
     if (by_p) {
         before_lo = wave_scan64(before_lo);
@@ -496,16 +540,18 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
     __syncthreads();
     if (tid < kSampleTiles) ws.tiles[(chunk0 + c) * kSampleTiles + tid] = sums[tid];
     else if (tid < kSampleTiles + 2) ws.sums[(chunk0 + c) * 2 + tid - kSampleTiles] = sums[tid];
+    if (tid == 0) ws.listed[chunk0 + c] = wide ? kSampleList + 1 : place;   // (wide: the row itself)
 }
 
 // 3. Each row: the borders among the listed logits (or, where those are too many for the list, among the
 // row's), and the draw. Fine bins of the listed logits, the few of a border's fine bin ranked by a wave, then the
 // tile that the draw falls into and the token; as above every wave searches for itself.
 struct SampleLds {
-    u64 list[kSampleList];
+    u64 list[kSampleList], weight[kSampleList];   // places and their weights
+    uint16_t bin[kSampleList];                    // fine bins, the top bit set where it is not in [lo, hi]
     u64 mass[kSampleBins];
     uint32_t counts[kSampleBins];
-    u64 few[2][kWave];
+    u64 few[2][kWave], few_weight[2][kWave];
     u64 digit[256], digit_weight[256];
     u64 scratch[kSampleWaves];
     u64 found[3];
@@ -523,6 +569,7 @@ __device__ __forceinline__ SampleBorder sample_rank(u64 c, u64 w, int n, u64 las
 {
     const bool in = (int)(threadIdx.x & (kWave - 1)) < n && c <= last;
     u64 sum = 0, weights = 0;
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
         const u64 ci = lane_value64(c, i), wi = lane_value64(w, i);
         const bool upto = ci <= c && ci <= last;
@@ -532,6 +579,7 @@ __device__ __forceinline__ SampleBorder sample_rank(u64 c, u64 w, int n, u64 las
     // the first in order that reaches it, else the last
     SampleBorder b{0, 0};
     bool reached = false;
+#pragma unroll 1
     for (uint64_t todo = __ballot(in); todo; todo &= todo - 1) {
         const int i = __ffsll((unsigned long long)todo) - 1;
         const u64 ci = lane_value64(c, i);
@@ -542,103 +590,122 @@ __device__ __forceinline__ SampleBorder sample_rank(u64 c, u64 w, int n, u64 las
     return b;
 }
 
-__global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs a, SampleWs ws)
+// What the borders' search needs of a row.
+struct SampleSearch {
+    const float* x;
+    SampleRow s;
+    SampleFound f;
+    float step;
+    int grid, V, frac, index_bits, lead, tiles, n;
+    u64 least;
+};
+
+// The last place that is kept; the weights of those in [lo, hi] are added to their tiles. LIST: among the n listed
+// places, else among the row's.
+template <bool LIST>
+__device__ __forceinline__ u64 sample_borders(const SampleSearch& q, SampleLds& lds)
 {
-    extern __shared__ u64 sample_lds[];
-    SampleLds& lds = *reinterpret_cast<SampleLds*>(sample_lds);
-    const int r = blockIdx.x, row = ws.row0 + r, tid = threadIdx.x, lane = tid & (kWave - 1), V = a.vocab;
-    const float* const x = a.logits + row * a.stride;
-    const int lead = sample_lead(x);
-    // everything that lies at a known place is loaded before any of it is waited for
-    const SampleRow s = sample_row(a, row);
-    const SampleFound f = ws.found[r];
-    const int64_t chunk0 = (int64_t)r * ws.chunks;
-    const int tiles = ws.chunks * kSampleTiles;
-    u64 early[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) early[i] = ws.list[(int64_t)r * kSampleList + i * kSampleThreads + tid];
-    u64 sum0 = 0, sum1 = 0;
-    for (int i = tid; i < ws.chunks; i += kSampleThreads) {
-        sum0 += ws.sums[(chunk0 + i) * 2];
-        sum1 += ws.sums[(chunk0 + i) * 2 + 1];
-    }
-    for (int i = tid; i < tiles; i += kSampleThreads) lds.tiles[i] = ws.tiles[chunk0 * kSampleTiles + i];
-    if (s.greedy || f.answered) return;
-    const float step = sample_step(s);
-    const int grid = sample_grid(f.top, step);
-    const u64 least = sample_least(s, a.frac);
-    const int n = (int)f.listed;   // 0: the row itself
-    u64 last = ~0ull;
-    auto weight = [&](float l) { return sample_weight(l, f.top, s, a.frac); };
-    auto place_weight = [&](u64 c) { return weight(sample_unkey((uint32_t)(c >> ws.index_bits))); };
-    if (f.lo < kSampleBins) {
-        const bool two = f.by_k && f.by_p && f.bk > f.hi;
-        // fine bins: as many to each bin that is listed, by the logit's place in it
-        const int fine = kSampleBins / min(f.hi - f.lo + 1 + two, kSampleBins);
-        auto fine_bin = [&](float l, int b) {
-            const float q = l * step, part = 1.0f - (q - floorf(q));
-            const int k = b == kSampleBins - 1 || !(part >= 0.0f) ? fine - 1 : min((int)(part * (float)fine), fine - 1);
-            return min((b > f.hi ? f.hi + 1 - f.lo : b - f.lo) * fine + k, kSampleBins - 1);
-        };
-        // every listed place: fn(place, logit, fine bin, whether in [lo, hi])
-        auto each = [&](auto&& fn) {
-            const int m = n ? n : V;
-            for (int i = tid; i < m; i += kSampleThreads) {
-                const u64 c = n ? lds.list[i] : sample_place(sample_logit(x[i]), i, ws.index_bits);
-                const float l = sample_unkey((uint32_t)(c >> ws.index_bits));
-                if (l == -__builtin_inff()) continue;
-                const int b = sample_bin(l, grid, step);
-                if ((b >= f.lo && b <= f.hi) || (two && b == f.bk)) fn(c, l, fine_bin(l, b), b <= f.hi);
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const SampleFound& f = q.f;
+    const bool two = f.by_k && f.by_p && f.bk > f.hi;
+    // fine bins: as many to each bin that is listed, by the logit's place in it
+    const int fine = kSampleBins / min(f.hi - f.lo + 1 + two, kSampleBins);
+    auto weigh = [&](u64 c) { return sample_weight(sample_unkey((uint32_t)(c >> q.index_bits)), (double)f.top, q.s, q.frac); };
+    auto fine_bin = [&](float l) {
+        const float g = l * q.step, part = 1.0f - (g - floorf(g));
+        const int b = sample_bin(l, q.grid, q.step);
+        const int k = b == kSampleBins - 1 || !(part >= 0.0f) ? fine - 1 : min((int)(part * (float)fine), fine - 1);
+        const int base = b > f.hi ? f.hi + 1 - f.lo : b - f.lo;
+        const bool in = b >= f.lo && (b <= f.hi || (two && b == f.bk));
+        return in ? min(base * fine + k, kSampleBins - 1) | (b > f.hi ? 0x8000 : 0) : 0x7fff;
+    };
+    // every place in question: fn(place, weight, fine bin, whether in [lo, hi])
+    auto each = [&](auto&& fn) {
+#pragma unroll 1
+        for (int i = tid; i < (LIST ? q.n : q.V); i += kSampleThreads) {
+            if constexpr (LIST) {
+                const uint32_t b = lds.bin[i];
+                fn(lds.list[i], lds.weight[i], (int)(b & 0x7fff), b < 0x8000);
+            } else {
+                const float l = sample_logit(q.x[i]);
+                if (!(((double)l - f.top) * q.s.scale >= kSampleNone)) continue;
+                const int b = fine_bin(l);
+                const u64 c = sample_place(l, i, q.index_bits);
+                if (b != 0x7fff) fn(c, weigh(c), b & 0x7fff, b < 0x8000);
             }
-        };
-        if (tid < kSampleBins) {
-            lds.mass[tid] = 0;
-            lds.counts[tid] = 0;
         }
-        if (tid < 2) {
-            lds.sums[tid] = 0;
-            lds.n_few[tid] = 0;
+    };
+    if constexpr (LIST) {
+#pragma unroll 1
+        for (int i = tid; i < q.n; i += kSampleThreads) {
+            const u64 c = lds.list[i], w = weigh(c);
+            const int b = fine_bin(sample_unkey((uint32_t)(c >> q.index_bits)));
+            lds.weight[i] = w;
+            lds.bin[i] = (uint16_t)b;
+            atomicAdd(&lds.counts[b & (kSampleBins - 1)], 1);
+            atomicAdd(&lds.mass[b & (kSampleBins - 1)], w);
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (i * kSampleThreads + tid < n) lds.list[i * kSampleThreads + tid] = early[i];
-        for (int i = 2 * kSampleThreads + tid; i < n; i += kSampleThreads) lds.list[i] = ws.list[(int64_t)r * kSampleList + i];
-        __syncthreads();
-        if (f.by_p && sum0 | sum1) {
-            atomicAdd(&lds.sums[0], sum0);
-            atomicAdd(&lds.sums[1], sum1);
-        }
-        each([&](u64, float l, int k, bool) {
-            atomicAdd(&lds.counts[k], 1);
-            if (f.by_p) atomicAdd(&lds.mass[k], weight(l));
+    } else {
+        each([&](u64, u64 w, int b, bool) {
+            atomicAdd(&lds.counts[b], 1);
+            atomicAdd(&lds.mass[b], w);
         });
-        __syncthreads();
-        SampleSums<uint32_t> counts;
-        SampleSums<u64> mass;
+    }
+    __syncthreads();
+    SampleSums<uint32_t> counts;
+    SampleSums<u64> mass;
 #pragma unroll
-        for (int e = 0; e < kSampleEach; ++e) {
-            counts.up[e] = lds.counts[kSampleEach * lane + e];
-            mass.up[e] = lds.mass[kSampleEach * lane + e];
-        }
-        counts.scan();
-        mass.scan();
-        // The place in fine bin k at which the counts or weights of its places, up to `up_to`, sum to `target`,
-        // and their sum of weights up to it.
-        auto border = [&](int slot, int k, u64 up_to, u64 target, bool count) -> SampleBorder {
-            const int m = (int)(counts.at(k) - counts.at(k - 1));
-            if (m <= kWave) {
-                each([&](u64 c, float, int b, bool) {
-                    if (b == k)
-                        if (const uint32_t to = atomicAdd(&lds.n_few[slot], 1); to < kWave) lds.few[slot][to] = c;
-                });
-                __syncthreads();
-                const u64 c = lds.few[slot][lane];
-                return sample_rank(c, place_weight(c), m, up_to, target, count);
+    for (int e = 0; e < kSampleEach; ++e) {
+        counts.up[e] = lds.counts[kSampleEach * lane + e];
+        mass.up[e] = lds.mass[kSampleEach * lane + e];
+    }
+    counts.scan();
+    mass.scan();
+    // The place in fine bin k at which the counts or weights of its places, up to `up_to`, sum to `target`,
+    // and their sum of weights up to it: first k's, then p's.
+    u64 last = ~0ull, whole = lds.sums[1];
+    const u64 before = lds.sums[0];
+#pragma unroll 1
+    for (int slot = f.by_k ? 0 : 1; slot < (f.by_p ? 2 : 1); ++slot) {
+        const bool count = slot == 0;
+        const int first = (two ? f.hi + 1 - f.lo : f.bk - f.lo) * fine;   // bk's first fine bin
+        u64 target;
+        int k;
+        bool there;
+        if (count) {
+            target = (uint32_t)q.s.k - f.k_before + counts.at(first - 1);
+            k = counts.reach((uint32_t)target);
+            there = counts.at(kSampleBins - 1) >= target;
+            target -= counts.at(k - 1);
+        } else {
+            const u64 all = sample_part(q.s.p, whole, true);
+            if (all <= before) {   // (as the rough sums have it, it is not)
+                last = 0;
+                break;
             }
+            target = all - before;
+            k = mass.reach(target);
+            there = mass.at(kSampleBins - 1) >= target;
+            target -= min(mass.at(k - 1), target - 1);
+        }
+        SampleBorder b{last, mass.at(k) - mass.at(k - 1)};   // (fewer with a weight: all of them)
+        const int m = (int)(counts.at(k) - counts.at(k - 1));
+        if (!there) {
+        } else if (m <= kWave) {
+            each([&](u64 c, u64 w, int b, bool) {
+                if (b == k)
+                    if (const uint32_t to = atomicAdd(&lds.n_few[slot], 1); to < kWave) {
+                        lds.few[slot][to] = c;
+                        lds.few_weight[slot][to] = w;
+                    }
+            });
+            __syncthreads();
+            b = sample_rank(lds.few[slot][lane], lds.few_weight[slot][lane], m, last, target, count);
+        } else {
             // many, as equal logits are: by digits of 8 bits below what they have in common
             u64 low = ~0ull, high = 0;
-            each([&](u64 c, float, int b, bool) {
-                if (b == k && c <= up_to) {
+            each([&](u64 c, u64, int b, bool) {
+                if (b == k && c <= last) {
                     low = min(low, c);
                     high = max(high, c);
                 }
@@ -651,19 +718,18 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
             __syncthreads();
             low = lds.found[0];
             high = lds.found[1];
-            if (low >= high) return {high, place_weight(high)};
-            int above = 64 - __builtin_clzll(low ^ high);
-            u64 prefix = above < 64 ? low >> above : 0, before = 0, weights = 0;
+            int above = low < high ? 64 - __builtin_clzll(low ^ high) : 0;
+            u64 prefix = low < high ? above < 64 ? low >> above : 0 : high, sum = 0, weights = 0;
+#pragma unroll 1
             while (above > 0) {
                 const int shift = max(0, above - 8);
                 __syncthreads();
                 if (tid < 256) lds.digit[tid] = lds.digit_weight[tid] = 0;
                 if (tid < 2) lds.found[tid] = 0;
                 __syncthreads();
-                each([&](u64 c, float l, int b, bool) {
-                    if (b != k || c > up_to || (above < 64 && c >> above != prefix)) return;
+                each([&](u64 c, u64 w, int b, bool) {
+                    if (b != k || c > last || (above < 64 && c >> above != prefix)) return;
                     const int d = (int)(c >> shift) & ((1 << (above - shift)) - 1);
-                    const u64 w = weight(l);
                     atomicAdd(&lds.digit_weight[d], w);
                     atomicAdd(&lds.digit[d], count ? 1 : w);
                     atomicMax(&lds.found[0], (u64)d);   // the last there is, should the target not be reached
@@ -671,7 +737,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
                 __syncthreads();
                 const u64 mine = tid < 256 ? lds.digit[tid] : 0, heavy = tid < 256 ? lds.digit_weight[tid] : 0;
                 const int end = (int)lds.found[0];
-                const u64 up = before + block_scan(mine, lds.scratch);
+                const u64 up = sum + block_scan(mine, lds.scratch);
                 __syncthreads();
                 const u64 up_weights = weights + block_scan(heavy, lds.scratch);
                 if (tid <= end && up - mine < target && (up >= target || tid == end)) {
@@ -681,53 +747,107 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
                 }
                 __syncthreads();
                 prefix = prefix << (above - shift) | lds.found[1];
-                before = lds.found[0];
+                sum = lds.found[0];
                 weights = lds.found[2];
                 above = shift;
             }
-            return {prefix, weights + place_weight(prefix)};
-        };
-        u64 whole = lds.sums[1];   // what p is a part of
-        if (f.by_k) {
-            const int first = (two ? f.hi + 1 - f.lo : f.bk - f.lo) * fine;   // bk's first fine bin
-            const uint32_t target = (uint32_t)s.k - f.k_before + counts.at(first - 1);
-            const int k = counts.reach(target);
-            const SampleBorder q = border(0, k, ~0ull, target - counts.at(k - 1), true);
-            last = q.place;
-            whole += mass.at(k - 1) - mass.at(first - 1) + q.sum;
+            b = {prefix, weights + weigh(prefix)};
         }
-        if (f.by_p) {
-            const u64 all = sample_part(s.p, whole, true), before = lds.sums[0], target = all > before ? all - before : 0;
-            const int k = mass.reach(target);
-            last = target ? border(1, k, last, target - min(mass.at(k - 1), target - 1), false).place : 0;
+        last = b.place;
+        if (count) whole += mass.at(k - 1) - mass.at(first - 1) + b.sum;
+    }
+    each([&](u64 c, u64 w, int, bool kept) {
+        const int tile = (((uint32_t)c & ((1u << q.index_bits) - 1)) + q.lead) / kSampleTile;
+        if (kept && c <= last && w >= q.least && tile < q.tiles) atomicAdd(&lds.tiles[tile], w);
+    });
+    return last;
+}
+
+__global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs a, SampleWs ws)
+{
+    extern __shared__ u64 sample_lds[];
+    SampleLds& lds = *reinterpret_cast<SampleLds*>(sample_lds);
+    const int r = blockIdx.x, row = ws.row0 + r, tid = threadIdx.x, lane = tid & (kWave - 1), V = a.vocab;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float* const x = a.logits + row * a.stride;
+    const int lead = sample_lead(x);
+    // everything that lies at a known place is loaded before any of it is waited for
+    const SampleRow s = sample_row(a, row);
+    const SampleFound f = ws.found[r];
+    const int64_t chunk0 = (int64_t)r * ws.chunks;
+    const int tiles = ws.chunks * kSampleTiles;
+    const u64* const lists = ws.list + chunk0 * kSampleListChunk;
+    const u64 early = wave < ws.chunks ? lists[(int64_t)wave * kSampleListChunk + lane] : 0;   // (what is no list's is not used)
+    u64 sum0 = 0, sum1 = 0;
+    for (int i = tid; i < ws.chunks; i += kSampleThreads) {
+        sum0 += ws.sums[(chunk0 + i) * 2];
+        sum1 += ws.sums[(chunk0 + i) * 2 + 1];
+    }
+    for (int i = tid; i < tiles; i += kSampleThreads) lds.tiles[i] = ws.tiles[chunk0 * kSampleTiles + i];
+    if (s.greedy || f.answered) return;
+    const float step = sample_step(s);
+    const int grid = sample_grid(f.top, step);
+    const u64 least = sample_least(s, a.frac);
+    u64 last = ~0ull;
+    if (f.lo < kSampleBins) {
+        if (tid < kSampleBins) {
+            lds.mass[tid] = 0;
+            lds.counts[tid] = 0;
         }
-        each([&](u64 c, float l, int, bool kept) {
-            const u64 w = weight(l);
-            const int tile = (((uint32_t)c & ((1u << ws.index_bits) - 1)) + lead) / kSampleTile;
-            if (kept && c <= last && w >= least && tile < tiles) atomicAdd(&lds.tiles[tile], w);
-        });
+        if (tid < 2) {
+            lds.sums[tid] = 0;
+            lds.n_few[tid] = 0;
+        }
+        // the chunks' lists, one behind the other
+        int n = 0;
+        bool fits = true;
+        for (int base = 0; base < ws.chunks && fits; base += kWave) {
+            const int m = min(ws.chunks - base, kWave);
+            const uint32_t mine = lane < m ? ws.listed[chunk0 + base + lane] : 0;
+            const uint32_t up = wave_sums(min(mine, (uint32_t)kSampleListChunk));
+            const int all = __builtin_amdgcn_readlane((int)up, kWave - 1);
+            fits = !__ballot(mine > kSampleListChunk) && n + all <= kSampleList;
+            if (fits)
+                for (int i = wave; i < m; i += kSampleWaves) {
+                    const int count = __builtin_amdgcn_readlane((int)mine, i), to = n + __builtin_amdgcn_readlane((int)up, i) - count;
+#pragma unroll 1
+                    for (int e = lane; e < count; e += kWave)
+                        lds.list[to + e] = base == 0 && i < kSampleWaves && e < kWave ? early : lists[(int64_t)(base + i) * kSampleListChunk + e];
+                }
+            n += all;
+        }
+        __syncthreads();
+        if (f.by_p && (sum0 | sum1)) {
+            atomicAdd(&lds.sums[0], sum0);
+            atomicAdd(&lds.sums[1], sum1);
+        }
+        const SampleSearch q{x, s, f, step, grid, V, a.frac, ws.index_bits, lead, tiles, n, least};
+        last = fits ? sample_borders<true>(q, lds) : sample_borders<false>(q, lds);
     }
     __syncthreads();
 
     // the tile that the draw falls into: a run of tiles to a lane
     const int run = (tiles + kWave - 1) / kWave;
     u64 sum = 0;
+#pragma unroll 1
     for (int i = lane * run; i < min((lane + 1) * run, tiles); ++i) sum += lds.tiles[i];
     const u64 runs = wave_scan64(sum), total = lane_value64(runs, kWave - 1);
     u64 target = sample_part(s.u, total, false);
     const uint64_t past = __ballot(runs > target);
     int tile = (past ? __ffsll((unsigned long long)past) - 1 : 0) * run;
     target -= past ? lane_value64(runs - sum, tile / run) : 0;
+#pragma unroll 1
     for (; tile < tiles - 1 && lds.tiles[tile] <= target; ++tile) target -= lds.tiles[tile];
     // its token
     const int at = tile * kSampleTile + 4 * tid - lead;
-    u64 w[4], mine = 0;
-    const floatx4_t v = sample_load(x, at, V);
+    u64 w[4], raw[4], mine = 0;
+    const floatx4_t v = sample_logits(at >= 0 && at + 3 < V ? *reinterpret_cast<const floatx4_t*>(x + at) : sample_edge(x, at, V));
+    sample_weights(v, (double)f.top, s, a.frac, raw);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const bool kept = v[e] > -__builtin_inff() &&
                           (sample_place(v[e], at + e, ws.index_bits) <= last || sample_bin(v[e], grid, step) < f.lo);
-        const u64 we = kept ? weight(v[e]) : 0;
+        const u64 we = kept ? raw[e] - kSampleBits : 0;
         w[e] = we >= least ? we : 0;
         mine += w[e];
     }

@@ -66,7 +66,7 @@ struct SampleArgs {
     int64_t stride;
 };
 constexpr int kSampleBins = 512;                 // of logits, by which a border is first looked for
-constexpr int kSampleList = 8192;                // logits of the bins that a border lies in
+constexpr int kSampleList = 6144, kSampleListChunk = 1536;   // logits of the bins that a border lies in, at most
 constexpr int kSampleChunk = 16384;              // tokens of a workgroup of the first two launches
 // What the second launch finds out about a row.
 struct SampleFound {
@@ -74,19 +74,19 @@ struct SampleFound {
     int lo, hi, bk;            // bins: where the last token kept may lie, and the k-th token's (kSampleBins: none)
     int by_k, by_p;
     uint32_t k_before;         // tokens before bin bk
-    uint32_t listed;           // 0: nothing, or more than the list holds
-    int answered, unused;      // the row's answer is there
+    int answered;              // the row's answer is there
 };
 // The workspace of `batch` rows: rows are taken so many at a time.
 struct SampleWs {
     unsigned long long* hist;  // [rows][chunks][kSampleBins]
-    unsigned long long* list;  // [rows][kSampleList]
+    unsigned long long* list;  // [rows][chunks][kSampleListChunk]
     unsigned long long* tiles; // [rows][chunks][4]: kept weights
     unsigned long long* sums;  // [rows][chunks][2]
     unsigned long long* all;   // [rows][chunks]: the sum of a chunk's bins
     SampleFound* found;        // [rows]
     float* top;                // [rows][chunks]: largest logit
     int32_t* first;            // [rows][chunks]: its index
+    uint32_t* listed;          // [rows][chunks]
     int row0, chunks, index_bits;
 };
 struct SamplePlan {
