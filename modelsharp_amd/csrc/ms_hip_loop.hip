@@ -147,7 +147,7 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
         const dim3 grid(plan.chunks, rows), block(kSampleThreads);
         hipLaunchKernelGGL(sample_scan_kernel, grid, block, 0, s, p, ws);
         hipLaunchKernelGGL(sample_sum_kernel, grid, block, 0, s, p, ws);
-        hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), block, lds, s, p, ws);
+        hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), dim3(kDrawThreads), lds, s, p, ws);
         if (hipError_t e = hipGetLastError()) return e;
     }
     return hipSuccess;

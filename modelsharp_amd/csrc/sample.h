@@ -34,46 +34,6 @@ __device__ __forceinline__ float sample_unkey(uint32_t k)
 // A logit and its index in one number, the index in the low `bits`.
 __device__ __forceinline__ u64 sample_place(float l, int i, int bits) { return (u64)sample_key(l) << bits | (uint32_t)i; }
 
-// 2^y by 2^k 2^f, k the nearest whole number, f in [-1/2, 1/2] by a polynomial (through 2^f at the zeros of a
-// Chebyshev polynomial, 1 at 0; off by 2^-50), as a whole multiple of 2^-frac in the low bits of a double's (the sum
-// with 2^52 rounds it): kSampleBits above it. y from -64 on; below that, and for NaN, it is 0. A logit's 17 operations
-// in 64 bits are most of what bounds sampling by p, where every logit's weight counts.
-// Four at a time, so that the operations of one wait for nothing.
-constexpr u64 kSampleBits = 0x433ull << 52;
-template <int N>
-__device__ __forceinline__ void sample_raw(const double (&x)[N], int frac, u64 (&out)[N])
-{
-    constexpr double c[11] = {1.0,
-                              0.6931471805599462,
-                              0.24022650695910075,
-                              0.05550410866465167,
-                              0.009618129107618665,
-                              0.0013333558200794592,
-                              0.00015403530424776529,
-                              1.5252672924850737e-05,
-                              1.3215451633221434e-06,
-                              1.0205905413765595e-07,
-                              7.070977866508138e-09};
-    double t[N], f[N], s[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const double y = __builtin_fmax(x[i], -64.0);
-        t[i] = y + 0x1.8p52;   // y's whole part in t's low bits
-        f[i] = y - (t[i] - 0x1.8p52);
-        s[i] = c[10];
-    }
-#pragma unroll
-    for (int n = 9; n >= 0; --n)
-#pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = __builtin_fma(s[i], f[i], c[n]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const u64 b = __builtin_bit_cast(u64, s[i]);
-        const uint32_t hi = (uint32_t)(b >> 32) + (((uint32_t)__builtin_bit_cast(u64, t[i]) + frac) << 20);
-        out[i] = __builtin_bit_cast(u64, __builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)b) + 0x1p52);
-    }
-}
-
 // What a row's settings say.
 struct SampleRow {
     double scale;    // log2(e) / t
@@ -84,8 +44,8 @@ struct SampleRow {
 __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int r)
 {
     SampleRow s;
-    s.t = a.temperature ? a.temperature[r] : 1.0f;
-    s.greedy = !(s.t > 0.0f);
+    s.t = fminf(a.temperature ? a.temperature[r] : 1.0f, 1e30f);
+    s.greedy = !(s.t > 0.0f) || (a.temperature && a.temperature[r] != a.temperature[r]);
     s.scale = 1.4426950408889634074 / (double)s.t;
     const int k = a.top_k ? a.top_k[r] : 0;
     s.k = k <= 0 || k > a.vocab ? a.vocab : k;
@@ -94,17 +54,84 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int r)
     s.u = a.random[r];
     return s;
 }
-__device__ __forceinline__ void sample_weights(floatx4_t l, double top, const SampleRow& s, int frac, u64 (&raw)[4])
+// A value that is the same in every lane, in scalar registers (there is no scalar arithmetic on floats, so the
+// compiler holds a row's numbers once for each lane: spills at 64 registers, 10 of 43 us).
+template <typename T>
+__device__ __forceinline__ T uniform(T x)
 {
-    const double y[4] = {((double)l[0] - top) * s.scale, ((double)l[1] - top) * s.scale, ((double)l[2] - top) * s.scale,
-                         ((double)l[3] - top) * s.scale};
-    sample_raw<4>(y, frac, raw);
+    if constexpr (sizeof(T) == 8) {
+        const u64 b = __builtin_bit_cast(u64, x);
+        const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b), hi = __builtin_amdgcn_readfirstlane((int)(b >> 32));
+        return __builtin_bit_cast(T, (u64)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+    }
 }
-__device__ __forceinline__ u64 sample_weight(float l, double top, const SampleRow& s, int frac)
+
+// The weights of a row whose largest logit is `top`. Those below `low` are 0, and scale (l - top) above -160: where a
+// step of fp32 at `top` is worth more than 2^64, no other logit than `top` counts and the scale may be less.
+struct SampleScale {
+    double top, scale;
+    float low;
+};
+__device__ __forceinline__ SampleScale sample_scale(float top, const SampleRow& s)
 {
-    const double y[1] = {((double)l - top) * s.scale};
+    const uint32_t b = __float_as_uint(top);
+    const float below = top > 0.0f ? __uint_as_float(b - 1) : top < 0.0f ? __uint_as_float(b + 1) : -0x1p-149f;
+    SampleScale e;
+    e.top = top;
+    e.scale = __builtin_fmin(s.scale, 64.0 / (below > -__builtin_inff() ? (double)top - (double)below : 0x1p104));
+    const float low = (float)((double)top - 60.0 / e.scale);
+    const uint32_t c = __float_as_uint(low);
+    e.low = fmaxf(low > 0.0f ? __uint_as_float(c - 1) : low < 0.0f ? __uint_as_float(c + 1) : -0x1p-149f, -3.402823466e38f);
+    return {uniform(e.top), uniform(e.scale), uniform(e.low)};
+}
+// A logit as its weight needs it: NaN and what is lower than `low` as that, +infinity as the largest finite value.
+__device__ __forceinline__ float sample_clamp(float l, float low) { return __builtin_amdgcn_fmed3f(l, low, 3.402823466e38f); }
+
+// 2^y, y = scale (l - top), by 2^k 2^f, k the nearest whole number, f in [-1/2, 1/2] by a polynomial (through 2^f at
+// the zeros of a Chebyshev polynomial, 1 at 0; off by 2^-44 of it), as a whole multiple of 2^-frac in the low bits of
+// a double's (the sum with 2^52 rounds it): kSampleBits above it. A logit's 15 operations in 64 bits are most of what
+// bounds sampling by p, where every logit's weight counts. Four at a time, so that none waits for its own.
+constexpr u64 kSampleBits = 0x433ull << 52;
+template <int N>
+__device__ __forceinline__ void sample_raw(const float (&l)[N], const SampleScale& e, int frac, u64 (&out)[N])
+{
+    constexpr double c[10] = {1.0,
+                              0.6931471805599453,
+                              0.2402265069581299,
+                              0.055504108664760424,
+                              0.009618129159402558,
+                              0.0013333558179043112,
+                              0.00015403455852453838,
+                              1.525268684626772e-05,
+                              1.3255224878668817e-06,
+                              1.0203121063391729e-07};
+    const double magic = 0x1.8p52 + frac;
+    double t[N], f[N], s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const double d = (double)l[i] - e.top;
+        t[i] = __builtin_fma(d, e.scale, magic);   // k + frac in the low bits
+        f[i] = __builtin_fma(d, e.scale, -(t[i] - magic));
+        s[i] = c[9];
+    }
+#pragma unroll
+    for (int n = 8; n >= 0; --n)
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = __builtin_fma(s[i], f[i], c[n]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const u64 b = __builtin_bit_cast(u64, s[i]);
+        const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)__builtin_bit_cast(u64, t[i]) << 20);
+        out[i] = __builtin_bit_cast(u64, __builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)b) + 0x1p52);
+    }
+}
+__device__ __forceinline__ u64 sample_weight(float l, const SampleScale& e, int frac)
+{
+    const float x[1] = {sample_clamp(l, e.low)};
     u64 raw[1];
-    sample_raw<1>(y, frac, raw);
+    sample_raw<1>(x, e, frac, raw);
     return raw[0] - kSampleBits;
 }
 // The least whole number a sum has to reach to be at least x of w, and the largest it must pass to be above it.
@@ -159,7 +186,8 @@ __device__ __forceinline__ float wave_max_all(float x)
     return fmaxf(x, xor32_value(x));
 }
 // Inclusive sums of x over the workgroup's threads. The scratch is used again behind the next barrier.
-__device__ __forceinline__ u64 block_scan(u64 x, u64 (&scratch)[kSampleWaves])
+template <int WAVES>
+__device__ __forceinline__ u64 block_scan(u64 x, u64 (&scratch)[WAVES])
 {
     const int wave = threadIdx.x >> 6;
     x = wave_scan64(x);
@@ -167,7 +195,7 @@ __device__ __forceinline__ u64 block_scan(u64 x, u64 (&scratch)[kSampleWaves])
     __syncthreads();
     u64 before = 0;
 #pragma unroll
-    for (int w = 0; w < kSampleWaves - 1; ++w) {
+    for (int w = 0; w < WAVES - 1; ++w) {
         const u64 y = scratch[w];
         before += w < wave ? y : 0;
     }
@@ -240,12 +268,6 @@ __device__ __forceinline__ floatx4_t sample_edge(const float* x, int i, int V)
     for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < V ? x[i + e] : -__builtin_inff();
     return v;
 }
-__device__ __forceinline__ floatx4_t sample_logits(floatx4_t v)
-{
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = sample_logit(v[e]);
-    return v;
-}
 // A thread's four tokens of each of a chunk's tiles. What follows goes from tile to tile in loops that are not
 // unrolled (a code of 23 KB run through once took 12 us for a row, most of it for the instructions), so the
 // tiles move down a place each time.
@@ -267,7 +289,7 @@ struct SampleChunk {
         const floatx4_t x = v[0];
 #pragma unroll
         for (int j = 0; j + 1 < kSampleTiles; ++j) v[j] = v[j + 1];
-        return sample_logits(x);
+        return x;
     }
 };
 
@@ -283,10 +305,11 @@ __device__ __forceinline__ int sample_bin(float l, int top_grid, float step)
 {
     return min(top_grid - sample_grid(l, step), kSampleBins - 1);
 }
-// Where the grid's lines are no whole numbers in fp32, or t is next to infinity, the bins say nothing.
-__device__ __forceinline__ bool sample_wide(float top, float step, const SampleRow& s)
+// Where the grid's lines are no whole numbers in fp32, or t is next to infinity, the bins say nothing; where the
+// largest logit is next to the lowest value there is, `low` does not tell -infinity from it.
+__device__ __forceinline__ bool sample_wide(float top, float step, bool borders, const SampleRow& s)
 {
-    return !(fabsf(top * step) < 0x1p22f) || !(s.t < 1e30f);
+    return (borders && (!(fabsf(top * step) < 0x1p22f) || !(s.t < 1e29f))) || top < -1e37f;
 }
 constexpr float kSampleNone = -46.0f;   // weights of 2^-46 and less are 0: such logits need not be counted
 
@@ -331,7 +354,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleAr
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = at + j * kSampleTile + e;
-                mine = v[e] == top && i >= 0 ? min(mine, i) : mine;
+                mine = sample_logit(v[e]) == top && i >= 0 ? min(mine, i) : mine;
             }
         }
         if (mine != INT32_MAX) atomicMin(&first, mine);
@@ -387,7 +410,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
     if (tid == 0) place = 0;
     float top = -__builtin_inff();
     for (int i = lane; i < ws.chunks; i += kWave) top = fmaxf(top, ws.top[chunk0 + i]);
-    top = wave_max_all(top);
+    top = uniform(wave_max_all(top));
     if (s.greedy || top == -__builtin_inff()) {   // the first chunk that has it; nothing to draw from
         if (c == 0 && wave == 0) {
             int i = INT32_MAX;
@@ -403,10 +426,10 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
         }
         return;
     }
-    const float step = sample_step(s), scale = (float)s.scale;
-    const int grid = sample_grid(top, step);
+    const float step = uniform(sample_step(s)), scale = uniform((float)s.scale);
+    const int grid = uniform(sample_grid(top, step));
     bool by_k = s.k < a.vocab;
-    const bool by_p = s.p < 1.0f, borders = by_k || by_p, wide = borders && sample_wide(top, step, s);
+    const bool by_p = s.p < 1.0f, borders = by_k || by_p, wide = sample_wide(top, step, borders, s);
     int lo = kSampleBins, hi = kSampleBins, bk = kSampleBins;
     uint32_t k_before = 0;
     if (wide) {   // any bin
@@ -479,55 +502,65 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
     if (c == 0 && tid == 0) ws.found[r] = {top, lo, hi, bk, by_k, by_p, k_before, 0};
 
     // sums: each tile's kept weights before `lo`; the weights before `lo`; all weights that p is a part of
-    const u64 least = sample_least(s, a.frac);
+    const u64 least = uniform(sample_least(s, a.frac));
+    const SampleScale es = sample_scale(top, s);
     const bool every = by_p && !by_k, two = by_p && by_k && bk > hi;
     // Logits from which on a tile has something to keep or to list (on the grid), or, without borders, to keep.
     const int deep = by_k ? max(hi, bk) : hi;
-    const float slack = 0.01f + 0x1p-21f * fabsf(top * scale);   // of the divisions and sums here
-    const float none = top + (kSampleNone - slack) / scale;
-    const float from = lo == kSampleBins && least ? top + (__builtin_amdgcn_logf(fminf(s.m, 1.0f)) - slack) / scale : none;
-    const float line = deep < kSampleBins - 1 ? (float)(grid - deep) : -__builtin_inff();
-    const float line_lo = lo < kSampleBins ? (float)(grid - lo + 1) : -__builtin_inff();   // in a bin before lo
-    const float line_hi = hi < kSampleBins - 1 ? (float)(grid - hi) : -__builtin_inff();
-    const float line_k = by_k ? (float)(grid - bk + 1) : __builtin_inff();   // in a bin before bk
-    const float line_k_end = bk < kSampleBins - 1 ? (float)(grid - bk) : -__builtin_inff();
+    const double slack = 0.01 + 0x1p-21 * fabs(es.top * es.scale);   // of the sums here
+    const float none = uniform(fmaxf((float)(es.top + (kSampleNone - slack) / es.scale), es.low));
+    const float from = uniform(lo == kSampleBins && least ? (float)(es.top + (__builtin_amdgcn_logf(fminf(s.m, 1.0f)) - slack) / es.scale) : none);
+    const float line = uniform(deep < kSampleBins - 1 ? (float)(grid - deep) : -__builtin_inff());
+    const float line_lo = uniform(lo < kSampleBins ? (float)(grid - lo + 1) : -__builtin_inff());   // in a bin before lo
+    const float line_hi = uniform(hi < kSampleBins - 1 ? (float)(grid - hi) : -__builtin_inff());
+    const float line_k = uniform(by_k ? (float)(grid - bk + 1) : __builtin_inff());   // in a bin before bk
+    const float line_k_end = uniform(two ? bk < kSampleBins - 1 ? (float)(grid - bk) : -__builtin_inff() : __builtin_inff());
     u64* const out = ws.list + (chunk0 + c) * kSampleListChunk;
     u64 before_lo = 0, part = 0;
 #pragma unroll 1
     for (int j = 0; j < kSampleTiles; ++j) {
         const floatx4_t v = chunk.next();
-        const float high = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-        const bool some = __ballot(high >= from && high * step >= line) && !wide;
+        float l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l[e] = sample_clamp(v[e], es.low);
+        const float high = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+        const bool some = __ballot((high >= from) & (high * step >= line)) && !wide;
         if (!some && !every) continue;
         u64 raw[4];
-        sample_weights(v, (double)top, s, a.frac, raw);
-        if (every) part += (raw[0] + raw[1]) + (raw[2] + raw[3]) - 4 * kSampleBits;
+        sample_raw<4>(l, es, a.frac, raw);
+        const u64 all = (raw[0] + raw[1]) + (raw[2] + raw[3]) - 4 * kSampleBits;
+        if (every) part += all;
         if (!some) continue;
         u64 tile = 0;
-        uint32_t listed = 0;
+        if (lo == kSampleBins && !least) {
+            tile = all;
+        } else {
+            uint32_t listed = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float g = v[e] * step;
-            const u64 w = raw[e] - kSampleBits, before = g >= line_lo ? w : 0;
-            tile += before >= least ? before : 0;
-            before_lo += before;
-            if (!every) part += g >= line_k ? w : 0;
-            const bool in = g < line_lo && v[e] >= none && (g >= line_hi || (two && g < line_k && g >= line_k_end));
-            listed |= in ? 1u << e : 0;
+            for (int e = 0; e < 4; ++e) {
+                const float g = l[e] * step;
+                const u64 w = raw[e] - kSampleBits, before = g >= line_lo ? w : 0;
+                tile += before >= least ? before : 0;
+                before_lo += before;
+                if (!every) part += g >= line_k ? w : 0;
+                const bool in = (g < line_lo) & (l[e] >= none) & ((g >= line_hi) | ((g < line_k) & (g >= line_k_end)));
+                listed |= in ? 1u << e : 0;
+            }
+            while (const uint64_t ready = __ballot(listed != 0)) {   // (a lane's in order)
+                uint32_t to = 0;
+                if (lane == 0) to = atomicAdd(&place, __popcll(ready));
+                to = __builtin_amdgcn_readfirstlane(to) +
+                     __builtin_amdgcn_mbcnt_hi((uint32_t)(ready >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ready, 0));
+                if (listed) {
+                    const int e = __ffs(listed) - 1;
+                    const float x = e & 2 ? e & 1 ? l[3] : l[2] : e & 1 ? l[1] : l[0];
+                    if (to < kSampleListChunk) out[to] = sample_place(x, at + j * kSampleTile + e, ws.index_bits);
+                    listed &= listed - 1;
+                }
+            }
         }
         tile = wave_scan64(tile);
         if (lane == kWave - 1) atomicAdd(&sums[j], tile);
-        while (const uint64_t ready = __ballot(listed != 0)) {   // (a lane's in order)
-            uint32_t to = 0;
-            if (lane == 0) to = atomicAdd(&place, __popcll(ready));
-            to = __builtin_amdgcn_readfirstlane(to) + __builtin_amdgcn_mbcnt_hi((uint32_t)(ready >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ready, 0));
-            if (listed) {
-                const int e = __ffs(listed) - 1;
-                const float l = e & 2 ? e & 1 ? v[3] : v[2] : e & 1 ? v[1] : v[0];
-                if (to < kSampleListChunk) out[to] = sample_place(l, at + j * kSampleTile + e, ws.index_bits);
-                listed &= listed - 1;
-            }
-        }
     }
     if (by_p) {
         before_lo = wave_scan64(before_lo);
@@ -545,7 +578,9 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
 
 // 3. Each row: the borders among the listed logits (or, where those are too many for the list, among the
 // row's), and the draw. Fine bins of the listed logits, the few of a border's fine bin ranked by a wave, then the
-// tile that the draw falls into and the token; as above every wave searches for itself.
+// tile that the draw falls into and the token; as above every wave searches for itself. (Four waves, one to a SIMD: with
+// sixteen the searches, the same in each, took 6 of 13 us.)
+constexpr int kDrawThreads = 512, kDrawWaves = kDrawThreads / kWave;
 struct SampleLds {
     u64 list[kSampleList], weight[kSampleList];   // places and their weights
     uint16_t bin[kSampleList];                    // fine bins, the top bit set where it is not in [lo, hi]
@@ -553,7 +588,7 @@ struct SampleLds {
     uint32_t counts[kSampleBins];
     u64 few[2][kWave], few_weight[2][kWave];
     u64 digit[256], digit_weight[256];
-    u64 scratch[kSampleWaves];
+    u64 scratch[kDrawWaves];
     u64 found[3];
     u64 sums[2];
     uint32_t n_few[2];
@@ -594,6 +629,7 @@ __device__ __forceinline__ SampleBorder sample_rank(u64 c, u64 w, int n, u64 las
 struct SampleSearch {
     const float* x;
     SampleRow s;
+    SampleScale e;
     SampleFound f;
     float step;
     int grid, V, frac, index_bits, lead, tiles, n;
@@ -610,7 +646,7 @@ __device__ __forceinline__ u64 sample_borders(const SampleSearch& q, SampleLds& 
     const bool two = f.by_k && f.by_p && f.bk > f.hi;
     // fine bins: as many to each bin that is listed, by the logit's place in it
     const int fine = kSampleBins / min(f.hi - f.lo + 1 + two, kSampleBins);
-    auto weigh = [&](u64 c) { return sample_weight(sample_unkey((uint32_t)(c >> q.index_bits)), (double)f.top, q.s, q.frac); };
+    auto weigh = [&](u64 c) { return sample_weight(sample_unkey((uint32_t)(c >> q.index_bits)), q.e, q.frac); };
     auto fine_bin = [&](float l) {
         const float g = l * q.step, part = 1.0f - (g - floorf(g));
         const int b = sample_bin(l, q.grid, q.step);
@@ -622,13 +658,13 @@ __device__ __forceinline__ u64 sample_borders(const SampleSearch& q, SampleLds& 
     // every place in question: fn(place, weight, fine bin, whether in [lo, hi])
     auto each = [&](auto&& fn) {
 #pragma unroll 1
-        for (int i = tid; i < (LIST ? q.n : q.V); i += kSampleThreads) {
+        for (int i = tid; i < (LIST ? q.n : q.V); i += kDrawThreads) {
             if constexpr (LIST) {
                 const uint32_t b = lds.bin[i];
                 fn(lds.list[i], lds.weight[i], (int)(b & 0x7fff), b < 0x8000);
             } else {
                 const float l = sample_logit(q.x[i]);
-                if (!(((double)l - f.top) * q.s.scale >= kSampleNone)) continue;
+                if (!(((double)l - q.e.top) * q.e.scale >= kSampleNone)) continue;
                 const int b = fine_bin(l);
                 const u64 c = sample_place(l, i, q.index_bits);
                 if (b != 0x7fff) fn(c, weigh(c), b & 0x7fff, b < 0x8000);
@@ -637,7 +673,7 @@ __device__ __forceinline__ u64 sample_borders(const SampleSearch& q, SampleLds& 
     };
     if constexpr (LIST) {
 #pragma unroll 1
-        for (int i = tid; i < q.n; i += kSampleThreads) {
+        for (int i = tid; i < q.n; i += kDrawThreads) {
             const u64 c = lds.list[i], w = weigh(c);
             const int b = fine_bin(sample_unkey((uint32_t)(c >> q.index_bits)));
             lds.weight[i] = w;
@@ -763,7 +799,7 @@ __device__ __forceinline__ u64 sample_borders(const SampleSearch& q, SampleLds& 
     return last;
 }
 
-__global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs a, SampleWs ws)
+__global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a, SampleWs ws)
 {
     extern __shared__ u64 sample_lds[];
     SampleLds& lds = *reinterpret_cast<SampleLds*>(sample_lds);
@@ -777,22 +813,25 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     const int64_t chunk0 = (int64_t)r * ws.chunks;
     const int tiles = ws.chunks * kSampleTiles;
     const u64* const lists = ws.list + chunk0 * kSampleListChunk;
-    const u64 early = wave < ws.chunks ? lists[(int64_t)wave * kSampleListChunk + lane] : 0;   // (what is no list's is not used)
+    u64 early[2];   // (what is no list's is not used)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) early[i] = lists[(int64_t)min(wave + i * kDrawWaves, ws.chunks - 1) * kSampleListChunk + lane];
     u64 sum0 = 0, sum1 = 0;
-    for (int i = tid; i < ws.chunks; i += kSampleThreads) {
+    for (int i = tid; i < ws.chunks; i += kDrawThreads) {
         sum0 += ws.sums[(chunk0 + i) * 2];
         sum1 += ws.sums[(chunk0 + i) * 2 + 1];
     }
-    for (int i = tid; i < tiles; i += kSampleThreads) lds.tiles[i] = ws.tiles[chunk0 * kSampleTiles + i];
+    for (int i = tid; i < tiles; i += kDrawThreads) lds.tiles[i] = ws.tiles[chunk0 * kSampleTiles + i];
     if (s.greedy || f.answered) return;
     const float step = sample_step(s);
     const int grid = sample_grid(f.top, step);
     const u64 least = sample_least(s, a.frac);
+    const SampleScale es = sample_scale(f.top, s);
     u64 last = ~0ull;
     if (f.lo < kSampleBins) {
-        if (tid < kSampleBins) {
-            lds.mass[tid] = 0;
-            lds.counts[tid] = 0;
+        for (int i = tid; i < kSampleBins; i += kDrawThreads) {
+            lds.mass[i] = 0;
+            lds.counts[i] = 0;
         }
         if (tid < 2) {
             lds.sums[tid] = 0;
@@ -808,11 +847,12 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
             const int all = __builtin_amdgcn_readlane((int)up, kWave - 1);
             fits = !__ballot(mine > kSampleListChunk) && n + all <= kSampleList;
             if (fits)
-                for (int i = wave; i < m; i += kSampleWaves) {
+                for (int i = wave; i < m; i += kDrawWaves) {
                     const int count = __builtin_amdgcn_readlane((int)mine, i), to = n + __builtin_amdgcn_readlane((int)up, i) - count;
 #pragma unroll 1
                     for (int e = lane; e < count; e += kWave)
-                        lds.list[to + e] = base == 0 && i < kSampleWaves && e < kWave ? early : lists[(int64_t)(base + i) * kSampleListChunk + e];
+                        if (base || i >= 2 * kDrawWaves || e >= kWave) lds.list[to + e] = lists[(int64_t)(base + i) * kSampleListChunk + e];
+                    if (base == 0 && i < 2 * kDrawWaves && lane < count) lds.list[to + lane] = i < kDrawWaves ? early[0] : early[1];
                 }
             n += all;
         }
@@ -821,7 +861,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
             atomicAdd(&lds.sums[0], sum0);
             atomicAdd(&lds.sums[1], sum1);
         }
-        const SampleSearch q{x, s, f, step, grid, V, a.frac, ws.index_bits, lead, tiles, n, least};
+        const SampleSearch q{x, s, es, f, step, grid, V, a.frac, ws.index_bits, lead, tiles, n, least};
         last = fits ? sample_borders<true>(q, lds) : sample_borders<false>(q, lds);
     }
     __syncthreads();
@@ -838,29 +878,55 @@ __global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs 
     target -= past ? lane_value64(runs - sum, tile / run) : 0;
 #pragma unroll 1
     for (; tile < tiles - 1 && lds.tiles[tile] <= target; ++tile) target -= lds.tiles[tile];
-    // its token
-    const int at = tile * kSampleTile + 4 * tid - lead;
-    u64 w[4], raw[4], mine = 0;
-    const floatx4_t v = sample_logits(at >= 0 && at + 3 < V ? *reinterpret_cast<const floatx4_t*>(x + at) : sample_edge(x, at, V));
-    sample_weights(v, (double)f.top, s, a.frac, raw);
+    // its token: sixteen to a thread
+    constexpr int kEach = kSampleTile / kDrawThreads / 4;
+    const int at = tile * kSampleTile + 4 * kEach * tid - lead;
+    floatx4_t v[kEach];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const bool kept = v[e] > -__builtin_inff() &&
-                          (sample_place(v[e], at + e, ws.index_bits) <= last || sample_bin(v[e], grid, step) < f.lo);
-        const u64 we = kept ? raw[e] - kSampleBits : 0;
-        w[e] = we >= least ? we : 0;
-        mine += w[e];
+    for (int i = 0; i < kEach; ++i)
+        v[i] = at + 4 * i >= 0 && at + 4 * i + 3 < V ? *reinterpret_cast<const floatx4_t*>(x + at + 4 * i) : sample_edge(x, at + 4 * i, V);
+    // the kept weights of four neighbours
+    auto kept = [&](floatx4_t y, int i, u64 (&w)[4]) {
+        float l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l[e] = sample_clamp(y[e], es.low);
+        sample_raw<4>(l, es, a.frac, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = y[e] > -__builtin_inff() &&
+                            (sample_place(l[e], at + 4 * i + e, ws.index_bits) <= last || sample_bin(l[e], grid, step) < f.lo);
+            const u64 we = in ? w[e] - kSampleBits : 0;
+            w[e] = we >= least ? we : 0;
+        }
+    };
+    u64 mine = 0;
+#pragma unroll 1
+    for (int i = 0; i < kEach; ++i) {
+        u64 w[4];
+        kept(v[0], i, w);
+        mine += (w[0] + w[1]) + (w[2] + w[3]);
+        const floatx4_t y = v[0];
+#pragma unroll
+        for (int k = 0; k + 1 < kEach; ++k) v[k] = v[k + 1];
+        v[kEach - 1] = y;   // all of them again in their places behind the loop
     }
     u64 up_to = block_scan(mine, lds.scratch);
     if (up_to > target && up_to - mine <= target) {
         up_to -= mine;
+#pragma unroll 1
+        for (int i = 0; i < kEach && up_to <= target; ++i) {
+            u64 w[4];
+            kept(v[0], i, w);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            up_to += w[e];
-            if (up_to > target) {
-                a.token[row] = at + e;
-                if (a.logprob) a.logprob[row] = (float)log((double)w[e] / (double)total);
-                break;
+            for (int k = 0; k + 1 < kEach; ++k) v[k] = v[k + 1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool here = up_to <= target && up_to + w[e] > target;
+                up_to += w[e];
+                if (here) {
+                    a.token[row] = at + 4 * i + e;
+                    if (a.logprob) a.logprob[row] = (float)log((double)w[e] / (double)total);
+                }
             }
         }
     }
