@@ -107,7 +107,7 @@ hipError_t launch_shared_attention(const SharedAttnArgs& args, const SharedPlan&
 namespace {
 int64_t sample_row_bytes(int64_t chunks)
 {
-    return chunks * ((kSampleBins + kSampleListChunk + kSampleTiles + 3) * 8 + 12) + sizeof(SampleFound);
+    return chunks * ((kSampleBins + kSampleListChunk + 3 * kSampleTiles + 1) * 8 + 12) + sizeof(SampleFound);
 }
 }  // namespace
 
@@ -133,7 +133,7 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     ws.list = ws.hist + c * kSampleBins;
     ws.tiles = ws.list + c * kSampleListChunk;
     ws.sums = ws.tiles + c * kSampleTiles;
-    ws.all = ws.sums + c * 2;
+    ws.all = ws.sums + c * 2 * kSampleTiles;
     ws.found = reinterpret_cast<SampleFound*>(ws.all + c);
     ws.top = reinterpret_cast<float*>(ws.found + n);
     ws.first = reinterpret_cast<int32_t*>(ws.top + c);

@@ -36,7 +36,7 @@ __device__ __forceinline__ u64 sample_place(float l, int i, int bits) { return (
 
 // What a row's settings say.
 struct SampleRow {
-    double scale;    // log2(e) / t
+    float scale;     // log2(e) / t, roughly
     float t, p, m, u;
     int k;
     bool greedy;
@@ -46,7 +46,7 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int r)
     SampleRow s;
     s.t = fminf(a.temperature ? a.temperature[r] : 1.0f, 1e30f);
     s.greedy = !(s.t > 0.0f) || (a.temperature && a.temperature[r] != a.temperature[r]);
-    s.scale = 1.4426950408889634074 / (double)s.t;
+    s.scale = 1.44269504f * __builtin_amdgcn_rcpf(s.t);
     const int k = a.top_k ? a.top_k[r] : 0;
     s.k = k <= 0 || k > a.vocab ? a.vocab : k;
     s.p = a.top_p ? a.top_p[r] : 1.0f;
@@ -68,23 +68,24 @@ __device__ __forceinline__ T uniform(T x)
     }
 }
 
-// The weights of a row whose largest logit is `top`. Those below `low` are 0, and scale (l - top) above -160: where a
-// step of fp32 at `top` is worth more than 2^64, no other logit than `top` counts and the scale may be less.
+// The weights of a row whose largest logit is `top`: scale = log2(e) / t, and 0 below `low`, where scale (l - top) is
+// -60 (above -160 at `low` itself: where a step of fp32 at `top` is worth more than 2^64, no other logit than
+// `top` counts and t may be more).
 struct SampleScale {
     double top, scale;
     float low;
 };
+__device__ __forceinline__ float sample_below(float x)
+{
+    const uint32_t b = __float_as_uint(x);
+    return x > 0.0f ? __uint_as_float(b - 1) : x < 0.0f ? __uint_as_float(b + 1) : -0x1p-149f;
+}
 __device__ __forceinline__ SampleScale sample_scale(float top, const SampleRow& s)
 {
-    const uint32_t b = __float_as_uint(top);
-    const float below = top > 0.0f ? __uint_as_float(b - 1) : top < 0.0f ? __uint_as_float(b + 1) : -0x1p-149f;
-    SampleScale e;
-    e.top = top;
-    e.scale = __builtin_fmin(s.scale, 64.0 / (below > -__builtin_inff() ? (double)top - (double)below : 0x1p104));
-    const float low = (float)((double)top - 60.0 / e.scale);
-    const uint32_t c = __float_as_uint(low);
-    e.low = fmaxf(low > 0.0f ? __uint_as_float(c - 1) : low < 0.0f ? __uint_as_float(c + 1) : -0x1p-149f, -3.402823466e38f);
-    return {uniform(e.top), uniform(e.scale), uniform(e.low)};
+    const float below = fmaxf(sample_below(top), -3.402823466e38f);
+    const double t = __builtin_fmax(s.t, below < top ? ((double)top - (double)below) * (1.4426950408889634074 / 64.0) : 0x1p98);
+    return {uniform((double)top), uniform(1.4426950408889634074 / t),
+            uniform(fmaxf(sample_below(top - 41.6f * s.t), -3.402823466e38f))};   // 60 ln 2
 }
 // A logit as its weight needs it: NaN and what is lower than `low` as that, +infinity as the largest finite value.
 __device__ __forceinline__ float sample_clamp(float l, float low) { return __builtin_amdgcn_fmed3f(l, low, 3.402823466e38f); }
@@ -151,7 +152,8 @@ __device__ __forceinline__ u64 sample_least(const SampleRow& s, int frac)
 }
 
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / kWave;
-constexpr int kSampleTile = 4 * kSampleThreads, kSampleTiles = 4;   // tokens of a tile; tiles of a chunk
+constexpr int kSampleLoads = 4;                                      // of a thread, 16 bytes each: a chunk's
+constexpr int kSampleTile = 4 * kWave * kSampleLoads, kSampleTiles = kSampleWaves;   // tokens of a wave; waves of a chunk
 constexpr int kSampleEach = kSampleBins / kWave;                     // bins of a lane
 
 // A 64-bit value moved by one DPP control; lanes whose source is outside the row, or whose row the mask leaves
@@ -268,27 +270,31 @@ __device__ __forceinline__ floatx4_t sample_edge(const float* x, int i, int V)
     for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < V ? x[i + e] : -__builtin_inff();
     return v;
 }
-// A thread's four tokens of each of a chunk's tiles. What follows goes from tile to tile in loops that are not
-// unrolled (a code of 23 KB run through once took 12 us for a row, most of it for the instructions), so the
-// tiles move down a place each time.
+// A thread's tokens of a chunk. What follows goes from load to load in loops that are not unrolled (a code of 23 KB
+// run through once took 12 us for a row, most of it for the instructions), so they move down a place each time.
 struct SampleChunk {
-    floatx4_t v[kSampleTiles];
+    floatx4_t v[kSampleLoads];
+    // the thread's first token of chunk c; its loads are 256 tokens apart
+    __device__ __forceinline__ static int first(const float* x, int c)
+    {
+        return c * kSampleChunk + (int)(threadIdx.x >> 6) * kSampleTile + 4 * (int)(threadIdx.x & (kWave - 1)) - sample_lead(x);
+    }
     __device__ __forceinline__ void load(const float* x, int at, int V)
     {
-        const int first = __builtin_amdgcn_readfirstlane(at - 4 * (int)threadIdx.x % (4 * kWave));
-        if (first >= 0 && first + kSampleTile * (kSampleTiles - 1) + 4 * kWave <= V) {   // all of the wave's
+        const int begin = __builtin_amdgcn_readfirstlane(at);
+        if (begin >= 0 && begin + kSampleTile <= V) {   // all of the wave's
 #pragma unroll
-            for (int j = 0; j < kSampleTiles; ++j) v[j] = *reinterpret_cast<const floatx4_t*>(x + at + j * kSampleTile);
+            for (int j = 0; j < kSampleLoads; ++j) v[j] = *reinterpret_cast<const floatx4_t*>(x + at + 4 * kWave * j);
         } else {
 #pragma unroll
-            for (int j = 0; j < kSampleTiles; ++j) v[j] = sample_edge(x, at + j * kSampleTile, V);
+            for (int j = 0; j < kSampleLoads; ++j) v[j] = sample_edge(x, at + 4 * kWave * j, V);
         }
     }
     __device__ __forceinline__ floatx4_t next()
     {
         const floatx4_t x = v[0];
 #pragma unroll
-        for (int j = 0; j + 1 < kSampleTiles; ++j) v[j] = v[j + 1];
+        for (int j = 0; j + 1 < kSampleLoads; ++j) v[j] = v[j + 1];
         return x;
     }
 };
@@ -296,7 +302,7 @@ struct SampleChunk {
 // Bins of logits on a grid that does not depend on the row: of a sixteenth, or a sixteenth of t where t is
 // below 1, so that the 512 from the largest logit's down reach weights of e^-32 (t up to 1) or 32 below it; the last
 // one holds all that is lower. A bin of 150,000 normal logits of deviation 2 has at most 1900.
-__device__ __forceinline__ float sample_step(const SampleRow& s) { return 16.0f / fminf(s.t, 1.0f); }
+__device__ __forceinline__ float sample_step(const SampleRow& s) { return 16.0f * __builtin_amdgcn_rcpf(fminf(s.t, 1.0f)); }
 __device__ __forceinline__ int sample_grid(float l, float step)
 {
     return (int)floorf(fminf(fmaxf(l * step, -0x1p29f), 0x1p29f));
@@ -326,9 +332,9 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleAr
     const int r = blockIdx.y, c = blockIdx.x, tid = threadIdx.x;
     const float* const x = a.logits + (ws.row0 + r) * a.stride;
     const SampleRow s = sample_row(a, ws.row0 + r);
-    const int at = c * kSampleTile * kSampleTiles + 4 * tid - sample_lead(x);
-    SampleChunk tiles;
-    tiles.load(x, at, a.vocab);
+    const int at = SampleChunk::first(x, c);
+    SampleChunk mine;
+    mine.load(x, at, a.vocab);
     if (tid < kSampleBins) hist[tid] = 0;
     if (tid == 0) {
         first = INT32_MAX;
@@ -336,9 +342,9 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleAr
     }
     float top = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < kSampleTiles; ++j)
+    for (int j = 0; j < kSampleLoads; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, tiles.v[j][e]);   // (NaN does not count)
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, mine.v[j][e]);   // (NaN does not count)
     top = wave_max_all(fminf(top, 3.402823466e38f));
     if ((tid & (kWave - 1)) == 0) tops[tid >> 6] = top;
     __syncthreads();
@@ -347,29 +353,29 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleAr
     const int64_t chunk = (int64_t)r * ws.chunks + c;
     if (tid == 0) ws.top[chunk] = top;
     if (s.greedy) {
-        int mine = INT32_MAX;
+        int here = INT32_MAX;
 #pragma unroll 1
-        for (int j = 0; j < kSampleTiles; ++j) {
-            const floatx4_t v = tiles.next();
+        for (int j = 0; j < kSampleLoads; ++j) {
+            const floatx4_t v = mine.next();
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = at + j * kSampleTile + e;
-                mine = sample_logit(v[e]) == top && i >= 0 ? min(mine, i) : mine;
+                const int i = at + 4 * kWave * j + e;
+                here = sample_logit(v[e]) == top && i >= 0 ? min(here, i) : here;
             }
         }
-        if (mine != INT32_MAX) atomicMin(&first, mine);
+        if (here != INT32_MAX) atomicMin(&first, here);
         __syncthreads();
         if (tid == 0) ws.first[chunk] = first;
         return;
     }
     if (s.k == a.vocab && !(s.p < 1.0f)) return;
     u64 sum = 0;
-    const float step = sample_step(s), grid = floorf(top * step), shift = 31.0f - top * (float)s.scale;
+    const float step = sample_step(s), grid = floorf(top * step), shift = 31.0f - top * s.scale;
     if (fabsf(shift) < __builtin_inff()) {   // (else nothing here counts beside another chunk, or the row is wide)
-        const float scale = (float)s.scale;
+        const float scale = s.scale;
 #pragma unroll 1
-        for (int j = 0; j < kSampleTiles; ++j) {
-            const floatx4_t v = tiles.next();
+        for (int j = 0; j < kSampleLoads; ++j) {
+            const floatx4_t v = mine.next();
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float l = v[e], y = __builtin_fmaf(l, scale, shift), g = floorf(l * step);
@@ -397,16 +403,21 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
 {
     __shared__ float mass[2][kSampleBins];
     __shared__ uint32_t counts[2][kSampleBins], place;
-    __shared__ u64 sums[kSampleTiles + 2];
     const int r = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t chunk0 = (int64_t)r * ws.chunks;
     const float* const x = a.logits + (ws.row0 + r) * a.stride;
     const SampleRow s = sample_row(a, ws.row0 + r);
-    const int at = c * kSampleTile * kSampleTiles + 4 * tid - sample_lead(x);
+    const int at = SampleChunk::first(x, c);
     SampleChunk chunk;
     chunk.load(x, at, a.vocab);
-    if (tid < kSampleTiles + 2) sums[tid] = 0;
+    // the bins of the first sixteen chunks, two threads to a place (where there are none, they are not used)
+    constexpr int kEarly = 8;
+    const int q = tid & (kSampleBins - 1), half = tid / kSampleBins;
+    const u64* const hists = ws.hist + chunk0 * kSampleBins + q;
+    u64 early[kEarly];
+#pragma unroll
+    for (int i = 0; i < kEarly; ++i) early[i] = hists[(int64_t)min(half + 2 * i, ws.chunks - 1) * kSampleBins];
     if (tid == 0) place = 0;
     float top = -__builtin_inff();
     for (int i = lane; i < ws.chunks; i += kWave) top = fmaxf(top, ws.top[chunk0 + i]);
@@ -426,7 +437,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
         }
         return;
     }
-    const float step = uniform(sample_step(s)), scale = uniform((float)s.scale);
+    const float step = uniform(sample_step(s)), scale = uniform(s.scale);
     const int grid = uniform(sample_grid(top, step));
     bool by_k = s.k < a.vocab;
     const bool by_p = s.p < 1.0f, borders = by_k || by_p, wide = sample_wide(top, step, borders, s);
@@ -438,18 +449,20 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
         bk = by_k ? 0 : kSampleBins;
     } else if (borders) {
         // place q of a chunk's bins holds grid line grid - b with b = (grid - q) mod 512, or one too far down
-        const int q = tid & (kSampleBins - 1), half = tid / kSampleBins, b0 = (grid - q) & (kSampleBins - 1);
-        const u64* const hists = ws.hist + chunk0 * kSampleBins + q;
+        const int b0 = (grid - q) & (kSampleBins - 1);
         float m = 0.0f;
         uint32_t n = 0;
-#pragma unroll 4
-        for (int i = half; i < ws.chunks; i += 2) {
-            const u64 h = hists[(int64_t)i * kSampleBins];
+        auto add = [&](int i, u64 h) {
             const float t = ws.top[chunk0 + i];
             const bool in = (float)b0 >= (float)grid - floorf(t * step);   // no higher than the chunk's largest
             n += in ? (uint32_t)(h & 0x7fff) : 0;
             m += in ? (float)(h >> 15) * __builtin_amdgcn_exp2f((t - top) * scale) : 0.0f;
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < kEarly; ++i)
+            if (half + 2 * i < ws.chunks) add(half + 2 * i, early[i]);
+#pragma unroll 1
+        for (int i = half + 2 * kEarly; i < ws.chunks; i += 2) add(i, hists[(int64_t)i * kSampleBins]);
         const bool last = b0 == kSampleBins - 1;
         mass[half][b0] = last ? 0.0f : m;
         counts[half][b0] = last ? 0 : n;
@@ -507,18 +520,18 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
     const bool every = by_p && !by_k, two = by_p && by_k && bk > hi;
     // Logits from which on a tile has something to keep or to list (on the grid), or, without borders, to keep.
     const int deep = by_k ? max(hi, bk) : hi;
-    const double slack = 0.01 + 0x1p-21 * fabs(es.top * es.scale);   // of the sums here
-    const float none = uniform(fmaxf((float)(es.top + (kSampleNone - slack) / es.scale), es.low));
-    const float from = uniform(lo == kSampleBins && least ? (float)(es.top + (__builtin_amdgcn_logf(fminf(s.m, 1.0f)) - slack) / es.scale) : none);
+    const float slack = 0.01f + 0x1p-20f * fminf(fabsf(top * scale), 0x1p30f), to_logit = 0.693147181f * s.t;   // of the sums here
+    const float none = uniform(fmaxf(top + (kSampleNone - slack) * to_logit, es.low));
+    const float from = uniform(lo == kSampleBins && least ? top + (__builtin_amdgcn_logf(fminf(s.m, 1.0f)) - slack) * to_logit : none);
     const float line = uniform(deep < kSampleBins - 1 ? (float)(grid - deep) : -__builtin_inff());
     const float line_lo = uniform(lo < kSampleBins ? (float)(grid - lo + 1) : -__builtin_inff());   // in a bin before lo
     const float line_hi = uniform(hi < kSampleBins - 1 ? (float)(grid - hi) : -__builtin_inff());
     const float line_k = uniform(by_k ? (float)(grid - bk + 1) : __builtin_inff());   // in a bin before bk
     const float line_k_end = uniform(two ? bk < kSampleBins - 1 ? (float)(grid - bk) : -__builtin_inff() : __builtin_inff());
     u64* const out = ws.list + (chunk0 + c) * kSampleListChunk;
-    u64 before_lo = 0, part = 0;
+    u64 tile = 0, before_lo = 0, part = 0;
 #pragma unroll 1
-    for (int j = 0; j < kSampleTiles; ++j) {
+    for (int j = 0; j < kSampleLoads; ++j) {
         const floatx4_t v = chunk.next();
         float l[4];
 #pragma unroll
@@ -531,9 +544,8 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
         const u64 all = (raw[0] + raw[1]) + (raw[2] + raw[3]) - 4 * kSampleBits;
         if (every) part += all;
         if (!some) continue;
-        u64 tile = 0;
         if (lo == kSampleBins && !least) {
-            tile = all;
+            tile += all;
         } else {
             uint32_t listed = 0;
 #pragma unroll
@@ -554,25 +566,24 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
                 if (listed) {
                     const int e = __ffs(listed) - 1;
                     const float x = e & 2 ? e & 1 ? l[3] : l[2] : e & 1 ? l[1] : l[0];
-                    if (to < kSampleListChunk) out[to] = sample_place(x, at + j * kSampleTile + e, ws.index_bits);
+                    if (to < kSampleListChunk) out[to] = sample_place(x, at + 4 * kWave * j + e, ws.index_bits);
                     listed &= listed - 1;
                 }
             }
         }
-        tile = wave_scan64(tile);
-        if (lane == kWave - 1) atomicAdd(&sums[j], tile);
     }
+    const int64_t mine = (chunk0 + c) * kSampleTiles + wave;
+    tile = wave_scan64(tile);
+    if (lane == kWave - 1) ws.tiles[mine] = tile;
     if (by_p) {
         before_lo = wave_scan64(before_lo);
         part = wave_scan64(part);
         if (lane == kWave - 1) {
-            atomicAdd(&sums[kSampleTiles], before_lo);
-            atomicAdd(&sums[kSampleTiles + 1], part);
+            ws.sums[2 * mine] = before_lo;
+            ws.sums[2 * mine + 1] = part;
         }
     }
-    __syncthreads();
-    if (tid < kSampleTiles) ws.tiles[(chunk0 + c) * kSampleTiles + tid] = sums[tid];
-    else if (tid < kSampleTiles + 2) ws.sums[(chunk0 + c) * 2 + tid - kSampleTiles] = sums[tid];
+    if (borders) __syncthreads();   // what the waves have listed
     if (tid == 0) ws.listed[chunk0 + c] = wide ? kSampleList + 1 : place;   // (wide: the row itself)
 }
 
@@ -816,12 +827,13 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     u64 early[2];   // (what is no list's is not used)
 #pragma unroll
     for (int i = 0; i < 2; ++i) early[i] = lists[(int64_t)min(wave + i * kDrawWaves, ws.chunks - 1) * kSampleListChunk + lane];
+    const uint32_t early_listed = ws.listed[chunk0 + min(lane, ws.chunks - 1)];
     u64 sum0 = 0, sum1 = 0;
-    for (int i = tid; i < ws.chunks; i += kDrawThreads) {
-        sum0 += ws.sums[(chunk0 + i) * 2];
-        sum1 += ws.sums[(chunk0 + i) * 2 + 1];
+    for (int i = tid; i < tiles; i += kDrawThreads) {
+        lds.tiles[i] = ws.tiles[chunk0 * kSampleTiles + i];
+        sum0 += ws.sums[(chunk0 * kSampleTiles + i) * 2];
+        sum1 += ws.sums[(chunk0 * kSampleTiles + i) * 2 + 1];
     }
-    for (int i = tid; i < tiles; i += kDrawThreads) lds.tiles[i] = ws.tiles[chunk0 * kSampleTiles + i];
     if (s.greedy || f.answered) return;
     const float step = sample_step(s);
     const int grid = sample_grid(f.top, step);
@@ -842,7 +854,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
         bool fits = true;
         for (int base = 0; base < ws.chunks && fits; base += kWave) {
             const int m = min(ws.chunks - base, kWave);
-            const uint32_t mine = lane < m ? ws.listed[chunk0 + base + lane] : 0;
+            const uint32_t mine = lane < m ? base ? ws.listed[chunk0 + base + lane] : early_listed : 0;
             const uint32_t up = wave_sums(min(mine, (uint32_t)kSampleListChunk));
             const int all = __builtin_amdgcn_readlane((int)up, kWave - 1);
             fits = !__ballot(mine > kSampleListChunk) && n + all <= kSampleList;
@@ -878,55 +890,35 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     target -= past ? lane_value64(runs - sum, tile / run) : 0;
 #pragma unroll 1
     for (; tile < tiles - 1 && lds.tiles[tile] <= target; ++tile) target -= lds.tiles[tile];
-    // its token: sixteen to a thread
-    constexpr int kEach = kSampleTile / kDrawThreads / 4;
-    const int at = tile * kSampleTile + 4 * kEach * tid - lead;
-    floatx4_t v[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-        v[i] = at + 4 * i >= 0 && at + 4 * i + 3 < V ? *reinterpret_cast<const floatx4_t*>(x + at + 4 * i) : sample_edge(x, at + 4 * i, V);
-    // the kept weights of four neighbours
-    auto kept = [&](floatx4_t y, int i, u64 (&w)[4]) {
+    // its token: four to a thread
+    static_assert(kSampleTile <= 4 * kDrawThreads, "a tile to a workgroup");
+    const int at = tile * kSampleTile + 4 * tid - lead;
+    u64 w[4] = {}, mine = 0;
+    if (4 * tid < kSampleTile) {
+        const floatx4_t v = at >= 0 && at + 3 < V ? *reinterpret_cast<const floatx4_t*>(x + at) : sample_edge(x, at, V);
         float l[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) l[e] = sample_clamp(y[e], es.low);
+        for (int e = 0; e < 4; ++e) l[e] = sample_clamp(v[e], es.low);
         sample_raw<4>(l, es, a.frac, w);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const bool in = y[e] > -__builtin_inff() &&
-                            (sample_place(l[e], at + 4 * i + e, ws.index_bits) <= last || sample_bin(l[e], grid, step) < f.lo);
+            const bool in = v[e] > -__builtin_inff() &&
+                            (sample_place(l[e], at + e, ws.index_bits) <= last || sample_bin(l[e], grid, step) < f.lo);
             const u64 we = in ? w[e] - kSampleBits : 0;
             w[e] = we >= least ? we : 0;
+            mine += w[e];
         }
-    };
-    u64 mine = 0;
-#pragma unroll 1
-    for (int i = 0; i < kEach; ++i) {
-        u64 w[4];
-        kept(v[0], i, w);
-        mine += (w[0] + w[1]) + (w[2] + w[3]);
-        const floatx4_t y = v[0];
-#pragma unroll
-        for (int k = 0; k + 1 < kEach; ++k) v[k] = v[k + 1];
-        v[kEach - 1] = y;   // all of them again in their places behind the loop
     }
     u64 up_to = block_scan(mine, lds.scratch);
     if (up_to > target && up_to - mine <= target) {
         up_to -= mine;
-#pragma unroll 1
-        for (int i = 0; i < kEach && up_to <= target; ++i) {
-            u64 w[4];
-            kept(v[0], i, w);
 #pragma unroll
-            for (int k = 0; k + 1 < kEach; ++k) v[k] = v[k + 1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool here = up_to <= target && up_to + w[e] > target;
-                up_to += w[e];
-                if (here) {
-                    a.token[row] = at + 4 * i + e;
-                    if (a.logprob) a.logprob[row] = (float)log((double)w[e] / (double)total);
-                }
+        for (int e = 0; e < 4; ++e) {
+            up_to += w[e];
+            if (up_to > target) {
+                a.token[row] = at + e;
+                if (a.logprob) a.logprob[row] = (float)log((double)w[e] / (double)total);
+                break;
             }
         }
     }

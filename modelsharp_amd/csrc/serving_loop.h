@@ -80,8 +80,8 @@ struct SampleFound {
 struct SampleWs {
     unsigned long long* hist;  // [rows][chunks][kSampleBins]
     unsigned long long* list;  // [rows][chunks][kSampleListChunk]
-    unsigned long long* tiles; // [rows][chunks][4]: kept weights
-    unsigned long long* sums;  // [rows][chunks][2]
+    unsigned long long* tiles; // [rows][chunks][16]: a wave's kept weights
+    unsigned long long* sums;  // [rows][chunks][16][2]
     unsigned long long* all;   // [rows][chunks]: the sum of a chunk's bins
     SampleFound* found;        // [rows]
     float* top;                // [rows][chunks]: largest logit
@@ -95,7 +95,7 @@ struct SamplePlan {
 };
 MS_INTERNAL SamplePlan sample_plan(int rows, int vocab, int cus);
 MS_INTERNAL hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* workspace, hipStream_t s);
-constexpr int kSampleVocab = 1 << 24, kSampleRows = 1 << 20;
+constexpr int kSampleVocab = 1 << 22, kSampleRows = 1 << 20;
 // Weights are at most 2^frac: no sum over the vocabulary passes 2^62.
 inline int sample_frac(int vocab)
 {
