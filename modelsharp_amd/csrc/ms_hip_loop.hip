@@ -107,14 +107,15 @@ hipError_t launch_shared_attention(const SharedAttnArgs& args, const SharedPlan&
 namespace {
 int64_t sample_row_bytes(int64_t chunks)
 {
-    return chunks * ((kSampleBins + kSampleListChunk + 3 * kSampleTiles + 1) * 8 + 12) + sizeof(SampleFound);
+    return chunks * ((kSampleBins + kSampleListChunk + 3 * kSampleTiles + 1) * 8 + 24) + sizeof(SampleFound);
 }
 }  // namespace
 
-SamplePlan sample_plan(int rows, int vocab, int)
+SamplePlan sample_plan(int rows, int vocab, int cus)
 {
     SamplePlan pl;
     pl.chunks = (vocab + 3 + kSampleChunk - 1) / kSampleChunk;   // (rows that begin up to 3 floats behind 16 bytes)
+    pl.parts = (int64_t)rows * pl.chunks * 4 <= 2 * cus ? 4 : 1;
     // rows at a time: what fits 64 MB, and 64 at the least
     pl.batch = (int)std::min<int64_t>(rows, std::max<int64_t>(64, (64ll << 20) / sample_row_bytes(pl.chunks)));
     pl.ws_bytes = (pl.batch * sample_row_bytes(pl.chunks) + 15) / 16 * 16;
@@ -128,6 +129,7 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     SampleWs ws{};
     const int64_t n = plan.batch, c = n * plan.chunks;
     ws.chunks = plan.chunks;
+    ws.parts = plan.parts;
     while ((1 << ws.index_bits) < p.vocab) ++ws.index_bits;
     ws.hist = static_cast<unsigned long long*>(workspace);
     ws.list = ws.hist + c * kSampleBins;
@@ -146,7 +148,10 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
         const int rows = std::min(plan.batch, p.rows - ws.row0);
         const dim3 grid(plan.chunks, rows), block(kSampleThreads);
         hipLaunchKernelGGL(sample_scan_kernel, grid, block, 0, s, p, ws);
-        hipLaunchKernelGGL(sample_sum_kernel, grid, block, 0, s, p, ws);
+        if (plan.parts == 1)
+            hipLaunchKernelGGL(sample_sum_kernel<kSampleWaves>, grid, block, 0, s, p, ws);
+        else
+            hipLaunchKernelGGL(sample_sum_kernel<kSampleWaves / 4>, dim3(4 * plan.chunks, rows), dim3(kSampleThreads / 4), 0, s, p, ws);
         hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), dim3(kDrawThreads), lds, s, p, ws);
         if (hipError_t e = hipGetLastError()) return e;
     }

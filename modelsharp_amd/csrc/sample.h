@@ -122,11 +122,8 @@ __device__ __forceinline__ void sample_raw(const float (&l)[N], const SampleScal
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] = __builtin_fma(s[i], f[i], c[n]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const u64 b = __builtin_bit_cast(u64, s[i]);
-        const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)__builtin_bit_cast(u64, t[i]) << 20);
-        out[i] = __builtin_bit_cast(u64, __builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)b) + 0x1p52);
-    }
+    for (int i = 0; i < N; ++i)
+        out[i] = __builtin_bit_cast(u64, __builtin_amdgcn_ldexp(s[i], (int)(uint32_t)__builtin_bit_cast(u64, t[i])) + 0x1p52);
 }
 __device__ __forceinline__ u64 sample_weight(float l, const SampleScale& e, int frac)
 {
@@ -274,10 +271,11 @@ __device__ __forceinline__ floatx4_t sample_edge(const float* x, int i, int V)
 // run through once took 12 us for a row, most of it for the instructions), so they move down a place each time.
 struct SampleChunk {
     floatx4_t v[kSampleLoads];
-    // the thread's first token of chunk c; its loads are 256 tokens apart
+    // the thread's first token of a workgroup of WAVES; its loads are 256 tokens apart
+    template <int WAVES>
     __device__ __forceinline__ static int first(const float* x, int c)
     {
-        return c * kSampleChunk + (int)(threadIdx.x >> 6) * kSampleTile + 4 * (int)(threadIdx.x & (kWave - 1)) - sample_lead(x);
+        return (c * WAVES + (int)(threadIdx.x >> 6)) * kSampleTile + 4 * (int)(threadIdx.x & (kWave - 1)) - sample_lead(x);
     }
     __device__ __forceinline__ void load(const float* x, int at, int V)
     {
@@ -332,7 +330,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleAr
     const int r = blockIdx.y, c = blockIdx.x, tid = threadIdx.x;
     const float* const x = a.logits + (ws.row0 + r) * a.stride;
     const SampleRow s = sample_row(a, ws.row0 + r);
-    const int at = SampleChunk::first(x, c);
+    const int at = SampleChunk::first<kSampleWaves>(x, c);
     SampleChunk mine;
     mine.load(x, at, a.vocab);
     if (tid < kSampleBins) hist[tid] = 0;
@@ -397,27 +395,34 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleAr
 // for the rough sums' error: [lo, hi] for the last token kept, and k's where p needs the sum of the first k. Their
 // logits go to the chunk's list (as places); what lies before them is kept and summed exactly, tile by tile. Every
 // workgroup adds up the chunks' bins for itself (4 KB each, from L2), two threads to a bin's place, and every wave
-// finds the borders' bins for itself: one round of loads and one barrier. (With a barrier at each step of the search
+// finds the borders' bins for itself: one round of loads and one barrier. A chunk to a workgroup, or where that leaves
+// CUs idle a quarter. (With a barrier at each step of the search
 // this launch took 54 us for 64 x 151936 of mixed settings, with additions in LDS 40.)
-__global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
 {
-    __shared__ float mass[2][kSampleBins];
-    __shared__ uint32_t counts[2][kSampleBins], place;
+    constexpr int kParts = kSampleWaves / WAVES;             // workgroups to a chunk
+    constexpr int kHalves = WAVES >= 16 ? 2 : 1, kPlaces = WAVES >= 8 ? 1 : 2;   // threads to a place, places to a thread
+    __shared__ float mass[kHalves][kSampleBins];
+    __shared__ uint32_t counts[kHalves][kSampleBins], place;
     const int r = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t chunk0 = (int64_t)r * ws.chunks;
     const float* const x = a.logits + (ws.row0 + r) * a.stride;
     const SampleRow s = sample_row(a, ws.row0 + r);
-    const int at = SampleChunk::first(x, c);
+    const int at = SampleChunk::first<WAVES>(x, c);
     SampleChunk chunk;
     chunk.load(x, at, a.vocab);
-    // the bins of the first sixteen chunks, two threads to a place (where there are none, they are not used)
+    // the bins of the first chunks (where there are none, they are not used)
     constexpr int kEarly = 8;
-    const int q = tid & (kSampleBins - 1), half = tid / kSampleBins;
+    const int q = tid & (kSampleBins - 1), half = kHalves == 2 ? tid / kSampleBins : 0;
     const u64* const hists = ws.hist + chunk0 * kSampleBins + q;
-    u64 early[kEarly];
+    u64 early[kPlaces][kEarly];
 #pragma unroll
-    for (int i = 0; i < kEarly; ++i) early[i] = hists[(int64_t)min(half + 2 * i, ws.chunks - 1) * kSampleBins];
+    for (int n = 0; n < kPlaces; ++n)
+#pragma unroll
+        for (int i = 0; i < kEarly; ++i)
+            early[n][i] = hists[(int64_t)min(half + kHalves * i, ws.chunks - 1) * kSampleBins + n * WAVES * kWave];
     if (tid == 0) place = 0;
     float top = -__builtin_inff();
     for (int i = lane; i < ws.chunks; i += kWave) top = fmaxf(top, ws.top[chunk0 + i]);
@@ -449,23 +454,26 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
         bk = by_k ? 0 : kSampleBins;
     } else if (borders) {
         // place q of a chunk's bins holds grid line grid - b with b = (grid - q) mod 512, or one too far down
-        const int b0 = (grid - q) & (kSampleBins - 1);
-        float m = 0.0f;
-        uint32_t n = 0;
-        auto add = [&](int i, u64 h) {
-            const float t = ws.top[chunk0 + i];
-            const bool in = (float)b0 >= (float)grid - floorf(t * step);   // no higher than the chunk's largest
-            n += in ? (uint32_t)(h & 0x7fff) : 0;
-            m += in ? (float)(h >> 15) * __builtin_amdgcn_exp2f((t - top) * scale) : 0.0f;
-        };
 #pragma unroll
-        for (int i = 0; i < kEarly; ++i)
-            if (half + 2 * i < ws.chunks) add(half + 2 * i, early[i]);
+        for (int k = 0; k < kPlaces; ++k) {
+            const int b0 = (grid - q - k * WAVES * kWave) & (kSampleBins - 1);
+            float m = 0.0f;
+            uint32_t n = 0;
+            auto add = [&](int i, u64 h) {
+                const float t = ws.top[chunk0 + i];
+                const bool in = (float)b0 >= (float)grid - floorf(t * step);   // no higher than the chunk's largest
+                n += in ? (uint32_t)(h & 0x7fff) : 0;
+                m += in ? (float)(h >> 15) * __builtin_amdgcn_exp2f((t - top) * scale) : 0.0f;
+            };
+#pragma unroll
+            for (int i = 0; i < kEarly; ++i)
+                if (half + kHalves * i < ws.chunks) add(half + kHalves * i, early[k][i]);
 #pragma unroll 1
-        for (int i = half + 2 * kEarly; i < ws.chunks; i += 2) add(i, hists[(int64_t)i * kSampleBins]);
-        const bool last = b0 == kSampleBins - 1;
-        mass[half][b0] = last ? 0.0f : m;
-        counts[half][b0] = last ? 0 : n;
+            for (int i = half + kHalves * kEarly; i < ws.chunks; i += kHalves) add(i, hists[(int64_t)i * kSampleBins + k * WAVES * kWave]);
+            const bool last = b0 == kSampleBins - 1;
+            mass[half][b0] = last ? 0.0f : m;
+            counts[half][b0] = last ? 0 : n;
+        }
         float all_mass = 0.0f;
         uint32_t all_count = 0;
         for (int i = lane; i < ws.chunks; i += kWave) {
@@ -483,8 +491,12 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
         SampleSums<uint32_t> ns;
 #pragma unroll
         for (int e = 0; e < kSampleEach; ++e) {
-            ms.up[e] = mass[0][kSampleEach * lane + e] + mass[1][kSampleEach * lane + e];
-            ns.up[e] = counts[0][kSampleEach * lane + e] + counts[1][kSampleEach * lane + e];
+            ms.up[e] = mass[0][kSampleEach * lane + e];
+            ns.up[e] = counts[0][kSampleEach * lane + e];
+            if (kHalves == 2) {
+                ms.up[e] += mass[kHalves - 1][kSampleEach * lane + e];
+                ns.up[e] += counts[kHalves - 1][kSampleEach * lane + e];
+            }
         }
         ms.scan();
         ns.scan();
@@ -528,7 +540,9 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
     const float line_hi = uniform(hi < kSampleBins - 1 ? (float)(grid - hi) : -__builtin_inff());
     const float line_k = uniform(by_k ? (float)(grid - bk + 1) : __builtin_inff());   // in a bin before bk
     const float line_k_end = uniform(two ? bk < kSampleBins - 1 ? (float)(grid - bk) : -__builtin_inff() : __builtin_inff());
-    u64* const out = ws.list + (chunk0 + c) * kSampleListChunk;
+    constexpr int kListed = kSampleListChunk / kParts;
+    const int64_t part0 = chunk0 * kParts + c;
+    u64* const out = ws.list + part0 * kListed;
     u64 tile = 0, before_lo = 0, part = 0;
 #pragma unroll 1
     for (int j = 0; j < kSampleLoads; ++j) {
@@ -566,13 +580,13 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
                 if (listed) {
                     const int e = __ffs(listed) - 1;
                     const float x = e & 2 ? e & 1 ? l[3] : l[2] : e & 1 ? l[1] : l[0];
-                    if (to < kSampleListChunk) out[to] = sample_place(x, at + 4 * kWave * j + e, ws.index_bits);
+                    if (to < kListed) out[to] = sample_place(x, at + 4 * kWave * j + e, ws.index_bits);
                     listed &= listed - 1;
                 }
             }
         }
     }
-    const int64_t mine = (chunk0 + c) * kSampleTiles + wave;
+    const int64_t mine = chunk0 * kSampleTiles + c * WAVES + wave;
     tile = wave_scan64(tile);
     if (lane == kWave - 1) ws.tiles[mine] = tile;
     if (by_p) {
@@ -584,7 +598,7 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_sum_kernel(SampleArg
         }
     }
     if (borders) __syncthreads();   // what the waves have listed
-    if (tid == 0) ws.listed[chunk0 + c] = wide ? kSampleList + 1 : place;   // (wide: the row itself)
+    if (tid == 0) ws.listed[part0] = wide || place > kListed ? kSampleList + 1 : place;   // (too many: the row itself)
 }
 
 // 3. Each row: the borders among the listed logits (or, where those are too many for the list, among the
@@ -823,11 +837,13 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     const SampleFound f = ws.found[r];
     const int64_t chunk0 = (int64_t)r * ws.chunks;
     const int tiles = ws.chunks * kSampleTiles;
-    const u64* const lists = ws.list + chunk0 * kSampleListChunk;
+    const int parts = ws.chunks * ws.parts, listed = kSampleListChunk / ws.parts;
+    const int64_t part0 = chunk0 * ws.parts;
+    const u64* const lists = ws.list + part0 * listed;
     u64 early[2];   // (what is no list's is not used)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) early[i] = lists[(int64_t)min(wave + i * kDrawWaves, ws.chunks - 1) * kSampleListChunk + lane];
-    const uint32_t early_listed = ws.listed[chunk0 + min(lane, ws.chunks - 1)];
+    for (int i = 0; i < 2; ++i) early[i] = lists[(int64_t)min(wave + i * kDrawWaves, parts - 1) * listed + lane];
+    const uint32_t early_listed = ws.listed[part0 + min(lane, parts - 1)];
     u64 sum0 = 0, sum1 = 0;
     for (int i = tid; i < tiles; i += kDrawThreads) {
         lds.tiles[i] = ws.tiles[chunk0 * kSampleTiles + i];
@@ -852,18 +868,18 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
         // the chunks' lists, one behind the other
         int n = 0;
         bool fits = true;
-        for (int base = 0; base < ws.chunks && fits; base += kWave) {
-            const int m = min(ws.chunks - base, kWave);
-            const uint32_t mine = lane < m ? base ? ws.listed[chunk0 + base + lane] : early_listed : 0;
-            const uint32_t up = wave_sums(min(mine, (uint32_t)kSampleListChunk));
+        for (int base = 0; base < parts && fits; base += kWave) {
+            const int m = min(parts - base, kWave);
+            const uint32_t mine = lane < m ? base ? ws.listed[part0 + base + lane] : early_listed : 0;
+            const uint32_t up = wave_sums(min(mine, (uint32_t)listed));
             const int all = __builtin_amdgcn_readlane((int)up, kWave - 1);
-            fits = !__ballot(mine > kSampleListChunk) && n + all <= kSampleList;
+            fits = !__ballot(mine > (uint32_t)listed) && n + all <= kSampleList;
             if (fits)
                 for (int i = wave; i < m; i += kDrawWaves) {
                     const int count = __builtin_amdgcn_readlane((int)mine, i), to = n + __builtin_amdgcn_readlane((int)up, i) - count;
 #pragma unroll 1
                     for (int e = lane; e < count; e += kWave)
-                        if (base || i >= 2 * kDrawWaves || e >= kWave) lds.list[to + e] = lists[(int64_t)(base + i) * kSampleListChunk + e];
+                        if (base || i >= 2 * kDrawWaves || e >= kWave) lds.list[to + e] = lists[(int64_t)(base + i) * listed + e];
                     if (base == 0 && i < 2 * kDrawWaves && lane < count) lds.list[to + lane] = i < kDrawWaves ? early[0] : early[1];
                 }
             n += all;

@@ -86,11 +86,12 @@ struct SampleWs {
     SampleFound* found;        // [rows]
     float* top;                // [rows][chunks]: largest logit
     int32_t* first;            // [rows][chunks]: its index
-    uint32_t* listed;          // [rows][chunks]
+    uint32_t* listed;          // [rows][chunks][parts]
     int row0, chunks, index_bits;
+    int parts;                 // workgroups to a chunk in the second launch: the list is theirs in equal parts
 };
 struct SamplePlan {
-    int chunks = 0, batch = 0;
+    int chunks = 0, batch = 0, parts = 1;
     int64_t ws_bytes = 0;
 };
 MS_INTERNAL SamplePlan sample_plan(int rows, int vocab, int cus);
