@@ -36,24 +36,40 @@ SharedPlan shared_attention_plan(int64_t tokens, int requests, int64_t max_new, 
                                  int H, int kvH, int D, int f16, int cus)
 {
     SharedPlan pl;
-    if (groups <= 0) return pl;
-    const int64_t grp = H / kvH, size = f16 ? 2 : 4;
+    const int64_t grp = H / kvH, size = f16 ? 2 : 4, row_bytes = kvH * D * size * 2;
+    // Shared where that leaves out 16 MB and more of keys and values (which lie in the caches all the same). us, alone
+    // and shared: four requests behind 700 (1 MB) 9.8 and 10.9, eight tokens each behind 800 (5 MB) 11.4 and 11.6, two
+    // chunks of 100 behind 8000 (16 MB) 76 and 72, four behind 3000 of 8 kv heads (37 MB) 15.1 and 12.8, 64 behind 500
+    // (65 MB) 16.2 and 14.4, 64 behind 16000 (2 GB) 152 and 59.
+    if (groups <= 0 || (requests - groups) * prefix * row_bytes < 16 << 20) return pl;
     const bool fit = f16 || D <= 128;   // an fp32 block's three parts in LDS
     pl.few_rows = f16 ? 64 : 128;
-    pl.prefix_blocks = fit && tokens * grp > (int64_t)pl.few_rows * groups;
-    const int64_t far = pl.prefix_blocks ? tokens * grp / 128 + groups : tokens * grp / 16 + groups;
+    // A prefix's rows by tiles of 128 or of 16, for all groups alike: a CU takes about 2400 rows by keys a us in the
+    // larger, 1700 in the smaller, without 5 us of the larger ones' start. us, by 128 and by 16 at their best
+    // splits: 32 single tokens of 28 / 4 heads behind 4000 26 and 21, 64 behind 16000 59 and 83, 64 of 16 / 2 heads of 256
+    // behind 4000 46 and 43, four groups of 16 of 32 / 8 heads behind 8000 65 and 65, eight chunks of 64 behind 6000
+    // 114 and 229. (fp32, page of 24: 24 and 27 for two groups of eight, 35 and 35 for 32 behind 4000.)
+    const int64_t group_rows = (tokens * grp + groups - 1) / groups, work = prefix * groups * kvH;
+    const int64_t rows128 = (group_rows + 127) / 128 * 128, rows16 = (group_rows + 15) / 16 * 16;
+    pl.prefix_blocks = fit && rows128 * work / 2400 + 5 * cus < rows16 * work / 1700;
+    const int64_t far = tokens * grp / (pl.prefix_blocks ? 128 : 16) + groups;   // tiles at the most; likely
+    const int64_t far_likely = groups * (pl.prefix_blocks ? rows128 / 128 : rows16 / 16);
     const bool few = max_new * grp <= pl.few_rows || !fit;
     const int64_t blocks = few ? 0 : tokens * grp / 128 + std::min<int64_t>(requests, tokens * grp / (pl.few_rows + 1) + 1);
-    const int64_t rows16 = tokens * grp / 16 + requests;
-    const int64_t rows = few ? rows16 : std::min<int64_t>(rows16, (int64_t)requests * (pl.few_rows / 16));
+    const int64_t tiles16 = tokens * grp / 16 + requests;
+    const int64_t rows = few ? tiles16 : std::min<int64_t>(tiles16, (int64_t)requests * (pl.few_rows / 16));
     const int64_t near = few ? std::max<int64_t>(1, std::min(rows, (max_new * grp + 15) / 16 * requests))
                              : tokens * grp / 128 + 1 + std::min<int64_t>(requests, tokens);
-    auto count = [&](int64_t tiles, int64_t keys, int64_t most) {
-        const int64_t bytes = keys * D * size;
-        return std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)cus / std::max<int64_t>(1, tiles * kvH), bytes >> 15, most}));
+    // A workgroup to a CU for tiles of 16 (32 tokens behind 4000 in 2, 4, 8 splits: 27, 21, 26 us), with 64 KB of keys
+    // or more (four requests behind 3000 in 8, 12, 16: 14.1, 12.8, 15), and for the requests' own keys; 128 rows: two, or
+    // one and a half beside single tokens (64 behind 16000 in 16, 24, 32: 68, 59, 69; chunks: in 2, 4, 8 147, 114, 128).
+    auto count = [&](int64_t tiles, int64_t wgs, int64_t keys, int64_t bytes, int64_t most) {
+        const int64_t n = std::max<int64_t>(1, tiles * kvH);
+        return std::max<int64_t>(1, std::min<int64_t>({wgs / n, keys * D * size / bytes, most}));
     };
-    pl.prefix_splits = (int)count(far, prefix, 32);
-    pl.splits = pl.prefix_splits + (int)count(near, rest, 16);
+    pl.prefix_splits = (int)(pl.prefix_blocks ? count(far_likely, few ? 3 * cus / 2 : 2 * cus, prefix, 32 << 10, 48)
+                                              : count(far_likely, cus, prefix, 64 << 10, 48));
+    pl.splits = pl.prefix_splits + (int)count(near, cus, rest, 32 << 10, 16);
     pl.prefix_min = (int)((prefix + pl.prefix_splits - 1) / pl.prefix_splits);
     pl.split_min = (int)((rest + pl.splits - pl.prefix_splits - 1) / (pl.splits - pl.prefix_splits));
     pl.prefix_grid = far * pl.prefix_splits * kvH;
