@@ -498,8 +498,9 @@ int ms_hip_paged_attention(const ms_hip_paged_desc* desc, const float* dQ, const
  * (int32 [groups]) hold the same keys and values, cached by each of them (past[r] >= dShared[i]), as a
  * rule in the same pages. They are read from the pages of the group's first request; a prefix need not
  * end with a page. The result is that of ms_hip_paged_attention, of the same accuracy; where a group's
- * requests do not agree so, its rows are unspecified. A call with local_window_size >= 0, without groups or without the workspace
- * shares nothing, and is ms_hip_paged_attention.
+ * requests do not agree so, its rows are unspecified. A call with local_window_size >= 0, without the workspace, or where
+ * sharing would by the bounds save less than 16 MB of reading, (requests - groups) * max_shared positions, shares
+ * nothing, and is ms_hip_paged_attention.
  *   max_shared, max_rest   bounds of the shared positions of a group and of any request's positions
  *                          behind its prefix, new tokens among them (0: not known). They choose the
  *                          launch, as max_new and max_total do. */

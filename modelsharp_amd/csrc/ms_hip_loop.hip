@@ -41,7 +41,7 @@ SharedPlan shared_attention_plan(int64_t tokens, int requests, int64_t max_new, 
     // and shared: four requests behind 700 (1 MB) 9.8 and 10.9, eight tokens each behind 800 (5 MB) 11.4 and 11.6, two
     // chunks of 100 behind 8000 (16 MB) 76 and 72, four behind 3000 of 8 kv heads (37 MB) 15.1 and 12.8, 64 behind 500
     // (65 MB) 16.2 and 14.4, 64 behind 16000 (2 GB) 152 and 59.
-    if (groups <= 0 || (requests - groups) * prefix * row_bytes < 16 << 20) return pl;
+    if (groups <= 0 || (double)(requests - groups) * prefix * row_bytes < 16 << 20) return pl;   // (bounds may be anything)
     const bool fit = f16 || D <= 128;   // an fp32 block's three parts in LDS
     pl.few_rows = f16 ? 64 : 128;
     // A prefix's rows by tiles of 128 or of 16, for all groups alike: a CU takes about 2400 rows by keys a us in the
@@ -49,7 +49,8 @@ SharedPlan shared_attention_plan(int64_t tokens, int requests, int64_t max_new, 
     // splits: 32 single tokens of 28 / 4 heads behind 4000 26 and 21, 64 behind 16000 59 and 83, 64 of 16 / 2 heads of 256
     // behind 4000 46 and 43, four groups of 16 of 32 / 8 heads behind 8000 65 and 65, eight chunks of 64 behind 6000
     // 114 and 229. (fp32, page of 24: 24 and 27 for two groups of eight, 35 and 35 for 32 behind 4000.)
-    const int64_t group_rows = (tokens * grp + groups - 1) / groups, work = prefix * groups * kvH;
+    const int64_t group_rows = (tokens * grp + groups - 1) / groups;
+    const double work = (double)prefix * groups * kvH;
     const int64_t rows128 = (group_rows + 127) / 128 * 128, rows16 = (group_rows + 15) / 16 * 16;
     pl.prefix_blocks = fit && rows128 * work / 2400 + 5 * cus < rows16 * work / 1700;
     const int64_t far = tokens * grp / (pl.prefix_blocks ? 128 : 16) + groups;   // tiles at the most; likely

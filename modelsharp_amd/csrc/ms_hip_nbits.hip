@@ -3507,7 +3507,8 @@ int ms_hip_paged_shared_attention_check(const ms_hip_paged_desc* d, const ms_hip
     if (s->groups > d->requests)
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] paged_shared_attention: %d groups of %d requests", s->groups, d->requests);
     const SharedPlan plan = shared_plan(*d, *s);
-    if (plan.prefix_grid + plan.blocks_grid + plan.rows_grid >= 1 << 24)   // a launch has fewer than 2^32 threads
+    if (plan.prefix_grid + plan.blocks_grid + plan.rows_grid >= 1 << 24 ||   // a launch has fewer than 2^32 threads
+        (plan.splits && (int64_t)d->tokens * d->num_heads / 4 >= 1 << 24))
         return fail(MS_HIP_ERR_UNSUPPORTED, "[ms_hip] paged_shared_attention: %d tokens of %d requests need too many workgroups",
                     d->tokens, d->requests);
     return MS_HIP_OK;

@@ -13,11 +13,18 @@ pytestmark = pytest.mark.gpu
 F16, F32, I32 = np.float16, np.float32, np.int32
 
 
-def batch(seed, groups, G, D, page, dtype, spare_rows=0, extra_columns=0):
+WORTH = 16 << 20   # bytes that a call has to leave out, by its bounds, to share anything
+
+
+def batch(seed, groups, G, D, page, dtype, spare_rows=0, extra_columns=0, roomy=True):
     """(batch, bounds, shared) of groups [(shared positions, [(new, own cached), ...]), ...]. Whole pages of a prefix
-    are the same pages; a part of one is a copy in each request's own. A group of shared 0 shares nothing."""
+    are the same pages; a part of one is a copy in each request's own. A group of shared 0 shares nothing. A roomy
+    batch's table is wide enough that a call without other bounds shares."""
     news = [n for _, members in groups for n, _ in members]
     pasts = [s + o for s, members in groups for _, o in members]
+    if roomy:
+        saved = max(1, len(news) - len(groups)) * page * 2 * G * D * np.dtype(dtype).itemsize   # by a page's positions
+        extra_columns += -(-WORTH // saved)
     b = ref.Batch(seed, news, pasts, G, D, page, dtype, spare_rows=spare_rows, extra_columns=extra_columns)
     bounds, r = [0], 0
     for shared, members in groups:
@@ -33,7 +40,9 @@ def batch(seed, groups, G, D, page, dtype, spare_rows=0, extra_columns=0):
     return b, np.array(bounds, I32), np.array([s for s, _ in groups], I32)
 
 
-def run_shared(b, bounds, shared, q, H, window=-1, scale=0.0, workspace=True, hints=True, stride=0, out=None):
+def run_shared(b, bounds, shared, q, H, window=-1, scale=0.0, workspace=True, hints=False, stride=0, out=None):
+    """paged_shared_attention's output, by the table's width or with exact bounds (hints); the call is one that
+    shares but where the test says otherwise."""
     import torch
     d = desc_of(b, H, local_window_size=window, scale=scale, q_stride=stride)
     s = native.SharedDesc(groups=len(shared))
@@ -44,6 +53,9 @@ def run_shared(b, bounds, shared, q, H, window=-1, scale=0.0, workspace=True, hi
         for g in range(len(shared)):
             mine[max(bounds[g], 0):max(bounds[g + 1], 0)] = shared[g]
         s.max_shared, s.max_rest = max(0, int(max(shared, default=0))), max(0, int((total - mine).max()))
+    if workspace and 0 < len(shared) < len(b.news):
+        prefix = s.max_shared or b.max_pages * b.page
+        assert (len(b.news) - len(shared)) * prefix * 2 * b.G * b.D * b.k.itemsize >= WORTH
     o = torch.full((b.tokens, H * b.D), float("nan"), device="cuda") if out is None else dev(out)
     n = native.paged_shared_attention_workspace_size(d, s) if workspace else 0
     ws = torch.full((n // 4 + 64,), float("nan"), device="cuda")
@@ -71,7 +83,7 @@ CASES = [
     ([(1000, [(3, 2)] * 9)], 4, 4, 256, 16),
     ([(75, [(20, 3)] * 3)], 8, 2, 80, 7),
     ([(2050, [(1, i) for i in range(20)])], 16, 1, 128, 64),
-    ([(40, [(2, 1)])] * 70, 2, 1, 64, 8),                                      # more groups than lanes
+    ([(40, [(2, 1)] * 2)] * 70, 2, 1, 64, 8),                                  # more groups than lanes
     ([(300, [(1, 3)] * 33), (299, [(1, 3)] * 2), (301, [(40, 0)])], 8, 2, 40, 24),
     ([(4100, [(1, 10)] * 5)], 32, 8, 128, 128),
 ]
@@ -85,7 +97,66 @@ def test_shared_attention(gpu, case, dtype, workspace):
     log(f"shared {case} {dtype.__name__} workspace={workspace}")
     b, bounds, shared = batch(2000 + case, groups, G, D, page, dtype, spare_rows=3 * (case % 2), extra_columns=case % 3)
     q = queries(b, H)
-    check_attention(run_shared(b, bounds, shared, q, H, workspace=workspace, hints=bool(case % 3)), b, q, H)
+    check_attention(run_shared(b, bounds, shared, q, H, workspace=workspace), b, q, H)
+
+
+# with bounds as they are: groups, H, G, D, page
+LARGE = [
+    ([(2100, [(1, 3)] * 3)], 8, 8, 128, 16),
+    ([(1100, [(1, i) for i in range(32)])], 28, 4, 128, 16),
+    ([(3001, [(40, 7)] * 8)], 14, 2, 128, 16),
+    ([(900, [(1, 5)] * 20), (1200, [(2, 0)] * 15)], 16, 2, 256, 24),
+    ([(1000, [(1, 9)] * 16), (0, [(1, 30)] * 4), (1500, [(100, 3), (1, 0)])], 8, 4, 64, 32),
+    ([(4005, [(1, 2)] * 40)], 4, 4, 40, 10),
+    ([(640, [(3, 90)] * 33)], 12, 4, 96, 16),
+    ([(3000, [(1, 400)] * 24)], 32, 1, 64, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_shared_attention_by_its_bounds(gpu, case, dtype):
+    groups, H, G, D, page = LARGE[case]
+    log(f"large {case} {dtype.__name__}")
+    b, bounds, shared = batch(2100 + case, groups, G, D, page, dtype, spare_rows=2 * (case % 2), roomy=False)
+    q = queries(b, H)
+    check_attention(run_shared(b, bounds, shared, q, H, hints=True), b, q, H)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+def test_bounds_that_are_too_small(gpu, dtype):
+    """They choose the launch alone."""
+    import torch
+    groups, H, G, D, page = LARGE[4]
+    b, bounds, shared = batch(9, groups, G, D, page, dtype)
+    q = queries(b, H)
+    bufs = [dev(x) for x in (q, b.cu, b.past, b.table, bounds, shared, b.k, b.v)]
+    for new, total, prefix, rest in ((1, 0, 0, 1), (1, 0, 1500, 1), (2, 0, 900, 2), (0, 950, 900, 1)):
+        d = desc_of(b, H, max_new=new, max_total=total)
+        s = native.SharedDesc(groups=len(shared), max_shared=prefix, max_rest=rest)
+        n = native.paged_shared_attention_workspace_size(d, s)
+        out, ws = torch.full((b.tokens, H * D), float("nan"), device="cuda"), torch.empty(n // 4 + 4, device="cuda")
+        log(f"bounds {new} {total} {prefix} {rest}")
+        native.paged_shared_attention(d, s, *map(ptr, bufs), ptr(out), ptr(ws), n, stream())
+        check_attention(out.cpu().numpy(), b, q, H)
+
+
+@pytest.mark.parametrize("new", [1, 40], ids=["tokens", "chunks"])
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+def test_a_prefix_is_read_from_its_first_request(gpu, dtype, new):
+    """The others' entries of the table for it are not looked at, which shows that it is shared."""
+    H, G, D, page = 8, 2, 64, 16
+    b, bounds, shared = batch(10, [(100, [(new, 30)] * 5), (64, [(new, 0)] * 2)], G, D, page, dtype)
+    q = queries(b, H)
+    want, mass, longest = ref.attention(b, q, H)
+    tol = ref.attention_tolerance(mass, longest, D, float(np.abs(b.v).max()))
+    bad = b.num_pages - 1 if b.num_pages - 1 not in b.table else int(np.setdiff1d(np.arange(b.num_pages), b.table)[0])
+    b.k[bad], b.v[bad] = np.nan, np.nan
+    log(f"first request {dtype.__name__} {new}")
+    b.table[1:5, :6], b.table[6, :4] = bad, -1
+    got = run_shared(b, bounds, shared, q, H)
+    assert np.abs(got - want).max() <= tol
+    assert np.isnan(run_shared(b, bounds, shared, q, H, workspace=False)).any()
 
 
 @pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
@@ -97,7 +168,7 @@ def test_requests_outside_the_groups(gpu, dtype):
     log(f"outside {dtype.__name__}")
     check_attention(run_shared(b, bounds[1:3], shared[1:2], q, 8), b, q, 8)
     check_attention(run_shared(b, bounds[:1], shared[:0], q, 8), b, q, 8)
-    assert np.array_equal(run_shared(b, bounds[:1], shared[:0], q, 8), run_attention(b, q, 8))
+    assert np.array_equal(run_shared(b, bounds[:1], shared[:0], q, 8), run_attention(b, q, 8, hints=False))
 
 
 @pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
@@ -106,7 +177,7 @@ def test_a_window_shares_nothing(gpu, dtype):
     q = queries(b, 4)
     log(f"window {dtype.__name__}")
     for window in (0, 1, 50, 1000):
-        assert np.array_equal(run_shared(b, bounds, shared, q, 4, window), run_attention(b, q, 4, window))
+        assert np.array_equal(run_shared(b, bounds, shared, q, 4, window), run_attention(b, q, 4, window, hints=False))
     check_attention(run_shared(b, bounds, shared, q, 4, 50), b, q, 4, 50)
 
 
@@ -190,18 +261,18 @@ def test_groups_that_make_no_sense(gpu):
     for bad, lengths in (([5, 2, 5, 9], [64, 64, 64]), ([-7, -3, 5, 9], [64, 64, 64]), ([0, 0, 5, 10 ** 6], [big, 64, 64]),
                          ([0, 3, 5, big], [-5, big, 64])):
         log(f"groups {bad} {lengths}")
-        got = run_shared(b, np.array(bad, I32), np.array(lengths, I32), q, H, hints=False)
+        got = run_shared(b, np.array(bad, I32), np.array(lengths, I32), q, H)
         assert np.abs(got[last] - want[last]).max() < 1e-4
     cu = b.cu.copy()
     for bad in ([0, 5, 3, 9, -4, 2, 70, 7, 8, 9], [big] * 10, [-big] * 10):
         log(f"cu {bad}")
         b.cu = np.array(bad, I32)
-        run_shared(b, bounds, shared, q, H, hints=False)
+        run_shared(b, bounds, shared, q, H)
     b.cu = cu
     b.past[:] = big
-    run_shared(b, bounds, shared, q, H, hints=False)
+    run_shared(b, bounds, shared, q, H)
     b.past[:] = -big
-    run_shared(b, bounds, shared, q, H, hints=False)
+    run_shared(b, bounds, shared, q, H)
 
 
 def test_shared_attention_replayed_from_a_graph(gpu):
@@ -209,7 +280,7 @@ def test_shared_attention_replayed_from_a_graph(gpu):
     captured graphs with workspaces of their own."""
     import torch
     H, G, D, page = 8, 2, 128, 16
-    first = batch(8, [(96, [(1, 60)] * 4), (32, [(3, 9)] * 4)], G, D, page, F16, extra_columns=6)   # (room for the others)
+    first = batch(8, [(96, [(1, 60)] * 4), (32, [(3, 9)] * 4)], G, D, page, F16, extra_columns=6)
     b, bounds, shared = first
     d = desc_of(b, H)
     s = native.SharedDesc(groups=2)
@@ -229,7 +300,7 @@ def test_shared_attention_replayed_from_a_graph(gpu):
         graphs.append((g, out, ws))
     for i, groups in enumerate([[(96, [(1, 20)] * 4), (32, [(3, 9)] * 4)], [(16, [(1, 60)] * 2), (80, [(2, 3)] * 6)],
                                 [(0, [(1, 50)] * 5), (112, [(1, 0)] * 3)]]):
-        b, bounds, shared = batch(20 + i, groups, G, D, page, F16)
+        b, bounds, shared = batch(20 + i, groups, G, D, page, F16, roomy=False)
         q = np.zeros((bufs[0].shape), F32)
         q[:b.tokens] = queries(b, H)
         table = np.full(bufs[3].shape, -1, I32)
