@@ -582,6 +582,11 @@ class SampleDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("rows", "vocab", "stride")]
 
 
+def step_check(desc: StepDesc):
+    """Raises for a descriptor that paged_plan and paged_commit do not take."""
+    check(load().ms_hip_step_check(ctypes.byref(desc)))
+
+
 def paged_plan(desc: StepDesc, dWant, dPast, dFree, dFreeCount, dTable, dCu, dUsed, dRequests, dPositions, dSlots,
                stream=None):
     """A step's cumulative lengths, new pages and rows from what each request wants."""
@@ -592,6 +597,11 @@ def paged_plan(desc: StepDesc, dWant, dPast, dFree, dFreeCount, dTable, dCu, dUs
 def paged_commit(desc: StepDesc, dCu, dUsed, dDone, dKeep, dPast, dTable, dFree, dFreeCount, stream=None):
     """The step's end: lengths advance, pages leave the free stack, those of requests that ended return."""
     check(load().ms_hip_paged_commit(ctypes.byref(desc), dCu, dUsed, dDone, dKeep, dPast, dTable, dFree, dFreeCount, stream))
+
+
+def sample_check(desc: SampleDesc):
+    """Raises for a descriptor that sample does not take."""
+    check(load().ms_hip_sample_check(ctypes.byref(desc)))
 
 
 def sample_workspace_size(desc: SampleDesc) -> int:

@@ -4,9 +4,12 @@ interface (IKernel, KernelRegistry), next to the decoder-layer operators of deco
   PagedAttention    com.microsoft's operator (the reference has no paged cache): rotation of the
                     new queries and keys, their append to the pages, and attention of each
                     request's new tokens over its own; with norms of queries and keys per head
-                    as two further inputs
+                    as two further inputs, and prefixes that groups of requests share as two more
   QkNormRotary      the norms and the rotation alone, before GroupQueryAttention with do_rotary=0
   LoraMatMulNBits   MatMulNBits with low-rank adapters of many requests beside it
+  PagedStepPlan     rows, positions, cache slots and new pages of a step, from what requests want
+  PagedStepCommit   lengths behind the step, and the pages of requests that have ended
+  SampleTokens      next tokens by temperature, top-k, top-p and min-p
 
 Activations are torch tensors on the device (host arrays are uploaded once per call); caches are
 device tensors and are written in place. Nothing here computes on the CPU: an input that the
@@ -94,7 +97,9 @@ class HipPagedAttentionKernel(_Serving):
     [num_blocks, block_size, kv_num_heads, D] (fp32 or fp16 device tensors, written in place),
     cumulative_sequence_length [requests + 1], past_seqlens [requests], block_table [requests,
     max_blocks], cos_cache, sin_cache, then q_norm and k_norm weights [D] (optional, with
-    attribute epsilon). Rows past the last request's of the output are zeros."""
+    attribute epsilon), then group_bounds [groups + 1] and shared_lengths [groups] (optional:
+    requests [group_bounds[i], group_bounds[i + 1]) begin with the same shared_lengths[i] cached
+    positions, as a rule in the same blocks). Rows past the last request's of the output are zeros."""
     op_type = "PagedAttention"
 
     def _check(self, node):
@@ -157,21 +162,53 @@ class HipPagedAttentionKernel(_Serving):
             cos, sin = self._rotary(node, ctx, 8, q.device)
             d.cos_rows, d.cos_cols = int(cos.shape[0]), int(cos.shape[1])
         gq, gk = (self._gamma(ctx, _optional(node, i), D, q.device) for i in (10, 11))
-        native.paged_attention_check(d)   # before the caches are written
+        shared = self._shared(node, ctx, d, q.device)
+        if shared is None:   # before the caches are written
+            native.paged_attention_check(d)
+        else:
+            native.paged_shared_attention_check(d, shared[0])
         turned = torch.empty((T, H * D), dtype=torch.float32, device=q.device)
         out = torch.zeros_like(turned)
         st = _stream(q)
         native.paged_append(d, pq, pk, pv, _ptr(gq), _ptr(gk), cu.data_ptr(), past.data_ptr(), table.data_ptr(), _ptr(cos),
                             _ptr(sin), turned.data_ptr(), caches[0].data_ptr(), caches[1].data_ptr(), st)
         d.q_stride = 0
-        n = native.paged_attention_workspace_size(d)
+        if shared is None:
+            n = native.paged_attention_workspace_size(d)
+        else:
+            n = native.paged_shared_attention_workspace_size(d, shared[0])
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        native.paged_attention(d, turned.data_ptr(), cu.data_ptr(), past.data_ptr(), table.data_ptr(),
-                               caches[0].data_ptr(), caches[1].data_ptr(), out.data_ptr(), _ptr(ws), n, st)
+        lists = [t.data_ptr() for t in (cu, past, table)]
+        rest = (caches[0].data_ptr(), caches[1].data_ptr(), out.data_ptr(), _ptr(ws), n, st)
+        if shared is None:
+            native.paged_attention(d, turned.data_ptr(), *lists, *rest)
+        else:
+            native.paged_shared_attention(d, shared[0], turned.data_ptr(), *lists, shared[1].data_ptr(), shared[2].data_ptr(),
+                                          *rest)
         ctx.set(node.outputs[0], out)
         for i in (1, 2):
             if _present(node, i):
                 ctx.set(node.outputs[i], caches[i - 1])
+
+    def _shared(self, node, ctx, d, device):
+        """(descriptor, bounds, lengths) of the groups at inputs 12 and 13, or None."""
+        names = [_optional(node, i) for i in (12, 13)]
+        if not any(names):
+            return None
+        if not all(names):
+            raise ModelSharpException("PagedAttention group_bounds and shared_lengths must be given together.")
+        sources = [ctx.get_tensor(name) for name in names]
+        groups = int(np.prod(sources[1].shape))
+        s = native.SharedDesc(groups=groups)
+        if d.max_total and groups and all(isinstance(t, np.ndarray) for t in sources):
+            # known to the host as the lengths are, from which max_total is
+            bounds, lengths = (t.reshape(-1).astype(np.int64) for t in sources)
+            cu, past = (ctx.get_tensor(node.inputs[i]).reshape(-1).astype(np.int64) for i in (5, 6))
+            at = np.searchsorted(bounds, np.arange(d.requests), side="right") - 1
+            mine = np.where((at >= 0) & (at < groups), lengths[np.clip(at, 0, groups - 1)], 0)
+            s.max_shared = int(np.clip(lengths.max(), 0, d.max_total))
+            s.max_rest = int(np.clip((np.diff(cu) + past - mine).max(), 0, d.max_total))
+        return s, self._lengths(ctx, names[0], groups + 1, device), self._lengths(ctx, names[1], groups, device)
 
 
 class HipQkNormRotaryKernel(_Serving):
@@ -281,9 +318,125 @@ class HipLoraMatMulNBitsKernel(_Serving):
         ctx.set(node.outputs[0], y)
 
 
+class _Step(_Serving):
+    """What the nodes around a step's attention share: lists in device memory, written in place."""
+
+    def _list(self, ctx, name, rank=1):
+        torch = _torch()
+        t = ctx.get_tensor(name)
+        if isinstance(t, np.ndarray) or t.dtype != torch.int32 or t.dim() != rank or not t.is_contiguous():
+            raise ModelSharpException(f"{self.op_type} '{name}' must be a contiguous {rank}-D int32 device tensor (it may be "
+                                      "written in place).")
+        return t
+
+    def _pool(self, ctx, names):
+        """block_table, past_seqlens, free_blocks and free_count, on one device, and their descriptor (tokens and
+        page_size are the caller's)."""
+        table, past, free, count = (self._list(ctx, name, 2 if i == 0 else 1) for i, name in enumerate(names))
+        R = int(past.numel())
+        if int(table.shape[0]) != R or count.numel() != 1 or free.numel() == 0:
+            raise ModelSharpException(f"{self.op_type} block_table must be [{R}, max_blocks], free_blocks [num_blocks] and "
+                                      "free_count [1].")
+        if any(t.device != table.device for t in (past, free, count)):
+            raise ModelSharpException(f"{self.op_type} '{names[0]}' is on {table.device}; the other lists must be as well.")
+        return table, past, free, count, native.StepDesc(requests=R, num_pages=int(free.numel()), max_pages=int(table.shape[1]))
+
+
+class HipPagedStepPlanKernel(_Step):
+    """PagedStepPlan(block_table [requests, max_blocks], past_seqlens [requests], free_blocks
+    [num_blocks], free_count [1], wanted [requests]) -> (cumulative_sequence_length [requests + 1],
+    request_ids, position_ids, slots [tokens], used_blocks [1]), with attributes tokens (the step's rows)
+    and block_size: the first four inputs are int32 device tensors, of which free_blocks[0 ..
+    free_count) are free; a request that finds no room has no rows in this step. The new
+    blocks are written to block_table; PagedStepCommit takes them off the free ones."""
+    op_type = "PagedStepPlan"
+
+    def _check(self, node):
+        if node.attr_int("tokens", -1) < 0 or node.attr_int("block_size", 0) <= 0:
+            raise ModelSharpException("PagedStepPlan requires 'tokens' of at least 0 and a positive 'block_size'.")
+
+    def _run(self, node: GraphNode, ctx: GraphContext) -> None:
+        torch = _torch()
+        table, past, free, count, d = self._pool(ctx, node.inputs[:4])
+        d.tokens, d.page_size = node.attr_int("tokens", 0), node.attr_int("block_size", 0)
+        native.step_check(d)
+        want = self._lengths(ctx, node.inputs[4], d.requests, table.device)
+        cu, *rows, used = (torch.empty(n, dtype=torch.int32, device=table.device)
+                           for n in (d.requests + 1, d.tokens, d.tokens, d.tokens, 1))
+        native.paged_plan(d, want.data_ptr(), past.data_ptr(), free.data_ptr(), count.data_ptr(), table.data_ptr(),
+                          cu.data_ptr(), used.data_ptr(), *[t.data_ptr() for t in rows], _stream(table))
+        for i, t in enumerate((cu, *rows, used)):
+            if _present(node, i):
+                ctx.set(node.outputs[i], t)
+
+
+class HipPagedStepCommitKernel(_Step):
+    """PagedStepCommit(block_table, past_seqlens, free_blocks, free_count, cumulative_sequence_length,
+    used_blocks, done [requests], keep [requests]) -> (block_table, past_seqlens, free_blocks,
+    free_count), all written in place: lengths grow by the step's rows and its blocks leave the
+    free ones; requests with a done of not 0 (optional) give theirs back from column keep (optional: 0) on."""
+    op_type = "PagedStepCommit"
+
+    def _run(self, node: GraphNode, ctx: GraphContext) -> None:
+        table, past, free, count, d = self._pool(ctx, node.inputs[:4])
+        d.page_size = node.attr_int("block_size", 0)
+        native.step_check(d)
+        cu = self._lengths(ctx, node.inputs[4], d.requests + 1, table.device)
+        used = self._lengths(ctx, node.inputs[5], 1, table.device)
+        done, keep = (self._lengths(ctx, node.inputs[i], d.requests, table.device) if _optional(node, i) else None
+                      for i in (6, 7))
+        native.paged_commit(d, cu.data_ptr(), used.data_ptr(), _ptr(done), _ptr(keep), past.data_ptr(), table.data_ptr(),
+                            free.data_ptr(), count.data_ptr(), _stream(table))
+        for i, t in enumerate((table, past, free, count)):
+            if _present(node, i):
+                ctx.set(node.outputs[i], t)
+
+
+class HipSampleTokensKernel(_Serving):
+    """SampleTokens(logits [..., vocab], random, temperature, top_k, top_p, min_p) -> (tokens int32 [...],
+    log_probs [...]): the inputs behind logits hold one value for each row, all but random (in
+    [0, 1)) optional; a temperature of 0 takes the likeliest token, a row without a logit above
+    -infinity has token -1."""
+    op_type = "SampleTokens"
+
+    def _run(self, node: GraphNode, ctx: GraphContext) -> None:
+        torch = _torch()
+        x = self._dev.input(ctx, node.inputs[0])
+        if x.dim() < 1:
+            raise ModelSharpException("SampleTokens logits must be [..., vocab].")
+        vocab = int(x.shape[-1])
+        rows = int(np.prod(x.shape[:-1]))
+        if not _optional(node, 1):
+            raise ModelSharpException("SampleTokens requires random (input 1).")
+
+        def each(i):
+            if not _optional(node, i):
+                return None
+            if i == 3:
+                return self._lengths(ctx, node.inputs[i], rows, x.device)
+            t = self._input(ctx, node.inputs[i], x.device).reshape(-1)
+            if t.numel() != rows:
+                raise ModelSharpException(f"SampleTokens '{node.inputs[i]}' has {t.numel()} elements; expected {rows}.")
+            return t
+
+        u, t, k, p, m = (each(i) for i in (1, 2, 3, 4, 5))
+        d = native.SampleDesc(rows=rows, vocab=vocab)
+        native.sample_check(d)
+        token = torch.empty(x.shape[:-1], dtype=torch.int32, device=x.device)
+        lp = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if _present(node, 1) else None
+        n = native.sample_workspace_size(d)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
+        native.sample(d, x.data_ptr(), _ptr(t), _ptr(k), _ptr(p), _ptr(m), u.data_ptr(), token.data_ptr(), _ptr(lp),
+                      ws.data_ptr(), n, _stream(x))
+        ctx.set(node.outputs[0], token)
+        if lp is not None:
+            ctx.set(node.outputs[1], lp)
+
+
 def register_serving_kernels(registry: KernelRegistry) -> KernelRegistry:
     """Registers the device kernels of a serving step (last registration wins,
     KernelRegistry.cs:20-24)."""
-    for k in (HipPagedAttentionKernel(), HipQkNormRotaryKernel(), HipLoraMatMulNBitsKernel()):
+    for k in (HipPagedAttentionKernel(), HipQkNormRotaryKernel(), HipLoraMatMulNBitsKernel(), HipPagedStepPlanKernel(),
+              HipPagedStepCommitKernel(), HipSampleTokensKernel()):
         registry.register(k)
     return registry
