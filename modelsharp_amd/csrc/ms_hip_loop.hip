@@ -128,11 +128,10 @@ int64_t sample_row_bytes(int64_t chunks)
 }
 }  // namespace
 
-SamplePlan sample_plan(int rows, int vocab, int cus)
+SamplePlan sample_plan(int rows, int vocab)
 {
     SamplePlan pl;
     pl.chunks = (vocab + 3 + kSampleChunk - 1) / kSampleChunk;   // (rows that begin up to 3 floats behind 16 bytes)
-    pl.parts = (int64_t)rows * pl.chunks * 4 <= 2 * cus ? 4 : 1;
     // rows at a time: what fits 64 MB, and 64 at the least
     pl.batch = (int)std::min<int64_t>(rows, std::max<int64_t>(64, (64ll << 20) / sample_row_bytes(pl.chunks)));
     pl.ws_bytes = (pl.batch * sample_row_bytes(pl.chunks) + 15) / 16 * 16;
@@ -146,7 +145,6 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     SampleWs ws{};
     const int64_t n = plan.batch, c = n * plan.chunks;
     ws.chunks = plan.chunks;
-    ws.parts = plan.parts;
     while ((1 << ws.index_bits) < p.vocab) ++ws.index_bits;
     ws.hist = static_cast<unsigned long long*>(workspace);
     ws.list = ws.hist + c * kSampleBins;
@@ -165,10 +163,13 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
         const int rows = std::min(plan.batch, p.rows - ws.row0);
         const dim3 grid(plan.chunks, rows), block(kSampleThreads);
         hipLaunchKernelGGL(sample_scan_kernel, grid, block, 0, s, p, ws);
-        if (plan.parts == 1)
-            hipLaunchKernelGGL(sample_sum_kernel<kSampleWaves>, grid, block, 0, s, p, ws);
-        else
-            hipLaunchKernelGGL(sample_sum_kernel<kSampleWaves / 4>, dim3(4 * plan.chunks, rows), dim3(kSampleThreads / 4), 0, s, p, ws);
+        const dim3 parts(kSampleParts * plan.chunks, rows);
+        if (p.top_k || p.top_p) {
+            hipLaunchKernelGGL(sample_find_kernel, dim3(rows), block, 0, s, p, ws);
+            hipLaunchKernelGGL(sample_sum_kernel<false>, parts, dim3(kSumWaves * kWave), 0, s, p, ws);
+        } else {
+            hipLaunchKernelGGL(sample_sum_kernel<true>, parts, dim3(kSumWaves * kWave), 0, s, p, ws);
+        }
         hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), dim3(kDrawThreads), lds, s, p, ws);
         if (hipError_t e = hipGetLastError()) return e;
     }

@@ -3749,7 +3749,7 @@ int ms_hip_sample_check(const ms_hip_sample_desc* d)
 int64_t ms_hip_sample_workspace_size(const ms_hip_sample_desc* d)
 {
     if (!d || ms_hip_sample_check(d) != MS_HIP_OK || d->rows == 0) return 0;
-    return sample_plan(d->rows, d->vocab, device_cus()).ws_bytes;
+    return sample_plan(d->rows, d->vocab).ws_bytes;
 }
 
 int ms_hip_sample(const ms_hip_sample_desc* d, const float* dLogits, const float* dTemperature, const int32_t* dTopK,
@@ -3763,7 +3763,7 @@ int ms_hip_sample(const ms_hip_sample_desc* d, const float* dLogits, const float
     for (const void* x : {(const void*)dLogits, (const void*)dTemperature, (const void*)dTopK, (const void*)dTopP,
                           (const void*)dMinP, (const void*)dRandom, (const void*)dTokens, (const void*)dLogProbs})
         if (misaligned4(x)) return fail(MS_HIP_ERR_INVALID, "[ms_hip] sample: buffers must be 4-byte aligned");
-    const SamplePlan plan = sample_plan(d->rows, d->vocab, device_cus());
+    const SamplePlan plan = sample_plan(d->rows, d->vocab);
     if (plan.ws_bytes && (!dWorkspace || misaligned16(dWorkspace) || workspace_bytes < plan.ws_bytes))
         return fail(MS_HIP_ERR_INVALID, "[ms_hip] sample needs a 16-byte aligned workspace of %lld bytes (got %lld)",
                     (long long)plan.ws_bytes, (long long)(dWorkspace ? workspace_bytes : 0));

@@ -68,13 +68,8 @@ __device__ __forceinline__ T uniform(T x)
     }
 }
 
-// The weights of a row whose largest logit is `top`: scale = log2(e) / t, and 0 below `low`, where scale (l - top) is
-// -60 (above -160 at `low` itself: where a step of fp32 at `top` is worth more than 2^64, no other logit than
-// `top` counts and t may be more).
-struct SampleScale {
-    double top, scale;
-    float low;
-};
+// scale = log2(e) / t, `low` where scale (l - top) is -60 (above -160 at `low` itself: where a step of fp32 at `top` is
+// worth more than 2^64, no other logit than `top` counts and t may be more).
 __device__ __forceinline__ float sample_below(float x)
 {
     const uint32_t b = __float_as_uint(x);
@@ -300,7 +295,11 @@ struct SampleChunk {
 // Bins of logits on a grid that does not depend on the row: of a sixteenth, or a sixteenth of t where t is
 // below 1, so that the 512 from the largest logit's down reach weights of e^-32 (t up to 1) or 32 below it; the last
 // one holds all that is lower. A bin of 150,000 normal logits of deviation 2 has at most 1900.
-__device__ __forceinline__ float sample_step(const SampleRow& s) { return 16.0f * __builtin_amdgcn_rcpf(fminf(s.t, 1.0f)); }
+// (t below 2^-100: that of 2^-100, since 1 / t may be infinite.)
+__device__ __forceinline__ float sample_step(const SampleRow& s)
+{
+    return 16.0f * __builtin_amdgcn_rcpf(fminf(fmaxf(s.t, 0x1p-100f), 1.0f));
+}
 __device__ __forceinline__ int sample_grid(float l, float step)
 {
     return (int)floorf(fminf(fmaxf(l * step, -0x1p29f), 0x1p29f));
@@ -391,55 +390,84 @@ __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleAr
     if (tid == 0) ws.all[chunk] = all;
 }
 
-// 2. Each chunk again, with the whole row's largest logit and bins. The bins that a border may lie in are known but
-// for the rough sums' error: [lo, hi] for the last token kept, and k's where p needs the sum of the first k. Their
-// logits go to the chunk's list (as places); what lies before them is kept and summed exactly, tile by tile. Every
-// workgroup adds up the chunks' bins for itself (4 KB each, from L2), two threads to a bin's place, and every wave
-// finds the borders' bins for itself: one round of loads and one barrier. A chunk to a workgroup, or where that leaves
-// CUs idle a quarter. (With a barrier at each step of the search
-// this launch took 54 us for 64 x 151936 of mixed settings, with additions in LDS 40.)
-template <int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
+// What the later launches need of a row. The weights' numbers and the logits from which on a tile has something to keep
+// or to list: from (or, without borders, to keep), none (what is lower weighs nothing), and on the grid line (of all
+// that is kept or listed), line_lo (in a bin before lo), line_hi (before or in hi), line_k (before bk), line_k_end (in bk).
+__device__ __forceinline__ SampleFound sample_limits(const SampleArgs& a, const SampleRow& s, float top, bool wide, int lo, int hi,
+                                                     int bk, bool by_k, bool by_p, uint32_t k_before)
 {
-    constexpr int kParts = kSampleWaves / WAVES;             // workgroups to a chunk
-    constexpr int kHalves = WAVES >= 16 ? 2 : 1, kPlaces = WAVES >= 8 ? 1 : 2;   // threads to a place, places to a thread
-    __shared__ float mass[kHalves][kSampleBins];
-    __shared__ uint32_t counts[kHalves][kSampleBins], place;
-    const int r = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
+    const float step = sample_step(s), inf = __builtin_inff();
+    const int grid = sample_grid(top, step), deep = by_k ? max(hi, bk) : hi;
+    const u64 least = sample_least(s, a.frac);
+    const SampleScale es = sample_scale(top, s);
+    const float slack = 0.01f + 0x1p-20f * fminf(fabsf(top * s.scale), 0x1p30f), to_logit = 0.693147181f * s.t;   // of the sums here
+    const float none = fmaxf(top + (kSampleNone - slack) * to_logit, es.low);
+    SampleFound f{};
+    f.weights = es;
+    f.least = least;
+    f.top = top;
+    f.lo = lo;
+    f.hi = hi;
+    f.bk = bk;
+    f.by_k = by_k;
+    f.by_p = by_p;
+    f.k_before = k_before;
+    f.wide = wide;
+    f.step = step;
+    f.none = none;
+    f.from = lo == kSampleBins && least ? top + (__builtin_amdgcn_logf(fminf(s.m, 1.0f)) - slack) * to_logit : none;
+    f.line = deep < kSampleBins - 1 ? (float)(grid - deep) : -inf;
+    f.line_lo = lo < kSampleBins ? (float)(grid - lo + 1) : -inf;
+    f.line_hi = hi < kSampleBins - 1 ? (float)(grid - hi) : -inf;
+    f.line_k = by_k ? (float)(grid - bk + 1) : inf;
+    f.line_k_end = by_p && by_k && bk > hi ? bk < kSampleBins - 1 ? (float)(grid - bk) : -inf : inf;
+    return f;
+}
+// By a wave: the row's answer where nothing is drawn, the likeliest token or none (top of -infinity).
+__device__ __forceinline__ void sample_answer(const SampleArgs& a, const SampleWs& ws, int r, float top)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t chunk0 = (int64_t)r * ws.chunks;
+    int i = INT32_MAX;
+    if (top > -__builtin_inff())   // the first chunk that has it
+        for (int j = lane; j < ws.chunks; j += kWave) i = ws.top[chunk0 + j] == top ? min(i, j) : i;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) i = min(i, __shfl_xor(i, o));
+    if (lane == 0) {
+        a.token[ws.row0 + r] = i < ws.chunks ? ws.first[chunk0 + i] : -1;
+        if (a.logprob) a.logprob[ws.row0 + r] = i < ws.chunks ? 0.0f : __builtin_nanf("");
+        ws.found[r].answered = 1;
+    }
+}
+__device__ __forceinline__ float sample_top(const SampleWs& ws, int64_t chunk0)
+{
+    float top = -__builtin_inff();
+    for (int i = threadIdx.x & (kWave - 1); i < ws.chunks; i += kWave) top = fmaxf(top, ws.top[chunk0 + i]);
+    return uniform(wave_max_all(top));
+}
+
+// 2. Each row, where k or p is set for any: the bins that a border may lie in are known but for the rough sums'
+// error: [lo, hi] for the last token kept, and k's where p needs the sum of the first k. The chunks' bins are added up two
+// threads to a bin's place; then one wave searches. (By every workgroup of the next launch for itself, that launch took
+// 38 us for 200 x 50001 by p, 22 of its 27 thousand cycles before the first weight.)
+__global__ __launch_bounds__(kSampleThreads, 4) void sample_find_kernel(SampleArgs a, SampleWs ws)
+{
+    __shared__ float mass[2][kSampleBins];
+    __shared__ uint32_t counts[2][kSampleBins];
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t chunk0 = (int64_t)r * ws.chunks;
-    const float* const x = a.logits + (ws.row0 + r) * a.stride;
     const SampleRow s = sample_row(a, ws.row0 + r);
-    const int at = SampleChunk::first<WAVES>(x, c);
-    SampleChunk chunk;
-    chunk.load(x, at, a.vocab);
     // the bins of the first chunks (where there are none, they are not used)
     constexpr int kEarly = 8;
-    const int q = tid & (kSampleBins - 1), half = kHalves == 2 ? tid / kSampleBins : 0;
+    const int q = tid & (kSampleBins - 1), half = tid / kSampleBins;
     const u64* const hists = ws.hist + chunk0 * kSampleBins + q;
-    u64 early[kPlaces][kEarly];
+    u64 early[kEarly];
 #pragma unroll
-    for (int n = 0; n < kPlaces; ++n)
-#pragma unroll
-        for (int i = 0; i < kEarly; ++i)
-            early[n][i] = hists[(int64_t)min(half + kHalves * i, ws.chunks - 1) * kSampleBins + n * WAVES * kWave];
-    if (tid == 0) place = 0;
-    float top = -__builtin_inff();
-    for (int i = lane; i < ws.chunks; i += kWave) top = fmaxf(top, ws.top[chunk0 + i]);
-    top = uniform(wave_max_all(top));
-    if (s.greedy || top == -__builtin_inff()) {   // the first chunk that has it; nothing to draw from
-        if (c == 0 && wave == 0) {
-            int i = INT32_MAX;
-            if (top > -__builtin_inff())
-                for (int j = lane; j < ws.chunks; j += kWave) i = ws.top[chunk0 + j] == top ? min(i, j) : i;
-#pragma unroll
-            for (int o = 32; o; o >>= 1) i = min(i, __shfl_xor(i, o));
-            if (lane == 0) {
-                a.token[ws.row0 + r] = i < ws.chunks ? ws.first[chunk0 + i] : -1;
-                if (a.logprob) a.logprob[ws.row0 + r] = i < ws.chunks ? 0.0f : __builtin_nanf("");
-                ws.found[r].answered = 1;
-            }
-        }
+    for (int i = 0; i < kEarly; ++i) early[i] = hists[(int64_t)min(half + 2 * i, ws.chunks - 1) * kSampleBins];
+    const float top = sample_top(ws, chunk0);
+    if (s.greedy || top == -__builtin_inff()) {
+        if (wave == 0) sample_answer(a, ws, r, top);
         return;
     }
     const float step = uniform(sample_step(s)), scale = uniform(s.scale);
@@ -454,26 +482,29 @@ __global__ __launch_bounds__(WAVES * kWave, 8) void sample_sum_kernel(SampleArgs
         bk = by_k ? 0 : kSampleBins;
     } else if (borders) {
         // place q of a chunk's bins holds grid line grid - b with b = (grid - q) mod 512, or one too far down
-#pragma unroll
-        for (int k = 0; k < kPlaces; ++k) {
-            const int b0 = (grid - q - k * WAVES * kWave) & (kSampleBins - 1);
-            float m = 0.0f;
-            uint32_t n = 0;
-            auto add = [&](int i, u64 h) {
-                const float t = ws.top[chunk0 + i];
-                const bool in = (float)b0 >= (float)grid - floorf(t * step);   // no higher than the chunk's largest
-                n += in ? (uint32_t)(h & 0x7fff) : 0;
-                m += in ? (float)(h >> 15) * __builtin_amdgcn_exp2f((t - top) * scale) : 0.0f;
-            };
+        const int b0 = (grid - q) & (kSampleBins - 1);
+        float m = 0.0f;
+        uint32_t n = 0;
+        auto add = [&](int i, u64 h) {
+            const float t = ws.top[chunk0 + i];
+            const bool in = (float)b0 >= (float)grid - floorf(t * step);   // no higher than the chunk's largest
+            n += in ? (uint32_t)(h & 0x7fff) : 0;
+            m += in ? (float)(h >> 15) * __builtin_amdgcn_exp2f((t - top) * scale) : 0.0f;
+        };
+        for (int i0 = 0;;) {
 #pragma unroll
             for (int i = 0; i < kEarly; ++i)
-                if (half + kHalves * i < ws.chunks) add(half + kHalves * i, early[k][i]);
-#pragma unroll 1
-            for (int i = half + kHalves * kEarly; i < ws.chunks; i += kHalves) add(i, hists[(int64_t)i * kSampleBins + k * WAVES * kWave]);
-            const bool last = b0 == kSampleBins - 1;
-            mass[half][b0] = last ? 0.0f : m;
-            counts[half][b0] = last ? 0 : n;
+                if (i0 + half + 2 * i < ws.chunks) add(i0 + half + 2 * i, early[i]);
+            i0 += 2 * kEarly;
+            if (i0 >= ws.chunks) break;
+#pragma unroll
+            for (int i = 0; i < kEarly; ++i) early[i] = hists[(int64_t)min(i0 + half + 2 * i, ws.chunks - 1) * kSampleBins];
         }
+        const bool last = b0 == kSampleBins - 1;
+        mass[half][b0] = last ? 0.0f : m;
+        counts[half][b0] = last ? 0 : n;
+        __syncthreads();
+        if (wave) return;
         float all_mass = 0.0f;
         uint32_t all_count = 0;
         for (int i = lane; i < ws.chunks; i += kWave) {
@@ -486,17 +517,12 @@ __global__ __launch_bounds__(WAVES * kWave, 8) void sample_sum_kernel(SampleArgs
         }
         all_mass = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_sums(all_mass)), kWave - 1));
         all_count = (uint32_t)__builtin_amdgcn_readlane((int)wave_sums(all_count), kWave - 1);
-        __syncthreads();
         SampleSums<float> ms;
         SampleSums<uint32_t> ns;
 #pragma unroll
         for (int e = 0; e < kSampleEach; ++e) {
-            ms.up[e] = mass[0][kSampleEach * lane + e];
-            ns.up[e] = counts[0][kSampleEach * lane + e];
-            if (kHalves == 2) {
-                ms.up[e] += mass[kHalves - 1][kSampleEach * lane + e];
-                ns.up[e] += counts[kHalves - 1][kSampleEach * lane + e];
-            }
+            ms.up[e] = mass[0][kSampleEach * lane + e] + mass[1][kSampleEach * lane + e];
+            ns.up[e] = counts[0][kSampleEach * lane + e] + counts[1][kSampleEach * lane + e];
         }
         ms.scan();
         ns.scan();
@@ -520,28 +546,58 @@ __global__ __launch_bounds__(WAVES * kWave, 8) void sample_sum_kernel(SampleArgs
         } else if (by_k) {
             lo = hi = bk;
         }
-    } else {
-        __syncthreads();   // the sums are zero
     }
-    if (wide) __syncthreads();
-    if (c == 0 && tid == 0) ws.found[r] = {top, lo, hi, bk, by_k, by_p, k_before, 0};
+    if (tid == 0) ws.found[r] = sample_limits(a, s, top, wide, lo, hi, bk, by_k, by_p, k_before);
+}
 
+// 3. Each chunk again, by four workgroups: what lies before bin lo is kept and summed exactly, tile by tile, the logits
+// of the bins in question go to the workgroup's list (as places). ALONE: no row has k or p, and each
+// workgroup finds the row's numbers for itself.
+constexpr int kSumWaves = kSampleWaves / kSampleParts;
+template <bool ALONE>
+__global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
+{
+    __shared__ uint32_t place;
+    const int r = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t chunk0 = (int64_t)r * ws.chunks;
+    const float* const x = a.logits + (ws.row0 + r) * a.stride;
+    const int at = SampleChunk::first<kSumWaves>(x, c);
+    SampleChunk chunk;
+    chunk.load(x, at, a.vocab);
+    SampleFound f;
+    if constexpr (ALONE) {
+        const SampleRow s = sample_row(a, ws.row0 + r);
+        const float top = sample_top(ws, chunk0);
+        if (s.greedy || top == -__builtin_inff()) {
+            if (c == 0 && wave == 0) sample_answer(a, ws, r, top);
+            return;
+        }
+        f = sample_limits(a, s, top, sample_wide(top, sample_step(s), false, s), kSampleBins, kSampleBins, kSampleBins, false,
+                          false, 0);
+        if (f.wide) {
+            f.lo = 0;
+            f.hi = kSampleBins - 1;
+        }
+        if (c == 0 && tid == 0) ws.found[r] = f;
+    } else {
+        f = ws.found[r];
+        if (f.answered) return;
+    }
+    const bool borders = f.lo < kSampleBins;
+    if (borders) {
+        if (tid == 0) place = 0;
+        __syncthreads();
+    }
     // sums: each tile's kept weights before `lo`; the weights before `lo`; all weights that p is a part of
-    const u64 least = uniform(sample_least(s, a.frac));
-    const SampleScale es = sample_scale(top, s);
-    const bool every = by_p && !by_k, two = by_p && by_k && bk > hi;
-    // Logits from which on a tile has something to keep or to list (on the grid), or, without borders, to keep.
-    const int deep = by_k ? max(hi, bk) : hi;
-    const float slack = 0.01f + 0x1p-20f * fminf(fabsf(top * scale), 0x1p30f), to_logit = 0.693147181f * s.t;   // of the sums here
-    const float none = uniform(fmaxf(top + (kSampleNone - slack) * to_logit, es.low));
-    const float from = uniform(lo == kSampleBins && least ? top + (__builtin_amdgcn_logf(fminf(s.m, 1.0f)) - slack) * to_logit : none);
-    const float line = uniform(deep < kSampleBins - 1 ? (float)(grid - deep) : -__builtin_inff());
-    const float line_lo = uniform(lo < kSampleBins ? (float)(grid - lo + 1) : -__builtin_inff());   // in a bin before lo
-    const float line_hi = uniform(hi < kSampleBins - 1 ? (float)(grid - hi) : -__builtin_inff());
-    const float line_k = uniform(by_k ? (float)(grid - bk + 1) : __builtin_inff());   // in a bin before bk
-    const float line_k_end = uniform(two ? bk < kSampleBins - 1 ? (float)(grid - bk) : -__builtin_inff() : __builtin_inff());
-    constexpr int kListed = kSampleListChunk / kParts;
-    const int64_t part0 = chunk0 * kParts + c;
+    const u64 least = uniform(f.least);
+    const SampleScale es = {uniform(f.weights.top), uniform(f.weights.scale), uniform(f.weights.low)};
+    const bool every = f.by_p && !f.by_k, simple = !borders && !least;
+    const float step = uniform(f.step), none = uniform(f.none), from = uniform(f.from), line = uniform(f.line);
+    const float line_lo = uniform(f.line_lo), line_hi = uniform(f.line_hi), line_k = uniform(f.line_k);
+    const float line_k_end = uniform(f.line_k_end);
+    constexpr int kListed = kSampleListChunk / kSampleParts;
+    const int64_t part0 = chunk0 * kSampleParts + c;
     u64* const out = ws.list + part0 * kListed;
     u64 tile = 0, before_lo = 0, part = 0;
 #pragma unroll 1
@@ -551,14 +607,14 @@ __global__ __launch_bounds__(WAVES * kWave, 8) void sample_sum_kernel(SampleArgs
 #pragma unroll
         for (int e = 0; e < 4; ++e) l[e] = sample_clamp(v[e], es.low);
         const float high = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
-        const bool some = __ballot((high >= from) & (high * step >= line)) && !wide;
+        const bool some = __ballot((high >= from) & (high * step >= line)) && !f.wide;
         if (!some && !every) continue;
         u64 raw[4];
         sample_raw<4>(l, es, a.frac, raw);
         const u64 all = (raw[0] + raw[1]) + (raw[2] + raw[3]) - 4 * kSampleBits;
         if (every) part += all;
         if (!some) continue;
-        if (lo == kSampleBins && !least) {
+        if (simple) {
             tile += all;
         } else {
             uint32_t listed = 0;
@@ -586,10 +642,10 @@ __global__ __launch_bounds__(WAVES * kWave, 8) void sample_sum_kernel(SampleArgs
             }
         }
     }
-    const int64_t mine = chunk0 * kSampleTiles + c * WAVES + wave;
+    const int64_t mine = chunk0 * kSampleTiles + c * kSumWaves + wave;
     tile = wave_scan64(tile);
     if (lane == kWave - 1) ws.tiles[mine] = tile;
-    if (by_p) {
+    if (f.by_p) {
         before_lo = wave_scan64(before_lo);
         part = wave_scan64(part);
         if (lane == kWave - 1) {
@@ -597,11 +653,13 @@ __global__ __launch_bounds__(WAVES * kWave, 8) void sample_sum_kernel(SampleArgs
             ws.sums[2 * mine + 1] = part;
         }
     }
-    if (borders) __syncthreads();   // what the waves have listed
-    if (tid == 0) ws.listed[part0] = wide || place > kListed ? kSampleList + 1 : place;   // (too many: the row itself)
+    if (borders) {
+        __syncthreads();   // what the waves have listed
+        if (tid == 0) ws.listed[part0] = f.wide || place > kListed ? kSampleList + 1 : place;   // (too many: the row itself)
+    }
 }
 
-// 3. Each row: the borders among the listed logits (or, where those are too many for the list, among the
+// 4. Each row: the borders among the listed logits (or, where those are too many for the list, among the
 // row's), and the draw. Fine bins of the listed logits, the few of a border's fine bin ranked by a wave, then the
 // tile that the draw falls into and the token; as above every wave searches for itself. (Four waves, one to a SIMD: with
 // sixteen the searches, the same in each, took 6 of 13 us.)
@@ -837,12 +895,14 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     const SampleFound f = ws.found[r];
     const int64_t chunk0 = (int64_t)r * ws.chunks;
     const int tiles = ws.chunks * kSampleTiles;
-    const int parts = ws.chunks * ws.parts, listed = kSampleListChunk / ws.parts;
-    const int64_t part0 = chunk0 * ws.parts;
+    constexpr int listed = kSampleListChunk / kSampleParts;
+    const int parts = ws.chunks * kSampleParts;
+    const int64_t part0 = chunk0 * kSampleParts;
     const u64* const lists = ws.list + part0 * listed;
-    u64 early[2];   // (what is no list's is not used)
+    constexpr int kEarly = 6;
+    u64 early[kEarly];   // (what is no list's is not used)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) early[i] = lists[(int64_t)min(wave + i * kDrawWaves, parts - 1) * listed + lane];
+    for (int i = 0; i < kEarly; ++i) early[i] = lists[(int64_t)min(wave + i * kDrawWaves, parts - 1) * listed + lane];
     const uint32_t early_listed = ws.listed[part0 + min(lane, parts - 1)];
     u64 sum0 = 0, sum1 = 0;
     for (int i = tid; i < tiles; i += kDrawThreads) {
@@ -850,11 +910,11 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
         sum0 += ws.sums[(chunk0 * kSampleTiles + i) * 2];
         sum1 += ws.sums[(chunk0 * kSampleTiles + i) * 2 + 1];
     }
-    if (s.greedy || f.answered) return;
-    const float step = sample_step(s);
+    if (f.answered) return;
+    const float step = f.step;
     const int grid = sample_grid(f.top, step);
-    const u64 least = sample_least(s, a.frac);
-    const SampleScale es = sample_scale(f.top, s);
+    const u64 least = f.least;
+    const SampleScale es = f.weights;
     u64 last = ~0ull;
     if (f.lo < kSampleBins) {
         for (int i = tid; i < kSampleBins; i += kDrawThreads) {
@@ -875,12 +935,16 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
             const int all = __builtin_amdgcn_readlane((int)up, kWave - 1);
             fits = !__ballot(mine > (uint32_t)listed) && n + all <= kSampleList;
             if (fits)
+#pragma unroll 1
                 for (int i = wave; i < m; i += kDrawWaves) {
                     const int count = __builtin_amdgcn_readlane((int)mine, i), to = n + __builtin_amdgcn_readlane((int)up, i) - count;
+                    const bool there = base == 0 && i < kEarly * kDrawWaves;
 #pragma unroll 1
-                    for (int e = lane; e < count; e += kWave)
-                        if (base || i >= 2 * kDrawWaves || e >= kWave) lds.list[to + e] = lists[(int64_t)(base + i) * listed + e];
-                    if (base == 0 && i < 2 * kDrawWaves && lane < count) lds.list[to + lane] = i < kDrawWaves ? early[0] : early[1];
+                    for (int e = there ? lane + kWave : lane; e < count; e += kWave)
+                        lds.list[to + e] = lists[(int64_t)(base + i) * listed + e];
+                    if (there && lane < count) lds.list[to + lane] = early[0];
+#pragma unroll
+                    for (int j = 0; j + 1 < kEarly; ++j) early[j] = early[j + 1];
                 }
             n += all;
         }

@@ -68,13 +68,23 @@ struct SampleArgs {
 constexpr int kSampleBins = 512;                 // of logits, by which a border is first looked for
 constexpr int kSampleList = 6144, kSampleListChunk = 1536;   // logits of the bins that a border lies in, at most
 constexpr int kSampleChunk = 16384;              // tokens of a workgroup of the first two launches
-// What the second launch finds out about a row.
+constexpr int kSampleParts = 4;                  // workgroups to a chunk of the launch that sums: the list is theirs in equal parts
+// The weights of a row whose largest logit is `top`: 2^(scale (l - top)), and 0 below `low`.
+struct SampleScale {
+    double top, scale;
+    float low;
+};
+// What is found out about a row from its bins.
 struct SampleFound {
+    SampleScale weights;
+    unsigned long long least;  // lower weights are cut by m
     float top;
     int lo, hi, bk;            // bins: where the last token kept may lie, and the k-th token's (kSampleBins: none)
     int by_k, by_p;
     uint32_t k_before;         // tokens before bin bk
+    int wide;                  // the bins say nothing
     int answered;              // the row's answer is there
+    float step, from, none, line, line_lo, line_hi, line_k, line_k_end;
 };
 // The workspace of `batch` rows: rows are taken so many at a time.
 struct SampleWs {
@@ -86,15 +96,14 @@ struct SampleWs {
     SampleFound* found;        // [rows]
     float* top;                // [rows][chunks]: largest logit
     int32_t* first;            // [rows][chunks]: its index
-    uint32_t* listed;          // [rows][chunks][parts]
+    uint32_t* listed;          // [rows][chunks][kSampleParts]
     int row0, chunks, index_bits;
-    int parts;                 // workgroups to a chunk in the second launch: the list is theirs in equal parts
 };
 struct SamplePlan {
-    int chunks = 0, batch = 0, parts = 1;
+    int chunks = 0, batch = 0;
     int64_t ws_bytes = 0;
 };
-MS_INTERNAL SamplePlan sample_plan(int rows, int vocab, int cus);
+MS_INTERNAL SamplePlan sample_plan(int rows, int vocab);
 MS_INTERNAL hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* workspace, hipStream_t s);
 constexpr int kSampleVocab = 1 << 22, kSampleRows = 1 << 20;
 // Weights are at most 2^frac: no sum over the vocabulary passes 2^62.

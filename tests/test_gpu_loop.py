@@ -341,6 +341,19 @@ def test_sample_odd_logits(gpu, vocab):
     check_sample(logits, k=[2] * n, u=u)
 
 
+def test_sample_tiny_temperatures(gpu):
+    """Down to the type's smallest: the likeliest tokens share the draw."""
+    rng = np.random.default_rng(14)
+    for top in (0.0, -1.5, 3.0, 1e-39):
+        x = (np.minimum(rng.standard_normal((6, 9000)) - 6, -0.5) + top).astype(F32)
+        x[:, 4000], x[:, 7000] = top, top
+        t = np.array([1e-30, 1e-37, 1e-38, 1e-40, 1e-45, 2.0 ** -100], F32)
+        log(f"tiny temperatures below {top}")
+        for u, token in ((0.3, 4000), (0.7, 7000)):
+            for s in (dict(), dict(m=[0.5] * 6), dict(p=[0.9] * 6), dict(k=[4] * 6)):
+                assert (check_sample(x, t=t, u=[u] * 6, **s) == token).all()
+
+
 def test_sample_of_a_long_row(gpu):
     rng = np.random.default_rng(9)
     vocab = 2 ** 22 - 3
