@@ -124,7 +124,7 @@ hipError_t launch_shared_attention(const SharedAttnArgs& args, const SharedPlan&
 namespace {
 int64_t sample_row_bytes(int64_t chunks)
 {
-    return chunks * ((kSampleBins + kSampleListChunk + 3 * kSampleTiles + 1) * 8 + 24) + sizeof(SampleFound);
+    return chunks * ((kSampleBins + 3 * kSampleTiles + 1) * 8 + 8) + kSampleList * 8 + 8 + sizeof(SampleFound);
 }
 }  // namespace
 
@@ -148,7 +148,7 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     while ((1 << ws.index_bits) < p.vocab) ++ws.index_bits;
     ws.hist = static_cast<unsigned long long*>(workspace);
     ws.list = ws.hist + c * kSampleBins;
-    ws.tiles = ws.list + c * kSampleListChunk;
+    ws.tiles = ws.list + n * kSampleList;
     ws.sums = ws.tiles + c * kSampleTiles;
     ws.all = ws.sums + c * 2 * kSampleTiles;
     ws.found = reinterpret_cast<SampleFound*>(ws.all + c);

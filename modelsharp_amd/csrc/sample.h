@@ -547,17 +547,22 @@ __global__ __launch_bounds__(kSampleThreads, 4) void sample_find_kernel(SampleAr
             lo = hi = bk;
         }
     }
-    if (tid == 0) ws.found[r] = sample_limits(a, s, top, wide, lo, hi, bk, by_k, by_p, k_before);
+    if (tid == 0) {
+        ws.found[r] = sample_limits(a, s, top, wide, lo, hi, bk, by_k, by_p, k_before);
+        ws.listed[r] = 0;
+    }
 }
 
 // 3. Each chunk again, by four workgroups: what lies before bin lo is kept and summed exactly, tile by tile, the logits
-// of the bins in question go to the workgroup's list (as places). ALONE: no row has k or p, and each
+// of the bins in question go to the row's list (as places, in any order: what is done with them does not depend on it),
+// by way of LDS so that a workgroup asks for its places in the list once. ALONE: no row has k or p, and each
 // workgroup finds the row's numbers for itself.
-constexpr int kSumWaves = kSampleWaves / kSampleParts;
+constexpr int kSumWaves = kSampleWaves / kSampleParts, kSumList = 1024;
 template <bool ALONE>
 __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
 {
-    __shared__ uint32_t place;
+    __shared__ u64 out[kSumList];
+    __shared__ uint32_t place, place0;
     const int r = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t chunk0 = (int64_t)r * ws.chunks;
@@ -596,9 +601,6 @@ __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(Sample
     const float step = uniform(f.step), none = uniform(f.none), from = uniform(f.from), line = uniform(f.line);
     const float line_lo = uniform(f.line_lo), line_hi = uniform(f.line_hi), line_k = uniform(f.line_k);
     const float line_k_end = uniform(f.line_k_end);
-    constexpr int kListed = kSampleListChunk / kSampleParts;
-    const int64_t part0 = chunk0 * kSampleParts + c;
-    u64* const out = ws.list + part0 * kListed;
     u64 tile = 0, before_lo = 0, part = 0;
 #pragma unroll 1
     for (int j = 0; j < kSampleLoads; ++j) {
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(Sample
                 if (listed) {
                     const int e = __ffs(listed) - 1;
                     const float x = e & 2 ? e & 1 ? l[3] : l[2] : e & 1 ? l[1] : l[0];
-                    if (to < kListed) out[to] = sample_place(x, at + 4 * kWave * j + e, ws.index_bits);
+                    if (to < kSumList) out[to] = sample_place(x, at + 4 * kWave * j + e, ws.index_bits);
                     listed &= listed - 1;
                 }
             }
@@ -655,7 +657,13 @@ __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(Sample
     }
     if (borders) {
         __syncthreads();   // what the waves have listed
-        if (tid == 0) ws.listed[part0] = f.wide || place > kListed ? kSampleList + 1 : place;   // (too many: the row itself)
+        const uint32_t n = place;
+        if (n == 0) return;
+        if (tid == 0) place0 = atomicAdd(&ws.listed[r], n <= kSumList ? n : kSampleList + 1);   // (too many: the row itself)
+        __syncthreads();
+        u64* const list = ws.list + (int64_t)r * kSampleList;
+        for (uint32_t i = tid; i < min(n, (uint32_t)kSumList); i += kSumWaves * kWave)
+            if (place0 + i < kSampleList) list[place0 + i] = out[i];
     }
 }
 
@@ -887,7 +895,6 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     extern __shared__ u64 sample_lds[];
     SampleLds& lds = *reinterpret_cast<SampleLds*>(sample_lds);
     const int r = blockIdx.x, row = ws.row0 + r, tid = threadIdx.x, lane = tid & (kWave - 1), V = a.vocab;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* const x = a.logits + row * a.stride;
     const int lead = sample_lead(x);
     // everything that lies at a known place is loaded before any of it is waited for
@@ -895,15 +902,12 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
     const SampleFound f = ws.found[r];
     const int64_t chunk0 = (int64_t)r * ws.chunks;
     const int tiles = ws.chunks * kSampleTiles;
-    constexpr int listed = kSampleListChunk / kSampleParts;
-    const int parts = ws.chunks * kSampleParts;
-    const int64_t part0 = chunk0 * kSampleParts;
-    const u64* const lists = ws.list + part0 * listed;
-    constexpr int kEarly = 6;
-    u64 early[kEarly];   // (what is no list's is not used)
+    const u64* const list = ws.list + (int64_t)r * kSampleList;
+    constexpr int kEarly = 4;
+    u64 early[kEarly];   // (what is not listed is not used)
 #pragma unroll
-    for (int i = 0; i < kEarly; ++i) early[i] = lists[(int64_t)min(wave + i * kDrawWaves, parts - 1) * listed + lane];
-    const uint32_t early_listed = ws.listed[part0 + min(lane, parts - 1)];
+    for (int i = 0; i < kEarly; ++i) early[i] = list[i * kDrawThreads + tid];
+    const uint32_t listed = ws.listed[r];
     u64 sum0 = 0, sum1 = 0;
     for (int i = tid; i < tiles; i += kDrawThreads) {
         lds.tiles[i] = ws.tiles[chunk0 * kSampleTiles + i];
@@ -925,29 +929,12 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a,
             lds.sums[tid] = 0;
             lds.n_few[tid] = 0;
         }
-        // the chunks' lists, one behind the other
-        int n = 0;
-        bool fits = true;
-        for (int base = 0; base < parts && fits; base += kWave) {
-            const int m = min(parts - base, kWave);
-            const uint32_t mine = lane < m ? base ? ws.listed[part0 + base + lane] : early_listed : 0;
-            const uint32_t up = wave_sums(min(mine, (uint32_t)listed));
-            const int all = __builtin_amdgcn_readlane((int)up, kWave - 1);
-            fits = !__ballot(mine > (uint32_t)listed) && n + all <= kSampleList;
-            if (fits)
-#pragma unroll 1
-                for (int i = wave; i < m; i += kDrawWaves) {
-                    const int count = __builtin_amdgcn_readlane((int)mine, i), to = n + __builtin_amdgcn_readlane((int)up, i) - count;
-                    const bool there = base == 0 && i < kEarly * kDrawWaves;
-#pragma unroll 1
-                    for (int e = there ? lane + kWave : lane; e < count; e += kWave)
-                        lds.list[to + e] = lists[(int64_t)(base + i) * listed + e];
-                    if (there && lane < count) lds.list[to + lane] = early[0];
+        const bool fits = !f.wide && listed <= kSampleList;
+        const int n = fits ? (int)listed : 0;
 #pragma unroll
-                    for (int j = 0; j + 1 < kEarly; ++j) early[j] = early[j + 1];
-                }
-            n += all;
-        }
+        for (int i = 0; i < kEarly; ++i)
+            if (i * kDrawThreads + tid < n) lds.list[i * kDrawThreads + tid] = early[i];
+        for (int i = kEarly * kDrawThreads + tid; i < n; i += kDrawThreads) lds.list[i] = list[i];
         __syncthreads();
         if (f.by_p && (sum0 | sum1)) {
             atomicAdd(&lds.sums[0], sum0);

@@ -66,9 +66,9 @@ struct SampleArgs {
     int64_t stride;
 };
 constexpr int kSampleBins = 512;                 // of logits, by which a border is first looked for
-constexpr int kSampleList = 6144, kSampleListChunk = 1536;   // logits of the bins that a border lies in, at most
+constexpr int kSampleList = 6144;                // logits of the bins that a border lies in, at most
 constexpr int kSampleChunk = 16384;              // tokens of a workgroup of the first two launches
-constexpr int kSampleParts = 4;                  // workgroups to a chunk of the launch that sums: the list is theirs in equal parts
+constexpr int kSampleParts = 4;                  // workgroups to a chunk of the launch that sums
 // The weights of a row whose largest logit is `top`: 2^(scale (l - top)), and 0 below `low`.
 struct SampleScale {
     double top, scale;
@@ -89,14 +89,14 @@ struct SampleFound {
 // The workspace of `batch` rows: rows are taken so many at a time.
 struct SampleWs {
     unsigned long long* hist;  // [rows][chunks][kSampleBins]
-    unsigned long long* list;  // [rows][chunks][kSampleListChunk]
+    unsigned long long* list;  // [rows][kSampleList]
     unsigned long long* tiles; // [rows][chunks][16]: a wave's kept weights
     unsigned long long* sums;  // [rows][chunks][16][2]
     unsigned long long* all;   // [rows][chunks]: the sum of a chunk's bins
     SampleFound* found;        // [rows]
     float* top;                // [rows][chunks]: largest logit
     int32_t* first;            // [rows][chunks]: its index
-    uint32_t* listed;          // [rows][chunks][kSampleParts]
+    uint32_t* listed;          // [rows]
     int row0, chunks, index_bits;
 };
 struct SamplePlan {
