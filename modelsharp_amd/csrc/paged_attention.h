@@ -1111,7 +1111,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void paged_attention_kernel
 }
 
 // Attention behind shared prefixes: the prefixes' tiles first (128 rows, or 16), then those of the requests'
-// own keys, all of a launch beside each other. MODE as above; both kinds where either has both.
+// own keys, all of a launch beside each other. MODE as above; both kinds where either has both. A prefix's keys
+// are read once for all rows of a tile instead of once for each request: 64 tokens of 28 / 4 heads behind 16,000
+// shared keys 59 us with the merge (152 by themselves), bound by the products of tiles of 128 rows; 32 behind
+// 4000 21 us, in tiles of 16.
 template <typename T, int DP, bool WHOLE, PagedMode MODE>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void shared_attention_kernel(SharedAttnArgs p)
 {

@@ -320,7 +320,8 @@ constexpr float kSampleNone = -46.0f;   // weights of 2^-46 and less are 0: such
 // is set, how many logits fall into each bin and, roughly, their weights relative to the chunk's largest: a count in
 // the low 15 bits (a chunk has 2^14), the weights in fp32 as multiples of 2^-31 above, in one whole number, so that an
 // addition in LDS does both and the order of additions does not matter. A bin's place is its grid line modulo
-// 512, the same in every chunk.
+// 512, the same in every chunk. 17 us for 200 rows of 50001 (2.3 TB/s; the copy's 5.1 would be 8): the loads wait for
+// each other at the barrier behind the largest logit.
 __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleArgs a, SampleWs ws)
 {
     __shared__ u64 hist[kSampleBins], all;
@@ -536,10 +537,12 @@ __global__ __launch_bounds__(kSampleThreads, 4) void sample_find_kernel(SampleAr
             k_before = ns.at(bk - 1);
         }
         if (by_p) {
-            // two of fp32's exponentials: arguments of up to 64 with three roundings (2^-16 of it each) and a shift by the
-            // chunk's largest logit (half a step of that), sums in fp32, a step of 2^-31 each
+            // In units of 2^-20 of a weight: 6.1 for scale (2^-22.4 of it, at 46 bits below the largest), 1.4 for the
+            // argument in the scan (31 at the most), 4 for the one here (46, two roundings), 3 for the exponentials and
+            // the sums of bins, a sixteenth for each chunk's sum: held as 32 and an eighth. The shift by a chunk's
+            // largest logit is off by two of its roundings, each weight by a step of 2^-31.
             const float all = ms.at(kSampleBins - 1);
-            const float off = (0x1p-13f + 0x1p-22f * fabsf(top * scale)) * all + (float)ns.at(kSampleBins - 1);
+            const float off = (0x1p-15f + 0x1p-23f * ws.chunks + 0x1p-22f * fabsf(top * scale)) * all + (float)ns.at(kSampleBins - 1);
             const float w0 = by_k ? ms.at(bk - 1) : all, w1 = by_k ? ms.at(bk) : all, p = fmaxf(s.p, 0.0f);
             hi = min(ms.reach(p * w1 + off), by_k ? bk : kSampleBins - 1);
             lo = min(ms.reach(p * w0 - off), hi);
@@ -556,7 +559,8 @@ __global__ __launch_bounds__(kSampleThreads, 4) void sample_find_kernel(SampleAr
 // 3. Each chunk again, by four workgroups: what lies before bin lo is kept and summed exactly, tile by tile, the logits
 // of the bins in question go to the row's list (as places, in any order: what is done with them does not depend on it),
 // by way of LDS so that a workgroup asks for its places in the list once. ALONE: no row has k or p, and each
-// workgroup finds the row's numbers for itself.
+// workgroup finds the row's numbers for itself. 24 us for 200 rows of 50001 by p, where each logit's weight counts, 16 for
+// 64 of 151936 of mixed settings: issue, 17 operations in 64 bits of a logit and its tests.
 constexpr int kSumWaves = kSampleWaves / kSampleParts, kSumList = 1024;
 template <bool ALONE>
 __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
@@ -670,7 +674,8 @@ __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(Sample
 // 4. Each row: the borders among the listed logits (or, where those are too many for the list, among the
 // row's), and the draw. Fine bins of the listed logits, the few of a border's fine bin ranked by a wave, then the
 // tile that the draw falls into and the token; as above every wave searches for itself. (Four waves, one to a SIMD: with
-// sixteen the searches, the same in each, took 6 of 13 us, with eight a row 9.3 instead of 8.5.)
+// sixteen the searches, the same in each, took 6 of 13 us, with eight a row 9.3 instead of 8.5.) Where the list is too
+// long the row itself is searched: 150,000 logits of deviation 0.1 by p 0.6 ms, all equal 2.7 ms.
 constexpr int kDrawThreads = 256, kDrawWaves = kDrawThreads / kWave;
 struct SampleLds {
     u64 list[kSampleList], weight[kSampleList];   // places and their weights
@@ -748,17 +753,30 @@ __device__ __forceinline__ u64 sample_borders(const SampleSearch& q, SampleLds& 
     };
     // every place in question: fn(place, weight, fine bin, whether in [lo, hi])
     auto each = [&](auto&& fn) {
+        if constexpr (LIST) {
 #pragma unroll 1
-        for (int i = tid; i < (LIST ? q.n : q.V); i += kDrawThreads) {
-            if constexpr (LIST) {
+            for (int i = tid; i < q.n; i += kDrawThreads) {
                 const uint32_t b = lds.bin[i];
                 fn(lds.list[i], lds.weight[i], (int)(b & 0x7fff), b < 0x8000);
-            } else {
-                const float l = sample_logit(q.x[i]);
-                if (!(((double)l - q.e.top) * q.e.scale >= kSampleNone)) continue;
-                const int b = fine_bin(l);
-                const u64 c = sample_place(l, i, q.index_bits);
-                if (b != 0x7fff) fn(c, weigh(c), b & 0x7fff, b < 0x8000);
+            }
+        } else {   // (the next four under way)
+            auto load = [&](int i) {
+                return i >= 0 && i + 3 < q.V ? *reinterpret_cast<const floatx4_t*>(q.x + i) : sample_edge(q.x, i, q.V);
+            };
+            floatx4_t next = load(4 * tid - q.lead);
+#pragma unroll 1
+            for (int i = 4 * tid - q.lead; i < q.V; i += 4 * kDrawThreads) {
+                floatx4_t v = next;
+                next = load(min(i + 4 * kDrawThreads, q.V));
+#pragma unroll 1
+                for (int e = 0; e < 4; ++e) {
+                    const float l = sample_logit(v[0]);
+                    v = floatx4_t{v[1], v[2], v[3], v[3]};
+                    if (!(((double)l - q.e.top) * q.e.scale >= kSampleNone)) continue;
+                    const int b = fine_bin(l);
+                    const u64 c = sample_place(l, i + e, q.index_bits);
+                    if (b != 0x7fff) fn(c, weigh(c), b & 0x7fff, b < 0x8000);
+                }
             }
         }
     };

@@ -341,6 +341,18 @@ def test_sample_odd_logits(gpu, vocab):
     check_sample(logits, k=[2] * n, u=u)
 
 
+@pytest.mark.parametrize("vocab", [30011, 151936])
+def test_sample_shares_next_to_one(gpu, vocab):
+    """Borders far down, where the rough sums say least."""
+    rng = np.random.default_rng(vocab)
+    p = 1 - np.array([3e-2, 1e-2, 1e-3, 3e-4, 1e-4, 4e-5, 1e-5, 1e-6, 2.0 ** -24])
+    log(f"shares next to one of {vocab}")
+    for t, dev_ in ((1.0, 2.0), (0.7, 1.5), (1.7, 1.0), (1.0, 0.1)):
+        x = (rng.standard_normal((len(p), vocab)) * dev_).astype(F32)
+        check_sample(x, t=[t] * len(p), p=p, u=1 - (rng.random(len(p)) * 0.02).astype(F32))
+        check_sample(x, t=[t] * len(p), p=p, k=rng.integers(vocab // 50, vocab, len(p)), u=1 - (rng.random(len(p)) * 0.02).astype(F32))
+
+
 def test_sample_tiny_temperatures(gpu):
     """Down to the type's smallest: the likeliest tokens share the draw."""
     rng = np.random.default_rng(14)
