@@ -596,7 +596,7 @@ int ms_hip_paged_commit(const ms_hip_step_desc* desc, const int32_t* dCu, const 
  * of its own value a row: dTemperature fp32 (null: 1; 0 or less or NaN: the likeliest token), dTopK
  * int32 (null, 0 or less: all), dTopP fp32 (null, 1 or more or NaN: all; 0 or less: the
  * likeliest), dMinP fp32 (null, 0 or less or NaN: none), dRandom fp32 in [0, 1) (what is outside counts
- * as its nearest end). A NaN logit counts as -infinity, +infinity as the largest finite value, a temperature above
+ * as its nearest end, NaN as 0). A NaN logit counts as -infinity, +infinity as the largest finite value, a temperature above
  * 1e30 as that; a row without a logit above -infinity has token -1 and log-probability NaN. Weights count in
  * 64 bits, as multiples of 2^-44 (vocabularies above 2^18: of 2^-62 times the next power of two), so a
  * token is that of the 64-bit definition but where that lies within such a step, and the same on
