@@ -165,7 +165,7 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
         hipLaunchKernelGGL(sample_scan_kernel, grid, block, 0, s, p, ws);
         const dim3 parts(kSampleParts * plan.chunks, rows);
         if (p.top_k || p.top_p) {
-            hipLaunchKernelGGL(sample_find_kernel, dim3(rows), block, 0, s, p, ws);
+            hipLaunchKernelGGL(sample_find_kernel, dim3(rows), dim3(kFindThreads), 0, s, p, ws);
             hipLaunchKernelGGL(sample_sum_kernel<false>, parts, dim3(kSumWaves * kWave), 0, s, p, ws);
         } else {
             hipLaunchKernelGGL(sample_sum_kernel<true>, parts, dim3(kSumWaves * kWave), 0, s, p, ws);

@@ -143,7 +143,7 @@ __device__ __forceinline__ u64 sample_least(const SampleRow& s, int frac)
     return s.m > 0.0f ? (u64)__builtin_rint(__builtin_ldexp((double)fminf(s.m, 1.0f), frac)) : 0;
 }
 
-constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / kWave;
+constexpr int kSampleThreads = 512, kSampleWaves = kSampleThreads / kWave;
 constexpr int kSampleLoads = 4;                                      // of a thread, 16 bytes each: a chunk's
 constexpr int kSampleTile = 4 * kWave * kSampleLoads, kSampleTiles = kSampleWaves;   // tokens of a wave; waves of a chunk
 constexpr int kSampleEach = kSampleBins / kWave;                     // bins of a lane
@@ -318,10 +318,10 @@ constexpr float kSampleNone = -46.0f;   // weights of 2^-46 and less are 0: such
 
 // 1. Each chunk of a row: its largest logit (and that one's index, for the likeliest token), and, where k or p
 // is set, how many logits fall into each bin and, roughly, their weights relative to the chunk's largest: a count in
-// the low 15 bits (a chunk has 2^14), the weights in fp32 as multiples of 2^-31 above, in one whole number, so that an
+// the low 15 bits (a chunk has 2^13), the weights in fp32 as multiples of 2^-31 above, in one whole number, so that an
 // addition in LDS does both and the order of additions does not matter. A bin's place is its grid line modulo
-// 512, the same in every chunk. 17 us for 200 rows of 50001 (2.3 TB/s; the copy's 5.1 would be 8): the loads wait for
-// each other at the barrier behind the largest logit.
+// 512, the same in every chunk. 13 us for 200 rows of 50001 (3.0 TB/s; the copy's 5.1 would be 8): the loads wait for
+// each other at the barrier behind the largest logit (17 in workgroups of 1024 threads).
 __global__ __launch_bounds__(kSampleThreads, 8) void sample_scan_kernel(SampleArgs a, SampleWs ws)
 {
     __shared__ u64 hist[kSampleBins], all;
@@ -451,7 +451,8 @@ __device__ __forceinline__ float sample_top(const SampleWs& ws, int64_t chunk0)
 // error: [lo, hi] for the last token kept, and k's where p needs the sum of the first k. The chunks' bins are added up two
 // threads to a bin's place; then one wave searches. (By every workgroup of the next launch for itself, that launch took
 // 38 us for 200 x 50001 by p, 22 of its 27 thousand cycles before the first weight.)
-__global__ __launch_bounds__(kSampleThreads, 4) void sample_find_kernel(SampleArgs a, SampleWs ws)
+constexpr int kFindThreads = 2 * kSampleBins;
+__global__ __launch_bounds__(kFindThreads, 4) void sample_find_kernel(SampleArgs a, SampleWs ws)
 {
     __shared__ float mass[2][kSampleBins];
     __shared__ uint32_t counts[2][kSampleBins];
@@ -459,8 +460,8 @@ __global__ __launch_bounds__(kSampleThreads, 4) void sample_find_kernel(SampleAr
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t chunk0 = (int64_t)r * ws.chunks;
     const SampleRow s = sample_row(a, ws.row0 + r);
-    // the bins of the first chunks (where there are none, they are not used)
-    constexpr int kEarly = 8;
+    // the bins of the first chunks (where there are none, they are not used; 20 take in vocabularies of 152,000)
+    constexpr int kEarly = 10;
     const int q = tid & (kSampleBins - 1), half = tid / kSampleBins;
     const u64* const hists = ws.hist + chunk0 * kSampleBins + q;
     u64 early[kEarly];
@@ -556,10 +557,10 @@ __global__ __launch_bounds__(kSampleThreads, 4) void sample_find_kernel(SampleAr
     }
 }
 
-// 3. Each chunk again, by four workgroups: what lies before bin lo is kept and summed exactly, tile by tile, the logits
+// 3. Each chunk again, by two workgroups: what lies before bin lo is kept and summed exactly, tile by tile, the logits
 // of the bins in question go to the row's list (as places, in any order: what is done with them does not depend on it),
 // by way of LDS so that a workgroup asks for its places in the list once. ALONE: no row has k or p, and each
-// workgroup finds the row's numbers for itself. 24 us for 200 rows of 50001 by p, where each logit's weight counts, 16 for
+// workgroup finds the row's numbers for itself. 21 us for 200 rows of 50001 by p, where each logit's weight counts, 14 for
 // 64 of 151936 of mixed settings: issue, 17 operations in 64 bits of a logit and its tests.
 constexpr int kSumWaves = kSampleWaves / kSampleParts, kSumList = 1024;
 template <bool ALONE>
