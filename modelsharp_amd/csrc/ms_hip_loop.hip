@@ -17,9 +17,9 @@ hipError_t launch_plan(const PlanArgs& p, int cus, hipStream_t s)
     const int64_t items = std::max<int64_t>(p.tokens, p.requests);
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, 2 * cus));
     const unsigned lds = 2 * (p.requests + 1) * sizeof(uint32_t);
-    if (lds > 63 * 1024)   // beside the kernel's own
+    if (lds > 63 * 1024)   // beside the kernel's own; always the most there is, for calls of two threads
         if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(paged_plan_kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds))
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, 2 * (kPlanRequests + 1) * 4))
             return e;
     hipLaunchKernelGGL(paged_plan_kernel, dim3(grid), dim3(256), lds, s, p);
     return hipGetLastError();
@@ -155,9 +155,12 @@ hipError_t launch_sample(const SampleArgs& p, const SamplePlan& plan, void* work
     ws.top = reinterpret_cast<float*>(ws.found + n);
     ws.first = reinterpret_cast<int32_t*>(ws.top + c);
     ws.listed = reinterpret_cast<uint32_t*>(ws.first + c);
-    const int lds = (int)(sizeof(SampleLds) + plan.chunks * kSampleTiles * 8);
+    constexpr int kMostChunks = (kSampleVocab + 3 + kSampleChunk - 1) / kSampleChunk;
+    constexpr int kMostLds = (int)sizeof(SampleLds) + kMostChunks * kSampleTiles * 8;
+    static_assert(kMostLds <= 160 * 1024, "a CU's LDS");
+    const int lds = (int)sizeof(SampleLds) + plan.chunks * kSampleTiles * 8;
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sample_draw_kernel),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds))
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds))
         return e;
     for (; ws.row0 < p.rows; ws.row0 += plan.batch) {
         const int rows = std::min(plan.batch, p.rows - ws.row0);

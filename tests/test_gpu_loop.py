@@ -419,6 +419,45 @@ def test_sample_follows_the_distribution(gpu):
     assert np.abs(np.bincount(token, minlength=50) - share * n).max() <= 1.0
 
 
+def test_sample_rows_in_batches(gpu):
+    """More rows than the workspace holds at a time, each with settings of its own."""
+    rng = np.random.default_rng(15)
+    rows, vocab = 2900, 301
+    one = native.sample_workspace_size(native.SampleDesc(rows=1, vocab=vocab))
+    assert native.sample_workspace_size(native.SampleDesc(rows=rows, vocab=vocab)) < rows * one   # batches
+    log(f"batches of {rows}")
+    s = settings(rng, rows)
+    s["u"] = (np.floor(s["u"] * 1000) + F32(0.37)) / F32(1000)
+    check_sample((rng.standard_normal((rows, vocab)) * 2).astype(F32), **s)
+
+
+def test_two_samples_at_once(gpu):
+    """On two streams, of different vocabularies, each with a workspace of its own; as one after the other."""
+    import torch
+    rng = np.random.default_rng(16)
+    calls = []
+    for rows, vocab in ((40, 150001), (64, 30000)):
+        s = settings(rng, rows)
+        d = native.SampleDesc(rows=rows, vocab=vocab)
+        n = native.sample_workspace_size(d)
+        bufs = [dev((rng.standard_normal((rows, vocab)) * 2).astype(F32)), *(dev(s[x]) for x in "tkpmu")]
+        calls.append((d, bufs, torch.empty(n, dtype=torch.uint8, device="cuda"), n, torch.cuda.Stream()))
+    results = []
+    for together in (False, True):
+        outs = [[(dev(np.zeros(c[0].rows, I32)), dev(np.zeros(c[0].rows, F32))) for _ in range(6)] for c in calls]
+        torch.cuda.synchronize()
+        log(f"together {together}")
+        for i in range(6):
+            for (d, bufs, ws, n, st), out in zip(calls, outs):
+                native.sample(d, *map(ptr, bufs), *map(ptr, out[i]), ptr(ws), n, st.cuda_stream)
+                if not together:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        results.append([[t.cpu().numpy() for t in pair] for out in outs for pair in out])
+    for a, b in zip(*results):
+        assert all(np.array_equal(x, y) for x, y in zip(a, b))
+
+
 def test_sample_replayed_from_a_graph(gpu):
     """Captured once, replayed with other logits and settings; every replay as an eager call."""
     import torch
