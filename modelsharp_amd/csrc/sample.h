@@ -561,7 +561,7 @@ __global__ __launch_bounds__(kFindThreads, 4) void sample_find_kernel(SampleArgs
 // of the bins in question go to the row's list (as places, in any order: what is done with them does not depend on it),
 // by way of LDS so that a workgroup asks for its places in the list once. ALONE: no row has k or p, and each
 // workgroup finds the row's numbers for itself. 21 us for 200 rows of 50001 by p, where each logit's weight counts, 14 for
-// 64 of 151936 of mixed settings: issue, 17 operations in 64 bits of a logit and its tests.
+// 64 of 151936 of mixed settings: issue (VALU busy 81% of the cycles), 17 operations in 64 bits of a logit and its tests.
 constexpr int kSumWaves = kSampleWaves / kSampleParts, kSumList = 1024;
 template <bool ALONE>
 __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
