@@ -67,7 +67,7 @@ struct SampleArgs {
 };
 constexpr int kSampleBins = 512;                 // of logits, by which a border is first looked for
 constexpr int kSampleList = 6144;                // logits of the bins that a border lies in, at most
-constexpr int kSampleChunk = 8192;               // tokens of a workgroup of the first two launches
+constexpr int kSampleChunk = 8192;               // tokens of a workgroup of the first launch
 constexpr int kSampleParts = 2;                  // workgroups to a chunk of the launch that sums
 // The weights of a row whose largest logit is `top`: 2^(scale (l - top)), and 0 below `low`.
 struct SampleScale {
