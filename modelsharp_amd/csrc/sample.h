@@ -602,7 +602,7 @@ __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(Sample
     // sums: each tile's kept weights before `lo`; the weights before `lo`; all weights that p is a part of
     const u64 least = uniform(f.least);
     const SampleScale es = {uniform(f.weights.top), uniform(f.weights.scale), uniform(f.weights.low)};
-    const bool every = f.by_p && !f.by_k, simple = !borders && !least;
+    const bool every = f.by_p && !f.by_k && !f.wide, simple = !borders && !least;   // (wide: the draw weighs the row)
     const float step = uniform(f.step), none = uniform(f.none), from = uniform(f.from), line = uniform(f.line);
     const float line_lo = uniform(f.line_lo), line_hi = uniform(f.line_hi), line_k = uniform(f.line_k);
     const float line_k_end = uniform(f.line_k_end);
@@ -809,7 +809,9 @@ __device__ __forceinline__ u64 sample_borders(const SampleSearch& q, SampleLds& 
     mass.scan();
     // The place in fine bin k at which the counts or weights of its places, up to `up_to`, sum to `target`,
     // and their sum of weights up to it: first k's, then p's.
-    u64 last = ~0ull, whole = lds.sums[1];
+    // (Of a wide row the bins hold all that weighs anything, and not -infinity, which the sums take for `low`, the
+    // largest logit itself in rows of the lowest values.)
+    u64 last = ~0ull, whole = f.wide && !f.by_k ? mass.at(kSampleBins - 1) : lds.sums[1];
     const u64 before = lds.sums[0];
 #pragma unroll 1
     for (int slot = f.by_k ? 0 : 1; slot < (f.by_p ? 2 : 1); ++slot) {

@@ -341,6 +341,32 @@ def test_sample_odd_logits(gpu, vocab):
     check_sample(logits, k=[2] * n, u=u)
 
 
+@pytest.mark.parametrize("vocab", [5, 1000, 4097, 8192, 50001])
+def test_sample_shares_of_the_lowest_logits(gpu, vocab):
+    """Rows whose largest logit is the type's lowest value (or the next above it), by p alone: what is -infinity, NaN or
+    behind the row's end has no part in the total that p is a share of."""
+    rng = np.random.default_rng(vocab)
+    low = np.finfo(F32).min
+    next_up = np.nextafter(low, F32(0))
+    rows, t = [], []
+    for top in (low, next_up):
+        for below in ([], [-np.inf], [np.nan], [-np.inf, np.nan], [low], [low, -np.inf]):
+            for temperature in (1.0, 0.3, 1e30):   # (at 1e30 `low` weighs e^-20 beside the next above it)
+                x = np.full(vocab, top, F32)
+                for odd in below:
+                    x[rng.random(vocab) < 0.4] = odd
+                x[vocab // 2] = top
+                rows.append(x)
+                t.append(temperature)
+    n, logits = len(rows), np.stack(rows)
+    log(f"lowest logits at {vocab}")
+    for p in (0.0137, 0.43, 0.871):
+        u = (np.floor(rng.random(n) * 97) + 0.37) / 97
+        check_sample(logits, t=t, p=[p] * n, u=u)
+        check_sample(logits, t=t, p=[p] * n, m=[0.01] * n, u=u, stride=vocab + 3)
+    check_sample(logits, t=t, p=np.where(np.arange(n) % 2, 1.0, 0.43), k=np.where(np.arange(n) % 3, 0, vocab // 2 + 1), u=u)
+
+
 @pytest.mark.parametrize("vocab", [30011, 151936])
 def test_sample_shares_next_to_one(gpu, vocab):
     """Borders far down, where the rough sums say least."""
