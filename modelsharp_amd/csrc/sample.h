@@ -308,11 +308,13 @@ __device__ __forceinline__ int sample_bin(float l, int top_grid, float step)
 {
     return min(top_grid - sample_grid(l, step), kSampleBins - 1);
 }
-// Where the grid's lines are no whole numbers in fp32, or t is next to infinity, the bins say nothing; where the
+// Where the grid's lines are no whole numbers in fp32, or t is next to infinity, the bins say nothing; nor where t is
+// so small that a weight's exponent cannot be had by `scale` in fp32 (below 2^-100 alone: from there on top * scale is
+// below 2^19 where top * step is below 2^22; an infinite scale times 0 is NaN). Where the
 // largest logit is next to the lowest value there is, `low` does not tell -infinity from it.
 __device__ __forceinline__ bool sample_wide(float top, float step, bool borders, const SampleRow& s)
 {
-    return (borders && (!(fabsf(top * step) < 0x1p22f) || !(s.t < 1e29f))) || top < -1e37f;
+    return (borders && (!(fabsf(top * step) < 0x1p22f) || !(fabsf(top * s.scale) < 0x1p20f) || !(s.t < 1e29f))) || top < -1e37f;
 }
 constexpr float kSampleNone = -46.0f;   // weights of 2^-46 and less are 0: such logits need not be counted
 

@@ -392,6 +392,68 @@ def test_sample_tiny_temperatures(gpu):
                 assert (check_sample(x, t=t, u=[u] * 6, **s) == token).all()
 
 
+@pytest.mark.parametrize("top", [0.0, -0.0, 1e-39, 2.0 ** -85, -2.0 ** -85, 2.0 ** -100])
+def test_sample_limits_at_tiny_temperatures(gpu, top):
+    """Where 1 / t is infinite or next to it and the largest logit next to zero: k and p cut as ever, ties by rising
+    index among them."""
+    rng = np.random.default_rng(17)
+    t = np.array([1e-30, 2.0 ** -100, 2.0 ** -101, 2.0 ** -120, 2.0 ** -126, 2.0 ** -130, 1e-40, 1e-42, 1e-45], F32)
+    n, ties = len(t), [1234, 4000, 7000]
+    x = (np.minimum(rng.standard_normal((n, 9000)) - 6, -0.5) + top).astype(F32)
+    x[:, ties] = top
+    log(f"limits at tiny temperatures below {top}")
+    for s, kept in ((dict(k=[1] * n), 1), (dict(k=[2] * n), 2), (dict(p=[0.3] * n), 1), (dict(p=[0.6] * n), 2), (dict(p=[0.9] * n), 3),
+                    (dict(k=[2] * n, p=[0.4] * n), 1), (dict(k=[2] * n, p=[0.6] * n), 2)):
+        for u in (0.1, 0.6, 0.9):
+            assert (check_sample(x, t=t, u=[u] * n, **s) == ties[int(u * kept)]).all()
+    # logits a part of t apart, as far as there are such numbers next to `top`
+    for part in (0.25, 1.0, 7.0):
+        y = x.copy()
+        y[:, 100:180] = (F32(top) - part * t[:, None].astype(np.float64) * np.arange(80)).astype(F32)
+        for s in (dict(k=[3] * n), dict(p=[0.83] * n), dict(k=[17] * n, p=[0.771] * n), dict(p=[0.913] * n, m=[0.11] * n)):
+            check_sample(y, t=t, u=rng.random(n), **s)
+
+
+def test_half_of_two_ties_at_tiny_temperatures(gpu):
+    """p of 0.5 of two equal weights is reached by the first."""
+    t = np.array([1e-37, 2.0 ** -130, 1e-40, 1e-45], F32)
+    x = np.full((4, 9000), -3.0, F32)
+    x[:, 4000] = x[:, 7000] = 0.0
+    log("half of two ties")
+    assert (run_sample(x, t=t, p=[0.5] * 4, u=[0.7] * 4)[0] == 4000).all()
+
+
+@pytest.mark.parametrize("top", [0.0, -0.0, 1e-39, 2.0 ** -85, -2.0 ** -85, 2.0 ** -100])
+def test_sample_limits_at_tiny_temperatures(gpu, top):
+    """Where 1 / t is infinite or next to it and the largest logit next to zero: k and p cut as ever, ties by rising
+    index among them."""
+    rng = np.random.default_rng(17)
+    t = np.array([1e-30, 2.0 ** -100, 2.0 ** -101, 2.0 ** -120, 2.0 ** -126, 2.0 ** -130, 1e-40, 1e-42, 1e-45], F32)
+    n, ties = len(t), [1234, 4000, 7000]
+    x = (np.minimum(rng.standard_normal((n, 9000)) - 6, -0.5) + top).astype(F32)
+    x[:, ties] = top
+    log(f"limits at tiny temperatures below {top}")
+    for s, kept in ((dict(k=[1] * n), 1), (dict(k=[2] * n), 2), (dict(p=[0.3] * n), 1), (dict(p=[0.6] * n), 2), (dict(p=[0.9] * n), 3),
+                    (dict(k=[2] * n, p=[0.4] * n), 1), (dict(k=[2] * n, p=[0.6] * n), 2)):
+        for u in (0.1, 0.6, 0.9):
+            assert (check_sample(x, t=t, u=[u] * n, **s) == ties[int(u * kept)]).all()
+    # logits a part of t apart, as far as there are such numbers next to `top`
+    for part in (0.25, 1.0, 7.0):
+        y = x.copy()
+        y[:, 100:180] = (F32(top) - part * t[:, None].astype(np.float64) * np.arange(80)).astype(F32)
+        for s in (dict(k=[3] * n), dict(p=[0.83] * n), dict(k=[17] * n, p=[0.771] * n), dict(p=[0.913] * n, m=[0.11] * n)):
+            check_sample(y, t=t, u=rng.random(n), **s)
+
+
+def test_half_of_two_ties_at_tiny_temperatures(gpu):
+    """p of 0.5 of two equal weights is reached by the first."""
+    t = np.array([1e-37, 2.0 ** -130, 1e-40, 1e-45], F32)
+    x = np.full((4, 9000), -3.0, F32)
+    x[:, 4000] = x[:, 7000] = 0.0
+    log("half of two ties")
+    assert (run_sample(x, t=t, p=[0.5] * 4, u=[0.7] * 4)[0] == 4000).all()
+
+
 def test_sample_of_a_long_row(gpu):
     rng = np.random.default_rng(9)
     vocab = 2 ** 22 - 3
