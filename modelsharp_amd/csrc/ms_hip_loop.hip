@@ -105,7 +105,8 @@ hipError_t launch_shared_attention(const SharedAttnArgs& args, const SharedPlan&
     p.prefix_blocks = plan.prefix_blocks;
     p.prefix_grid = (int)plan.prefix_grid;
     p.blocks_grid = (int)plan.blocks_grid;
-    p.few_rows = plan.few_rows;
+    // without tiles of 128 for the requests' own keys those of 16 take requests of any length (max_new may be too small)
+    p.few_rows = plan.blocks_grid ? plan.few_rows : INT32_MAX;
     const unsigned grid = (unsigned)(plan.prefix_grid + plan.blocks_grid + plan.rows_grid);
     const bool whole = p.b.page.div % 16 == 0, both = plan.prefix_blocks || plan.blocks_grid;
     if (p.f16)

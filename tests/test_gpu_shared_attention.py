@@ -141,6 +141,31 @@ def test_bounds_that_are_too_small(gpu, dtype):
         check_attention(out.cpu().numpy(), b, q, H)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
+def test_bounds_of_new_tokens_that_are_too_small_beside_large_tiles(gpu, dtype):
+    """The prefix in tiles of 128 rows, the requests' own keys in tiles of 16 by a bound of few new tokens, and requests
+    of more: every row has its own keys' records."""
+    import torch
+    H, G, D, prefix = 8, 2, 64, 5000
+    b, bounds, shared = batch(11, [(prefix, [(40, 30)] * 6 + [(1, 500), (64, 0)])], G, D, 16, dtype, roomy=False)
+    q = queries(b, H)
+    rows, cus = b.tokens * H // G, torch.cuda.get_device_properties(0).multi_processor_count
+    pad = lambda n: -(-rows // n) * n   # noqa: E731
+    bufs = [dev(x) for x in (q, b.cu, b.past, b.table, bounds, shared, b.k, b.v)]
+    for new in (1, 9, 16):
+        d = desc_of(b, H, max_new=new)
+        s = native.SharedDesc(groups=1, max_shared=prefix, max_rest=600)
+        assert (len(b.news) - 1) * prefix * 2 * G * D * b.k.itemsize >= WORTH
+        # what the launch goes by: few rows to a request, so many to the prefix that tiles of 128 take it
+        assert new * H // G <= 64 < 40 * H // G and pad(128) * prefix * G / 2400 + 5 * cus < pad(16) * prefix * G / 1700
+        n = native.paged_shared_attention_workspace_size(d, s)
+        assert n > 2 * b.tokens * H * (D + 2) * 4   # shared, in several records
+        out, ws = (torch.full((m,), float("nan"), device="cuda") for m in (b.tokens * H * D, n // 4 + 4))
+        log(f"bound of {new} beside tiles of 128 rows, {dtype.__name__}")
+        native.paged_shared_attention(d, s, *map(ptr, bufs), ptr(out), ptr(ws), n, stream())
+        check_attention(out.reshape(b.tokens, -1).cpu().numpy(), b, q, H)
+
+
 @pytest.mark.parametrize("new", [1, 40], ids=["tokens", "chunks"])
 @pytest.mark.parametrize("dtype", [F16, F32], ids=["f16", "f32"])
 def test_a_prefix_is_read_from_its_first_request(gpu, dtype, new):
