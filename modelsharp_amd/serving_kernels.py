@@ -206,8 +206,9 @@ class HipPagedAttentionKernel(_Serving):
             cu, past = (ctx.get_tensor(node.inputs[i]).reshape(-1).astype(np.int64) for i in (5, 6))
             at = np.searchsorted(bounds, np.arange(d.requests), side="right") - 1
             mine = np.where((at >= 0) & (at < groups), lengths[np.clip(at, 0, groups - 1)], 0)
-            s.max_shared = int(np.clip(lengths.max(), 0, d.max_total))
-            s.max_rest = int(np.clip((np.diff(cu) + past - mine).max(), 0, d.max_total))
+            # (at least 1: the entry's 0 is "not known")
+            s.max_shared = int(np.clip(lengths.max(), 1, d.max_total))
+            s.max_rest = int(np.clip((np.diff(cu) + past - mine).max(), 1, d.max_total))
         return s, self._lengths(ctx, names[0], groups + 1, device), self._lengths(ctx, names[1], groups, device)
 
 

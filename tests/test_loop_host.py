@@ -344,6 +344,18 @@ def test_attention_node_takes_groups(on_the_host):
     assert on_the_host[5][1][1].groups == 0
 
 
+def test_attention_node_knows_lengths_of_zero(on_the_host):
+    """The entry's 0 is "not known": host lengths that are all zero are a bound of 1, not of the table's width."""
+    node, ctx = attention_node({"g": np.array([0, 2, 4], I32), "s": np.zeros(2, I32)})
+    HipPagedAttentionKernel()._run(node, ctx)
+    s = on_the_host[1][1][1]
+    assert (s.groups, s.max_shared, s.max_rest) == (2, 1, 34)
+    node, ctx = attention_node({"g": np.array([0, 4], I32), "s": np.array([48], I32), "past": np.full(4, 48, I32), "cu": np.zeros(5, I32)})
+    HipPagedAttentionKernel()._run(node, ctx)
+    s = on_the_host[3][1][1]
+    assert (s.groups, s.max_shared, s.max_rest) == (1, 48, 1)
+
+
 @pytest.mark.parametrize("values,groups,words", [
     (dict(g=np.array([0, 3], I32)), ("g",), "given together"), (dict(s=np.array([3], I32)), ("", "s"), "given together"),
     (dict(g=np.array([0, 3, 4], I32), s=np.array([3], I32)), ("g", "s"), "3 elements; expected 2"),
