@@ -5,7 +5,8 @@
 //           fits the step's rows, and need is 0 or its sum fits the free pages
 //   cu = sums of want over the served; page j of the step is the j-th from the top of the stack
 //
-// (sums over the requests that could be served alone), and the step's end: lengths advance, the
+// (sums over the requests whose pages fit the table, served or not, so that what waits is not passed by what comes
+// behind it), and the step's end: lengths advance, the
 // pages of requests that ended go back to the stack.
 #pragma once
 #include "serving_loop.h"

@@ -87,8 +87,9 @@ __device__ __forceinline__ float sample_clamp(float l, float low) { return __bui
 
 // 2^y, y = scale (l - top), by 2^k 2^f, k the nearest whole number, f in [-1/2, 1/2] by a polynomial (through 2^f at
 // the zeros of a Chebyshev polynomial, 1 at 0; off by 2^-44 of it), as a whole multiple of 2^-frac in the low bits of
-// a double's (the sum with 2^52 rounds it): kSampleBits above it. A logit's 15 operations in 64 bits are most of what
-// bounds sampling by p, where every logit's weight counts. Four at a time, so that none waits for its own.
+// a double's (the sum with 2^52 rounds it): kSampleBits above it. A logit's 16 operations in 64 bits (3 additions, 11
+// fma, a conversion and a ldexp) are most of what bounds sampling by p, where every logit's weight counts. Four at a
+// time, so that none waits for its own.
 constexpr u64 kSampleBits = 0x433ull << 52;
 template <int N>
 __device__ __forceinline__ void sample_raw(const float (&l)[N], const SampleScale& e, int frac, u64 (&out)[N])
@@ -145,7 +146,8 @@ __device__ __forceinline__ u64 sample_least(const SampleRow& s, int frac)
 
 constexpr int kSampleThreads = 512, kSampleWaves = kSampleThreads / kWave;
 constexpr int kSampleLoads = 4;                                      // of a thread, 16 bytes each: a chunk's
-constexpr int kSampleTile = 4 * kWave * kSampleLoads, kSampleTiles = kSampleWaves;   // tokens of a wave; waves of a chunk
+constexpr int kSampleTile = 4 * kWave * kSampleLoads;                // tokens of a wave
+static_assert(kSampleTiles == kSampleWaves, "a chunk's tiles to the waves of a workgroup");
 constexpr int kSampleEach = kSampleBins / kWave;                     // bins of a lane
 
 // A 64-bit value moved by one DPP control; lanes whose source is outside the row, or whose row the mask leaves
@@ -416,6 +418,7 @@ __device__ __forceinline__ SampleFound sample_limits(const SampleArgs& a, const 
     f.by_p = by_p;
     f.k_before = k_before;
     f.wide = wide;
+    f.every = by_p && !by_k && !wide;   // (of a wide row the draw weighs them)
     f.step = step;
     f.none = none;
     f.from = lo == kSampleBins && least ? top + (__builtin_amdgcn_logf(fminf(s.m, 1.0f)) - slack) * to_logit : none;
@@ -563,7 +566,8 @@ __global__ __launch_bounds__(kFindThreads, 4) void sample_find_kernel(SampleArgs
 // of the bins in question go to the row's list (as places, in any order: what is done with them does not depend on it),
 // by way of LDS so that a workgroup asks for its places in the list once. ALONE: no row has k or p, and each
 // workgroup finds the row's numbers for itself. 21 us for 200 rows of 50001 by p, where each logit's weight counts, 14 for
-// 64 of 151936 of mixed settings: issue (VALU busy 81% of the cycles), 17 operations in 64 bits of a logit and its tests.
+// 64 of 151936 of mixed settings: issue (VALU busy for more than 80% of the cycles), a logit's 16 operations in 64 bits, the
+// sum of its weight, and its tests.
 constexpr int kSumWaves = kSampleWaves / kSampleParts, kSumList = 1024;
 template <bool ALONE>
 __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(SampleArgs a, SampleWs ws)
@@ -604,7 +608,7 @@ __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(Sample
     // sums: each tile's kept weights before `lo`; the weights before `lo`; all weights that p is a part of
     const u64 least = uniform(f.least);
     const SampleScale es = {uniform(f.weights.top), uniform(f.weights.scale), uniform(f.weights.low)};
-    const bool every = f.by_p && !f.by_k && !f.wide, simple = !borders && !least;   // (wide: the draw weighs the row)
+    const bool every = f.every, simple = !borders && !least;
     const float step = uniform(f.step), none = uniform(f.none), from = uniform(f.from), line = uniform(f.line);
     const float line_lo = uniform(f.line_lo), line_hi = uniform(f.line_hi), line_k = uniform(f.line_k);
     const float line_k_end = uniform(f.line_k_end);
@@ -678,7 +682,8 @@ __global__ __launch_bounds__(kSumWaves * kWave, 8) void sample_sum_kernel(Sample
 // row's), and the draw. Fine bins of the listed logits, the few of a border's fine bin ranked by a wave, then the
 // tile that the draw falls into and the token; as above every wave searches for itself. (Four waves, one to a SIMD: with
 // sixteen the searches, the same in each, took 6 of 13 us, with eight a row 9.3 instead of 8.5.) Where the list is too
-// long the row itself is searched: 150,000 logits of deviation 0.1 by p 0.6 ms, all equal 2.7 ms.
+// long the row itself is searched, by its one workgroup, slower than the plain form, which sorts it (0.35 ms): 150,000
+// logits of deviation 0.1 by p 0.6 ms, all equal 2.7 ms.
 constexpr int kDrawThreads = 256, kDrawWaves = kDrawThreads / kWave;
 struct SampleLds {
     u64 list[kSampleList], weight[kSampleList];   // places and their weights

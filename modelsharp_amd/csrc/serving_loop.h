@@ -68,6 +68,7 @@ struct SampleArgs {
 constexpr int kSampleBins = 512;                 // of logits, by which a border is first looked for
 constexpr int kSampleList = 6144;                // logits of the bins that a border lies in, at most
 constexpr int kSampleChunk = 8192;               // tokens of a workgroup of the first launch
+constexpr int kSampleTiles = 8;                  // tiles of a chunk: what a wave sums
 constexpr int kSampleParts = 2;                  // workgroups to a chunk of the launch that sums
 // The weights of a row whose largest logit is `top`: 2^(scale (l - top)), and 0 below `low`.
 struct SampleScale {
@@ -83,6 +84,7 @@ struct SampleFound {
     int by_k, by_p;
     uint32_t k_before;         // tokens before bin bk
     int wide;                  // the bins say nothing
+    int every;                 // the sums weigh each logit: p, without k, where the bins say something
     int answered;              // the row's answer is there
     float step, from, none, line, line_lo, line_hi, line_k, line_k_end;
 };
@@ -90,8 +92,8 @@ struct SampleFound {
 struct SampleWs {
     unsigned long long* hist;  // [rows][chunks][kSampleBins]
     unsigned long long* list;  // [rows][kSampleList]
-    unsigned long long* tiles; // [rows][chunks][16]: a wave's kept weights
-    unsigned long long* sums;  // [rows][chunks][16][2]
+    unsigned long long* tiles; // [rows][chunks][kSampleTiles]: a wave's kept weights
+    unsigned long long* sums;  // [rows][chunks][kSampleTiles][2]
     unsigned long long* all;   // [rows][chunks]: the sum of a chunk's bins
     SampleFound* found;        // [rows]
     float* top;                // [rows][chunks]: largest logit
