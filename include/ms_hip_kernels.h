@@ -559,7 +559,10 @@ int ms_hip_lora(const ms_hip_lora_desc* desc, const float* dX, const void* dA, c
  * [num_pages] of which [0, dFreeCount[0]) are free. A request is served as a whole or not at
  * all: if its pages fit the table, the sum of what is wanted up to and with it is at most
  * `tokens`, and it needs no new page or the sum of the pages needed up to and with it is at
- * most the free ones (sums over the requests whose pages fit the table). Written:
+ * most the free ones (sums over the requests whose pages fit the table). One that waits stays in the sums,
+ * so that those behind it do not pass it: one whose pages are not free keeps those that need a page
+ * waiting, and a want above `tokens`, which is never served, all of them, until the host makes it smaller (a
+ * prompt longer than a step is wanted in parts). Written:
  *   dCu int32 [requests + 1]   the step's rows, cu of ms_hip_paged_append and _attention: request
  *                              r is served where cu[r] < cu[r + 1]
  *   dTable int32 [requests, max_pages]   the new pages of those served, from the top of the stack in

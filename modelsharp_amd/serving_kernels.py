@@ -348,7 +348,9 @@ class HipPagedStepPlanKernel(_Step):
     [num_blocks], free_count [1], wanted [requests]) -> (cumulative_sequence_length [requests + 1],
     request_ids, position_ids, slots [tokens], used_blocks [1]), with attributes tokens (the step's rows)
     and block_size: the first four inputs are int32 device tensors, of which free_blocks[0 ..
-    free_count) are free; a request that finds no room has no rows in this step. The new
+    free_count) are free; a request that finds no room has no rows in this step, nor have those
+    behind it that would pass it (a wanted above tokens is never served, and none behind it). Rows
+    are those of the requests served; request_ids says whose (-1: nobody's). The new
     blocks are written to block_table; PagedStepCommit takes them off the free ones."""
     op_type = "PagedStepPlan"
 
@@ -395,9 +397,9 @@ class HipPagedStepCommitKernel(_Step):
 
 class HipSampleTokensKernel(_Serving):
     """SampleTokens(logits [..., vocab], random, temperature, top_k, top_p, min_p) -> (tokens int32 [...],
-    log_probs [...]): the inputs behind logits hold one value for each row, all but random (in
-    [0, 1)) optional; a temperature of 0 takes the likeliest token, a row without a logit above
-    -infinity has token -1."""
+    log_probs [...]): the inputs behind logits hold one value for each row (of a step's rows: its
+    request's), all but random (in [0, 1)) optional; a temperature of 0 takes the likeliest token, a
+    row without a logit above -infinity has token -1."""
     op_type = "SampleTokens"
 
     def _run(self, node: GraphNode, ctx: GraphContext) -> None:

@@ -144,6 +144,17 @@ def test_plan_lengths_that_make_no_sense(gpu):
     run_commit(pool, pool.table, np.arange(7), 0, np.ones(6, I32), np.array([0, 1, 2, -5, 9, big], I32))
 
 
+def test_what_waits_is_not_passed(gpu):
+    """A want above the step's rows holds back all behind it; one whose pages are not free those that need a page."""
+    pool = ref.Pool(8, [5, 16, 3, 32, 7], 16, 2, 4)
+    for want, tokens, served in (([9, 1, 1, 1, 1], 8, [0, 0, 0, 0, 0]), ([1, 9, 1, 1, 1], 8, [1, 0, 0, 0, 0]),
+                                 # 5 + 40 fill 3 pages of 16, 2 of them new and both free; 5 + 50 need 3
+                                 ([40, 1, 1, 1, 1], 60, [40, 0, 1, 0, 1]), ([50, 1, 1, 1, 1], 60, [0, 0, 1, 0, 1]),
+                                 ([8, 1, 1, 1, 1], 8, [8, 0, 0, 0, 0])):
+        log(f"want {want} of {tokens}")
+        assert np.diff(run_plan(pool, want, tokens)[0]).tolist() == served
+
+
 def test_pages_that_are_not_there(gpu):
     """Table and stack entries outside the pool: their rows have no slot and nothing returns them."""
     pool = ref.Pool(5, [40, 20, 70, 1], 16, 12, 6)
